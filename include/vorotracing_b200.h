@@ -401,6 +401,62 @@ VT_API vt_status vt_pad_u8x4(const uint8_t *src, uint64_t texels, void *dst, vt_
 VT_API vt_status vt_quantize_u8(const float *src, uint64_t count, float scale, float offset,
                                 uint8_t *dst, vt_stream stream);
 
+/* ---- low-precision operators of a learned layer ----
+ *
+ * No reference counterpart.  Microscaled formats: a row is cut into blocks of
+ * 32 columns (the last one padded with zeros), each with one exponent byte E.
+ *   8 bits: codes (rows, 32 B) i8, exps (rows, B) u8, B = ceil(cols / 32);
+ *           value = code * 2^(E - 133), E >= 7
+ *   4 bits: codes (rows, 16 B) u8, the even column in the low nibble, exps
+ *           (rows, B) u8; value = e2m1 * 2^(E - 127), E >= 1
+ * E = 255 marks a block that held a NaN or an infinity: its values are NaN.
+ * Codes are 16-byte aligned.  Other matrices are row-major with a row stride
+ * in elements; outputs are dense.  An element type is VT_F32, VT_F16 or
+ * VT_BF16 (products: 16-bit types), an activation one of VT_ACT_*. */
+#define VT_F32 0
+#define VT_F16 1
+#define VT_BF16 2
+#define VT_ACT_IDENTITY 0
+#define VT_ACT_RELU 1
+#define VT_ACT_SILU 2
+#define VT_ACT_GELU_TANH 3
+
+/* h = act(z) and z in 8 bits, in one pass: what a training step keeps of z. */
+VT_API vt_status vt_mx8_checkpoint(const void *z, int dtype, uint64_t rows, uint32_t cols,
+                                   uint64_t z_stride, int act, void *h, int8_t *codes,
+                                   uint8_t *exps, vt_stream stream);
+/* dz = dh * act'(z8). */
+VT_API vt_status vt_mx8_act_bwd(const void *dh, int dtype, uint64_t rows, uint32_t cols,
+                                uint64_t dh_stride, const int8_t *codes, const uint8_t *exps,
+                                int act, void *dz, vt_stream stream);
+/* The values of 8-bit codes. */
+VT_API vt_status vt_mx8_dequantize(const int8_t *codes, const uint8_t *exps, uint64_t rows,
+                                   uint32_t cols, int dtype, void *out, vt_stream stream);
+/* Gradients of y = act(z) W^T + b, weight (outs, cols), from the 8-bit z:
+ * dz (rows, cols) = (dy W) * act'(z8), dw (outs, cols) = dy^T act(z8),
+ * db (outs) = column sums of dy.  Any output may be null. */
+VT_API uint64_t vt_mx8_linear_bwd_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs);
+VT_API vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const void *weight,
+                                   uint64_t weight_stride, int dtype, uint64_t rows, uint32_t cols,
+                                   uint32_t outs, const int8_t *codes, const uint8_t *exps, int act,
+                                   void *dz, void *dw, void *db, void *workspace,
+                                   uint64_t workspace_bytes, uint32_t *err, vt_stream stream);
+/* x to 4 bits, and 4 bits to values. */
+VT_API vt_status vt_mx4_quantize(const void *x, int dtype, uint64_t rows, uint32_t cols,
+                                 uint64_t x_stride, uint8_t *codes, uint8_t *exps,
+                                 vt_stream stream);
+VT_API vt_status vt_mx4_dequantize(const uint8_t *codes, const uint8_t *exps, uint64_t rows,
+                                   uint32_t cols, int dtype, void *out, vt_stream stream);
+/* y (rows, outs) = act(q4(x) w4^T + bias): x (rows, cols) is rounded to 4 bits
+ * on the way, codes / exps are the weight (outs, cols) in 4 bits, bias (outs)
+ * may be null. */
+VT_API uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs);
+VT_API vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, uint64_t rows,
+                               uint32_t cols, uint32_t outs, const uint8_t *codes,
+                               const uint8_t *exps, const void *bias, int act, void *y,
+                               void *workspace, uint64_t workspace_bytes, uint32_t *err,
+                               vt_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,208 @@
+// vt_mx.cuh -- microscaled block formats and the activations of a learned layer.
+//
+// A row is cut into blocks of 32 columns; the last block may be short and is
+// padded with zeros.  Each block has one exponent byte E and its values are
+// small codes times a power of two:
+//   8 bits: e = max(floor(log2 max|x|), -120), E = e + 127,
+//           code = clamp(rne(x 2^(6 - e)), -127, 127), value = code 2^(e - 6)
+//   4 bits: e = max(floor(log2 max|x|) - 2, -126), E = e + 127,
+//           code = e2m1(x 2^-e) rounded to nearest even, saturated at 6,
+//           value = e2m1 2^e, e2m1 in {0, .5, 1, 1.5, 2, 3, 4, 6} and negatives
+// A block that holds a NaN or an infinity has E = 255 and stands for NaN.
+// Scaling by a power of two is exact in binary32, so the code's rounding is the
+// only rounding, and an 8-bit value fits bfloat16 without another one.  The
+// lower bounds of e keep 2^(6 - e), 2^-e and the scales normal numbers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "vt_abi.cuh"
+
+namespace vt {
+
+enum : int { ACT_IDENTITY = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
+constexpr uint32_t MX_BLOCK = 32;
+
+// ---- types ----
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v)
+{
+    return __bfloat162float(v);
+}
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v)
+{
+    return __float2bfloat16_rn(v);
+}
+
+// 8 values of a row, as 16-byte words (one, or two for binary32)
+template <typename T> struct Vec8 {
+    static constexpr int WORDS = sizeof(T) * 8 / 16;
+    uint4 w[WORDS];
+    __device__ __forceinline__ void load(const T *p)
+    {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    }
+    __device__ __forceinline__ void store(T *p) const
+    {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
+    }
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void unpack(float *v) const
+    {
+        const T *t = reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(t[i]);
+    }
+    __device__ __forceinline__ void pack(const float *v)
+    {
+        T *t = reinterpret_cast<T *>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(v[i]);
+    }
+};
+
+// ---- formats ----
+
+// Exponent field of a block from the bits of its largest magnitude (sign bit clear).
+__device__ __forceinline__ uint32_t mx8_exponent(uint32_t top_bits)
+{
+    const uint32_t f = top_bits >> 23;
+    return f < 7u ? 7u : f;
+}
+__device__ __forceinline__ uint32_t mx4_exponent(uint32_t top_bits)
+{
+    const uint32_t f = top_bits >> 23;
+    return f == 255u ? 255u : f < 3u ? 1u : f - 2u;
+}
+// 2^(6 - e) and 2^(e - 6) of an 8-bit block.  E = 255 gives 2^-122 (its codes are set to zero) and NaN.
+__device__ __forceinline__ float mx8_inverse(uint32_t E) { return __uint_as_float((260u - E) << 23); }
+__device__ __forceinline__ float mx8_scale(uint32_t E)
+{
+    return __uint_as_float(E == 255u ? 0x7fc00000u : (E - 6u) << 23);
+}
+// 2^-e and 2^e of a 4-bit block.
+__device__ __forceinline__ float mx4_inverse(uint32_t E) { return __uint_as_float((254u - E) << 23); }
+__device__ __forceinline__ float mx4_scale(uint32_t E)
+{
+    return __uint_as_float(E == 255u ? 0x7fc00000u : E << 23);
+}
+__device__ __forceinline__ int mx8_code(float x, float inverse)
+{
+    return __float2int_rn(fminf(fmaxf(x * inverse, -127.0f), 127.0f));
+}
+// Two e2m1 codes in a byte, `lo` in the low nibble; rounds to nearest even and saturates.
+__device__ __forceinline__ uint32_t mx4_pair(float lo, float hi)
+{
+    uint32_t r;
+    asm("{\n.reg .b8 t;\ncvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\ncvt.u32.u8 %0, t;\n}" : "=r"(r)
+        : "f"(hi), "f"(lo));
+    return r;
+}
+// e2m1 magnitudes doubled are 0 1 2 3 4 6 8 12
+__device__ __forceinline__ float mx4_value(uint32_t nibble)
+{
+    const float m = 0.5f * (float)((0xc8643210u >> ((nibble & 7u) * 4u)) & 15u);
+    return nibble & 8u ? -m : m;
+}
+
+// ---- activations (binary32 throughout; the caller rounds once) ----
+
+__device__ __forceinline__ float logistic(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+// gelu_tanh(x) = x logistic(c (x + 0.044715 x^3)), c = 2 sqrt(2 / pi).  Outside [-15, 15] the
+// logistic is 0 or 1 in binary32; the bound keeps x^3 finite.  A NaN passes both comparisons.
+constexpr float GELU_C = 1.5957691216057308f, GELU_A = 0.044715f;
+__device__ __forceinline__ float gelu_clip(float x)
+{
+    return x > 15.0f ? 15.0f : x < -15.0f ? -15.0f : x;
+}
+
+template <int ACT> __device__ __forceinline__ float act_value(float x)
+{
+    if constexpr (ACT == ACT_RELU) {
+        return x < 0.0f ? 0.0f : x;  // a NaN stays one
+    } else if constexpr (ACT == ACT_SILU) {
+        return x * logistic(x);
+    } else if constexpr (ACT == ACT_GELU) {
+        const float c = gelu_clip(x);
+        return x * logistic(GELU_C * c * fmaf(GELU_A * c, c, 1.0f));
+    } else {
+        return x;
+    }
+}
+
+template <int ACT> __device__ __forceinline__ float act_slope(float x)
+{
+    if constexpr (ACT == ACT_RELU) {
+        return x > 0.0f ? 1.0f : x <= 0.0f ? 0.0f : x;
+    } else if constexpr (ACT == ACT_SILU) {
+        const float p = logistic(x);
+        return fmaf(x * p, 1.0f - p, p);
+    } else if constexpr (ACT == ACT_GELU) {
+        const float c = gelu_clip(x), cc = c * c;
+        const float p = logistic(GELU_C * c * fmaf(GELU_A, cc, 1.0f));
+        return fmaf(c * p, (1.0f - p) * GELU_C * fmaf(3.0f * GELU_A, cc, 1.0f), p);
+    } else {
+        return 1.0f;
+    }
+}
+
+// ---- dispatch: one instantiation per activation / type ----
+
+template <int V> struct IntC { static constexpr int value = V; };
+template <typename T> struct TypeC { using type = T; };
+
+template <typename F> inline vt_status with_act(int act, F f)
+{
+    switch (act) {
+    case ACT_IDENTITY: return f(IntC<ACT_IDENTITY>());
+    case ACT_RELU: return f(IntC<ACT_RELU>());
+    case ACT_SILU: return f(IntC<ACT_SILU>());
+    case ACT_GELU: return f(IntC<ACT_GELU>());
+    }
+    return set_error(VT_ERR_INVALID, "unknown activation %d", act);
+}
+
+template <typename F> inline vt_status with_type(int dtype, F f)
+{
+    switch (dtype) {
+    case VT_F32: return f(TypeC<float>());
+    case VT_F16: return f(TypeC<__half>());
+    case VT_BF16: return f(TypeC<__nv_bfloat16>());
+    }
+    return set_error(VT_ERR_INVALID, "unknown element type %d", dtype);
+}
+
+template <typename F> inline vt_status with_type16(int dtype, F f)
+{
+    switch (dtype) {
+    case VT_F16: return f(TypeC<__half>());
+    case VT_BF16: return f(TypeC<__nv_bfloat16>());
+    }
+    return set_error(VT_ERR_INVALID, "products take binary16 or bfloat16 (type %d given)", dtype);
+}
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline uint32_t mx_blocks(uint32_t cols) { return cols / MX_BLOCK + (cols % MX_BLOCK != 0); }
+inline int sm_count()
+{
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+
+}  // namespace vt

@@ -1,0 +1,291 @@
+"""Microscaled low-precision operators for a learned layer beside the tracer.
+
+No counterpart in the reference.  Two formats, both in blocks of 32 columns
+with one power-of-two scale a block (``include/vorotracing_b200.h`` has the
+layouts): 8 bits for what a training step keeps of a layer's pre-activations,
+4 bits for weights and activations at inference.
+
+    h, ckpt = act_checkpoint(z, "silu")        # h = act(z); z kept in 8 bits
+    y = h @ weight.t() + bias
+    dz, dw, db = linear_backward(dy, weight, ckpt)   # from the 8-bit z
+
+    w4 = quantize4(weight)                     # once
+    y = linear4(x, w4, bias, "silu")           # act(q4(x) w4^T + b)
+
+``act_linear`` is the training pair as an autograd function.  Tensors live on
+a CUDA device, kernels run on torch's current stream, outputs are new tensors
+there; matrices may have any row stride.  Elementwise operators take float32,
+float16 and bfloat16, products the 16-bit types.  A block of 32 columns that
+holds a NaN or an infinity is NaN in either format.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ._lib import check, lib
+
+BLOCK = 32
+ACTS = {"identity": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_P, _U64, _U32, _I = C.c_void_p, C.c_uint64, C.c_uint32, C.c_int
+
+_ARGS = {
+    "vt_mx8_checkpoint": (_P, _I, _U64, _U32, _U64, _I, _P, _P, _P, _P),
+    "vt_mx8_act_bwd": (_P, _I, _U64, _U32, _U64, _P, _P, _I, _P, _P),
+    "vt_mx8_dequantize": (_P, _P, _U64, _U32, _I, _P, _P),
+    "vt_mx8_linear_bwd_workspace_bytes": (_U64, _U32, _U32),
+    "vt_mx8_linear_bwd": (_P, _U64, _P, _U64, _I, _U64, _U32, _U32, _P, _P, _I, _P, _P, _P, _P,
+                          _U64, _P, _P),
+    "vt_mx4_quantize": (_P, _I, _U64, _U32, _U64, _P, _P, _P),
+    "vt_mx4_dequantize": (_P, _P, _U64, _U32, _I, _P, _P),
+    "vt_mx4_linear_workspace_bytes": (_U64, _U32, _U32),
+    "vt_mx4_linear": (_P, _U64, _I, _U64, _U32, _U32, _P, _P, _P, _I, _P, _P, _U64, _P, _P),
+}
+_fn = {}
+
+
+def _call(name):
+    """The C entry point with its argument types declared, so that plain integers can be passed."""
+    f = _fn.get(name)
+    if f is None:
+        f = getattr(lib(), name)
+        f.argtypes = _ARGS[name]
+        f.restype = C.c_uint64 if name.endswith("_bytes") else C.c_int
+        _fn[name] = f
+    return f
+
+
+def _fail(msg: str):
+    raise RuntimeError(msg)
+
+
+def _act_code(act: str) -> int:
+    code = ACTS.get(act)
+    if code is None:
+        _fail(f"unknown activation {act!r}, expected one of {', '.join(ACTS)}")
+    return code
+
+
+def _matrix(t, name: str, types=_DTYPES):
+    """A tensor as rows of its last dimension with unit column stride: (tensor, rows, cols, row stride)."""
+    if not t.is_cuda:
+        _fail(f"{name} must be on CUDA device")
+    if t.dtype not in types:
+        _fail(f"{name} had dtype {str(t.dtype).replace('torch.', '')}, expected one of "
+              + ", ".join(str(d).replace("torch.", "") for d in types))
+    if t.dim() == 0:
+        _fail(f"{name} must have at least one dimension")
+    cols = t.size(-1)
+    if t.dim() == 2 and (t.stride(1) == 1 or cols <= 1) and (t.stride(0) >= cols or t.size(0) <= 1):
+        return t, t.size(0), cols, t.stride(0) if t.size(0) > 1 else cols
+    t = t.contiguous()
+    rows = 1
+    for n in t.shape[:-1]:
+        rows *= n
+    return t, rows, cols, cols
+
+
+_PRODUCT_TYPES = {torch.float16: 1, torch.bfloat16: 2}
+
+
+def _same(a, b, name: str, other: str):
+    if a.device != b.device:
+        _fail(f"{name} must be on the same device as {other}")
+
+
+def _launch(name: str, device, *args):
+    """Calls an entry point on the tensors' device and torch's current stream there."""
+    f = _call(name)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            check(f(*args, torch.cuda.current_stream(device).cuda_stream), name)
+    else:
+        check(f(*args, torch.cuda.current_stream(device).cuda_stream), name)
+
+
+def _check_parts(codes, exps, cols, code_dtype, per_block, what):
+    if codes.dim() != 2 or exps.dim() != 2:
+        _fail(f"{what}: codes and exponents are matrices")
+    blocks = -(-cols // BLOCK)
+    if codes.dtype != code_dtype or exps.dtype != torch.uint8:
+        _fail(f"{what}: codes must be {str(code_dtype).replace('torch.', '')} and exponents uint8")
+    if codes.size(1) != blocks * per_block or exps.size(1) != blocks or codes.size(0) != exps.size(0):
+        _fail(f"{what}: {cols} columns take codes (rows, {blocks * per_block}) and exponents "
+              f"(rows, {blocks}), got {tuple(codes.shape)} and {tuple(exps.shape)}")
+    if not codes.is_cuda or codes.device != exps.device:
+        _fail(f"{what}: codes and exponents must be on the same CUDA device")
+    if not codes.is_contiguous() or not exps.is_contiguous():
+        _fail(f"{what}: codes and exponents must be contiguous")
+    if codes.data_ptr() % 16:
+        _fail(f"{what}: codes must be 16-byte aligned")
+
+
+class Checkpoint:
+    """A matrix of pre-activations in 8 bits and the activation it goes through.
+
+    codes (rows, 32 B) int8, exps (rows, B) uint8, B = ceil(cols / 32)."""
+
+    __slots__ = ("codes", "exps", "cols", "act", "_act")
+
+    def __init__(self, codes, exps, cols: int, act: str):
+        self._act = _act_code(act)
+        _check_parts(codes, exps, cols, torch.int8, BLOCK, "Checkpoint")
+        self.codes, self.exps, self.cols, self.act = codes, exps, cols, act
+
+    @property
+    def rows(self) -> int:
+        return self.codes.size(0)
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The 8-bit values, (rows, cols)."""
+        if dtype not in _DTYPES:
+            _fail(f"cannot dequantise to {str(dtype).replace('torch.', '')}")
+        out = torch.empty((self.rows, self.cols), dtype=dtype, device=self.codes.device)
+        _launch("vt_mx8_dequantize", out.device, self.codes.data_ptr(), self.exps.data_ptr(),
+                self.rows, self.cols, _DTYPES[dtype], out.data_ptr())
+        return out
+
+
+class MX4:
+    """A matrix in 4-bit microscaled blocks: codes (rows, 16 B) uint8, two columns a
+    byte with the even one in the low nibble, exps (rows, B) uint8."""
+
+    __slots__ = ("codes", "exps", "cols")
+
+    def __init__(self, codes, exps, cols: int):
+        _check_parts(codes, exps, cols, torch.uint8, BLOCK // 2, "MX4")
+        self.codes, self.exps, self.cols = codes, exps, cols
+
+    @property
+    def rows(self) -> int:
+        return self.codes.size(0)
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The 4-bit values, (rows, cols)."""
+        if dtype not in _DTYPES:
+            _fail(f"cannot dequantise to {str(dtype).replace('torch.', '')}")
+        out = torch.empty((self.rows, self.cols), dtype=dtype, device=self.codes.device)
+        _launch("vt_mx4_dequantize", out.device, self.codes.data_ptr(), self.exps.data_ptr(),
+                self.rows, self.cols, _DTYPES[dtype], out.data_ptr())
+        return out
+
+
+def act_checkpoint(z: torch.Tensor, act: str = "silu"):
+    """(act(z), 8-bit checkpoint of z) for z (..., cols), in one pass."""
+    code = _act_code(act)
+    m, rows, cols, stride = _matrix(z, "z")
+    blocks = -(-cols // BLOCK)
+    h = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    codes = torch.empty((rows, blocks * BLOCK), dtype=torch.int8, device=z.device)
+    exps = torch.empty((rows, blocks), dtype=torch.uint8, device=z.device)
+    _launch("vt_mx8_checkpoint", z.device, m.data_ptr(), _DTYPES[z.dtype], rows, cols, stride,
+            code, h.data_ptr(), codes.data_ptr(), exps.data_ptr())
+    ckpt = Checkpoint.__new__(Checkpoint)
+    ckpt.codes, ckpt.exps, ckpt.cols, ckpt.act, ckpt._act = codes, exps, cols, act, code
+    return h, ckpt
+
+
+def act_backward(dh: torch.Tensor, ckpt: Checkpoint) -> torch.Tensor:
+    """dz = dh * act'(z8), in dh's type and shape."""
+    m, rows, cols, stride = _matrix(dh, "dh")
+    if rows != ckpt.rows or cols != ckpt.cols:
+        _fail(f"dh had {rows} rows of {cols}, the checkpoint has {ckpt.rows} of {ckpt.cols}")
+    _same(dh, ckpt.codes, "dh", "the checkpoint")
+    dz = torch.empty(dh.shape, dtype=dh.dtype, device=dh.device)
+    _launch("vt_mx8_act_bwd", dh.device, m.data_ptr(), _DTYPES[dh.dtype], rows, cols, stride,
+            ckpt.codes.data_ptr(), ckpt.exps.data_ptr(), ckpt._act, dz.data_ptr())
+    return dz
+
+
+def linear_backward(dy: torch.Tensor, weight: torch.Tensor, ckpt: Checkpoint, bias: bool = True,
+                    need_dz: bool = True, need_dw: bool = True):
+    """Gradients of y = act(z) W^T + b from the 8-bit checkpoint of z.
+
+    dy (..., outs) and weight (outs, cols) in the same 16-bit type.  Returns
+    (dz, dw, db) in that type: dz (..., cols) = (dy W) * act'(z8), dw (outs,
+    cols) = dy^T act(z8) and db (outs) = column sums of dy; None for those not
+    asked for."""
+    m, rows, outs, dy_stride = _matrix(dy, "dy", _PRODUCT_TYPES)
+    w, w_rows, cols, w_stride = _matrix(weight, "weight", _PRODUCT_TYPES)
+    if weight.dim() != 2 or w_rows != outs:
+        _fail(f"weight had shape {tuple(weight.shape)}, expected ({outs}, columns)")
+    if weight.dtype != dy.dtype:
+        _fail("weight must have the dtype of dy")
+    if rows != ckpt.rows or cols != ckpt.cols:
+        _fail(f"dy has {rows} rows and weight {cols} columns, the checkpoint has {ckpt.rows} "
+              f"rows of {ckpt.cols}")
+    _same(weight, dy, "weight", "dy")
+    _same(ckpt.codes, dy, "the checkpoint", "dy")
+    dev, dt = dy.device, dy.dtype
+    dz = torch.empty((*dy.shape[:-1], cols), dtype=dt, device=dev) if need_dz else None
+    dw = torch.empty((outs, cols), dtype=dt, device=dev) if need_dw else None
+    db = torch.empty(outs, dtype=dt, device=dev) if bias else None
+    n = _call("vt_mx8_linear_bwd_workspace_bytes")(rows, cols, outs)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    _launch("vt_mx8_linear_bwd", dev, m.data_ptr(), dy_stride, w.data_ptr(), w_stride,
+            _DTYPES[dt], rows, cols, outs, ckpt.codes.data_ptr(), ckpt.exps.data_ptr(), ckpt._act,
+            dz.data_ptr() if need_dz else None, dw.data_ptr() if need_dw else None,
+            db.data_ptr() if bias else None, ws.data_ptr() if n else None, n, None)
+    return dz, dw, db
+
+
+class _ActLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, weight, bias, act):
+        h, ckpt = act_checkpoint(z, act)
+        ctx.ckpt, ctx.has_bias = ckpt, bias is not None
+        ctx.save_for_backward(weight)
+        return torch.nn.functional.linear(h, weight, bias)
+
+    @staticmethod
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        dz, dw, db = linear_backward(dy, ctx.saved_tensors[0], ctx.ckpt,
+                                     bias=ctx.has_bias and need[2], need_dz=need[0],
+                                     need_dw=need[1])
+        return dz, dw, db, None
+
+
+def act_linear(z: torch.Tensor, weight: torch.Tensor, bias=None, act: str = "silu"):
+    """y = act(z) W^T + b for training: between forward and backward only the
+    8-bit form of z is kept (33/32 byte a value), neither z nor act(z)."""
+    return _ActLinear.apply(z, weight, bias, act)
+
+
+def quantize4(x: torch.Tensor) -> MX4:
+    """x (..., cols) in 4-bit microscaled blocks, as (rows, cols)."""
+    m, rows, cols, stride = _matrix(x, "x")
+    blocks = -(-cols // BLOCK)
+    q = MX4.__new__(MX4)
+    q.codes = torch.empty((rows, blocks * BLOCK // 2), dtype=torch.uint8, device=x.device)
+    q.exps = torch.empty((rows, blocks), dtype=torch.uint8, device=x.device)
+    q.cols = cols
+    _launch("vt_mx4_quantize", x.device, m.data_ptr(), _DTYPES[x.dtype], rows, cols, stride,
+            q.codes.data_ptr(), q.exps.data_ptr())
+    return q
+
+
+def linear4(x: torch.Tensor, w: MX4, bias=None, act: str = "identity") -> torch.Tensor:
+    """y = act(q4(x) w4^T + bias): x (..., cols) in a 16-bit type is rounded to
+    4 bits on the way, w is the weight (outs, cols) in 4 bits, bias (outs) has
+    x's type.  y (..., outs) has x's type."""
+    code = _act_code(act)
+    m, rows, cols, stride = _matrix(x, "x", _PRODUCT_TYPES)
+    outs = w.rows
+    if cols != w.cols:
+        _fail(f"x had {cols} columns, the weight has {w.cols}")
+    _same(w.codes, x, "the weight", "x")
+    if bias is not None:
+        if bias.dtype != x.dtype or bias.dim() != 1 or bias.size(0) != outs:
+            _fail(f"bias must have the dtype of x and shape ({outs},)")
+        _same(bias, x, "bias", "x")
+        bias = bias.contiguous()
+    y = torch.empty((*x.shape[:-1], outs), dtype=x.dtype, device=x.device)
+    n = _call("vt_mx4_linear_workspace_bytes")(rows, cols, outs)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _launch("vt_mx4_linear", x.device, m.data_ptr(), stride, _DTYPES[x.dtype], rows, cols, outs,
+            w.codes.data_ptr(), w.exps.data_ptr(), bias.data_ptr() if bias is not None else None,
+            code, y.data_ptr(), ws.data_ptr() if n else None, n, None)
+    return y
