@@ -217,7 +217,7 @@ extern "C" vt_status vt_mx8_checkpoint(const void *z, int dtype, uint64_t rows, 
     MX_COMMON("vt_mx8_checkpoint");
     VT_REQUIRE(z && h && codes && exps, "vt_mx8_checkpoint: null pointer");
     VT_REQUIRE(z_stride >= cols, "vt_mx8_checkpoint: the row stride is less than a row");
-    VT_REQUIRE(vt::aligned16(codes), "vt_mx8_checkpoint: codes must be 16-byte aligned");
+    VT_REQUIRE(vt::aligned32(codes), "vt_mx8_checkpoint: codes must be 32-byte aligned");
     return vt::with_type(dtype, [&](auto ty) {
         using T = typename decltype(ty)::type;
         return vt::with_act(act, [&](auto a) {
@@ -235,7 +235,7 @@ extern "C" vt_status vt_mx8_act_bwd(const void *dh, int dtype, uint64_t rows, ui
     MX_COMMON("vt_mx8_act_bwd");
     VT_REQUIRE(dh && codes && exps && dz, "vt_mx8_act_bwd: null pointer");
     VT_REQUIRE(dh_stride >= cols, "vt_mx8_act_bwd: the row stride is less than a row");
-    VT_REQUIRE(vt::aligned16(codes), "vt_mx8_act_bwd: codes must be 16-byte aligned");
+    VT_REQUIRE(vt::aligned32(codes), "vt_mx8_act_bwd: codes must be 32-byte aligned");
     return vt::with_type(dtype, [&](auto ty) {
         using T = typename decltype(ty)::type;
         return vt::with_act(act, [&](auto a) {
@@ -252,7 +252,7 @@ extern "C" vt_status vt_mx8_dequantize(const int8_t *codes, const uint8_t *exps,
 {
     MX_COMMON("vt_mx8_dequantize");
     VT_REQUIRE(codes && exps && out, "vt_mx8_dequantize: null pointer");
-    VT_REQUIRE(vt::aligned16(codes), "vt_mx8_dequantize: codes must be 16-byte aligned");
+    VT_REQUIRE(vt::aligned32(codes), "vt_mx8_dequantize: codes must be 32-byte aligned");
     return vt::with_type(dtype, [&](auto ty) {
         using T = typename decltype(ty)::type;
         const vt::MxShape s = vt::mx_shape<T>(rows, cols, out, cols, out, cols);

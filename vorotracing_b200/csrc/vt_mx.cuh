@@ -160,6 +160,24 @@ template <int ACT> __device__ __forceinline__ float act_slope(float x)
     }
 }
 
+// Both at once; one logistic serves both.
+template <int ACT> __device__ __forceinline__ void act_both(float x, float &value, float &slope)
+{
+    if constexpr (ACT == ACT_SILU) {
+        const float p = logistic(x);
+        value = x * p;
+        slope = fmaf(value, 1.0f - p, p);
+    } else if constexpr (ACT == ACT_GELU) {
+        const float c = gelu_clip(x), cc = c * c;
+        const float p = logistic(GELU_C * c * fmaf(GELU_A, cc, 1.0f));
+        value = x * p;
+        slope = fmaf(c * p, (1.0f - p) * GELU_C * fmaf(3.0f * GELU_A, cc, 1.0f), p);
+    } else {
+        value = act_value<ACT>(x);
+        slope = act_slope<ACT>(x);
+    }
+}
+
 // ---- dispatch: one instantiation per activation / type ----
 
 template <int V> struct IntC { static constexpr int value = V; };
@@ -196,6 +214,7 @@ template <typename F> inline vt_status with_type16(int dtype, F f)
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned32(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 inline uint32_t mx_blocks(uint32_t cols) { return cols / MX_BLOCK + (cols % MX_BLOCK != 0); }
 inline int sm_count()
 {

@@ -1,0 +1,630 @@
+// vt_mx8_linear.cu -- gradients of y = act(z) W^T + b from an 8-bit checkpoint of z (vt_mx.cuh):
+//   dz = (dy W) * act'(z8),  dW = dy^T act(z8),  db = column sums of dy
+//
+// Layers with up to 256 outputs (narrow_kernel) make all three in one pass over the rows, so dy
+// and the checkpoint are read from HBM once and act(z8) never reaches memory.  A CTA owns a slab
+// of up to 128 columns of z and every G-th tile of 128 rows.  A tile of dy is staged once in
+// shared memory (TMA, 128-byte swizzle) and used twice: as the K-major A operand of
+// dH = dy W, and, the same bytes read the other way, as the MN-major A operand of
+// dW += dy^T act(z8), whose accumulator stays in tensor memory over all the CTA's rows.
+// Between the two products eight warps take dH out of tensor memory, read the 8-bit z, evaluate
+// act and act' together (one logistic serves both), write dz, and leave act(z8) in shared memory
+// as the second product's B operand, rounded to the operands' 16-bit type as the forward pass's
+// own activations are.  Two more warps add up dy's columns from the staged tile.  At its end a CTA
+// writes its part of dW in binary32; a second kernel adds the parts in order, so results do not
+// depend on timing.
+#include "vt_mx_tile.cuh"
+#include "vt_tc.cuh"
+
+#include <atomic>
+
+namespace vt {
+
+template <typename T, bool KIN> struct Rows {  // element (i, k) of a row-major matrix, or of its transpose
+    static constexpr bool K_INNER = KIN;
+    const T *p;
+    uint64_t stride;
+    __device__ float operator()(uint64_t i, uint64_t k) const
+    {
+        return to_f32<T>(__ldg(p + (KIN ? i * stride + k : k * stride + i)));
+    }
+};
+
+template <int ACT> struct Checkpoint8 {  // act(z8) at (column, row)
+    static constexpr bool K_INNER = false;
+    const int8_t *codes;
+    const uint8_t *exps;
+    uint32_t blocks;
+    __device__ float z(uint64_t row, uint32_t col) const
+    {
+        return (float)codes[row * blocks * MX_BLOCK + col] * mx8_scale(exps[row * blocks + col / MX_BLOCK]);
+    }
+    __device__ float operator()(uint64_t col, uint64_t row) const { return act_value<ACT>(z(row, (uint32_t)col)); }
+};
+
+template <typename T, int ACT> struct StoreDz {
+    Checkpoint8<ACT> ckpt;
+    T *p;
+    uint32_t cols;
+    __device__ void operator()(uint64_t i, uint32_t j, float v) const
+    {
+        p[i * cols + j] = from_f32<T>(v * act_slope<ACT>(ckpt.z(i, j)));
+    }
+};
+
+template <typename T> __global__ void column_sum_kernel(const T *p, uint64_t rows, uint32_t cols, uint64_t stride, T *out)
+{
+    __shared__ float part[256];
+    float v = 0.0f;
+    for (uint64_t i = threadIdx.x; i < rows; i += 256u) v += to_f32<T>(p[i * stride + blockIdx.x]);
+    part[threadIdx.x] = v;
+    __syncthreads();
+    for (int n = 128; n; n >>= 1) {
+        if (threadIdx.x < n) part[threadIdx.x] += part[threadIdx.x + n];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) out[blockIdx.x] = from_f32<T>(part[0]);
+}
+
+// ---- layers with up to 256 outputs ----
+
+constexpr uint32_t TILE_ROWS = 128, NARROW_OUTS = 256, NARROW_THREADS = 384;
+
+// OC: dy's columns in chunks of 64; NC: the slab's columns in chunks of 64.
+template <int OC, int NC> struct Narrow {
+    static constexpr uint32_t W_BYTES = OC * 8192u * NC, DY_BYTES = OC * 16384u, H_BYTES = NC * 16384u;
+    // as much staging as 227 KB hold
+    static constexpr uint32_t STAGES = OC >= 3 ? 2 : OC == 2 ? 3 : 4, H_BUFS = OC == 4 && NC == 2 ? 1 : 2;
+    static constexpr uint32_t DY_AT = W_BYTES, H_AT = DY_AT + STAGES * DY_BYTES, CTRL_AT = H_AT + H_BUFS * H_BYTES;
+    static constexpr uint32_t MT = (OC + 1) / 2;                 // accumulator tiles of 128 outputs
+    static constexpr uint32_t DW_COLS = MT * NC * 64u, DH_COLS = NC * 64u;
+    static constexpr uint32_t TMEM_USED = DW_COLS + 2u * DH_COLS;
+    static constexpr uint32_t TMEM = TMEM_USED <= 128 ? 128 : TMEM_USED <= 256 ? 256 : 512;
+    struct Ctrl {
+        uint64_t full[STAGES], empty[STAGES], dh_full[2], dh_empty[2], h_full[H_BUFS], h_empty[H_BUFS], w_full, done;
+        uint32_t tmem;
+        tc::Fail fail;
+    };
+    static constexpr uint32_t SMEM = CTRL_AT + sizeof(Ctrl);
+    static_assert(TMEM_USED <= 512 && SMEM <= 232448, "does not fit an SM");
+};
+
+struct NarrowArgs {
+    uint64_t rows;
+    uint32_t cols, outs, blocks, tiles, groups, slabs;
+    const int8_t *codes;
+    const uint8_t *exps;
+    void *dz;          // null: not wanted
+    float *dw_parts;   // [group][slab][NC * 64][MT * 128]; null: dW not wanted
+    float *db_parts;   // [group][2][OC * 64]; null: db not wanted
+    uint32_t *err;
+    bool dz_wide;      // dz's rows hold whole 32-byte pieces
+};
+
+__device__ __forceinline__ void store32(void *p, const uint32_t *w)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+__device__ __forceinline__ void load32(const void *p, uint32_t *w)
+{
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w)
+{
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
+{
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Byte i (0..3) of a word of codes, as a float: the byte with its sign bit turned goes under
+// the exponent of 2^23, which makes 2^23 + 128 + code.
+__device__ __forceinline__ float code_float(uint32_t turned, int i)
+{
+    return __uint_as_float(__byte_perm(turned, 0x4b000000u, 0x7440u | i)) - 8388736.0f;
+}
+
+// One warp's 32 rows by 32 columns (one block a lane): g = dH in, h and dz out as packed 16-bit pairs.
+template <typename T, int ACT>
+__device__ __forceinline__ void transform_block(const uint32_t *codes, uint32_t E, const uint32_t *g, uint32_t *h, uint32_t *dz)
+{
+    const float sc = mx8_scale(E);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        const uint32_t c = codes[w] ^ 0x80808080u;
+        float hv[4], gv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float z = code_float(c, i) * sc;
+            float slope;
+            act_both<ACT>(z, hv[i], slope);
+            gv[i] = __uint_as_float(g[4 * w + i]) * slope;
+        }
+        h[2 * w] = pack2<T>(hv[0], hv[1]);
+        h[2 * w + 1] = pack2<T>(hv[2], hv[3]);
+        dz[2 * w] = pack2<T>(gv[0], gv[1]);
+        dz[2 * w + 1] = pack2<T>(gv[2], gv[3]);
+    }
+}
+
+// 32 columns of a row of dz from packed pairs
+template <typename T>
+__device__ __forceinline__ void store_dz(const NarrowArgs &a, uint64_t row, uint32_t col, const uint32_t *w)
+{
+    T *p = (T *)a.dz + row * a.cols + col;
+    if (a.dz_wide) {
+        if (col < a.cols) store32(p, w);
+        if (col + 16u < a.cols) store32(p + 16, w + 8);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            const float2 v = unpack2<T>(w[i]);
+            if (col + 2 * i < a.cols) p[2 * i] = from_f32<T>(v.x);
+            if (col + 2 * i + 1 < a.cols) p[2 * i + 1] = from_f32<T>(v.y);
+        }
+    }
+}
+
+template <typename T, int ACT, int OC, int NC>
+__global__ void __launch_bounds__(NARROW_THREADS, 1)
+    narrow_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap w_map, const NarrowArgs a)
+{
+    using P = Narrow<OC, NC>;
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    typename P::Ctrl &s = *reinterpret_cast<typename P::Ctrl *>(smem + P::CTRL_AT);
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    const uint32_t slab = blockIdx.x % a.slabs, group = blockIdx.x / a.slabs;
+    // dy's chunks are shared out among the slabs for the column sums
+    const uint32_t sharers = a.slabs < OC ? a.slabs : OC;
+    const bool sums = a.db_parts && slab < sharers;
+    tc::Fail *const fail = &s.fail;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < P::STAGES; ++i) {
+            tc::mbar_init(&s.full[i], 1);
+            tc::mbar_init(&s.empty[i], sums ? 3 : 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            tc::mbar_init(&s.dh_full[i], 1);
+            tc::mbar_init(&s.dh_empty[i], 8);
+        }
+        for (uint32_t i = 0; i < P::H_BUFS; ++i) {
+            tc::mbar_init(&s.h_full[i], 8);
+            tc::mbar_init(&s.h_empty[i], 1);
+        }
+        tc::mbar_init(&s.w_full, 1);
+        tc::mbar_init(&s.done, 1);
+        s.fail.failed = 0;
+        tc::mbar_init_fence();
+        tc::tma_prefetch_map(&dy_map);
+        tc::tma_prefetch_map(&w_map);
+    }
+    if (warp == 1) tc::tmem_alloc<P::TMEM>(&s.tmem);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = s.tmem, dh_at = tmem + P::DW_COLS;
+
+    if (warp == 0) {
+        if (lane == 0) {  // TMA
+            uint32_t issued = 0;
+            tc::mbar_arrive_tx(&s.w_full, P::W_BYTES);
+            for (int n = 0; n < NC; ++n)
+                tc::tma_load_2d(smem + n * (OC * 8192), &w_map, (int)(slab * NC + n) * 64, 0, &s.w_full);
+            tc::Ring r;
+            for (uint32_t t = group; t < a.tiles; t += a.groups) {
+                if (!tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err)) break;
+                tc::mbar_arrive_tx(&s.full[r.i], P::DY_BYTES);
+                for (int c = 0; c < OC; ++c)
+                    tc::tma_load_2d(smem + P::DY_AT + r.i * P::DY_BYTES + c * 16384, &dy_map, c * 64, (int)(t * TILE_ROWS),
+                                    &s.full[r.i]);
+                ++issued;
+                r.next(P::STAGES);
+            }
+            if (s.fail.failed) {  // leave no copy in flight
+                tc::mbar_wait_slow(&s.w_full, 0, fail, a.err, true);
+                for (uint32_t i = 0; i < P::STAGES && i < issued; ++i)
+                    tc::mbar_wait_slow(&s.full[i], ((issued - 1 - i) / P::STAGES) & 1u, fail, a.err, true);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {  // products
+            constexpr uint32_t ID_DH = tc::idesc_f16<BF16>(128, P::DH_COLS, false, true);
+            constexpr uint32_t ID_DW = tc::idesc_f16<BF16>(128, P::DH_COLS, true, true);
+            const uint32_t w_addr = tc::smem_u32(smem), dy_addr = w_addr + P::DY_AT, h_addr = w_addr + P::H_AT;
+            tc::Ring r, dh, h, prev;
+            bool ok = tc::mbar_wait(&s.w_full, 0, fail, a.err), first = true;
+            // dW += dy^T h of the tile before the current one: its activations are ready only now.
+            // For an odd number of chunks the last accumulator tile's upper 64 rows come from
+            // whatever follows in shared memory; they are never read.
+            auto weight_product = [&]() -> bool {
+                if (!tc::mbar_wait(&s.h_full[h.i], h.phase, fail, a.err)) return false;
+                tc::fence_after();
+                if (a.dw_parts) {
+                    for (uint32_t m = 0; m < P::MT; ++m)
+                        for (uint32_t k = 0; k < 8; ++k)
+                            tc::mma_f16(tmem + m * P::DH_COLS,
+                                        tc::smem_desc(dy_addr + prev.i * P::DY_BYTES + m * 32768u + k * 2048u, 16384, 1024),
+                                        tc::smem_desc(h_addr + h.i * P::H_BYTES + k * 2048u, 16384, 1024), ID_DW,
+                                        !(first && k == 0));
+                    first = false;
+                }
+                tc::commit(&s.h_empty[h.i]);
+                tc::commit(&s.empty[prev.i]);
+                h.next(P::H_BUFS);
+                prev.next(P::STAGES);
+                return true;
+            };
+            for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
+                ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err) &&
+                     tc::mbar_wait(&s.dh_empty[dh.i], dh.phase ^ 1u, fail, a.err);
+                if (!ok) break;
+                tc::fence_after();
+                for (uint32_t c = 0; c < OC; ++c)
+                    for (uint32_t k = 0; k < 4; ++k)
+                        tc::mma_f16(dh_at + dh.i * P::DH_COLS,
+                                    tc::smem_desc(dy_addr + r.i * P::DY_BYTES + c * 16384u + k * 32u, 16, 1024),
+                                    tc::smem_desc(w_addr + c * 8192u + k * 2048u, OC * 8192u, 1024), ID_DH, c + k != 0);
+                tc::commit(&s.dh_full[dh.i]);
+                r.next(P::STAGES);
+                dh.next(2);
+                if (t != group) ok = weight_product();
+            }
+            if (ok) ok = weight_product();
+            tc::commit(&s.done);
+            if (!ok) tc::mbar_wait_slow(&s.done, 0, fail, a.err, true);  // leave no product in flight
+        }
+    } else if (warp < 4) {
+        if (sums) {  // column sums: each of the two warps takes half of a tile's rows, a lane two columns
+            tc::Ring r;
+            float2 total[OC] = {};
+            bool ok = true;
+            const uint32_t row0 = (warp - 2u) * 64u;
+            for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
+                ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
+                if (!ok) break;
+#pragma unroll
+                for (int c = 0; c < OC; ++c) {
+                    if (c % sharers != slab) continue;
+                    const uint8_t *p = smem + P::DY_AT + r.i * P::DY_BYTES + c * 16384 + row0 * 128u;
+                    float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+                    for (uint32_t i = 0; i < 64; ++i) {
+                        const float2 x = unpack2<T>(*reinterpret_cast<const uint32_t *>(p + i * 128u + ((lane * 4u) ^ (i & 7u) << 4)));
+                        v.x += x.x;
+                        v.y += x.y;
+                    }
+                    total[c].x += v.x;
+                    total[c].y += v.y;
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&s.empty[r.i]);
+                r.next(P::STAGES);
+            }
+#pragma unroll
+            for (int c = 0; c < OC; ++c)
+                if (c % sharers == slab)
+                    *reinterpret_cast<float2 *>(a.db_parts + ((uint64_t)group * 2u + (warp - 2u)) * (OC * 64u) + c * 64u + lane * 2u) =
+                        total[c];
+        }
+    } else {  // activations: warp w reads rows 32 (w % 4).. of the tile and half of the slab's columns
+        const uint32_t quad = warp % 4u, half = (warp - 4u) / 4u;
+        const uint32_t in_tile = quad * 32u + lane, block0 = (slab * NC * 2u) + half * NC;
+        uint32_t codes[NC][8], E[NC];
+        auto fetch = [&](uint32_t t, uint32_t (&c)[NC][8], uint32_t (&e)[NC]) {
+            const uint64_t row = (uint64_t)t * TILE_ROWS + in_tile;
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                const bool in = t < a.tiles && row < a.rows && block0 + j < a.blocks;
+                if (in) {
+                    const uint64_t b = row * a.blocks + block0 + j;
+                    load32(a.codes + b * 32u, c[j]);
+                    e[j] = __ldg(a.exps + b);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) c[j][i] = 0;
+                    e[j] = 127;
+                }
+            }
+        };
+        fetch(group, codes, E);
+        tc::Ring dh, h;
+        bool ok = true;
+        for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
+            const uint64_t row = (uint64_t)t * TILE_ROWS + in_tile;
+            uint32_t next[NC][8], next_E[NC];
+            fetch(t + a.groups, next, next_E);
+            ok = tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err) &&
+                 tc::mbar_wait(&s.h_empty[h.i], h.phase ^ 1u, fail, a.err);
+            if (!__all_sync(~0u, ok)) { ok = false; break; }
+            tc::fence_after();
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                uint32_t g[32], hv[16], dz[16];
+                tc::tmem_load32(dh_at + dh.i * P::DH_COLS + (quad * 32u << 16) + (half * NC + j) * 32u, g);
+                tc::tmem_wait_load();
+                if (j == NC - 1) {
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s.dh_empty[dh.i]);
+                }
+                transform_block<T, ACT>(codes[j], E[j], g, hv, dz);
+                // activations: 64-byte piece of row in_tile in the swizzled chunk
+                uint8_t *p = smem + P::H_AT + h.i * P::H_BYTES + (NC == 2 ? half * 16384u : 0u) + in_tile * 128u;
+                const uint32_t unit = (NC == 2 ? j : half) * 4u;
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u)
+                    *reinterpret_cast<uint4 *>(p + (((unit + u) ^ (in_tile & 7u)) << 4)) =
+                        make_uint4(hv[4 * u], hv[4 * u + 1], hv[4 * u + 2], hv[4 * u + 3]);
+                if (a.dz && row < a.rows) store_dz<T>(a, row, (block0 + j) * 32u, dz);
+            }
+            tc::fence_async_shared();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s.h_full[h.i]);
+            dh.next(2);
+            h.next(P::H_BUFS);
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) codes[j][i] = next[j][i];
+                E[j] = next_E[j];
+            }
+        }
+        if (a.dw_parts) {
+            ok = ok && tc::mbar_wait(&s.done, 0, fail, a.err);
+            if (__all_sync(~0u, ok)) {
+                tc::fence_after();
+                float *out = a.dw_parts + ((uint64_t)group * a.slabs + slab) * (NC * 64u) * (P::MT * 128u);
+                for (uint32_t m = 0; m < P::MT; ++m)
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) {
+                        uint32_t v[32];
+                        const uint32_t n0 = (half * NC + j) * 32u;
+                        tc::tmem_load32(tmem + m * P::DH_COLS + (quad * 32u << 16) + n0, v);
+                        tc::tmem_wait_load();
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i)
+                            out[(n0 + i) * (P::MT * 128u) + m * 128u + in_tile] = __uint_as_float(v[i]);
+                    }
+            }
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 1) tc::tmem_free<P::TMEM>(tmem);
+}
+
+// Adds the groups' parts in order: dw (outs, cols) and db (outs).
+template <typename T>
+__global__ void __launch_bounds__(256) narrow_reduce_kernel(const float *__restrict__ dw_parts, const float *__restrict__ db_parts,
+                                                            uint32_t groups, uint32_t slabs, uint32_t slab_cols, uint32_t part_outs,
+                                                            uint32_t cols, uint32_t outs, T *__restrict__ dw, T *__restrict__ db)
+{
+    const uint64_t per_group = (uint64_t)slabs * slab_cols * part_outs;
+    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    if (dw && i < per_group) {
+        const uint32_t o = (uint32_t)(i % part_outs), n = (uint32_t)(i / part_outs);
+        if (o < outs && n < cols) {
+            float v = 0.0f;
+#pragma unroll 8
+            for (uint32_t g = 0; g < groups; ++g) v += __ldg(dw_parts + g * per_group + i);
+            dw[(uint64_t)o * cols + n] = from_f32<T>(v);
+        }
+    }
+    if (db && i < outs) {
+        const uint32_t pad = (outs + 63u) / 64u * 64u;
+        float v = 0.0f;
+        for (uint32_t g = 0; g < 2u * groups; ++g) v += __ldg(db_parts + (uint64_t)g * pad + i);
+        db[i] = from_f32<T>(v);
+    }
+}
+
+// Rows of a matrix copied to a pitch of whole 16-byte words, which TMA asks for.
+template <typename T>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const T *__restrict__ src, uint64_t rows, uint32_t cols, uint64_t stride,
+                                                       T *__restrict__ dst, uint32_t pitch)
+{
+    const uint32_t words = pitch / 8u;
+    const uint64_t n = rows * words;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256u) {
+        const uint64_t row = i / words;
+        const uint32_t col = (uint32_t)(i % words) * 8u;
+        const T *p = src + row * stride + col;
+        Vec8<T> v;
+        T *e = reinterpret_cast<T *>(v.w);
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) e[k] = col + k < cols ? p[k] : from_f32<T>(0.0f);
+        v.store(dst + row * pitch + col);
+    }
+}
+
+static uint64_t align_up(uint64_t n, uint64_t a) { return (n + a - 1) / a * a; }
+
+// How a narrow call is cut, and where its workspace parts lie.  The copies of dy and the weight
+// are counted always: whether they are needed depends on pointers.
+struct NarrowPlan {
+    uint32_t oc, nc, slabs, tiles, groups, part_outs;
+    uint64_t dw_at, db_at, dy_at, w_at, bytes;
+};
+static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, uint32_t sms)
+{
+    NarrowPlan p;
+    p.oc = (outs + 63u) / 64u;
+    p.nc = cols <= 64u ? 1u : 2u;
+    p.slabs = (cols + p.nc * 64u - 1u) / (p.nc * 64u);
+    p.tiles = (uint32_t)((rows + TILE_ROWS - 1u) / TILE_ROWS);
+    // one CTA an SM; a slab more than there are SMs still gets its own
+    p.groups = p.slabs < sms ? sms / p.slabs : 1u;
+    if (p.groups > p.tiles) p.groups = p.tiles;
+    p.part_outs = (p.oc + 1u) / 2u * 128u;
+    p.dw_at = 0;
+    p.db_at = p.dw_at + align_up((uint64_t)p.groups * p.slabs * p.nc * 64u * p.part_outs * 4u, 256);
+    p.dy_at = p.db_at + align_up((uint64_t)p.groups * 2u * p.oc * 64u * 4u, 256);
+    p.w_at = p.dy_at + align_up(rows * align_up(outs, 8) * 2u, 256);
+    p.bytes = p.w_at + align_up((uint64_t)outs * align_up(cols, 8) * 2u, 256);
+    return p;
+}
+
+// A tensor map over p, or over a copy of it with whole 16-byte rows where p's are not.
+template <typename T>
+static vt_status map_rows(CUtensorMap *map, const void *p, uint64_t stride, uint64_t rows, uint32_t cols, void *copy,
+                          uint32_t box_rows, cudaStream_t stream)
+{
+    uint64_t pitch = stride * sizeof(T);
+    if (pitch % 16u || !aligned16(p)) {
+        const uint32_t to = (uint32_t)align_up(cols, 8);
+        const uint64_t items = rows * (to / 8u), want = (items + 255u) / 256u;
+        pad_rows_kernel<T><<<(unsigned)(want < 4096u ? want : 4096u), 256, 0, stream>>>((const T *)p, rows, cols, stride, (T *)copy, to);
+        if (vt_status s = check_launch("pad_rows_kernel")) return s;
+        p = copy;
+        pitch = (uint64_t)to * sizeof(T);
+    }
+    const CUtensorMapDataType type =
+        std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return tc::make_map(map, type, p, rows, cols, pitch, box_rows, 64);
+}
+
+// Lets a kernel have more shared memory than 48 KB, once a device.
+template <typename K> static vt_status allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return VT_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(VT_ERR_CUDA, "%u bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+    }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return VT_OK;
+}
+
+template <typename T, int ACT, int OC, int NC>
+static vt_status launch_narrow(const CUtensorMap &dy, const CUtensorMap &w, const NarrowArgs &a, cudaStream_t stream)
+{
+    static std::atomic<uint64_t> allowed{0};
+    using P = Narrow<OC, NC>;
+    if (vt_status s = allow_smem(narrow_kernel<T, ACT, OC, NC>, P::SMEM, allowed)) return s;
+    narrow_kernel<T, ACT, OC, NC><<<a.groups * a.slabs, NARROW_THREADS, P::SMEM, stream>>>(dy, w, a);
+    return check_launch("narrow_kernel");
+}
+
+template <typename T, int ACT>
+static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, uint64_t w_stride, uint64_t rows, uint32_t cols,
+                            uint32_t outs, const int8_t *codes, const uint8_t *exps, void *dz, void *dw, void *db,
+                            uint8_t *workspace, uint32_t *err, cudaStream_t stream)
+{
+    const NarrowPlan p = narrow_plan(rows, cols, outs, (uint32_t)sm_count());
+    CUtensorMap dy_map, w_map;
+    if (vt_status s = map_rows<T>(&dy_map, dy, dy_stride, rows, outs, workspace + p.dy_at, TILE_ROWS, stream)) return s;
+    if (vt_status s = map_rows<T>(&w_map, w, w_stride, outs, cols, workspace + p.w_at, p.oc * 64u, stream)) return s;
+    NarrowArgs a;
+    a.rows = rows;
+    a.cols = cols;
+    a.outs = outs;
+    a.blocks = mx_blocks(cols);
+    a.tiles = p.tiles;
+    a.groups = p.groups;
+    a.slabs = p.slabs;
+    a.codes = codes;
+    a.exps = exps;
+    a.dz = dz;
+    a.dw_parts = dw ? (float *)(workspace + p.dw_at) : nullptr;
+    a.db_parts = db ? (float *)(workspace + p.db_at) : nullptr;
+    a.err = err;
+    a.dz_wide = cols % 16u == 0 && (reinterpret_cast<uintptr_t>(dz) & 31u) == 0;
+    vt_status s = VT_OK;
+    switch (p.oc * 2u + p.nc) {
+    case 3: s = launch_narrow<T, ACT, 1, 1>(dy_map, w_map, a, stream); break;
+    case 4: s = launch_narrow<T, ACT, 1, 2>(dy_map, w_map, a, stream); break;
+    case 5: s = launch_narrow<T, ACT, 2, 1>(dy_map, w_map, a, stream); break;
+    case 6: s = launch_narrow<T, ACT, 2, 2>(dy_map, w_map, a, stream); break;
+    case 7: s = launch_narrow<T, ACT, 3, 1>(dy_map, w_map, a, stream); break;
+    case 8: s = launch_narrow<T, ACT, 3, 2>(dy_map, w_map, a, stream); break;
+    case 9: s = launch_narrow<T, ACT, 4, 1>(dy_map, w_map, a, stream); break;
+    default: s = launch_narrow<T, ACT, 4, 2>(dy_map, w_map, a, stream); break;
+    }
+    if (s || !(dw || db)) return s;
+    const uint64_t n = (uint64_t)p.slabs * p.nc * 64u * p.part_outs;
+    narrow_reduce_kernel<T><<<(unsigned)((n + 255u) / 256u), 256, 0, stream>>>(a.dw_parts, a.db_parts, p.groups, p.slabs, p.nc * 64u,
+                                                                           p.part_outs, cols, outs, (T *)dw, (T *)db);
+    return check_launch("narrow_reduce_kernel");
+}
+
+template <typename T>
+static vt_status zero(T *p, uint64_t n, cudaStream_t stream)
+{
+    if (!p || !n) return VT_OK;
+    cudaError_t e = cudaMemsetAsync(p, 0, n * sizeof(T), stream);
+    return e == cudaSuccess ? VT_OK : set_error(VT_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
+}
+
+}  // namespace vt
+
+extern "C" uint64_t vt_mx8_linear_bwd_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs)
+{
+    if (rows == 0 || cols == 0 || outs == 0 || outs > vt::NARROW_OUTS) return 0;
+    return vt::narrow_plan(rows, cols, outs, (uint32_t)vt::sm_count()).bytes;
+}
+
+extern "C" vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const void *weight, uint64_t weight_stride,
+                                       int dtype, uint64_t rows, uint32_t cols, uint32_t outs, const int8_t *codes,
+                                       const uint8_t *exps, int act, void *dz, void *dw, void *db, void *workspace,
+                                       uint64_t workspace_bytes, uint32_t *err, vt_stream stream)
+{
+    VT_REQUIRE(rows <= (1ull << 31) - 256, "vt_mx8_linear_bwd: too many rows");
+    VT_REQUIRE(cols <= (1u << 20) && outs <= (1u << 20), "vt_mx8_linear_bwd: layer too wide");
+    cudaStream_t st = (cudaStream_t)stream;
+    return vt::with_type16(dtype, [&](auto ty) -> vt_status {
+        using T = typename decltype(ty)::type;
+        if (rows == 0 || cols == 0 || outs == 0) {
+            if (vt_status s = vt::zero((T *)dz, rows * cols, st)) return s;
+            if (vt_status s = vt::zero((T *)dw, (uint64_t)outs * cols, st)) return s;
+            if (rows == 0 || outs == 0) return vt::zero((T *)db, outs, st);
+        }
+        VT_REQUIRE(dy && (cols == 0 || (weight && codes && exps)), "vt_mx8_linear_bwd: null pointer");
+        VT_REQUIRE(dy_stride >= outs && weight_stride >= cols,
+                   "vt_mx8_linear_bwd: a row stride is less than a row");
+        VT_REQUIRE(vt::aligned32(codes), "vt_mx8_linear_bwd: codes must be 32-byte aligned");
+        VT_REQUIRE(workspace_bytes >= vt_mx8_linear_bwd_workspace_bytes(rows, cols, outs) && vt::aligned16(workspace),
+                   "vt_mx8_linear_bwd: workspace too small or not 16-byte aligned");
+        return vt::with_act(act, [&](auto a) -> vt_status {
+            constexpr int ACT = decltype(a)::value;
+            if (cols && outs <= vt::NARROW_OUTS)
+                return vt::run_narrow<T, ACT>(dy, dy_stride, weight, weight_stride, rows, cols, outs, codes, exps, dz, dw, db,
+                                              (uint8_t *)workspace, err, st);
+            const vt::Checkpoint8<ACT> ckpt{codes, exps, vt::mx_blocks(cols)};
+            if (dz && cols) {
+                const dim3 grid((unsigned)((rows + 63) / 64), (cols + 63) / 64);
+                vt::tile_product_kernel<<<grid, 256, 0, st>>>(
+                    rows, cols, (uint64_t)outs, vt::Rows<T, true>{(const T *)dy, dy_stride},
+                    vt::Rows<T, false>{(const T *)weight, weight_stride}, vt::StoreDz<T, ACT>{ckpt, (T *)dz, cols});
+            }
+            if (dw && cols) {
+                const dim3 grid((outs + 63) / 64, (cols + 63) / 64);
+                vt::tile_product_kernel<<<grid, 256, 0, st>>>(
+                    (uint64_t)outs, cols, rows, vt::Rows<T, false>{(const T *)dy, dy_stride}, ckpt,
+                    vt::StoreY<T, vt::ACT_IDENTITY>{(T *)dw, nullptr, cols});
+            }
+            if (db) vt::column_sum_kernel<T><<<outs, 256, 0, st>>>((const T *)dy, rows, outs, dy_stride, (T *)db);
+            return vt::check_launch("vt_mx8_linear_bwd");
+        });
+    });
+}

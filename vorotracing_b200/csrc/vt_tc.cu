@@ -1,0 +1,44 @@
+// vt_tc.cu -- host side of the tensor-core plumbing: TMA tensor maps.
+#include "vt_tc.cuh"
+
+namespace vt {
+namespace tc {
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's entry point, looked up once: the library does not link against the driver.
+static EncodeTiled encode_tiled()
+{
+    static const EncodeTiled f = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return (EncodeTiled)p;
+    }();
+    return f;
+}
+
+vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint64_t cols,
+                   uint64_t pitch, uint32_t box_rows, uint32_t box_cols)
+{
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return set_error(VT_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+    const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
+    const CUresult r = encode(map, type, 2, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(VT_ERR_CUDA, "cuTensorMapEncodeTiled: error %d (%llu x %llu, pitch %llu)", (int)r,
+                         (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)pitch);
+    return VT_OK;
+}
+
+}  // namespace tc
+}  // namespace vt

@@ -1,0 +1,166 @@
+// vt_tc.cuh -- tensor-core plumbing for sm_100a: mbarriers, TMA tile loads,
+// tensor memory and tcgen05 products.  Thin wrappers over PTX; one kernel file
+// decides what they move.
+//
+// Every wait has an end.  A wait that lasts a second gives up, marks the CTA as
+// failed in shared memory and writes VT_ERR_CUDA to the caller's error word; all
+// other waits of that CTA then return too, its roles run to their ends, the
+// producer waits (as long again at most) for the copies it has in flight, and
+// tensor memory is freed.  The outputs of such a launch are not valid.
+#pragma once
+
+#include <cuda.h>
+
+#include "vt_abi.cuh"
+
+namespace vt {
+namespace tc {
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// ---- mbarriers ----
+
+struct Fail {  // in shared memory, one a CTA
+    volatile uint32_t failed;
+};
+
+__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_tx(uint64_t *bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok;
+}
+__device__ __forceinline__ uint64_t nanoseconds()
+{
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+constexpr uint64_t WAIT_LIMIT_NS = 1000000000ull;
+
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, Fail *fail, uint32_t *err, bool last)
+{
+    const uint64_t began = nanoseconds();
+    for (;;) {
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try(bar, parity)) return true;
+        if (fail->failed && !last) return false;
+        if (nanoseconds() - began > WAIT_LIMIT_NS) {
+            fail->failed = 1;
+            report(err, VT_ERR_CUDA);
+            return false;
+        }
+    }
+}
+// Waits for the phase of that parity to end; false: given up.
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, Fail *fail, uint32_t *err)
+{
+    for (int i = 0; i < 16; ++i)
+        if (mbar_try(bar, parity)) return true;
+    return mbar_wait_slow(bar, parity, fail, err, false);
+}
+
+// Counts through the stages of a ring: index and the parity of its current use.
+struct Ring {
+    uint32_t i = 0, phase = 0;
+    __device__ __forceinline__ void next(uint32_t stages)
+    {
+        if (++i == stages) { i = 0; phase ^= 1u; }
+    }
+};
+
+// ---- TMA ----
+
+__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+// Shared-memory writes of this thread before, reads by TMA or tcgen05 after.
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- tensor memory ----
+
+template <uint32_t COLS> __device__ __forceinline__ void tmem_alloc(uint32_t *slot)  // one warp
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "n"(COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <uint32_t COLS> __device__ __forceinline__ void tmem_free(uint32_t base)  // the same warp
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLS));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes: lane l gets row l of its quadrant
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+
+// ---- products ----
+
+// Shared-memory operand in the 128-byte swizzle.  Atoms are 8 rows of 128 bytes (1024-byte
+// aligned).  K-major operand: rows are the operand's rows, stride = bytes from 8 rows to the
+// next 8, lead unused.  MN-major operand: rows are steps of k, stride = bytes from 8 steps of k
+// to the next 8, lead = bytes from 64 rows of the operand to the next 64.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride)
+{
+    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 |
+           1ull << 46 | 2ull << 61;
+}
+// Instruction descriptor of kind::f16, binary32 accumulators.  mn: the operand is MN-major.
+template <bool BF16> __host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, bool a_mn, bool b_mn)
+{
+    return 1u << 4 | (BF16 ? 1u : 0u) << 7 | (BF16 ? 1u : 0u) << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 |
+           (n >> 3) << 17 | (m >> 4) << 24;
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate)
+{
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+// The barrier gets one arrival when the products issued so far by this thread are done.
+__device__ __forceinline__ void commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// ---- host: tensor maps ----
+
+// A row-major matrix (rows, cols) of `bytes`-wide elements with a row pitch in bytes, read in
+// boxes of (box_rows, box_cols) with 128-byte swizzle; outside of the matrix zeros are read.
+vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint64_t cols,
+                   uint64_t pitch, uint32_t box_rows, uint32_t box_cols);
+
+}  // namespace tc
+}  // namespace vt

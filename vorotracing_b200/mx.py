@@ -44,6 +44,28 @@ _ARGS = {
     "vt_mx4_linear": (_P, _U64, _I, _U64, _U32, _U32, _P, _P, _P, _I, _P, _P, _U64, _P, _P),
 }
 _fn = {}
+_error_words = {}
+
+
+def _error_word(device) -> torch.Tensor:
+    """The device word where a product's kernel reports that one of its waits has run out."""
+    t = _error_words.get(device.index)
+    if t is None:
+        t = _error_words[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+    return t
+
+
+def raise_errors(device=None):
+    """Waits for the device and raises if a product's kernel gave up there since the last call."""
+    i = torch.cuda.current_device() if device is None else torch.device(device).index
+    t = _error_words.get(torch.cuda.current_device() if i is None else i)
+    if t is not None:
+        torch.cuda.synchronize(t.device)
+        code = int(t.item())
+        if code:
+            t.zero_()
+            _fail(f"a microscaled product's kernel gave up waiting (status {code}); its outputs "
+                  "are not valid")
 
 
 def _call(name):
@@ -118,8 +140,9 @@ def _check_parts(codes, exps, cols, code_dtype, per_block, what):
         _fail(f"{what}: codes and exponents must be on the same CUDA device")
     if not codes.is_contiguous() or not exps.is_contiguous():
         _fail(f"{what}: codes and exponents must be contiguous")
-    if codes.data_ptr() % 16:
-        _fail(f"{what}: codes must be 16-byte aligned")
+    align = 32 if code_dtype == torch.int8 else 16
+    if codes.data_ptr() % align:
+        _fail(f"{what}: codes must be {align}-byte aligned")
 
 
 class Checkpoint:
@@ -227,7 +250,7 @@ def linear_backward(dy: torch.Tensor, weight: torch.Tensor, ckpt: Checkpoint, bi
     _launch("vt_mx8_linear_bwd", dev, m.data_ptr(), dy_stride, w.data_ptr(), w_stride,
             _DTYPES[dt], rows, cols, outs, ckpt.codes.data_ptr(), ckpt.exps.data_ptr(), ckpt._act,
             dz.data_ptr() if need_dz else None, dw.data_ptr() if need_dw else None,
-            db.data_ptr() if bias else None, ws.data_ptr() if n else None, n, None)
+            db.data_ptr() if bias else None, ws.data_ptr() if n else None, n, _error_word(dev).data_ptr())
     return dz, dw, db
 
 
@@ -287,5 +310,5 @@ def linear4(x: torch.Tensor, w: MX4, bias=None, act: str = "identity") -> torch.
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
     _launch("vt_mx4_linear", x.device, m.data_ptr(), stride, _DTYPES[x.dtype], rows, cols, outs,
             w.codes.data_ptr(), w.exps.data_ptr(), bias.data_ptr() if bias is not None else None,
-            code, y.data_ptr(), ws.data_ptr() if n else None, n, None)
+            code, y.data_ptr(), ws.data_ptr() if n else None, n, _error_word(x.device).data_ptr())
     return y
