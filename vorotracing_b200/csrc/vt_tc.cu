@@ -31,9 +31,15 @@ vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, ui
     if (!encode) return set_error(VT_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
     const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
     const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
-    const CUresult r = encode(map, type, 2, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const auto make = [&] {
+        return encode(map, type, 2, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = make();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread that has made no runtime call yet, as autograd's
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = make();
+    }
     if (r != CUDA_SUCCESS)
         return set_error(VT_ERR_CUDA, "cuTensorMapEncodeTiled: error %d (%llu x %llu, pitch %llu)", (int)r,
                          (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)pitch);
