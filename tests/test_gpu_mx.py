@@ -475,7 +475,7 @@ def test_entry_points_refuse():
     assert f("vt_mx8_checkpoint")(p, 2, 8, 64, 64, 4, p, p, p, None) == 1 and "activation" in err()
     assert f("vt_mx8_act_bwd")(p, 2, 8, 64, 64, p + 8, p, 0, p, None) == 1 and "aligned" in err()
     assert f("vt_mx4_quantize")(p, 2, 8, 64, 64, p, None, None) == 1 and "null pointer" in err()
-    assert f("vt_mx4_linear")(p, 64, 2, 8, 64, 4, p, p, None, 0, p, None, 0, None, None) == 1 and "workspace" in err()
+    assert f("vt_mx4_linear")(p, 64, 2, 8, 64, 300, p, p, None, 0, p, None, 0, None, None) == 1 and "workspace" in err()
     assert f("vt_mx4_linear")(p, 64, 0, 8, 64, 4, p, p, None, 0, p, p, 1 << 20, None, None) == 1 and "16" in err()
     assert f("vt_mx8_linear_bwd")(p, 4, p, 64, 2, 1 << 32, 64, 4, p, p, 0, p, p, p, p, 1 << 40, None, None) == 1 and "rows" in err()
     assert f("vt_mx8_linear_bwd")(p, 4, None, 64, 2, 8, 64, 4, p, p, 0, p, p, p, p, 1 << 40, None, None) == 1 and "null" in err()

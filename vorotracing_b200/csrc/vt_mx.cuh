@@ -74,6 +74,57 @@ template <typename T> struct Vec8 {
     }
 };
 
+// 32 bytes at a 32-byte boundary
+__device__ __forceinline__ void store32(void *p, const uint32_t *w)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+__device__ __forceinline__ void load32(const void *p, uint32_t *w)
+{
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w)
+{
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
+{
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// 32 columns of a row from packed pairs.  wide: the row starts on 32 bytes and holds whole
+// 32-byte pieces, which are whole sectors of L2.
+template <typename T>
+__device__ __forceinline__ void store_row32(T *row, uint32_t col, uint32_t cols, bool wide, const uint32_t *w)
+{
+    T *p = row + col;
+    if (wide) {
+        if (col < cols) store32(p, w);
+        if (col + 16u < cols) store32(p + 16, w + 8);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            const float2 v = unpack2<T>(w[i]);
+            if (col + 2 * i < cols) p[2 * i] = from_f32<T>(v.x);
+            if (col + 2 * i + 1 < cols) p[2 * i + 1] = from_f32<T>(v.y);
+        }
+    }
+}
+
 // ---- formats ----
 
 // Exponent field of a block from the bits of its largest magnitude (sign bit clear).

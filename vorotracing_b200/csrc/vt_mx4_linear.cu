@@ -1,23 +1,327 @@
 // vt_mx4_linear.cu -- y = act(q4(x) w4^T + b), both matrices in 4-bit microscaled blocks (vt_mx.cuh).
-#include "vt_mx_tile.cuh"
+//
+// The product runs on the tensor cores' block-scaled 4-bit path: 128 rows of x by TN outputs a
+// tile, 256 steps of k a stage.  The weight's codes come by TMA into the 128-byte swizzle; four
+// warps bring the scales of a stage into the order in which they are copied to tensor memory; one
+// thread issues copies and products; four warps take finished accumulators out of tensor memory,
+// add the bias, apply the activation and round once.
+//
+// x is rounded to 4 bits inside the same kernel while one tile spans all outputs (QUANT): eight
+// warps read x, which is then read from HBM once and nothing of its 4-bit form is written.
+// With more outputs the same rows would be rounded again for every tile of outputs, so a pass of
+// its own writes codes and scales first, 17/32 byte a value, and TMA brings them in.
+#include "vt_mx.cuh"
+#include "vt_tc.cuh"
 
 namespace vt {
 
-template <bool QUANT, typename T> struct Matrix4 {  // values of a 4-bit matrix at (row, column)
-    static constexpr bool K_INNER = true;
-    const uint8_t *codes, *exps;
-    uint32_t blocks;
-    __device__ float operator()(uint64_t row, uint64_t col) const
-    {
-        const uint32_t c = codes[(row * blocks * MX_BLOCK + col) / 2u];
-        return mx4_value(c >> (4u * (col & 1u)) & 15u) * mx4_scale(exps[row * blocks + col / MX_BLOCK]);
-    }
+constexpr uint32_t L4_ROWS = 128, L4_K = 256;
+
+template <int TN, bool QUANT> struct L4 {
+    static constexpr uint32_t A_BYTES = L4_ROWS * 128u, B_BYTES = TN * 128u;
+    static constexpr uint32_t B_PARTS = TN > 128 ? TN / 128 : 1;  // groups of 128 rows of scales
+    static constexpr uint32_t SF_BYTES = (1u + B_PARTS) * 1024u;
+    static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SF_BYTES;
+    static constexpr uint32_t STAGES = TN == 256 ? 4 : 5;
+    // two accumulators when they leave room for the scales
+    static constexpr uint32_t ACCS = TN == 256 ? 1 : 2;
+    static constexpr uint32_t SF_AT = ACCS * TN, SF_COLS = 8u + 8u * B_PARTS;
+    static constexpr uint32_t TMEM = SF_AT + SF_COLS <= 256 ? 256 : 512;
+    static constexpr uint32_t SCALE_WARPS = 4, QUANT_WARPS = QUANT ? 8 : 0;
+    // warps: 0 TMA, 1 products, 2 and 3 none, 4..7 results, 8..11 scales, 12.. x to 4 bits
+    static constexpr uint32_t THREADS = 32u * (8u + SCALE_WARPS + QUANT_WARPS);
+    static constexpr uint32_t FULL_COUNT = 1u + SCALE_WARPS + QUANT_WARPS;
+    struct Ctrl {
+        uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS];
+        uint32_t tmem;
+        tc::Fail fail;
+        float bias[TN];
+    };
+    static constexpr uint32_t CTRL_AT = STAGES * STAGE, SMEM = CTRL_AT + sizeof(Ctrl);
+    static_assert(SMEM <= 232448 && SF_AT + SF_COLS <= 512, "does not fit an SM");
 };
+
+struct L4Args {
+    uint64_t rows, x_stride;
+    uint32_t cols, outs, blocks, chunks, row_tiles, out_tiles;
+    uint32_t lanes_shift;  // QUANT: log2 of the lanes that share a row's part of a stage
+    const void *x;         // QUANT
+    const uint8_t *x_exps; // not QUANT
+    const uint8_t *w_exps;
+    const void *bias;
+    void *y;
+    uint32_t *err;
+    bool x_vec, y_wide;
+};
+
+// The scales of 8 blocks of a row, zeros (which multiply zero codes) behind its end.
+__device__ __forceinline__ uint2 load_scales(const uint8_t *exps, uint64_t row, uint32_t blocks, uint32_t b0)
+{
+    const uint8_t *p = exps + row * blocks + b0;
+    if (b0 + 8u <= blocks && (reinterpret_cast<uintptr_t>(p) & 7u) == 0) return __ldg(reinterpret_cast<const uint2 *>(p));
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+        if (b0 + i < blocks) w[i / 4] |= (uint32_t)__ldg(p + i) << (i % 4 * 8);
+    return make_uint2(w[0], w[1]);
+}
+// Place of a row's scales in a stage: 16 bytes for each of 32 rows, a word a group of 32.
+__device__ __forceinline__ uint32_t scale_place(uint32_t row) { return (row >> 7) * 1024u + (row & 31u) * 16u + ((row >> 5) & 3u) * 4u; }
+
+template <typename T, int ACT, int TN, bool QUANT>
+__global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
+    linear4_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const L4Args a)
+{
+    using P = L4<TN, QUANT>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    typename P::Ctrl &s = *reinterpret_cast<typename P::Ctrl *>(smem + P::CTRL_AT);
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    const uint32_t tiles = a.row_tiles * a.out_tiles;
+    tc::Fail *const fail = &s.fail;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < P::STAGES; ++i) {
+            tc::mbar_init(&s.full[i], P::FULL_COUNT);
+            tc::mbar_init(&s.empty[i], 1);
+        }
+        for (uint32_t i = 0; i < P::ACCS; ++i) {
+            tc::mbar_init(&s.acc_full[i], 1);
+            tc::mbar_init(&s.acc_empty[i], 4);
+        }
+        s.fail.failed = 0;
+        tc::mbar_init_fence();
+        tc::tma_prefetch_map(&w_map);
+        if (!QUANT) tc::tma_prefetch_map(&x_map);
+    }
+    if (warp == 1) tc::tmem_alloc<P::TMEM>(&s.tmem);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = s.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {  // TMA
+            tc::Ring r;
+            uint32_t issued = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                const int row0 = (int)(t / a.out_tiles * L4_ROWS), out0 = (int)(t % a.out_tiles * TN);
+                for (uint32_t c = 0; c < a.chunks; ++c) {
+                    ok = tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err);
+                    if (!ok) break;
+                    uint8_t *st = smem + r.i * P::STAGE;
+                    tc::mbar_arrive_tx(&s.full[r.i], P::B_BYTES + (QUANT ? 0u : P::A_BYTES));
+                    if (!QUANT) tc::tma_load_2d(st, &x_map, (int)(c * 128u), row0, &s.full[r.i]);
+                    tc::tma_load_2d(st + P::A_BYTES, &w_map, (int)(c * 128u), out0, &s.full[r.i]);
+                    ++issued;
+                    r.next(P::STAGES);
+                }
+            }
+            // A stage's barrier also waits for other warps, so a failed launch cannot use it to
+            // see that its copies are in: it waits for them by time, far longer than a copy takes.
+            if (s.fail.failed) {
+                const uint64_t began = tc::nanoseconds();
+                while (tc::nanoseconds() - began < 10000000ull) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {  // scales to tensor memory, products
+            const uint32_t base = tc::smem_u32(smem);
+            tc::Ring r, acc;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                ok = tc::mbar_wait(&s.acc_empty[acc.i], acc.phase ^ 1u, fail, a.err);
+                if (!ok) break;
+                const uint32_t d = tmem + acc.i * TN, sfa = tmem + P::SF_AT, sfb = sfa + 8u;
+                for (uint32_t c = 0; c < a.chunks; ++c) {
+                    ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
+                    if (!ok) break;
+                    tc::fence_after();
+                    const uint32_t st = base + r.i * P::STAGE, sf = st + P::A_BYTES + P::B_BYTES;
+                    const uint32_t steps = min(4u, (a.cols - c * L4_K + 63u) / 64u);
+                    for (uint32_t g = 0; 2u * g < steps; ++g) {
+                        tc::tmem_copy_scales(sfa + g * 4u, tc::scale_desc(sf + g * 512u));
+                        for (uint32_t p = 0; p < P::B_PARTS; ++p)
+                            tc::tmem_copy_scales(sfb + (g * P::B_PARTS + p) * 4u, tc::scale_desc(sf + 1024u + p * 1024u + g * 512u));
+                    }
+                    for (uint32_t k = 0; k < steps; ++k) {
+                        constexpr uint32_t ID0 = tc::idesc_mxf4(128, TN, 0), ID1 = tc::idesc_mxf4(128, TN, 1);
+                        tc::mma_mxf4(d, tc::smem_desc(st + k * 32u, 16, 1024), tc::smem_desc(st + P::A_BYTES + k * 32u, 16, 1024),
+                                     k & 1u ? ID1 : ID0, sfa + (k >> 1) * 4u, sfb + (k >> 1) * P::B_PARTS * 4u, c + k != 0);
+                    }
+                    tc::commit(&s.empty[r.i]);
+                    r.next(P::STAGES);
+                }
+                tc::commit(&s.acc_full[acc.i]);
+                if (!ok) {  // leave no product in flight
+                    tc::mbar_wait_slow(&s.acc_full[acc.i], acc.phase, fail, a.err, true);
+                    break;
+                }
+                acc.next(P::ACCS);
+            }
+        }
+    } else if (warp >= 4 && warp < 8) {  // results
+        const uint32_t quad = warp % 4u, in_tile = quad * 32u + lane;
+        tc::Ring acc;
+        for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+            const uint64_t row = (uint64_t)(t / a.out_tiles) * L4_ROWS + in_tile;
+            const uint32_t out0 = t % a.out_tiles * TN;
+            // the bias of the tile's outputs; the first barrier keeps the last tile's until it is used
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            for (uint32_t i = in_tile; i < TN; i += 128u)
+                s.bias[i] = a.bias && out0 + i < a.outs ? to_f32<T>(__ldg((const T *)a.bias + out0 + i)) : 0.0f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const bool ok = tc::mbar_wait(&s.acc_full[acc.i], acc.phase, fail, a.err);
+            if (!__all_sync(~0u, ok)) {  // failed: on to the next barrier with the other warps
+                acc.next(P::ACCS);
+                continue;
+            }
+            tc::fence_after();
+#pragma unroll 1
+            for (uint32_t n0 = 0; n0 < TN; n0 += 32u) {
+                uint32_t v[32], w[16];
+                tc::tmem_load32(tmem + acc.i * TN + (quad * 32u << 16) + n0, v);
+                tc::tmem_wait_load();
+                if (n0 + 32u == TN) {
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s.acc_empty[acc.i]);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i)
+                    w[i] = pack2<T>(act_value<ACT>(__uint_as_float(v[2 * i]) + s.bias[n0 + 2 * i]),
+                                    act_value<ACT>(__uint_as_float(v[2 * i + 1]) + s.bias[n0 + 2 * i + 1]));
+                if (row < a.rows) store_row32<T>((T *)a.y + row * a.outs, out0 + n0, a.outs, a.y_wide, w);
+            }
+            acc.next(P::ACCS);
+        }
+    } else if (warp >= 8 && warp < 12) {  // scales: a row of each operand's 128 a lane
+        const uint32_t i = (warp - 8u) * 32u + lane;
+        tc::Ring r;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            const uint64_t row = (uint64_t)(t / a.out_tiles) * L4_ROWS + i;
+            const uint32_t out = t % a.out_tiles * TN + i;
+            for (uint32_t c = 0; c < a.chunks; ++c) {
+                uint2 e[1 + P::B_PARTS];
+                if (!QUANT) e[0] = row < a.rows ? load_scales(a.x_exps, row, a.blocks, c * 8u) : make_uint2(0, 0);
+#pragma unroll
+                for (uint32_t p = 0; p < P::B_PARTS; ++p)
+                    e[1 + p] = i + p * 128u < TN && out + p * 128u < a.outs ? load_scales(a.w_exps, out + p * 128u, a.blocks, c * 8u)
+                                                                            : make_uint2(0, 0);
+                ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
+                if (!ok) break;
+                uint8_t *sf = smem + r.i * P::STAGE + P::A_BYTES + P::B_BYTES + scale_place(i);
+#pragma unroll
+                for (uint32_t p = QUANT ? 1 : 0; p < 1 + P::B_PARTS; ++p) {
+                    *reinterpret_cast<uint32_t *>(sf + p * 1024u) = e[p].x;
+                    *reinterpret_cast<uint32_t *>(sf + p * 1024u + 512u) = e[p].y;
+                }
+                tc::fence_async_shared();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
+                r.next(P::STAGES);
+            }
+        }
+    } else if (QUANT && warp >= 12) {  // x to 4 bits: 8 columns a lane, 4 lanes a block
+        const uint32_t q = warp - 12u, per = a.lanes_shift, rows_at_once = 32u >> per;
+        const uint32_t in_row = lane & ((1u << per) - 1u), first = (q << (5u - per)) + (lane >> per);
+        const uint32_t groups = 16u >> (5u - per);  // passes of 8 warps over the tile's 128 rows: 4, 8 or 16
+        tc::Ring r;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            const uint64_t row0 = (uint64_t)(t / a.out_tiles) * L4_ROWS;
+            for (uint32_t c = 0; c < a.chunks; ++c) {
+                const uint32_t col = c * L4_K + in_row * 8u;
+                const uint32_t n = col >= a.cols ? 0u : min(8u, a.cols - col);
+                ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
+                if (!ok) break;
+                uint8_t *st = smem + r.i * P::STAGE, *sf = st + P::A_BYTES + P::B_BYTES;
+#pragma unroll 1
+                for (uint32_t g = 0; g < groups; g += 4u) {
+                    Vec8<T> x[4];
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        const uint64_t row = row0 + first + (g + u) * 8u * rows_at_once;
+                        const bool in = row < a.rows && n;
+                        const T *p = (const T *)a.x + row * a.x_stride + col;
+                        if (in && a.x_vec) {
+                            x[u].load(p);
+                        } else {
+                            x[u].zero();
+                            if (in)
+                                for (uint32_t i = 0; i < n; ++i) reinterpret_cast<T *>(x[u].w)[i] = __ldg(p + i);
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        const uint32_t row = first + (g + u) * 8u * rows_at_once;
+                        float v[8];
+                        x[u].unpack(v);
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+                        top = max(top, __shfl_xor_sync(~0u, top, 1));
+                        top = max(top, __shfl_xor_sync(~0u, top, 2));
+                        const uint32_t E = mx4_exponent(top);
+                        const float inv = mx4_inverse(E == 255u ? 1u : E);
+                        uint32_t codes = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) codes |= mx4_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+                        const uint32_t block = in_row >> 2;
+                        *reinterpret_cast<uint32_t *>(st + row * 128u + ((block ^ (row & 7u)) << 4) + (in_row & 3u) * 4u) =
+                            E == 255u ? 0u : codes;
+                        if ((in_row & 3u) == 0) sf[scale_place(row) + (block >> 2) * 512u + (block & 3u)] = (uint8_t)E;
+                    }
+                }
+                tc::fence_async_shared();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
+                r.next(P::STAGES);
+            }
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 1) tc::tmem_free<P::TMEM>(tmem);
+}
+
+// No columns: the activation of the bias alone.
+template <typename T, int ACT> __global__ void bias_rows_kernel(const T *bias, uint64_t rows, uint32_t outs, T *y)
+{
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * outs; i += (uint64_t)gridDim.x * 256u)
+        y[i] = from_f32<T>(act_value<ACT>(bias ? to_f32<T>(bias[i % outs]) : 0.0f));
+}
+template <typename T, int ACT> static vt_status launch_bias(const L4Args &a, cudaStream_t stream)
+{
+    bias_rows_kernel<T, ACT><<<sm_count(), 256, 0, stream>>>((const T *)a.bias, a.rows, a.outs, (T *)a.y);
+    return check_launch("bias_rows_kernel");
+}
+
+template <typename T, int ACT, int TN, bool QUANT>
+static vt_status launch_linear4(const uint8_t *x_codes, const uint8_t *w_codes, L4Args a, cudaStream_t stream)
+{
+    static std::atomic<uint64_t> allowed{0};
+    using P = L4<TN, QUANT>;
+    CUtensorMap x_map = {}, w_map;
+    const uint64_t pitch = (uint64_t)a.blocks * 16u;
+    if (!QUANT)
+        if (vt_status s = tc::make_map(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, x_codes, a.rows, pitch, pitch, L4_ROWS, 128)) return s;
+    if (vt_status s = tc::make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w_codes, a.outs, pitch, pitch, TN, 128)) return s;
+    if (vt_status s = tc::allow_smem(linear4_kernel<T, ACT, TN, QUANT>, P::SMEM, allowed)) return s;
+    a.row_tiles = (uint32_t)((a.rows + L4_ROWS - 1u) / L4_ROWS);
+    a.out_tiles = (a.outs + TN - 1u) / TN;
+    const uint64_t tiles = (uint64_t)a.row_tiles * a.out_tiles;
+    const uint32_t sms = (uint32_t)sm_count();
+    linear4_kernel<T, ACT, TN, QUANT><<<(unsigned)(tiles < sms ? tiles : sms), P::THREADS, P::SMEM, stream>>>(x_map, w_map, a);
+    return check_launch("linear4_kernel");
+}
 
 }  // namespace vt
 
-extern "C" uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t)
+extern "C" uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs)
 {
+    if (outs <= 256u) return 0;  // x is rounded inside the kernel
     const uint64_t blocks = vt::mx_blocks(cols);
     return rows * blocks * 16u + (rows * blocks + 15u) / 16u * 16u;
 }
@@ -28,25 +332,44 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
 {
     VT_REQUIRE(rows <= (1ull << 31) - 256, "vt_mx4_linear: too many rows");
     VT_REQUIRE(cols <= (1u << 20) && outs <= (1u << 20), "vt_mx4_linear: layer too wide");
+    VT_REQUIRE((rows + 127) / 128 * ((outs + 63) / 64) < (1ull << 31), "vt_mx4_linear: too many outputs");
     if (rows == 0 || outs == 0) return VT_OK;
     VT_REQUIRE(y && (cols == 0 || (x && codes && exps)), "vt_mx4_linear: null pointer");
     VT_REQUIRE(x_stride >= cols, "vt_mx4_linear: the row stride is less than a row");
-    VT_REQUIRE(workspace_bytes >= vt_mx4_linear_workspace_bytes(rows, cols, outs) && (workspace || cols == 0) &&
-                   vt::aligned16(workspace),
+    VT_REQUIRE(vt::aligned16(codes), "vt_mx4_linear: codes must be 16-byte aligned");
+    VT_REQUIRE(workspace_bytes >= vt_mx4_linear_workspace_bytes(rows, cols, outs) && vt::aligned16(workspace),
                "vt_mx4_linear: workspace too small or not 16-byte aligned");
     cudaStream_t st = (cudaStream_t)stream;
-    const uint32_t blocks = vt::mx_blocks(cols);
-    uint8_t *xc = (uint8_t *)workspace, *xe = xc + rows * blocks * 16u;
     return vt::with_type16(dtype, [&](auto ty) -> vt_status {
         using T = typename decltype(ty)::type;
-        if (vt_status s = vt_mx4_quantize(x, dtype, rows, cols, x_stride, xc, xe, stream)) return s;
-        return vt::with_act(act, [&](auto a) -> vt_status {
-            const dim3 grid((unsigned)((rows + 63) / 64), (outs + 63) / 64);
-            vt::tile_product_kernel<<<grid, 256, 0, st>>>(
-                rows, outs, (uint64_t)cols, vt::Matrix4<true, T>{xc, xe, blocks},
-                vt::Matrix4<false, T>{codes, exps, blocks},
-                vt::StoreY<T, decltype(a)::value>{(T *)y, (const T *)bias, outs});
-            return vt::check_launch("vt_mx4_linear");
+        vt::L4Args a = {};
+        a.rows = rows;
+        a.x_stride = x_stride;
+        a.cols = cols;
+        a.outs = outs;
+        a.blocks = vt::mx_blocks(cols);
+        a.chunks = (cols + vt::L4_K - 1u) / vt::L4_K;
+        a.lanes_shift = cols <= 64u ? 3u : cols <= 128u ? 4u : 5u;
+        a.x = x;
+        a.w_exps = exps;
+        a.bias = bias;
+        a.y = y;
+        a.err = err;
+        a.x_vec = cols % 8u == 0 && x_stride % 8u == 0 && vt::aligned16(x);
+        a.y_wide = outs % 16u == 0 && vt::aligned32(y);
+        if (cols == 0) return vt::with_act(act, [&](auto f) { return vt::launch_bias<T, decltype(f)::value>(a, st); });
+        uint8_t *x_codes = (uint8_t *)workspace;
+        if (outs > 256u) {
+            uint8_t *x_exps = x_codes + rows * a.blocks * 16u;
+            if (vt_status s = vt_mx4_quantize(x, dtype, rows, cols, x_stride, x_codes, x_exps, stream)) return s;
+            a.x_exps = x_exps;
+        }
+        return vt::with_act(act, [&](auto f) -> vt_status {
+            constexpr int ACT = decltype(f)::value;
+            if (outs <= 64u) return vt::launch_linear4<T, ACT, 64, true>(nullptr, codes, a, st);
+            if (outs <= 128u) return vt::launch_linear4<T, ACT, 128, true>(nullptr, codes, a, st);
+            if (outs <= 256u) return vt::launch_linear4<T, ACT, 256, true>(nullptr, codes, a, st);
+            return vt::launch_linear4<T, ACT, 256, false>(x_codes, codes, a, st);
         });
     });
 }

@@ -16,8 +16,6 @@
 #include "vt_mx_tile.cuh"
 #include "vt_tc.cuh"
 
-#include <atomic>
-
 namespace vt {
 
 template <typename T, bool KIN> struct Rows {  // element (i, k) of a row-major matrix, or of its transpose
@@ -101,37 +99,6 @@ struct NarrowArgs {
     bool dz_wide;      // dz's rows hold whole 32-byte pieces
 };
 
-__device__ __forceinline__ void store32(void *p, const uint32_t *w)
-{
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-}
-__device__ __forceinline__ void load32(const void *p, uint32_t *w)
-{
-    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
-}
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
-{
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
-{
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
-template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w)
-{
-    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-}
-template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
-{
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-
 // Byte i (0..3) of a word of codes, as a float: the byte with its sign bit turned goes under
 // the exponent of 2^23, which makes 2^23 + 128 + code.
 __device__ __forceinline__ float code_float(uint32_t turned, int i)
@@ -159,24 +126,6 @@ __device__ __forceinline__ void transform_block(const uint32_t *codes, uint32_t 
         h[2 * w + 1] = pack2<T>(hv[2], hv[3]);
         dz[2 * w] = pack2<T>(gv[0], gv[1]);
         dz[2 * w + 1] = pack2<T>(gv[2], gv[3]);
-    }
-}
-
-// 32 columns of a row of dz from packed pairs
-template <typename T>
-__device__ __forceinline__ void store_dz(const NarrowArgs &a, uint64_t row, uint32_t col, const uint32_t *w)
-{
-    T *p = (T *)a.dz + row * a.cols + col;
-    if (a.dz_wide) {
-        if (col < a.cols) store32(p, w);
-        if (col + 16u < a.cols) store32(p + 16, w + 8);
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-            const float2 v = unpack2<T>(w[i]);
-            if (col + 2 * i < a.cols) p[2 * i] = from_f32<T>(v.x);
-            if (col + 2 * i + 1 < a.cols) p[2 * i + 1] = from_f32<T>(v.y);
-        }
     }
 }
 
@@ -372,7 +321,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 for (uint32_t u = 0; u < 4; ++u)
                     *reinterpret_cast<uint4 *>(p + (((unit + u) ^ (in_tile & 7u)) << 4)) =
                         make_uint4(hv[4 * u], hv[4 * u + 1], hv[4 * u + 2], hv[4 * u + 3]);
-                if (a.dz && row < a.rows) store_dz<T>(a, row, (block0 + j) * 32u, dz);
+                if (a.dz && row < a.rows) store_row32<T>((T *)a.dz + row * a.cols, (block0 + j) * 32u, a.cols, a.dz_wide, dz);
             }
             tc::fence_async_shared();
             __syncwarp();
@@ -500,28 +449,12 @@ static vt_status map_rows(CUtensorMap *map, const void *p, uint64_t stride, uint
     return tc::make_map(map, type, p, rows, cols, pitch, box_rows, 64);
 }
 
-// Lets a kernel have more shared memory than 48 KB, once a device.
-template <typename K> static vt_status allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done)
-{
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (done.load(std::memory_order_relaxed) & bit) return VT_OK;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return set_error(VT_ERR_CUDA, "%u bytes of shared memory: %s", bytes, cudaGetErrorString(e));
-    }
-    done.fetch_or(bit, std::memory_order_relaxed);
-    return VT_OK;
-}
-
 template <typename T, int ACT, int OC, int NC>
 static vt_status launch_narrow(const CUtensorMap &dy, const CUtensorMap &w, const NarrowArgs &a, cudaStream_t stream)
 {
     static std::atomic<uint64_t> allowed{0};
     using P = Narrow<OC, NC>;
-    if (vt_status s = allow_smem(narrow_kernel<T, ACT, OC, NC>, P::SMEM, allowed)) return s;
+    if (vt_status s = tc::allow_smem(narrow_kernel<T, ACT, OC, NC>, P::SMEM, allowed)) return s;
     narrow_kernel<T, ACT, OC, NC><<<a.groups * a.slabs, NARROW_THREADS, P::SMEM, stream>>>(dy, w, a);
     return check_launch("narrow_kernel");
 }

@@ -11,6 +11,8 @@
 
 #include <cuda.h>
 
+#include <atomic>
+
 #include "vt_abi.cuh"
 
 namespace vt {
@@ -149,6 +151,31 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
+// Shared-memory source of tmem_copy_scales: 32 rows of 16 bytes, unswizzled.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr)
+{
+    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(128u >> 4) << 32 | 1ull << 46;
+}
+// 512 bytes of shared memory to 4 columns of tensor memory, the same 32 lanes four times: the
+// scales of 128 rows of an operand and 4 blocks of k.  Row r and block b are byte b of word r / 32
+// of the 16 bytes at 16 (r % 32).  Copies and products of one thread run in the order of issue.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t d, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(d), "l"(desc) : "memory");
+}
+// Instruction descriptor of kind::mxf4: e2m1 operands, power-of-two scales for blocks of 32,
+// binary32 accumulators.  pair: which two of a word's four scales the product's 64 steps of k take.
+__host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t m, uint32_t n, uint32_t pair)
+{
+    return (2u * pair) << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (m >> 7) << 27 | (2u * pair) << 29;
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b,
+                                         bool accumulate)
+{
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"((uint32_t)accumulate) : "memory");
+}
 // The barrier gets one arrival when the products issued so far by this thread are done.
 __device__ __forceinline__ void commit(uint64_t *bar)
 {
@@ -161,6 +188,22 @@ __device__ __forceinline__ void commit(uint64_t *bar)
 // boxes of (box_rows, box_cols) with 128-byte swizzle; outside of the matrix zeros are read.
 vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint64_t cols,
                    uint64_t pitch, uint32_t box_rows, uint32_t box_cols);
+
+// Lets a kernel have more shared memory than 48 KB, once a device.
+template <typename K> inline vt_status allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return VT_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(VT_ERR_CUDA, "%u bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+    }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return VT_OK;
+}
 
 }  // namespace tc
 }  // namespace vt
