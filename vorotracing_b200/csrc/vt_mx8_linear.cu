@@ -13,56 +13,15 @@
 // own activations are.  Two more warps add up dy's columns from the staged tile.  At its end a CTA
 // writes its part of dW in binary32; a second kernel adds the parts in order, so results do not
 // depend on timing.
-#include "vt_mx_tile.cuh"
+//
+// Wider layers are two matrix products (wide_kernel), both on pairs of CTAs that share a 256 x 256
+// tile: dz = (dy W) * act'(z8), with the slope in the epilogue, and dW = dy^T h with h = act(z8)
+// written once, in the operands' type, by a pass before it: as an operand it is read once for
+// every 256 outputs, and evaluating it as often would cost more than the tensor cores' time.
+#include "vt_mx.cuh"
 #include "vt_tc.cuh"
 
 namespace vt {
-
-template <typename T, bool KIN> struct Rows {  // element (i, k) of a row-major matrix, or of its transpose
-    static constexpr bool K_INNER = KIN;
-    const T *p;
-    uint64_t stride;
-    __device__ float operator()(uint64_t i, uint64_t k) const
-    {
-        return to_f32<T>(__ldg(p + (KIN ? i * stride + k : k * stride + i)));
-    }
-};
-
-template <int ACT> struct Checkpoint8 {  // act(z8) at (column, row)
-    static constexpr bool K_INNER = false;
-    const int8_t *codes;
-    const uint8_t *exps;
-    uint32_t blocks;
-    __device__ float z(uint64_t row, uint32_t col) const
-    {
-        return (float)codes[row * blocks * MX_BLOCK + col] * mx8_scale(exps[row * blocks + col / MX_BLOCK]);
-    }
-    __device__ float operator()(uint64_t col, uint64_t row) const { return act_value<ACT>(z(row, (uint32_t)col)); }
-};
-
-template <typename T, int ACT> struct StoreDz {
-    Checkpoint8<ACT> ckpt;
-    T *p;
-    uint32_t cols;
-    __device__ void operator()(uint64_t i, uint32_t j, float v) const
-    {
-        p[i * cols + j] = from_f32<T>(v * act_slope<ACT>(ckpt.z(i, j)));
-    }
-};
-
-template <typename T> __global__ void column_sum_kernel(const T *p, uint64_t rows, uint32_t cols, uint64_t stride, T *out)
-{
-    __shared__ float part[256];
-    float v = 0.0f;
-    for (uint64_t i = threadIdx.x; i < rows; i += 256u) v += to_f32<T>(p[i * stride + blockIdx.x]);
-    part[threadIdx.x] = v;
-    __syncthreads();
-    for (int n = 128; n; n >>= 1) {
-        if (threadIdx.x < n) part[threadIdx.x] += part[threadIdx.x + n];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) out[blockIdx.x] = from_f32<T>(part[0]);
-}
 
 // ---- layers with up to 256 outputs ----
 
@@ -124,6 +83,22 @@ __device__ __forceinline__ void transform_block(const uint32_t *codes, uint32_t 
         }
         h[2 * w] = pack2<T>(hv[0], hv[1]);
         h[2 * w + 1] = pack2<T>(hv[2], hv[3]);
+        dz[2 * w] = pack2<T>(gv[0], gv[1]);
+        dz[2 * w + 1] = pack2<T>(gv[2], gv[3]);
+    }
+}
+
+// The same for dz alone.
+template <typename T, int ACT>
+__device__ __forceinline__ void slope_block(const uint32_t *codes, uint32_t E, const uint32_t *g, uint32_t *dz)
+{
+    const float sc = mx8_scale(E);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        const uint32_t c = codes[w] ^ 0x80808080u;
+        float gv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) gv[i] = __uint_as_float(g[4 * w + i]) * act_slope<ACT>(code_float(c, i) * sc);
         dz[2 * w] = pack2<T>(gv[0], gv[1]);
         dz[2 * w + 1] = pack2<T>(gv[2], gv[3]);
     }
@@ -403,6 +378,270 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const T *__restrict__ src
     }
 }
 
+
+// ---- wider layers ----
+
+constexpr uint32_t WIDE_STAGES = 6, WIDE_STAGE_BYTES = 32768, WIDE_THREADS = 256;
+struct WideCtrl {
+    uint64_t full[WIDE_STAGES], empty[WIDE_STAGES], acc_full[2], acc_empty[2];
+    uint32_t tmem;
+    tc::Fail fail;
+};
+constexpr uint32_t WIDE_SMEM = WIDE_STAGES * WIDE_STAGE_BYTES + sizeof(WideCtrl);
+
+struct WideArgs {
+    uint64_t m, n, k;          // sizes of the product C (m, n) = sum over k
+    uint32_t m_tiles, n_tiles, tile_n, chunks, splits, chunks_a_split;
+    uint32_t blocks;           // of a row of z
+    const int8_t *codes;       // dz: the checkpoint
+    const uint8_t *exps;
+    void *out;                 // dz or dW
+    float *parts;              // dW with splits > 1: [split][m][n]
+    uint32_t *err;
+    bool out_wide;
+};
+
+// C = A B on 256 x 256 tiles, 64 steps of k a stage.  DZ: A = dy (K-major), B = W, C = dz after the
+// slope.  Otherwise A = dy^T (MN-major: k runs over the rows of dy), B = h, C = dW or, where k is
+// split for want of tiles, parts of it.
+template <typename T, int ACT, bool DZ>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
+    wide_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const WideArgs a)
+{
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    WideCtrl &s = *reinterpret_cast<WideCtrl *>(smem + WIDE_STAGES * WIDE_STAGE_BYTES);
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = tc::cluster_rank();
+    const uint32_t units = a.m_tiles * a.n_tiles * a.splits, first = blockIdx.x / 2u, step = gridDim.x / 2u;
+    const uint32_t half_n = a.tile_n / 2u, b_boxes = half_n > 64u ? 2u : 1u;
+    tc::Fail *const fail = &s.fail;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < WIDE_STAGES; ++i) {
+            tc::mbar_init(&s.full[i], 1);
+            tc::mbar_init(&s.empty[i], 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            tc::mbar_init(&s.acc_full[i], 1);
+            tc::mbar_init(&s.acc_empty[i], 8);
+        }
+        s.fail.failed = 0;
+        tc::mbar_init_fence();
+        tc::tma_prefetch_map(&a_map);
+        tc::tma_prefetch_map(&b_map);
+    }
+    if (warp == 1) tc::tmem_alloc_pair<512>(&s.tmem);
+    tc::fence_before();
+    tc::cluster_sync();
+    tc::fence_after();
+    const uint32_t tmem = s.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {  // TMA, in each CTA; the leader's barriers count both CTAs' bytes
+            tc::Ring r;
+            bool ok = true;
+            for (uint32_t u = first; u < units && ok; u += step) {
+                const uint32_t t = u % (a.m_tiles * a.n_tiles), c0 = u / (a.m_tiles * a.n_tiles) * a.chunks_a_split;
+                const uint32_t c1 = min(a.chunks, c0 + a.chunks_a_split);
+                const int m0 = (int)(t / a.n_tiles * 256u + rank * 128u), n0 = (int)(t % a.n_tiles * a.tile_n + rank * half_n);
+                for (uint32_t c = c0; c < c1; ++c) {
+                    ok = tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err);
+                    if (!ok) break;
+                    uint8_t *st = smem + r.i * WIDE_STAGE_BYTES;
+                    const uint32_t bar = tc::leader_addr(&s.full[r.i]);
+                    if (rank == 0) tc::mbar_arrive_tx(&s.full[r.i], 2u * (16384u + b_boxes * 8192u));
+                    if (DZ) {
+                        tc::tma_load_2d_pair(st, &a_map, (int)(c * 64u), m0, bar);
+                    } else {
+                        tc::tma_load_2d_pair(st, &a_map, m0, (int)(c * 64u), bar);
+                        tc::tma_load_2d_pair(st + 8192, &a_map, m0 + 64, (int)(c * 64u), bar);
+                    }
+                    for (uint32_t b = 0; b < b_boxes; ++b)
+                        tc::tma_load_2d_pair(st + 16384 + b * 8192, &b_map, n0 + (int)(b * 64u), (int)(c * 64u), bar);
+                    r.next(WIDE_STAGES);
+                }
+            }
+            // The bytes of both CTAs are counted in the leader alone, so after a failure each CTA
+            // waits for its copies by time, far longer than they take.
+            if (s.fail.failed) {
+                const uint64_t began = tc::nanoseconds();
+                while (tc::nanoseconds() - began < 10000000ull) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {  // products, in the leader
+            const uint32_t base = tc::smem_u32(smem), id = tc::idesc_f16<BF16>(256, 0, !DZ, true) | (a.tile_n >> 3) << 17;
+            tc::Ring r, acc;
+            bool ok = true;
+            for (uint32_t u = first; u < units && ok; u += step) {
+                const uint32_t c0 = u / (a.m_tiles * a.n_tiles) * a.chunks_a_split, c1 = min(a.chunks, c0 + a.chunks_a_split);
+                ok = tc::mbar_wait(&s.acc_empty[acc.i], acc.phase ^ 1u, fail, a.err);
+                if (!ok) break;
+                for (uint32_t c = c0; c < c1; ++c) {
+                    ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
+                    if (!ok) break;
+                    tc::fence_after();
+                    const uint32_t st = base + r.i * WIDE_STAGE_BYTES;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        tc::mma_f16_pair(tmem + acc.i * 256u,
+                                         DZ ? tc::smem_desc(st + k * 32u, 16, 1024) : tc::smem_desc(st + k * 2048u, 8192, 1024),
+                                         tc::smem_desc(st + 16384u + k * 2048u, 8192, 1024), id, c != c0 || k != 0);
+                    tc::commit_pair(&s.empty[r.i]);
+                    r.next(WIDE_STAGES);
+                }
+                tc::commit_pair(&s.acc_full[acc.i]);
+                if (!ok) {  // leave no product in flight
+                    tc::mbar_wait_slow(&s.acc_full[acc.i], acc.phase, fail, a.err, true);
+                    break;
+                }
+                acc.next(2);
+            }
+        }
+    } else if (warp >= 4) {  // results: a lane has a row of this CTA's 128
+        const uint32_t quad = warp % 4u, in_tile = quad * 32u + lane;
+        tc::Ring acc;
+        for (uint32_t u = first; u < units; u += step) {
+            const uint32_t t = u % (a.m_tiles * a.n_tiles), split = u / (a.m_tiles * a.n_tiles);
+            const uint64_t row = (uint64_t)(t / a.n_tiles) * 256u + rank * 128u + in_tile;
+            const uint32_t n0 = t % a.n_tiles * a.tile_n;
+            const bool ok = tc::mbar_wait(&s.acc_full[acc.i], acc.phase, fail, a.err);
+            if (!__all_sync(~0u, ok)) break;
+            tc::fence_after();
+#pragma unroll 1
+            for (uint32_t j = 0; j < a.tile_n; j += 32u) {
+                const uint32_t col = n0 + j;
+                uint32_t v[32], w[16];
+                uint32_t codes[8], E = 127;
+                if (DZ) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) codes[i] = 0;
+                    if (row < a.m && col < a.n) {
+                        const uint64_t b = row * a.blocks + col / 32u;
+                        load32(a.codes + b * 32u, codes);
+                        E = __ldg(a.exps + b);
+                    }
+                }
+                tc::tmem_load32(tmem + acc.i * 256u + (quad * 32u << 16) + j, v);
+                tc::tmem_wait_load();
+                if (j + 32u >= a.tile_n) {
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive_cluster(tc::leader_addr(&s.acc_empty[acc.i]));
+                }
+                if (row >= a.m) continue;
+                if (DZ) {
+                    slope_block<T, ACT>(codes, E, v, w);
+                    store_row32<T>((T *)a.out + row * a.n, col, (uint32_t)a.n, a.out_wide, w);
+                } else if (a.splits > 1) {
+                    float *p = a.parts + ((uint64_t)split * a.m + row) * a.n + col;
+                    if (a.n % 8u == 0) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i)
+                            if (col + 8u * i < a.n) store32(p + 8u * i, v + 8 * i);
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i)
+                            if (col + i < a.n) p[i] = __uint_as_float(v[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) w[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                    store_row32<T>((T *)a.out + row * a.n, col, (uint32_t)a.n, a.out_wide, w);
+                }
+            }
+            acc.next(2);
+        }
+    }
+    __syncwarp();
+    tc::fence_before();
+    tc::cluster_sync();  // no CTA leaves while the other may still reach its barriers
+    if (warp == 1) tc::tmem_free_pair<512>(tmem);
+}
+
+// h = act(z8) in the operands' type, rows at a pitch of whole 16-byte words.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) activate_kernel(const int8_t *__restrict__ codes, const uint8_t *__restrict__ exps,
+                                                       uint64_t rows, uint32_t blocks, uint32_t pitch, T *__restrict__ h)
+{
+    const uint64_t items = rows * blocks;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < items * 4u; i += (uint64_t)gridDim.x * 256u) {
+        const uint64_t b = i >> 2;
+        const uint64_t row = items >> 32 ? b / blocks : (uint32_t)b / blocks;
+        const uint32_t col = (uint32_t)(b - row * blocks) * 32u + (uint32_t)(i & 3u) * 8u;
+        if (col >= pitch) continue;
+        const uint2 c = __ldg(reinterpret_cast<const uint2 *>(codes) + i);
+        const float sc = mx8_scale(__ldg(exps + b));
+        uint32_t w[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const uint32_t x = (p < 2 ? c.x : c.y) ^ 0x80808080u;
+            w[p] = pack2<T>(act_value<ACT>(code_float(x, p % 2 * 2) * sc), act_value<ACT>(code_float(x, p % 2 * 2 + 1) * sc));
+        }
+        *reinterpret_cast<uint4 *>(h + row * pitch + col) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Column sums of dy in parts: a block takes 256 columns, 8 a lane, and every gridDim.y-th group of 8 rows.
+template <typename T>
+__global__ void __launch_bounds__(256) column_parts_kernel(const T *__restrict__ dy, uint64_t rows, uint32_t cols, uint64_t pitch,
+                                                           float *__restrict__ parts)
+{
+    __shared__ float sum[8][257];
+    const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, col = blockIdx.x * 256u + lane * 8u;
+    float v[8] = {};
+    if (col < cols)
+        for (uint64_t row = blockIdx.y * 8u + warp; row < rows; row += gridDim.y * 8u) {
+            Vec8<T> x;
+            float f[8];
+            const T *p = dy + row * pitch + col;
+            if (col + 8u <= cols) {
+                x.load(p);
+            } else {
+                x.zero();
+                for (uint32_t i = 0; i < cols - col; ++i) reinterpret_cast<T *>(x.w)[i] = p[i];
+            }
+            x.unpack(f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += f[i];
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[warp][lane * 8u + i] = v[i];
+    __syncthreads();
+    const uint32_t c = blockIdx.x * 256u + threadIdx.x;
+    float total = 0.0f;
+    for (int w = 0; w < 8; ++w) total += sum[w][threadIdx.x];
+    if (c < cols) parts[(uint64_t)blockIdx.y * cols + c] = total;
+}
+
+// Column sums in one launch, for the rare matrix that no other kernel reads.
+template <typename T>
+__global__ void __launch_bounds__(256) column_sum_kernel(const T *__restrict__ p, uint64_t rows, uint32_t cols, uint64_t stride, T *__restrict__ out)
+{
+    __shared__ float part[256];
+    float v = 0.0f;
+    for (uint64_t i = threadIdx.x; i < rows; i += 256u) v += to_f32<T>(p[i * stride + blockIdx.x]);
+    part[threadIdx.x] = v;
+    __syncthreads();
+    for (int n = 128; n; n >>= 1) {
+        if (threadIdx.x < n) part[threadIdx.x] += part[threadIdx.x + n];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) out[blockIdx.x] = from_f32<T>(part[0]);
+}
+
+// out = the parts added in order
+template <typename T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const float *__restrict__ parts, uint32_t count, uint64_t n, T *__restrict__ out)
+{
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256u) {
+        float v = 0.0f;
+#pragma unroll 4
+        for (uint32_t p = 0; p < count; ++p) v += __ldg(parts + p * n + i);
+        out[i] = from_f32<T>(v);
+    }
+}
+
 static uint64_t align_up(uint64_t n, uint64_t a) { return (n + a - 1) / a * a; }
 
 // How a narrow call is cut, and where its workspace parts lie.  The copies of dy and the weight
@@ -430,23 +669,27 @@ static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, uint3
     return p;
 }
 
-// A tensor map over p, or over a copy of it with whole 16-byte rows where p's are not.
+// p and its row stride, or a copy's whose rows are whole 16-byte words where p's are not.
 template <typename T>
-static vt_status map_rows(CUtensorMap *map, const void *p, uint64_t stride, uint64_t rows, uint32_t cols, void *copy,
-                          uint32_t box_rows, cudaStream_t stream)
+static vt_status whole_rows(const void *&p, uint64_t &stride, uint64_t rows, uint32_t cols, void *copy, cudaStream_t stream)
 {
     uint64_t pitch = stride * sizeof(T);
     if (pitch % 16u || !aligned16(p)) {
         const uint32_t to = (uint32_t)align_up(cols, 8);
         const uint64_t items = rows * (to / 8u), want = (items + 255u) / 256u;
         pad_rows_kernel<T><<<(unsigned)(want < 4096u ? want : 4096u), 256, 0, stream>>>((const T *)p, rows, cols, stride, (T *)copy, to);
-        if (vt_status s = check_launch("pad_rows_kernel")) return s;
         p = copy;
-        pitch = (uint64_t)to * sizeof(T);
+        stride = to;
+        return check_launch("pad_rows_kernel");
     }
+    return VT_OK;
+}
+template <typename T>
+static vt_status map_rows(CUtensorMap *map, const void *p, uint64_t stride, uint64_t rows, uint64_t cols, uint32_t box_rows)
+{
     const CUtensorMapDataType type =
         std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    return tc::make_map(map, type, p, rows, cols, pitch, box_rows, 64);
+    return tc::make_map(map, type, p, rows, cols, stride * sizeof(T), box_rows, 64);
 }
 
 template <typename T, int ACT, int OC, int NC>
@@ -466,8 +709,10 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
 {
     const NarrowPlan p = narrow_plan(rows, cols, outs, (uint32_t)sm_count());
     CUtensorMap dy_map, w_map;
-    if (vt_status s = map_rows<T>(&dy_map, dy, dy_stride, rows, outs, workspace + p.dy_at, TILE_ROWS, stream)) return s;
-    if (vt_status s = map_rows<T>(&w_map, w, w_stride, outs, cols, workspace + p.w_at, p.oc * 64u, stream)) return s;
+    if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
+    if (vt_status s = whole_rows<T>(w, w_stride, outs, cols, workspace + p.w_at, stream)) return s;
+    if (vt_status s = map_rows<T>(&dy_map, dy, dy_stride, rows, outs, TILE_ROWS)) return s;
+    if (vt_status s = map_rows<T>(&w_map, w, w_stride, outs, cols, p.oc * 64u)) return s;
     NarrowArgs a;
     a.rows = rows;
     a.cols = cols;
@@ -482,7 +727,7 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     a.dw_parts = dw ? (float *)(workspace + p.dw_at) : nullptr;
     a.db_parts = db ? (float *)(workspace + p.db_at) : nullptr;
     a.err = err;
-    a.dz_wide = cols % 16u == 0 && (reinterpret_cast<uintptr_t>(dz) & 31u) == 0;
+    a.dz_wide = cols % 16u == 0 && aligned32(dz);
     vt_status s = VT_OK;
     switch (p.oc * 2u + p.nc) {
     case 3: s = launch_narrow<T, ACT, 1, 1>(dy_map, w_map, a, stream); break;
@@ -501,6 +746,107 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     return check_launch("narrow_reduce_kernel");
 }
 
+// How a wide call is cut, and where its workspace parts lie.
+struct WidePlan {
+    uint32_t splits, chunks_a_split, sum_parts;
+    uint64_t h_at, dw_at, db_at, dy_at, w_at, bytes;
+};
+static uint32_t wide_tile_n(uint32_t cols) { return cols >= 256u ? 256u : (cols + 31u) / 32u * 32u; }
+static WidePlan wide_plan(uint64_t rows, uint32_t cols, uint32_t outs, uint32_t sms)
+{
+    WidePlan p;
+    const uint32_t tn = wide_tile_n(cols), chunks = (uint32_t)((rows + 63u) / 64u);
+    const uint64_t tiles = (uint64_t)((outs + 255u) / 256u) * ((cols + tn - 1u) / tn);
+    // with fewer tiles than pairs of SMs the rows are split, down to 8 stages a split
+    const uint64_t room = tiles < sms / 2u ? sms / 2u / tiles : 1u, most = (chunks + 7u) / 8u;
+    p.splits = (uint32_t)(room < most ? room : most);
+    p.chunks_a_split = (chunks + p.splits - 1u) / p.splits;
+    p.splits = (chunks + p.chunks_a_split - 1u) / p.chunks_a_split;
+    p.sum_parts = (uint32_t)((rows + 255u) / 256u < 32u ? (rows + 255u) / 256u : 32u);
+    p.h_at = 0;
+    p.dw_at = p.h_at + align_up(rows * align_up(cols, 8) * 2u, 256);
+    p.db_at = p.dw_at + (p.splits > 1 ? align_up((uint64_t)p.splits * outs * cols * 4u, 256) : 0);
+    p.dy_at = p.db_at + align_up((uint64_t)p.sum_parts * outs * 4u, 256);
+    p.w_at = p.dy_at + align_up(rows * align_up(outs, 8) * 2u, 256);
+    p.bytes = p.w_at + align_up((uint64_t)outs * align_up(cols, 8) * 2u, 256);
+    return p;
+}
+
+template <typename T, int ACT, bool DZ>
+static vt_status launch_wide(const CUtensorMap &ma, const CUtensorMap &mb, const WideArgs &a, uint32_t sms, cudaStream_t stream)
+{
+    static std::atomic<uint64_t> allowed{0};
+    if (vt_status s = tc::allow_smem(wide_kernel<T, ACT, DZ>, WIDE_SMEM, allowed)) return s;
+    const uint64_t units = (uint64_t)a.m_tiles * a.n_tiles * a.splits;
+    VT_REQUIRE(units < (1ull << 31), "vt_mx8_linear_bwd: too many tiles");
+    const unsigned pairs = (unsigned)(units < sms / 2u ? units : sms / 2u);
+    wide_kernel<T, ACT, DZ><<<pairs * 2u, WIDE_THREADS, WIDE_SMEM, stream>>>(ma, mb, a);
+    return check_launch("wide_kernel");
+}
+
+template <typename T, int ACT>
+static vt_status run_wide(const void *dy, uint64_t dy_stride, const void *w, uint64_t w_stride, uint64_t rows, uint32_t cols,
+                          uint32_t outs, const int8_t *codes, const uint8_t *exps, void *dz, void *dw, void *db,
+                          uint8_t *workspace, uint32_t *err, cudaStream_t stream)
+{
+    const uint32_t sms = (uint32_t)sm_count();
+    const WidePlan p = wide_plan(rows, cols, outs, sms);
+    if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
+    WideArgs a = {};
+    a.tile_n = wide_tile_n(cols);
+    a.n_tiles = (cols + a.tile_n - 1u) / a.tile_n;
+    a.n = cols;
+    a.blocks = mx_blocks(cols);
+    a.codes = codes;
+    a.exps = exps;
+    a.err = err;
+    CUtensorMap ma, mb;
+    if (dz) {
+        if (vt_status s = whole_rows<T>(w, w_stride, outs, cols, workspace + p.w_at, stream)) return s;
+        if (vt_status s = map_rows<T>(&ma, dy, dy_stride, rows, outs, 128)) return s;
+        if (vt_status s = map_rows<T>(&mb, w, w_stride, outs, cols, 64)) return s;
+        a.m = rows;
+        a.k = outs;
+        a.m_tiles = (uint32_t)((rows + 255u) / 256u);
+        a.chunks = a.chunks_a_split = (outs + 63u) / 64u;
+        a.splits = 1;
+        a.out = dz;
+        a.out_wide = cols % 16u == 0 && aligned32(dz);
+        if (vt_status s = launch_wide<T, ACT, true>(ma, mb, a, sms, stream)) return s;
+    }
+    if (dw) {
+        T *h = (T *)(workspace + p.h_at);
+        const uint32_t pitch = (uint32_t)align_up(cols, 8);
+        const uint64_t want = (rows * a.blocks * 4u + 255u) / 256u;
+        activate_kernel<T, ACT><<<(unsigned)(want < sms * 32u ? want : sms * 32u), 256, 0, stream>>>(codes, exps, rows, a.blocks, pitch, h);
+        if (vt_status s = check_launch("activate_kernel")) return s;
+        if (vt_status s = map_rows<T>(&ma, dy, dy_stride, rows, outs, 64)) return s;
+        if (vt_status s = map_rows<T>(&mb, h, pitch, rows, cols, 64)) return s;
+        a.m = outs;
+        a.k = rows;
+        a.m_tiles = (outs + 255u) / 256u;
+        a.chunks = (uint32_t)((rows + 63u) / 64u);
+        a.chunks_a_split = p.chunks_a_split;
+        a.splits = p.splits;
+        a.out = dw;
+        a.parts = (float *)(workspace + p.dw_at);
+        a.out_wide = cols % 16u == 0 && aligned32(dw);
+        if (vt_status s = launch_wide<T, ACT_IDENTITY, false>(ma, mb, a, sms, stream)) return s;
+        if (p.splits > 1) {
+            const uint64_t n = (uint64_t)outs * cols, blocks = (n + 255u) / 256u;
+            add_parts_kernel<T><<<(unsigned)(blocks < sms * 8u ? blocks : sms * 8u), 256, 0, stream>>>(a.parts, p.splits, n, (T *)dw);
+            if (vt_status s = check_launch("add_parts_kernel")) return s;
+        }
+    }
+    if (db) {
+        float *parts = (float *)(workspace + p.db_at);
+        column_parts_kernel<T><<<dim3((outs + 255u) / 256u, p.sum_parts), 256, 0, stream>>>((const T *)dy, rows, outs, dy_stride, parts);
+        add_parts_kernel<T><<<(outs + 255u) / 256u, 256, 0, stream>>>(parts, p.sum_parts, outs, (T *)db);
+        if (vt_status s = check_launch("column_parts_kernel")) return s;
+    }
+    return VT_OK;
+}
+
 template <typename T>
 static vt_status zero(T *p, uint64_t n, cudaStream_t stream)
 {
@@ -513,8 +859,9 @@ static vt_status zero(T *p, uint64_t n, cudaStream_t stream)
 
 extern "C" uint64_t vt_mx8_linear_bwd_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs)
 {
-    if (rows == 0 || cols == 0 || outs == 0 || outs > vt::NARROW_OUTS) return 0;
-    return vt::narrow_plan(rows, cols, outs, (uint32_t)vt::sm_count()).bytes;
+    if (rows == 0 || cols == 0 || outs == 0) return 0;
+    const uint32_t sms = (uint32_t)vt::sm_count();
+    return outs <= vt::NARROW_OUTS ? vt::narrow_plan(rows, cols, outs, sms).bytes : vt::wide_plan(rows, cols, outs, sms).bytes;
 }
 
 extern "C" vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const void *weight, uint64_t weight_stride,
@@ -531,6 +878,7 @@ extern "C" vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const
             if (vt_status s = vt::zero((T *)dz, rows * cols, st)) return s;
             if (vt_status s = vt::zero((T *)dw, (uint64_t)outs * cols, st)) return s;
             if (rows == 0 || outs == 0) return vt::zero((T *)db, outs, st);
+            if (!db) return VT_OK;
         }
         VT_REQUIRE(dy && (cols == 0 || (weight && codes && exps)), "vt_mx8_linear_bwd: null pointer");
         VT_REQUIRE(dy_stride >= outs && weight_stride >= cols,
@@ -538,26 +886,17 @@ extern "C" vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const
         VT_REQUIRE(vt::aligned32(codes), "vt_mx8_linear_bwd: codes must be 32-byte aligned");
         VT_REQUIRE(workspace_bytes >= vt_mx8_linear_bwd_workspace_bytes(rows, cols, outs) && vt::aligned16(workspace),
                    "vt_mx8_linear_bwd: workspace too small or not 16-byte aligned");
+        if (cols == 0) {  // a layer without inputs has the bias alone
+            vt::column_sum_kernel<T><<<outs, 256, 0, st>>>((const T *)dy, rows, outs, dy_stride, (T *)db);
+            return vt::check_launch("column_sum_kernel");
+        }
         return vt::with_act(act, [&](auto a) -> vt_status {
             constexpr int ACT = decltype(a)::value;
-            if (cols && outs <= vt::NARROW_OUTS)
+            if (outs <= vt::NARROW_OUTS)
                 return vt::run_narrow<T, ACT>(dy, dy_stride, weight, weight_stride, rows, cols, outs, codes, exps, dz, dw, db,
                                               (uint8_t *)workspace, err, st);
-            const vt::Checkpoint8<ACT> ckpt{codes, exps, vt::mx_blocks(cols)};
-            if (dz && cols) {
-                const dim3 grid((unsigned)((rows + 63) / 64), (cols + 63) / 64);
-                vt::tile_product_kernel<<<grid, 256, 0, st>>>(
-                    rows, cols, (uint64_t)outs, vt::Rows<T, true>{(const T *)dy, dy_stride},
-                    vt::Rows<T, false>{(const T *)weight, weight_stride}, vt::StoreDz<T, ACT>{ckpt, (T *)dz, cols});
-            }
-            if (dw && cols) {
-                const dim3 grid((outs + 63) / 64, (cols + 63) / 64);
-                vt::tile_product_kernel<<<grid, 256, 0, st>>>(
-                    (uint64_t)outs, cols, rows, vt::Rows<T, false>{(const T *)dy, dy_stride}, ckpt,
-                    vt::StoreY<T, vt::ACT_IDENTITY>{(T *)dw, nullptr, cols});
-            }
-            if (db) vt::column_sum_kernel<T><<<outs, 256, 0, st>>>((const T *)dy, rows, outs, dy_stride, (T *)db);
-            return vt::check_launch("vt_mx8_linear_bwd");
+            return vt::run_wide<T, ACT>(dy, dy_stride, weight, weight_stride, rows, cols, outs, codes, exps, dz, dw, db,
+                                        (uint8_t *)workspace, err, st);
         });
     });
 }
