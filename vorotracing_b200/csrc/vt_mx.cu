@@ -105,18 +105,22 @@ __global__ void __launch_bounds__(256) mx8_checkpoint_kernel(MxShape s, const T 
             make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
         if ((t & 3u) == 0) exps[t >> 2] = (uint8_t)E;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_value<ACT>(v[i]);
+        for (int i = 0; i < 8; i += 2) {
+            const float2 a = unpair(act_value2<ACT>(pair(v[i], v[i + 1])));
+            v[i] = a.x;
+            v[i + 1] = a.y;
+        }
         mx_store(s, it, h, v);
     }
 }
 
-__device__ __forceinline__ void mx8_values(const int8_t *codes, const uint8_t *exps, uint64_t t, float *v)
+// The four pairs of values of item t
+__device__ __forceinline__ void mx8_values(const int8_t *codes, const uint8_t *exps, uint64_t t, f32x2 *v)
 {
     const uint2 c = __ldg(reinterpret_cast<const uint2 *>(codes) + t);
-    const float sc = mx8_scale(__ldg(exps + (t >> 2)));
+    const f32x2 sc = both(mx8_scale(__ldg(exps + (t >> 2))));
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v[i] = (float)(int8_t)((i < 4 ? c.x : c.y) >> (i % 4 * 8)) * sc;
+    for (int i = 0; i < 4; ++i) v[i] = mul2(code_pair((i < 2 ? c.x : c.y) ^ 0x80808080u, i % 2 * 2), sc);
 }
 
 template <typename T, int ACT>
@@ -127,11 +131,16 @@ __global__ void __launch_bounds__(256) mx8_act_bwd_kernel(MxShape s, const T *__
     const uint64_t items = s.items();
     for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; t < items; t += (uint64_t)gridDim.x * 256u) {
         const MxItem it = mx_item(s, t);
-        float v[8], g[8];
+        float g[8];
+        f32x2 v[4];
         mx_load(s, it, dh, s.in_stride, g);
         mx8_values(codes, exps, t, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] *= act_slope<ACT>(v[i]);
+        for (int i = 0; i < 4; ++i) {
+            const float2 a = unpair(mul2(pair(g[2 * i], g[2 * i + 1]), act_slope2<ACT>(v[i])));
+            g[2 * i] = a.x;
+            g[2 * i + 1] = a.y;
+        }
         mx_store(s, it, dz, g);
     }
 }
@@ -142,8 +151,15 @@ __global__ void __launch_bounds__(256) mx8_dequantize_kernel(MxShape s, const in
 {
     const uint64_t items = s.items();
     for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; t < items; t += (uint64_t)gridDim.x * 256u) {
+        f32x2 p[4];
         float v[8];
-        mx8_values(codes, exps, t, v);
+        mx8_values(codes, exps, t, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 a = unpair(p[i]);
+            v[2 * i] = a.x;
+            v[2 * i + 1] = a.y;
+        }
         mx_store(s, mx_item(s, t), out, v);
     }
 }

@@ -41,6 +41,45 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
     return __float2bfloat16_rn(v);
 }
 
+// ---- pairs of binary32 values in one 64-bit register ----
+//
+// sm_100 adds and multiplies two at once, which halves the instructions of the activations; they
+// share the issue slots with conversions and shared-memory traffic and are what the fused kernels
+// spend most of them on.
+
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float x, float y)
+{
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 both(float x) { return pair(x, x); }
+
 // 8 values of a row, as 16-byte words (one, or two for binary32)
 template <typename T> struct Vec8 {
     static constexpr int WORDS = sizeof(T) * 8 / 16;
@@ -95,6 +134,11 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
 {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(f32x2 v)
+{
+    const float2 x = unpair(v);
+    return pack2<T>(x.x, x.y);
 }
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w)
@@ -171,62 +215,88 @@ __device__ __forceinline__ float mx4_value(uint32_t nibble)
 
 // ---- activations (binary32 throughout; the caller rounds once) ----
 
-__device__ __forceinline__ float logistic(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
-
-// gelu_tanh(x) = x logistic(c (x + 0.044715 x^3)), c = 2 sqrt(2 / pi).  Outside [-15, 15] the
-// logistic is 0 or 1 in binary32; the bound keeps x^3 finite.  A NaN passes both comparisons.
-constexpr float GELU_C = 1.5957691216057308f, GELU_A = 0.044715f;
-__device__ __forceinline__ float gelu_clip(float x)
+__device__ __forceinline__ float exp2_approx(float x)  // within 2^-22 of 2^x, relative
 {
-    return x > 15.0f ? 15.0f : x < -15.0f ? -15.0f : x;
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_approx(float x)  // within 1 ulp
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b)  // a NaN stays one
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// 1 / (1 + 2^x): the logistic of -x ln 2
+__device__ __forceinline__ f32x2 logistic2(f32x2 x)
+{
+    const float2 a = unpair(x);
+    const float2 b = unpair(add2(pair(exp2_approx(a.x), exp2_approx(a.y)), both(1.0f)));
+    return pair(reciprocal_approx(b.x), reciprocal_approx(b.y));
 }
 
-template <int ACT> __device__ __forceinline__ float act_value(float x)
+// gelu_tanh(x) = x logistic(c (x + a x^3)), c = 2 sqrt(2 / pi), a = 0.044715.  Outside [-15, 15]
+// the logistic is 0 or 1 in binary32; the bound keeps x^3 finite.
+constexpr float GELU_C = 1.5957691216057308f, GELU_A = 0.044715f, LOG2_E = 1.4426950408889634f;
+
+// Value and slope of the activation of two numbers; what is not wanted is not computed.
+template <int ACT, bool VALUE, bool SLOPE>
+__device__ __forceinline__ void act_pair(f32x2 x, f32x2 &value, f32x2 &slope)
 {
     if constexpr (ACT == ACT_RELU) {
-        return x < 0.0f ? 0.0f : x;  // a NaN stays one
+        const float2 v = unpair(x);
+        value = pair(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
+        if constexpr (SLOPE)  // x * 0 hands a NaN on
+            slope = pair(v.x > 0.0f ? 1.0f : v.x * 0.0f, v.y > 0.0f ? 1.0f : v.y * 0.0f);
     } else if constexpr (ACT == ACT_SILU) {
-        return x * logistic(x);
+        const f32x2 p = logistic2(mul2(x, both(-LOG2_E)));
+        value = mul2(x, p);
+        if constexpr (SLOPE) slope = fma2(value, fma2(p, both(-1.0f), both(1.0f)), p);
     } else if constexpr (ACT == ACT_GELU) {
-        const float c = gelu_clip(x);
-        return x * logistic(GELU_C * c * fmaf(GELU_A * c, c, 1.0f));
+        const float2 v = unpair(x);
+        const f32x2 c = pair(min_nan(max_nan(v.x, -15.0f), 15.0f), min_nan(max_nan(v.y, -15.0f), 15.0f));
+        const f32x2 cc = mul2(c, c);
+        const f32x2 p = logistic2(mul2(c, fma2(cc, both(-LOG2_E * GELU_C * GELU_A), both(-LOG2_E * GELU_C))));
+        if constexpr (VALUE) value = mul2(x, p);
+        if constexpr (SLOPE)
+            slope = fma2(mul2(mul2(c, p), fma2(p, both(-1.0f), both(1.0f))), fma2(cc, both(3.0f * GELU_C * GELU_A), both(GELU_C)), p);
     } else {
-        return x;
+        value = x;
+        slope = both(1.0f);
     }
 }
-
-template <int ACT> __device__ __forceinline__ float act_slope(float x)
+template <int ACT> __device__ __forceinline__ f32x2 act_value2(f32x2 x)
 {
-    if constexpr (ACT == ACT_RELU) {
-        return x > 0.0f ? 1.0f : x <= 0.0f ? 0.0f : x;
-    } else if constexpr (ACT == ACT_SILU) {
-        const float p = logistic(x);
-        return fmaf(x * p, 1.0f - p, p);
-    } else if constexpr (ACT == ACT_GELU) {
-        const float c = gelu_clip(x), cc = c * c;
-        const float p = logistic(GELU_C * c * fmaf(GELU_A, cc, 1.0f));
-        return fmaf(c * p, (1.0f - p) * GELU_C * fmaf(3.0f * GELU_A, cc, 1.0f), p);
-    } else {
-        return 1.0f;
-    }
+    f32x2 v, s;
+    act_pair<ACT, true, false>(x, v, s);
+    return v;
+}
+template <int ACT> __device__ __forceinline__ f32x2 act_slope2(f32x2 x)
+{
+    f32x2 v, s;
+    act_pair<ACT, false, true>(x, v, s);
+    return s;
 }
 
-// Both at once; one logistic serves both.
-template <int ACT> __device__ __forceinline__ void act_both(float x, float &value, float &slope)
+// Two of a word's four 8-bit codes (bytes i and i + 1, sign bits turned) as numbers: a turned
+// byte under the exponent of 2^23 is 2^23 + 128 + code.
+__device__ __forceinline__ f32x2 code_pair(uint32_t turned, int i)
 {
-    if constexpr (ACT == ACT_SILU) {
-        const float p = logistic(x);
-        value = x * p;
-        slope = fmaf(value, 1.0f - p, p);
-    } else if constexpr (ACT == ACT_GELU) {
-        const float c = gelu_clip(x), cc = c * c;
-        const float p = logistic(GELU_C * c * fmaf(GELU_A, cc, 1.0f));
-        value = x * p;
-        slope = fmaf(c * p, (1.0f - p) * GELU_C * fmaf(3.0f * GELU_A, cc, 1.0f), p);
-    } else {
-        value = act_value<ACT>(x);
-        slope = act_slope<ACT>(x);
-    }
+    return add2(pair(__uint_as_float(__byte_perm(turned, 0x4b000000u, 0x7440u | i)),
+                     __uint_as_float(__byte_perm(turned, 0x4b000000u, 0x7440u | (i + 1)))),
+                both(-8388736.0f));
 }
 
 // ---- dispatch: one instantiation per activation / type ----

@@ -35,7 +35,7 @@ template <int TN, bool QUANT> struct L4 {
         uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS];
         uint32_t tmem;
         tc::Fail fail;
-        float bias[TN];
+        alignas(8) float bias[TN];
     };
     static constexpr uint32_t CTRL_AT = STAGES * STAGE, SMEM = CTRL_AT + sizeof(Ctrl);
     static_assert(SMEM <= 232448 && SF_AT + SF_COLS <= 512, "does not fit an SM");
@@ -189,8 +189,8 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
                 }
 #pragma unroll
                 for (uint32_t i = 0; i < 16; ++i)
-                    w[i] = pack2<T>(act_value<ACT>(__uint_as_float(v[2 * i]) + s.bias[n0 + 2 * i]),
-                                    act_value<ACT>(__uint_as_float(v[2 * i + 1]) + s.bias[n0 + 2 * i + 1]));
+                    w[i] = pack2<T>(act_value2<ACT>(add2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])),
+                                                         *reinterpret_cast<const f32x2 *>(&s.bias[n0 + 2 * i]))));
                 if (row < a.rows) store_row32<T>((T *)a.y + row * a.outs, out0 + n0, a.outs, a.y_wide, w);
             }
             acc.next(P::ACCS);
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
 template <typename T, int ACT> __global__ void bias_rows_kernel(const T *bias, uint64_t rows, uint32_t outs, T *y)
 {
     for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < rows * outs; i += (uint64_t)gridDim.x * 256u)
-        y[i] = from_f32<T>(act_value<ACT>(bias ? to_f32<T>(bias[i % outs]) : 0.0f));
+        y[i] = from_f32<T>(unpair(act_value2<ACT>(both(bias ? to_f32<T>(bias[i % outs]) : 0.0f))).x);
 }
 template <typename T, int ACT> static vt_status launch_bias(const L4Args &a, cudaStream_t stream)
 {

@@ -58,49 +58,23 @@ struct NarrowArgs {
     bool dz_wide;      // dz's rows hold whole 32-byte pieces
 };
 
-// Byte i (0..3) of a word of codes, as a float: the byte with its sign bit turned goes under
-// the exponent of 2^23, which makes 2^23 + 128 + code.
-__device__ __forceinline__ float code_float(uint32_t turned, int i)
-{
-    return __uint_as_float(__byte_perm(turned, 0x4b000000u, 0x7440u | i)) - 8388736.0f;
-}
-
-// One warp's 32 rows by 32 columns (one block a lane): g = dH in, h and dz out as packed 16-bit pairs.
-template <typename T, int ACT>
+// One row's block of 32 columns: g = dH (binary32) in, h and dz out as packed 16-bit pairs.
+template <typename T, int ACT, bool VALUE>
 __device__ __forceinline__ void transform_block(const uint32_t *codes, uint32_t E, const uint32_t *g, uint32_t *h, uint32_t *dz)
 {
-    const float sc = mx8_scale(E);
+    const f32x2 sc = both(mx8_scale(E));
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
         const uint32_t c = codes[w] ^ 0x80808080u;
-        float hv[4], gv[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float z = code_float(c, i) * sc;
-            float slope;
-            act_both<ACT>(z, hv[i], slope);
-            gv[i] = __uint_as_float(g[4 * w + i]) * slope;
+        for (int i = 0; i < 2; ++i) {
+            f32x2 v, slope;
+            act_pair<ACT, VALUE, true>(mul2(code_pair(c, 2 * i), sc), v, slope);
+            const int at = 2 * w + i;
+            if (VALUE) h[at] = pack2<T>(v);
+            const f32x2 gp = pair(__uint_as_float(g[2 * at]), __uint_as_float(g[2 * at + 1]));
+            dz[at] = pack2<T>(ACT == ACT_IDENTITY ? gp : mul2(gp, slope));
         }
-        h[2 * w] = pack2<T>(hv[0], hv[1]);
-        h[2 * w + 1] = pack2<T>(hv[2], hv[3]);
-        dz[2 * w] = pack2<T>(gv[0], gv[1]);
-        dz[2 * w + 1] = pack2<T>(gv[2], gv[3]);
-    }
-}
-
-// The same for dz alone.
-template <typename T, int ACT>
-__device__ __forceinline__ void slope_block(const uint32_t *codes, uint32_t E, const uint32_t *g, uint32_t *dz)
-{
-    const float sc = mx8_scale(E);
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        const uint32_t c = codes[w] ^ 0x80808080u;
-        float gv[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) gv[i] = __uint_as_float(g[4 * w + i]) * act_slope<ACT>(code_float(c, i) * sc);
-        dz[2 * w] = pack2<T>(gv[0], gv[1]);
-        dz[2 * w + 1] = pack2<T>(gv[2], gv[3]);
     }
 }
 
@@ -288,7 +262,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.dh_empty[dh.i]);
                 }
-                transform_block<T, ACT>(codes[j], E[j], g, hv, dz);
+                transform_block<T, ACT, true>(codes[j], E[j], g, hv, dz);
                 // activations: 64-byte piece of row in_tile in the swizzled chunk
                 uint8_t *p = smem + P::H_AT + h.i * P::H_BYTES + (NC == 2 ? half * 16384u : 0u) + in_tile * 128u;
                 const uint32_t unit = (NC == 2 ? j : half) * 4u;
@@ -531,7 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
                 }
                 if (row >= a.m) continue;
                 if (DZ) {
-                    slope_block<T, ACT>(codes, E, v, w);
+                    transform_block<T, ACT, false>(codes, E, v, nullptr, w);
                     store_row32<T>((T *)a.out + row * a.n, col, (uint32_t)a.n, a.out_wide, w);
                 } else if (a.splits > 1) {
                     float *p = a.parts + ((uint64_t)split * a.m + row) * a.n + col;
@@ -571,12 +545,12 @@ __global__ void __launch_bounds__(256) activate_kernel(const int8_t *__restrict_
         const uint32_t col = (uint32_t)(b - row * blocks) * 32u + (uint32_t)(i & 3u) * 8u;
         if (col >= pitch) continue;
         const uint2 c = __ldg(reinterpret_cast<const uint2 *>(codes) + i);
-        const float sc = mx8_scale(__ldg(exps + b));
+        const f32x2 sc = both(mx8_scale(__ldg(exps + b)));
         uint32_t w[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             const uint32_t x = (p < 2 ? c.x : c.y) ^ 0x80808080u;
-            w[p] = pack2<T>(act_value<ACT>(code_float(x, p % 2 * 2) * sc), act_value<ACT>(code_float(x, p % 2 * 2 + 1) * sc));
+            w[p] = pack2<T>(act_value2<ACT>(mul2(code_pair(x, p % 2 * 2), sc)));
         }
         *reinterpret_cast<uint4 *>(h + row * pitch + col) = make_uint4(w[0], w[1], w[2], w[3]);
     }
