@@ -434,8 +434,13 @@ VT_API vt_status vt_mx8_dequantize(const int8_t *codes, const uint8_t *exps, uin
                                    uint32_t cols, int dtype, void *out, vt_stream stream);
 /* Gradients of y = act(z) W^T + b, weight (outs, cols), from the 8-bit z:
  * dz (rows, cols) = (dy W) * act'(z8), dw (outs, cols) = dy^T act(z8),
- * db (outs) = column sums of dy.  Any output may be null. */
-VT_API uint64_t vt_mx8_linear_bwd_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs);
+ * db (outs) = column sums of dy.  Any output may be null.  copies: 1 if dy's
+ * rows do not start on 16 bytes (pointer or stride), plus 2 if the weight's do
+ * not; the workspace then has room for copies that do.  err gets VT_ERR_CUDA
+ * if a wait inside a kernel has run out (a second); the outputs are then not
+ * valid. */
+VT_API uint64_t vt_mx8_linear_bwd_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs,
+                                                  int copies);
 VT_API vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const void *weight,
                                    uint64_t weight_stride, int dtype, uint64_t rows, uint32_t cols,
                                    uint32_t outs, const int8_t *codes, const uint8_t *exps, int act,
@@ -449,8 +454,10 @@ VT_API vt_status vt_mx4_dequantize(const uint8_t *codes, const uint8_t *exps, ui
                                    uint32_t cols, int dtype, void *out, vt_stream stream);
 /* y (rows, outs) = act(q4(x) w4^T + bias): x (rows, cols) is rounded to 4 bits
  * on the way, codes / exps are the weight (outs, cols) in 4 bits, bias (outs)
- * may be null. */
-VT_API uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs);
+ * may be null.  copies: 1 if x's rows do not start on 16 bytes.  err as for
+ * vt_mx8_linear_bwd. */
+VT_API uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs,
+                                              int copies);
 VT_API vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, uint64_t rows,
                                uint32_t cols, uint32_t outs, const uint8_t *codes,
                                const uint8_t *exps, const void *bias, int act, void *y,

@@ -49,4 +49,9 @@ def test_workspace_sizes_cover_the_layout():
     n = mx._call("vt_mx4_linear_workspace_bytes")
     for rows, cols in ((1, 1), (77, 1000), (1 << 20, 192)):
         blocks = -(-cols // 32)
-        assert n(rows, cols, 8) >= rows * blocks * 17
+        assert n(rows, cols, 300, 0) >= rows * blocks * 17
+        assert n(rows, cols, 8, 0) == 0 and n(rows, cols, 8, 1) >= rows * cols * 2
+    n = mx._call("vt_mx8_linear_bwd_workspace_bytes")
+    for rows, cols, outs in ((1, 1, 1), (1000, 200, 77), (1000, 200, 777)):
+        assert n(rows, cols, outs, 1) - n(rows, cols, outs, 0) >= rows * outs * 2
+        assert n(rows, cols, outs, 2) - n(rows, cols, outs, 0) >= cols * outs * 2

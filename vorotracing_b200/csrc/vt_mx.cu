@@ -174,10 +174,10 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(MxShape s, const T *_
         mx_load(s, mx_item(s, t), x, s.in_stride, v);
         const uint32_t E = mx4_exponent(block_top(v));
         const float inv = mx4_inverse(E == 255u ? 1u : E);
-        uint32_t c = 0;
+        f32x2 p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c |= mx4_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
-        codes[t] = E == 255u ? 0u : c;
+        for (int i = 0; i < 4; ++i) p[i] = mul2(pair(v[2 * i], v[2 * i + 1]), both(inv));
+        codes[t] = E == 255u ? 0u : mx4_word(p);
         if ((t & 3u) == 0) exps[t >> 2] = (uint8_t)E;
     }
 }

@@ -140,6 +140,13 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(f32x2 v)
     const float2 x = unpair(v);
     return pack2<T>(x.x, x.y);
 }
+// Binary32 bits of the larger magnitude of two 16-bit numbers whose sign bits are clear
+template <typename T> __device__ __forceinline__ uint32_t top_of_pair(uint32_t w);
+template <> __device__ __forceinline__ uint32_t top_of_pair<__half>(uint32_t w)
+{
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(w & 0xffffu, w >> 16))));
+}
+template <> __device__ __forceinline__ uint32_t top_of_pair<__nv_bfloat16>(uint32_t w) { return max(w << 16, w & 0xffff0000u); }
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w)
 {
@@ -198,12 +205,16 @@ __device__ __forceinline__ int mx8_code(float x, float inverse)
 {
     return __float2int_rn(fminf(fmaxf(x * inverse, -127.0f), 127.0f));
 }
-// Two e2m1 codes in a byte, `lo` in the low nibble; rounds to nearest even and saturates.
-__device__ __forceinline__ uint32_t mx4_pair(float lo, float hi)
+// Eight e2m1 codes in a word, the first in the lowest nibble; rounds to nearest even and saturates.
+__device__ __forceinline__ uint32_t mx4_word(const f32x2 *v)
 {
+    const float2 a = unpair(v[0]), b = unpair(v[1]), c = unpair(v[2]), d = unpair(v[3]);
     uint32_t r;
-    asm("{\n.reg .b8 t;\ncvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\ncvt.u32.u8 %0, t;\n}" : "=r"(r)
-        : "f"(hi), "f"(lo));
+    asm("{\n.reg .b8 p, q, r, s;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 p, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 q, %4, %3;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 r, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 s, %8, %7;\n"
+        "mov.b32 %0, {p, q, r, s};\n}"
+        : "=r"(r) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y), "f"(d.x), "f"(d.y));
     return r;
 }
 // e2m1 magnitudes doubled are 0 1 2 3 4 6 8 12

@@ -6,12 +6,13 @@
 // thread issues copies and products; four warps take finished accumulators out of tensor memory,
 // add the bias, apply the activation and round once.
 //
-// x is rounded to 4 bits inside the same kernel while one tile spans all outputs (QUANT): eight
-// warps read x, which is then read from HBM once and nothing of its 4-bit form is written.
+// x is rounded to 4 bits inside the same kernel while one tile spans all outputs (QUANT): TMA
+// brings x in as it is, deep enough ahead to keep HBM busy (112 to 128 KB), and eight warps round
+// it, a lane a block of 32 columns, into the operand's place.  x is then read from HBM once and
+// nothing of its 4-bit form is written.
 // With more outputs the same rows would be rounded again for every tile of outputs, so a pass of
 // its own writes codes and scales first, 17/32 byte a value, and TMA brings them in.
-#include "vt_mx.cuh"
-#include "vt_tc.cuh"
+#include "vt_mx_rows.cuh"
 
 namespace vt {
 
@@ -22,36 +23,35 @@ template <int TN, bool QUANT> struct L4 {
     static constexpr uint32_t B_PARTS = TN > 128 ? TN / 128 : 1;  // groups of 128 rows of scales
     static constexpr uint32_t SF_BYTES = (1u + B_PARTS) * 1024u;
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SF_BYTES;
-    static constexpr uint32_t STAGES = TN == 256 ? 4 : 5;
+    static constexpr uint32_t STAGES = QUANT ? (TN == 256 ? 2 : 3) : 4;
+    static constexpr uint32_t X_BYTES = L4_ROWS * 128u, X_STAGES = QUANT ? (TN == 64 ? 8 : 7) : 0;  // 64 columns of x each
     // two accumulators when they leave room for the scales
     static constexpr uint32_t ACCS = TN == 256 ? 1 : 2;
     static constexpr uint32_t SF_AT = ACCS * TN, SF_COLS = 8u + 8u * B_PARTS;
     static constexpr uint32_t TMEM = SF_AT + SF_COLS <= 256 ? 256 : 512;
     static constexpr uint32_t SCALE_WARPS = 4, QUANT_WARPS = QUANT ? 8 : 0;
-    // warps: 0 TMA, 1 products, 2 and 3 none, 4..7 results, 8..11 scales, 12.. x to 4 bits
+    // warps: 0 TMA, 1 products, 2 TMA of x, 3 none, 4..7 results, 8..11 scales, 12.. x to 4 bits
     static constexpr uint32_t THREADS = 32u * (8u + SCALE_WARPS + QUANT_WARPS);
     static constexpr uint32_t FULL_COUNT = 1u + SCALE_WARPS + QUANT_WARPS;
     struct Ctrl {
-        uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS];
+        uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS], x_full[X_STAGES + 1], x_empty[X_STAGES + 1];
         uint32_t tmem;
         tc::Fail fail;
         alignas(8) float bias[TN];
     };
-    static constexpr uint32_t CTRL_AT = STAGES * STAGE, SMEM = CTRL_AT + sizeof(Ctrl);
+    static constexpr uint32_t X_AT = STAGES * STAGE, CTRL_AT = X_AT + X_STAGES * X_BYTES, SMEM = CTRL_AT + sizeof(Ctrl);
     static_assert(SMEM <= 232448 && SF_AT + SF_COLS <= 512, "does not fit an SM");
 };
 
 struct L4Args {
-    uint64_t rows, x_stride;
+    uint64_t rows;
     uint32_t cols, outs, blocks, chunks, row_tiles, out_tiles;
-    uint32_t lanes_shift;  // QUANT: log2 of the lanes that share a row's part of a stage
-    const void *x;         // QUANT
-    const uint8_t *x_exps; // not QUANT
+    const uint8_t *x_exps;  // not QUANT
     const uint8_t *w_exps;
     const void *bias;
     void *y;
     uint32_t *err;
-    bool x_vec, y_wide;
+    bool y_wide;
 };
 
 // The scales of 8 blocks of a row, zeros (which multiply zero codes) behind its end.
@@ -88,10 +88,14 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             tc::mbar_init(&s.acc_full[i], 1);
             tc::mbar_init(&s.acc_empty[i], 4);
         }
+        for (uint32_t i = 0; i < P::X_STAGES; ++i) {
+            tc::mbar_init(&s.x_full[i], 1);
+            tc::mbar_init(&s.x_empty[i], P::QUANT_WARPS);
+        }
         s.fail.failed = 0;
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&w_map);
-        if (!QUANT) tc::tma_prefetch_map(&x_map);
+        tc::tma_prefetch_map(&x_map);
     }
     if (warp == 1) tc::tmem_alloc<P::TMEM>(&s.tmem);
     tc::fence_before();
@@ -102,7 +106,6 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
     if (warp == 0) {
         if (lane == 0) {  // TMA
             tc::Ring r;
-            uint32_t issued = 0;
             bool ok = true;
             for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
                 const int row0 = (int)(t / a.out_tiles * L4_ROWS), out0 = (int)(t % a.out_tiles * TN);
@@ -113,7 +116,6 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
                     tc::mbar_arrive_tx(&s.full[r.i], P::B_BYTES + (QUANT ? 0u : P::A_BYTES));
                     if (!QUANT) tc::tma_load_2d(st, &x_map, (int)(c * 128u), row0, &s.full[r.i]);
                     tc::tma_load_2d(st + P::A_BYTES, &w_map, (int)(c * 128u), out0, &s.full[r.i]);
-                    ++issued;
                     r.next(P::STAGES);
                 }
             }
@@ -223,56 +225,71 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
                 r.next(P::STAGES);
             }
         }
-    } else if (QUANT && warp >= 12) {  // x to 4 bits: 8 columns a lane, 4 lanes a block
-        const uint32_t q = warp - 12u, per = a.lanes_shift, rows_at_once = 32u >> per;
-        const uint32_t in_row = lane & ((1u << per) - 1u), first = (q << (5u - per)) + (lane >> per);
-        const uint32_t groups = 16u >> (5u - per);  // passes of 8 warps over the tile's 128 rows: 4, 8 or 16
-        tc::Ring r;
+    } else if (QUANT && warp == 2) {
+        if (lane == 0) {  // TMA of x, 64 columns at a time
+            tc::Ring r;
+            uint32_t issued = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+                for (uint32_t col = 0; col < a.cols; col += 64u) {
+                    ok = tc::mbar_wait(&s.x_empty[r.i], r.phase ^ 1u, fail, a.err);
+                    if (!ok) break;
+                    tc::mbar_arrive_tx(&s.x_full[r.i], P::X_BYTES);
+                    tc::tma_load_2d(smem + P::X_AT + r.i * P::X_BYTES, &x_map, (int)col, (int)(t / a.out_tiles * L4_ROWS),
+                                    &s.x_full[r.i]);
+                    ++issued;
+                    r.next(P::X_STAGES);
+                }
+            if (s.fail.failed)  // leave no copy in flight
+                for (uint32_t i = 0; i < P::X_STAGES && i < issued; ++i)
+                    tc::mbar_wait_slow(&s.x_full[i], ((issued - 1 - i) / P::X_STAGES) & 1u, fail, a.err, true);
+        }
+    } else if (QUANT && warp >= 12) {  // x to 4 bits: a lane has a row, each half of the warps one of a chunk's two blocks
+        const uint32_t row = warp % 4u * 32u + lane, part = (warp - 12u) / 4u;
+        tc::Ring r, x;
         bool ok = true;
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const uint64_t row0 = (uint64_t)(t / a.out_tiles) * L4_ROWS;
-            for (uint32_t c = 0; c < a.chunks; ++c) {
-                const uint32_t col = c * L4_K + in_row * 8u;
-                const uint32_t n = col >= a.cols ? 0u : min(8u, a.cols - col);
+            for (uint32_t c = 0; c < a.chunks && ok; ++c) {
                 ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
                 if (!ok) break;
-                uint8_t *st = smem + r.i * P::STAGE, *sf = st + P::A_BYTES + P::B_BYTES;
-#pragma unroll 1
-                for (uint32_t g = 0; g < groups; g += 4u) {
-                    Vec8<T> x[4];
+                uint8_t *st = smem + r.i * P::STAGE, *sf = st + P::A_BYTES + P::B_BYTES + scale_place(row);
+                const uint32_t steps = min(4u, (a.cols - c * L4_K + 63u) / 64u);
+                for (uint32_t k = 0; k < steps; ++k) {
+                    ok = __all_sync(~0u, tc::mbar_wait(&s.x_full[x.i], x.phase, fail, a.err));
+                    if (!ok) break;
+                    const uint8_t *from = smem + P::X_AT + x.i * P::X_BYTES + row * 128u;
+                    uint4 w[4];
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const uint4 *>(from + (((part * 4u + u) ^ (row & 7u)) << 4));
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s.x_empty[x.i]);
+                    x.next(P::X_STAGES);
+                    uint32_t top = 0;
 #pragma unroll
                     for (uint32_t u = 0; u < 4; ++u) {
-                        const uint64_t row = row0 + first + (g + u) * 8u * rows_at_once;
-                        const bool in = row < a.rows && n;
-                        const T *p = (const T *)a.x + row * a.x_stride + col;
-                        if (in && a.x_vec) {
-                            x[u].load(p);
-                        } else {
-                            x[u].zero();
-                            if (in)
-                                for (uint32_t i = 0; i < n; ++i) reinterpret_cast<T *>(x[u].w)[i] = __ldg(p + i);
+                        top = __vmaxu2(top, w[u].x & 0x7fff7fffu);
+                        top = __vmaxu2(top, w[u].y & 0x7fff7fffu);
+                        top = __vmaxu2(top, w[u].z & 0x7fff7fffu);
+                        top = __vmaxu2(top, w[u].w & 0x7fff7fffu);
+                    }
+                    const uint32_t E = mx4_exponent(top_of_pair<T>(top));
+                    const f32x2 inv = both(E == 255u ? 0.0f : mx4_inverse(E));
+                    uint32_t codes[4];
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        const uint32_t in[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+                        f32x2 v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = unpack2<T>(in[i]);
+                            v[i] = mul2(pair(f.x, f.y), inv);
                         }
+                        codes[u] = mx4_word(v);
                     }
-#pragma unroll
-                    for (uint32_t u = 0; u < 4; ++u) {
-                        const uint32_t row = first + (g + u) * 8u * rows_at_once;
-                        float v[8];
-                        x[u].unpack(v);
-                        uint32_t top = 0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-                        top = max(top, __shfl_xor_sync(~0u, top, 1));
-                        top = max(top, __shfl_xor_sync(~0u, top, 2));
-                        const uint32_t E = mx4_exponent(top);
-                        const float inv = mx4_inverse(E == 255u ? 1u : E);
-                        uint32_t codes = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) codes |= mx4_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
-                        const uint32_t block = in_row >> 2;
-                        *reinterpret_cast<uint32_t *>(st + row * 128u + ((block ^ (row & 7u)) << 4) + (in_row & 3u) * 4u) =
-                            E == 255u ? 0u : codes;
-                        if ((in_row & 3u) == 0) sf[scale_place(row) + (block >> 2) * 512u + (block & 3u)] = (uint8_t)E;
-                    }
+                    const uint32_t block = k * 2u + part;
+                    *reinterpret_cast<uint4 *>(st + row * 128u + ((block ^ (row & 7u)) << 4)) =
+                        make_uint4(codes[0], codes[1], codes[2], codes[3]);
+                    sf[(block >> 2) * 512u + (block & 3u)] = (uint8_t)E;
                 }
                 tc::fence_async_shared();
                 __syncwarp();
@@ -299,14 +316,17 @@ template <typename T, int ACT> static vt_status launch_bias(const L4Args &a, cud
 }
 
 template <typename T, int ACT, int TN, bool QUANT>
-static vt_status launch_linear4(const uint8_t *x_codes, const uint8_t *w_codes, L4Args a, cudaStream_t stream)
+static vt_status launch_linear4(const void *x, uint64_t x_stride, const uint8_t *w_codes, L4Args a, cudaStream_t stream)
 {
     static std::atomic<uint64_t> allowed{0};
     using P = L4<TN, QUANT>;
-    CUtensorMap x_map = {}, w_map;
+    CUtensorMap x_map, w_map;
     const uint64_t pitch = (uint64_t)a.blocks * 16u;
-    if (!QUANT)
-        if (vt_status s = tc::make_map(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, x_codes, a.rows, pitch, pitch, L4_ROWS, 128)) return s;
+    if (QUANT) {  // x itself
+        if (vt_status s = map_rows<T>(&x_map, x, x_stride, a.rows, a.cols, L4_ROWS)) return s;
+    } else {  // its codes
+        if (vt_status s = tc::make_map(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, a.rows, pitch, pitch, L4_ROWS, 128)) return s;
+    }
     if (vt_status s = tc::make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w_codes, a.outs, pitch, pitch, TN, 128)) return s;
     if (vt_status s = tc::allow_smem(linear4_kernel<T, ACT, TN, QUANT>, P::SMEM, allowed)) return s;
     a.row_tiles = (uint32_t)((a.rows + L4_ROWS - 1u) / L4_ROWS);
@@ -319,11 +339,12 @@ static vt_status launch_linear4(const uint8_t *x_codes, const uint8_t *w_codes, 
 
 }  // namespace vt
 
-extern "C" uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs)
+// copies: x's rows do not start on 16 bytes
+extern "C" uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs, int copies)
 {
-    if (outs <= 256u) return 0;  // x is rounded inside the kernel
     const uint64_t blocks = vt::mx_blocks(cols);
-    return rows * blocks * 16u + (rows * blocks + 15u) / 16u * 16u;
+    if (outs <= 256u) return copies ? rows * vt::align_up(cols, 8) * 2u : 0;  // x is rounded inside the kernel
+    return rows * blocks * 16u + vt::align_up(rows * blocks, 16);
 }
 
 extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, uint64_t rows, uint32_t cols,
@@ -337,39 +358,40 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
     VT_REQUIRE(y && (cols == 0 || (x && codes && exps)), "vt_mx4_linear: null pointer");
     VT_REQUIRE(x_stride >= cols, "vt_mx4_linear: the row stride is less than a row");
     VT_REQUIRE(vt::aligned16(codes), "vt_mx4_linear: codes must be 16-byte aligned");
-    VT_REQUIRE(workspace_bytes >= vt_mx4_linear_workspace_bytes(rows, cols, outs) && vt::aligned16(workspace),
-               "vt_mx4_linear: workspace too small or not 16-byte aligned");
     cudaStream_t st = (cudaStream_t)stream;
     return vt::with_type16(dtype, [&](auto ty) -> vt_status {
         using T = typename decltype(ty)::type;
+        VT_REQUIRE(workspace_bytes >= vt_mx4_linear_workspace_bytes(rows, cols, outs, !vt::whole_words<T>(x, x_stride)) &&
+                       vt::aligned16(workspace),
+                   "vt_mx4_linear: workspace too small or not 16-byte aligned");
         vt::L4Args a = {};
         a.rows = rows;
-        a.x_stride = x_stride;
         a.cols = cols;
         a.outs = outs;
         a.blocks = vt::mx_blocks(cols);
         a.chunks = (cols + vt::L4_K - 1u) / vt::L4_K;
-        a.lanes_shift = cols <= 64u ? 3u : cols <= 128u ? 4u : 5u;
-        a.x = x;
         a.w_exps = exps;
         a.bias = bias;
         a.y = y;
         a.err = err;
-        a.x_vec = cols % 8u == 0 && x_stride % 8u == 0 && vt::aligned16(x);
         a.y_wide = outs % 16u == 0 && vt::aligned32(y);
         if (cols == 0) return vt::with_act(act, [&](auto f) { return vt::launch_bias<T, decltype(f)::value>(a, st); });
-        uint8_t *x_codes = (uint8_t *)workspace;
-        if (outs > 256u) {
-            uint8_t *x_exps = x_codes + rows * a.blocks * 16u;
-            if (vt_status s = vt_mx4_quantize(x, dtype, rows, cols, x_stride, x_codes, x_exps, stream)) return s;
-            a.x_exps = x_exps;
+        if (outs <= 256u) {
+            const void *from = x;
+            uint64_t stride = x_stride;
+            if (vt_status s = vt::whole_rows<T>(from, stride, rows, cols, workspace, st)) return s;
+            return vt::with_act(act, [&](auto f) -> vt_status {
+                constexpr int ACT = decltype(f)::value;
+                if (outs <= 64u) return vt::launch_linear4<T, ACT, 64, true>(from, stride, codes, a, st);
+                if (outs <= 128u) return vt::launch_linear4<T, ACT, 128, true>(from, stride, codes, a, st);
+                return vt::launch_linear4<T, ACT, 256, true>(from, stride, codes, a, st);
+            });
         }
+        uint8_t *x_codes = (uint8_t *)workspace, *x_exps = x_codes + rows * a.blocks * 16u;
+        if (vt_status s = vt_mx4_quantize(x, dtype, rows, cols, x_stride, x_codes, x_exps, stream)) return s;
+        a.x_exps = x_exps;
         return vt::with_act(act, [&](auto f) -> vt_status {
-            constexpr int ACT = decltype(f)::value;
-            if (outs <= 64u) return vt::launch_linear4<T, ACT, 64, true>(nullptr, codes, a, st);
-            if (outs <= 128u) return vt::launch_linear4<T, ACT, 128, true>(nullptr, codes, a, st);
-            if (outs <= 256u) return vt::launch_linear4<T, ACT, 256, true>(nullptr, codes, a, st);
-            return vt::launch_linear4<T, ACT, 256, false>(x_codes, codes, a, st);
+            return vt::launch_linear4<T, decltype(f)::value, 256, false>(x_codes, 0, codes, a, st);
         });
     });
 }

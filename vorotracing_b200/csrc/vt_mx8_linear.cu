@@ -18,8 +18,7 @@
 // tile: dz = (dy W) * act'(z8), with the slope in the epilogue, and dW = dy^T h with h = act(z8)
 // written once, in the operands' type, by a pass before it: as an operand it is read once for
 // every 256 outputs, and evaluating it as often would cost more than the tensor cores' time.
-#include "vt_mx.cuh"
-#include "vt_tc.cuh"
+#include "vt_mx_rows.cuh"
 
 namespace vt {
 
@@ -333,26 +332,6 @@ __global__ void __launch_bounds__(256) narrow_reduce_kernel(const float *__restr
     }
 }
 
-// Rows of a matrix copied to a pitch of whole 16-byte words, which TMA asks for.
-template <typename T>
-__global__ void __launch_bounds__(256) pad_rows_kernel(const T *__restrict__ src, uint64_t rows, uint32_t cols, uint64_t stride,
-                                                       T *__restrict__ dst, uint32_t pitch)
-{
-    const uint32_t words = pitch / 8u;
-    const uint64_t n = rows * words;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256u) {
-        const uint64_t row = i / words;
-        const uint32_t col = (uint32_t)(i % words) * 8u;
-        const T *p = src + row * stride + col;
-        Vec8<T> v;
-        T *e = reinterpret_cast<T *>(v.w);
-#pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) e[k] = col + k < cols ? p[k] : from_f32<T>(0.0f);
-        v.store(dst + row * pitch + col);
-    }
-}
-
-
 // ---- wider layers ----
 
 constexpr uint32_t WIDE_STAGES = 6, WIDE_STAGE_BYTES = 32768, WIDE_THREADS = 256;
@@ -616,15 +595,15 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float *__restrict_
     }
 }
 
-static uint64_t align_up(uint64_t n, uint64_t a) { return (n + a - 1) / a * a; }
+// Operands whose rows do not start on 16 bytes are copied
+enum : int { COPY_DY = 1, COPY_WEIGHT = 2 };
 
-// How a narrow call is cut, and where its workspace parts lie.  The copies of dy and the weight
-// are counted always: whether they are needed depends on pointers.
+// How a narrow call is cut, and where its workspace parts lie.
 struct NarrowPlan {
     uint32_t oc, nc, slabs, tiles, groups, part_outs;
     uint64_t dw_at, db_at, dy_at, w_at, bytes;
 };
-static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, uint32_t sms)
+static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, int copies, uint32_t sms)
 {
     NarrowPlan p;
     p.oc = (outs + 63u) / 64u;
@@ -638,32 +617,14 @@ static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, uint3
     p.dw_at = 0;
     p.db_at = p.dw_at + align_up((uint64_t)p.groups * p.slabs * p.nc * 64u * p.part_outs * 4u, 256);
     p.dy_at = p.db_at + align_up((uint64_t)p.groups * 2u * p.oc * 64u * 4u, 256);
-    p.w_at = p.dy_at + align_up(rows * align_up(outs, 8) * 2u, 256);
-    p.bytes = p.w_at + align_up((uint64_t)outs * align_up(cols, 8) * 2u, 256);
+    p.w_at = p.dy_at + (copies & COPY_DY ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
+    p.bytes = p.w_at + (copies & COPY_WEIGHT ? align_up((uint64_t)outs * align_up(cols, 8) * 2u, 256) : 0);
     return p;
 }
 
-// p and its row stride, or a copy's whose rows are whole 16-byte words where p's are not.
-template <typename T>
-static vt_status whole_rows(const void *&p, uint64_t &stride, uint64_t rows, uint32_t cols, void *copy, cudaStream_t stream)
+template <typename T> static int copies_of(const void *dy, uint64_t dy_stride, const void *w, uint64_t w_stride)
 {
-    uint64_t pitch = stride * sizeof(T);
-    if (pitch % 16u || !aligned16(p)) {
-        const uint32_t to = (uint32_t)align_up(cols, 8);
-        const uint64_t items = rows * (to / 8u), want = (items + 255u) / 256u;
-        pad_rows_kernel<T><<<(unsigned)(want < 4096u ? want : 4096u), 256, 0, stream>>>((const T *)p, rows, cols, stride, (T *)copy, to);
-        p = copy;
-        stride = to;
-        return check_launch("pad_rows_kernel");
-    }
-    return VT_OK;
-}
-template <typename T>
-static vt_status map_rows(CUtensorMap *map, const void *p, uint64_t stride, uint64_t rows, uint64_t cols, uint32_t box_rows)
-{
-    const CUtensorMapDataType type =
-        std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    return tc::make_map(map, type, p, rows, cols, stride * sizeof(T), box_rows, 64);
+    return (whole_words<T>(dy, dy_stride) ? 0 : COPY_DY) | (whole_words<T>(w, w_stride) ? 0 : COPY_WEIGHT);
 }
 
 template <typename T, int ACT, int OC, int NC>
@@ -681,7 +642,7 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
                             uint32_t outs, const int8_t *codes, const uint8_t *exps, void *dz, void *dw, void *db,
                             uint8_t *workspace, uint32_t *err, cudaStream_t stream)
 {
-    const NarrowPlan p = narrow_plan(rows, cols, outs, (uint32_t)sm_count());
+    const NarrowPlan p = narrow_plan(rows, cols, outs, copies_of<T>(dy, dy_stride, w, w_stride), (uint32_t)sm_count());
     CUtensorMap dy_map, w_map;
     if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
     if (vt_status s = whole_rows<T>(w, w_stride, outs, cols, workspace + p.w_at, stream)) return s;
@@ -726,7 +687,7 @@ struct WidePlan {
     uint64_t h_at, dw_at, db_at, dy_at, w_at, bytes;
 };
 static uint32_t wide_tile_n(uint32_t cols) { return cols >= 256u ? 256u : (cols + 31u) / 32u * 32u; }
-static WidePlan wide_plan(uint64_t rows, uint32_t cols, uint32_t outs, uint32_t sms)
+static WidePlan wide_plan(uint64_t rows, uint32_t cols, uint32_t outs, int copies, uint32_t sms)
 {
     WidePlan p;
     const uint32_t tn = wide_tile_n(cols), chunks = (uint32_t)((rows + 63u) / 64u);
@@ -741,8 +702,8 @@ static WidePlan wide_plan(uint64_t rows, uint32_t cols, uint32_t outs, uint32_t 
     p.dw_at = p.h_at + align_up(rows * align_up(cols, 8) * 2u, 256);
     p.db_at = p.dw_at + (p.splits > 1 ? align_up((uint64_t)p.splits * outs * cols * 4u, 256) : 0);
     p.dy_at = p.db_at + align_up((uint64_t)p.sum_parts * outs * 4u, 256);
-    p.w_at = p.dy_at + align_up(rows * align_up(outs, 8) * 2u, 256);
-    p.bytes = p.w_at + align_up((uint64_t)outs * align_up(cols, 8) * 2u, 256);
+    p.w_at = p.dy_at + (copies & COPY_DY ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
+    p.bytes = p.w_at + (copies & COPY_WEIGHT ? align_up((uint64_t)outs * align_up(cols, 8) * 2u, 256) : 0);
     return p;
 }
 
@@ -764,7 +725,7 @@ static vt_status run_wide(const void *dy, uint64_t dy_stride, const void *w, uin
                           uint8_t *workspace, uint32_t *err, cudaStream_t stream)
 {
     const uint32_t sms = (uint32_t)sm_count();
-    const WidePlan p = wide_plan(rows, cols, outs, sms);
+    const WidePlan p = wide_plan(rows, cols, outs, copies_of<T>(dy, dy_stride, w, w_stride), sms);
     if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
     WideArgs a = {};
     a.tile_n = wide_tile_n(cols);
@@ -831,11 +792,12 @@ static vt_status zero(T *p, uint64_t n, cudaStream_t stream)
 
 }  // namespace vt
 
-extern "C" uint64_t vt_mx8_linear_bwd_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs)
+extern "C" uint64_t vt_mx8_linear_bwd_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs, int copies)
 {
     if (rows == 0 || cols == 0 || outs == 0) return 0;
     const uint32_t sms = (uint32_t)vt::sm_count();
-    return outs <= vt::NARROW_OUTS ? vt::narrow_plan(rows, cols, outs, sms).bytes : vt::wide_plan(rows, cols, outs, sms).bytes;
+    return outs <= vt::NARROW_OUTS ? vt::narrow_plan(rows, cols, outs, copies, sms).bytes
+                                   : vt::wide_plan(rows, cols, outs, copies, sms).bytes;
 }
 
 extern "C" vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const void *weight, uint64_t weight_stride,
@@ -858,7 +820,8 @@ extern "C" vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const
         VT_REQUIRE(dy_stride >= outs && weight_stride >= cols,
                    "vt_mx8_linear_bwd: a row stride is less than a row");
         VT_REQUIRE(vt::aligned32(codes), "vt_mx8_linear_bwd: codes must be 32-byte aligned");
-        VT_REQUIRE(workspace_bytes >= vt_mx8_linear_bwd_workspace_bytes(rows, cols, outs) && vt::aligned16(workspace),
+        VT_REQUIRE(workspace_bytes >= vt_mx8_linear_bwd_workspace_bytes(rows, cols, outs, vt::copies_of<T>(dy, dy_stride, weight, weight_stride)) &&
+                       vt::aligned16(workspace),
                    "vt_mx8_linear_bwd: workspace too small or not 16-byte aligned");
         if (cols == 0) {  // a layer without inputs has the bias alone
             vt::column_sum_kernel<T><<<outs, 256, 0, st>>>((const T *)dy, rows, outs, dy_stride, (T *)db);

@@ -35,15 +35,18 @@ _ARGS = {
     "vt_mx8_checkpoint": (_P, _I, _U64, _U32, _U64, _I, _P, _P, _P, _P),
     "vt_mx8_act_bwd": (_P, _I, _U64, _U32, _U64, _P, _P, _I, _P, _P),
     "vt_mx8_dequantize": (_P, _P, _U64, _U32, _I, _P, _P),
-    "vt_mx8_linear_bwd_workspace_bytes": (_U64, _U32, _U32),
+    "vt_mx8_linear_bwd_workspace_bytes": (_U64, _U32, _U32, _I),
     "vt_mx8_linear_bwd": (_P, _U64, _P, _U64, _I, _U64, _U32, _U32, _P, _P, _I, _P, _P, _P, _P,
                           _U64, _P, _P),
     "vt_mx4_quantize": (_P, _I, _U64, _U32, _U64, _P, _P, _P),
     "vt_mx4_dequantize": (_P, _P, _U64, _U32, _I, _P, _P),
-    "vt_mx4_linear_workspace_bytes": (_U64, _U32, _U32),
+    "vt_mx4_linear_workspace_bytes": (_U64, _U32, _U32, _I),
     "vt_mx4_linear": (_P, _U64, _I, _U64, _U32, _U32, _P, _P, _P, _I, _P, _P, _U64, _P, _P),
 }
 _fn = {}
+_get_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 _error_words = {}
 
 
@@ -117,14 +120,21 @@ def _same(a, b, name: str, other: str):
         _fail(f"{name} must be on the same device as {other}")
 
 
-def _launch(name: str, device, *args):
+def _launch(name: str, index: int, *args):
     """Calls an entry point on the tensors' device and torch's current stream there."""
-    f = _call(name)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            check(f(*args, torch.cuda.current_stream(device).cuda_stream), name)
+    f = _fn.get(name) or _call(name)
+    if index == _get_device():
+        status = f(*args, _raw_stream(index))
     else:
-        check(f(*args, torch.cuda.current_stream(device).cuda_stream), name)
+        with torch.cuda.device(index):
+            status = f(*args, _raw_stream(index))
+    if status:
+        check(status, name)
+
+
+def _unaligned(ptr: int, stride: int) -> bool:
+    """Whether 16-bit rows at that address and stride do not all start on 16 bytes."""
+    return bool(ptr % 16 or stride % 8)
 
 
 def _check_parts(codes, exps, cols, code_dtype, per_block, what):
@@ -165,8 +175,8 @@ class Checkpoint:
         """The 8-bit values, (rows, cols)."""
         if dtype not in _DTYPES:
             _fail(f"cannot dequantise to {str(dtype).replace('torch.', '')}")
-        out = torch.empty((self.rows, self.cols), dtype=dtype, device=self.codes.device)
-        _launch("vt_mx8_dequantize", out.device, self.codes.data_ptr(), self.exps.data_ptr(),
+        out = self.codes.new_empty((self.rows, self.cols), dtype=dtype)
+        _launch("vt_mx8_dequantize", out.device.index, self.codes.data_ptr(), self.exps.data_ptr(),
                 self.rows, self.cols, _DTYPES[dtype], out.data_ptr())
         return out
 
@@ -189,8 +199,8 @@ class MX4:
         """The 4-bit values, (rows, cols)."""
         if dtype not in _DTYPES:
             _fail(f"cannot dequantise to {str(dtype).replace('torch.', '')}")
-        out = torch.empty((self.rows, self.cols), dtype=dtype, device=self.codes.device)
-        _launch("vt_mx4_dequantize", out.device, self.codes.data_ptr(), self.exps.data_ptr(),
+        out = self.codes.new_empty((self.rows, self.cols), dtype=dtype)
+        _launch("vt_mx4_dequantize", out.device.index, self.codes.data_ptr(), self.exps.data_ptr(),
                 self.rows, self.cols, _DTYPES[dtype], out.data_ptr())
         return out
 
@@ -200,10 +210,10 @@ def act_checkpoint(z: torch.Tensor, act: str = "silu"):
     code = _act_code(act)
     m, rows, cols, stride = _matrix(z, "z")
     blocks = -(-cols // BLOCK)
-    h = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    codes = torch.empty((rows, blocks * BLOCK), dtype=torch.int8, device=z.device)
-    exps = torch.empty((rows, blocks), dtype=torch.uint8, device=z.device)
-    _launch("vt_mx8_checkpoint", z.device, m.data_ptr(), _DTYPES[z.dtype], rows, cols, stride,
+    h = m.new_empty(z.shape)
+    codes = m.new_empty((rows, blocks * BLOCK), dtype=torch.int8)
+    exps = m.new_empty((rows, blocks), dtype=torch.uint8)
+    _launch("vt_mx8_checkpoint", z.device.index, m.data_ptr(), _DTYPES[z.dtype], rows, cols, stride,
             code, h.data_ptr(), codes.data_ptr(), exps.data_ptr())
     ckpt = Checkpoint.__new__(Checkpoint)
     ckpt.codes, ckpt.exps, ckpt.cols, ckpt.act, ckpt._act = codes, exps, cols, act, code
@@ -216,8 +226,8 @@ def act_backward(dh: torch.Tensor, ckpt: Checkpoint) -> torch.Tensor:
     if rows != ckpt.rows or cols != ckpt.cols:
         _fail(f"dh had {rows} rows of {cols}, the checkpoint has {ckpt.rows} of {ckpt.cols}")
     _same(dh, ckpt.codes, "dh", "the checkpoint")
-    dz = torch.empty(dh.shape, dtype=dh.dtype, device=dh.device)
-    _launch("vt_mx8_act_bwd", dh.device, m.data_ptr(), _DTYPES[dh.dtype], rows, cols, stride,
+    dz = m.new_empty(dh.shape)
+    _launch("vt_mx8_act_bwd", dh.device.index, m.data_ptr(), _DTYPES[dh.dtype], rows, cols, stride,
             ckpt.codes.data_ptr(), ckpt.exps.data_ptr(), ckpt._act, dz.data_ptr())
     return dz
 
@@ -242,12 +252,14 @@ def linear_backward(dy: torch.Tensor, weight: torch.Tensor, ckpt: Checkpoint, bi
     _same(weight, dy, "weight", "dy")
     _same(ckpt.codes, dy, "the checkpoint", "dy")
     dev, dt = dy.device, dy.dtype
-    dz = torch.empty((*dy.shape[:-1], cols), dtype=dt, device=dev) if need_dz else None
-    dw = torch.empty((outs, cols), dtype=dt, device=dev) if need_dw else None
-    db = torch.empty(outs, dtype=dt, device=dev) if bias else None
-    n = _call("vt_mx8_linear_bwd_workspace_bytes")(rows, cols, outs)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _launch("vt_mx8_linear_bwd", dev, m.data_ptr(), dy_stride, w.data_ptr(), w_stride,
+    dz = m.new_empty((*dy.shape[:-1], cols)) if need_dz else None
+    dw = m.new_empty((outs, cols)) if need_dw else None
+    db = m.new_empty(outs) if bias else None
+    m_ptr, w_ptr = m.data_ptr(), w.data_ptr()
+    n = _call("vt_mx8_linear_bwd_workspace_bytes")(
+        rows, cols, outs, _unaligned(m_ptr, dy_stride) + 2 * _unaligned(w_ptr, w_stride))
+    ws = m.new_empty(n, dtype=torch.uint8) if n else None
+    _launch("vt_mx8_linear_bwd", dev.index, m_ptr, dy_stride, w_ptr, w_stride,
             _DTYPES[dt], rows, cols, outs, ckpt.codes.data_ptr(), ckpt.exps.data_ptr(), ckpt._act,
             dz.data_ptr() if need_dz else None, dw.data_ptr() if need_dw else None,
             db.data_ptr() if bias else None, ws.data_ptr() if n else None, n, _error_word(dev).data_ptr())
@@ -282,10 +294,10 @@ def quantize4(x: torch.Tensor) -> MX4:
     m, rows, cols, stride = _matrix(x, "x")
     blocks = -(-cols // BLOCK)
     q = MX4.__new__(MX4)
-    q.codes = torch.empty((rows, blocks * BLOCK // 2), dtype=torch.uint8, device=x.device)
-    q.exps = torch.empty((rows, blocks), dtype=torch.uint8, device=x.device)
+    q.codes = m.new_empty((rows, blocks * BLOCK // 2), dtype=torch.uint8)
+    q.exps = m.new_empty((rows, blocks), dtype=torch.uint8)
     q.cols = cols
-    _launch("vt_mx4_quantize", x.device, m.data_ptr(), _DTYPES[x.dtype], rows, cols, stride,
+    _launch("vt_mx4_quantize", x.device.index, m.data_ptr(), _DTYPES[x.dtype], rows, cols, stride,
             q.codes.data_ptr(), q.exps.data_ptr())
     return q
 
@@ -305,10 +317,11 @@ def linear4(x: torch.Tensor, w: MX4, bias=None, act: str = "identity") -> torch.
             _fail(f"bias must have the dtype of x and shape ({outs},)")
         _same(bias, x, "bias", "x")
         bias = bias.contiguous()
-    y = torch.empty((*x.shape[:-1], outs), dtype=x.dtype, device=x.device)
-    n = _call("vt_mx4_linear_workspace_bytes")(rows, cols, outs)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _launch("vt_mx4_linear", x.device, m.data_ptr(), stride, _DTYPES[x.dtype], rows, cols, outs,
+    y = m.new_empty((*x.shape[:-1], outs))
+    m_ptr = m.data_ptr()
+    n = _call("vt_mx4_linear_workspace_bytes")(rows, cols, outs, _unaligned(m_ptr, stride))
+    ws = m.new_empty(n, dtype=torch.uint8) if n else None
+    _launch("vt_mx4_linear", x.device.index, m_ptr, stride, _DTYPES[x.dtype], rows, cols, outs,
             w.codes.data_ptr(), w.exps.data_ptr(), bias.data_ptr() if bias is not None else None,
             code, y.data_ptr(), ws.data_ptr() if n else None, n, _error_word(x.device).data_ptr())
     return y
