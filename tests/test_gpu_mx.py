@@ -277,7 +277,8 @@ def test_linear_backward_is_reproducible():
 
 
 LINEAR4 = [(1, 1, 1), (1, 64, 8), (1, 4096, 512), (2, 33, 3), (16, 1000, 333), (17, 256, 128), (64, 96, 130),
-           (77, 1000, 77), (130, 520, 264), (300, 192, 64), (1000, 75, 48), (513, 1024, 640)]
+           (77, 1000, 77), (130, 520, 264), (300, 192, 64), (1000, 75, 48), (513, 1024, 640), (128, 4100, 200),
+           (9600, 96, 40), (10000, 75, 8), (9999, 200, 128), (9700, 520, 200), (2000, 333, 1300), (5000, 256, 512)]
 
 
 @pytest.mark.parametrize("dtype", TYPES16)
@@ -475,7 +476,7 @@ def test_entry_points_refuse():
     assert f("vt_mx8_checkpoint")(p, 2, 8, 64, 64, 4, p, p, p, None) == 1 and "activation" in err()
     assert f("vt_mx8_act_bwd")(p, 2, 8, 64, 64, p + 8, p, 0, p, None) == 1 and "aligned" in err()
     assert f("vt_mx4_quantize")(p, 2, 8, 64, 64, p, None, None) == 1 and "null pointer" in err()
-    assert f("vt_mx4_linear")(p, 64, 2, 8, 64, 300, p, p, None, 0, p, None, 0, None, None) == 1 and "workspace" in err()
+    assert f("vt_mx4_linear")(p, 64, 2, 10000, 64, 300, p, p, None, 0, p, None, 0, None, None) == 1 and "workspace" in err()
     assert f("vt_mx4_linear")(p, 64, 0, 8, 64, 4, p, p, None, 0, p, p, 1 << 20, None, None) == 1 and "16" in err()
     assert f("vt_mx8_linear_bwd")(p, 4, p, 64, 2, 1 << 32, 64, 4, p, p, 0, p, p, p, p, 1 << 40, None, None) == 1 and "rows" in err()
     assert f("vt_mx8_linear_bwd")(p, 4, None, 64, 2, 8, 64, 4, p, p, 0, p, p, p, p, 1 << 40, None, None) == 1 and "null" in err()

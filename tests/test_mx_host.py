@@ -47,7 +47,8 @@ def test_workspace_sizes_cover_the_layout():
     from vorotracing_b200 import mx
 
     n = mx._call("vt_mx4_linear_workspace_bytes")
-    for rows, cols in ((1, 1), (77, 1000), (1 << 20, 192)):
+    assert n(1, 4096, 4096, 1) == 0
+    for rows, cols in ((9999, 1), (12345, 1000), (1 << 20, 192)):
         blocks = -(-cols // 32)
         assert n(rows, cols, 300, 0) >= rows * blocks * 17
         assert n(rows, cols, 8, 0) == 0 and n(rows, cols, 8, 1) >= rows * cols * 2

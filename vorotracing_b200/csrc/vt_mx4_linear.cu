@@ -14,6 +14,12 @@
 // its own writes codes and scales first, 17/32 byte a value, and TMA brings them in.
 #include "vt_mx_rows.cuh"
 
+// Too few tiles to occupy the GPU (few rows, as in serving one token at a time) go the other way
+// round (few_kernel): 128 outputs are the product's rows and up to 128 rows of x its columns, k is
+// split over a cluster of up to 8 CTAs, each CTA rounds its part of x itself, and the parts of the
+// sums meet in distributed shared memory, where they are added in the order of k.  One launch; the
+// weight is spread over as many SMs as there are.
+
 namespace vt {
 
 constexpr uint32_t L4_ROWS = 128, L4_K = 256;
@@ -24,7 +30,7 @@ template <int TN, bool QUANT> struct L4 {
     static constexpr uint32_t SF_BYTES = (1u + B_PARTS) * 1024u;
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SF_BYTES;
     static constexpr uint32_t STAGES = QUANT ? (TN == 256 ? 2 : 3) : 4;
-    static constexpr uint32_t X_BYTES = L4_ROWS * 128u, X_STAGES = QUANT ? (TN == 64 ? 8 : 7) : 0;  // 64 columns of x each
+    static constexpr uint32_t X_BYTES = L4_ROWS * 128u, X_STAGES = TN == 64 ? 8 : 7;  // QUANT: 64 columns of x each
     // two accumulators when they leave room for the scales
     static constexpr uint32_t ACCS = TN == 256 ? 1 : 2;
     static constexpr uint32_t SF_AT = ACCS * TN, SF_COLS = 8u + 8u * B_PARTS;
@@ -34,12 +40,12 @@ template <int TN, bool QUANT> struct L4 {
     static constexpr uint32_t THREADS = 32u * (8u + SCALE_WARPS + QUANT_WARPS);
     static constexpr uint32_t FULL_COUNT = 1u + SCALE_WARPS + QUANT_WARPS;
     struct Ctrl {
-        uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS], x_full[X_STAGES + 1], x_empty[X_STAGES + 1];
+        uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS], x_full[X_STAGES], x_empty[X_STAGES];
         uint32_t tmem;
         tc::Fail fail;
         alignas(8) float bias[TN];
     };
-    static constexpr uint32_t X_AT = STAGES * STAGE, CTRL_AT = X_AT + X_STAGES * X_BYTES, SMEM = CTRL_AT + sizeof(Ctrl);
+    static constexpr uint32_t X_AT = STAGES * STAGE, CTRL_AT = X_AT + (QUANT ? X_STAGES * X_BYTES : 0u), SMEM = CTRL_AT + sizeof(Ctrl);
     static_assert(SMEM <= 232448 && SF_AT + SF_COLS <= 512, "does not fit an SM");
 };
 
@@ -67,6 +73,34 @@ __device__ __forceinline__ uint2 load_scales(const uint8_t *exps, uint64_t row, 
 }
 // Place of a row's scales in a stage: 16 bytes for each of 32 rows, a word a group of 32.
 __device__ __forceinline__ uint32_t scale_place(uint32_t row) { return (row >> 7) * 1024u + (row & 31u) * 16u + ((row >> 5) & 3u) * 4u; }
+
+// A block of 32 16-bit numbers to 4 bits: codes and exponent byte
+template <typename T> __device__ __forceinline__ uint4 block_codes(const uint4 *w, uint32_t &E)
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+        top = __vmaxu2(top, w[u].x & 0x7fff7fffu);
+        top = __vmaxu2(top, w[u].y & 0x7fff7fffu);
+        top = __vmaxu2(top, w[u].z & 0x7fff7fffu);
+        top = __vmaxu2(top, w[u].w & 0x7fff7fffu);
+    }
+    E = mx4_exponent(top_of_pair<T>(top));
+    const f32x2 inv = both(E == 255u ? 0.0f : mx4_inverse(E));
+    uint32_t codes[4];
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t in[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+        f32x2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2<T>(in[i]);
+            v[i] = mul2(pair(f.x, f.y), inv);
+        }
+        codes[u] = mx4_word(v);
+    }
+    return make_uint4(codes[0], codes[1], codes[2], codes[3]);
+}
 
 template <typename T, int ACT, int TN, bool QUANT>
 __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
@@ -264,31 +298,10 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.x_empty[x.i]);
                     x.next(P::X_STAGES);
-                    uint32_t top = 0;
-#pragma unroll
-                    for (uint32_t u = 0; u < 4; ++u) {
-                        top = __vmaxu2(top, w[u].x & 0x7fff7fffu);
-                        top = __vmaxu2(top, w[u].y & 0x7fff7fffu);
-                        top = __vmaxu2(top, w[u].z & 0x7fff7fffu);
-                        top = __vmaxu2(top, w[u].w & 0x7fff7fffu);
-                    }
-                    const uint32_t E = mx4_exponent(top_of_pair<T>(top));
-                    const f32x2 inv = both(E == 255u ? 0.0f : mx4_inverse(E));
-                    uint32_t codes[4];
-#pragma unroll
-                    for (uint32_t u = 0; u < 4; ++u) {
-                        const uint32_t in[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-                        f32x2 v[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 f = unpack2<T>(in[i]);
-                            v[i] = mul2(pair(f.x, f.y), inv);
-                        }
-                        codes[u] = mx4_word(v);
-                    }
+                    uint32_t E;
+                    const uint4 codes = block_codes<T>(w, E);
                     const uint32_t block = k * 2u + part;
-                    *reinterpret_cast<uint4 *>(st + row * 128u + ((block ^ (row & 7u)) << 4)) =
-                        make_uint4(codes[0], codes[1], codes[2], codes[3]);
+                    *reinterpret_cast<uint4 *>(st + row * 128u + ((block ^ (row & 7u)) << 4)) = codes;
                     sf[(block >> 2) * 512u + (block & 3u)] = (uint8_t)E;
                 }
                 tc::fence_async_shared();
@@ -301,6 +314,173 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
     tc::fence_before();
     __syncthreads();
     if (warp == 1) tc::tmem_free<P::TMEM>(tmem);
+}
+
+// ---- few tiles ----
+
+constexpr uint32_t FEW_STAGES = 6, FEW_STAGE = 2u * 16384u + 2048u, FEW_THREADS = 512;
+struct FewCtrl {
+    uint64_t full[FEW_STAGES], empty[FEW_STAGES], acc_full;
+    uint32_t tmem;
+    tc::Fail fail;
+};
+constexpr uint32_t FEW_SMEM = FEW_STAGES * FEW_STAGE + sizeof(FewCtrl);
+
+struct FewArgs {
+    uint64_t rows, x_stride;
+    uint32_t cols, outs, blocks, chunks, chunks_a_split;
+    const void *x;
+    const uint8_t *w_exps;
+    const void *bias;
+    void *y;
+    uint32_t *err;
+    bool x_vec;
+};
+
+// grid: (splits of k = the cluster, tiles of 128 outputs, tiles of 128 rows)
+template <typename T, int ACT>
+__global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_constant__ CUtensorMap w_map, const FewArgs a)
+{
+    extern __shared__ __align__(1024) uint8_t smem[];
+    FewCtrl &s = *reinterpret_cast<FewCtrl *>(smem + FEW_STAGES * FEW_STAGE);
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, splits = gridDim.x, rank = blockIdx.x;
+    const uint32_t out0 = blockIdx.y * 128u, c0 = rank * a.chunks_a_split, c1 = min(a.chunks, c0 + a.chunks_a_split);
+    const uint64_t row0 = (uint64_t)blockIdx.z * 128u;
+    const uint32_t rows = (uint32_t)(a.rows - row0 < 128u ? a.rows - row0 : 128u), n = (rows + 15u) / 16u * 16u;
+    tc::Fail *const fail = &s.fail;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < FEW_STAGES; ++i) {
+            tc::mbar_init(&s.full[i], 1 + 4 + 8);
+            tc::mbar_init(&s.empty[i], 1);
+        }
+        tc::mbar_init(&s.acc_full, 1);
+        s.fail.failed = 0;
+        tc::mbar_init_fence();
+        tc::tma_prefetch_map(&w_map);
+    }
+    if (warp == 1) tc::tmem_alloc<256>(&s.tmem);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = s.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {  // TMA of the weight's codes
+            tc::Ring r;
+            for (uint32_t c = c0; c < c1; ++c) {
+                if (!tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err)) break;
+                tc::mbar_arrive_tx(&s.full[r.i], 16384);
+                tc::tma_load_2d(smem + r.i * FEW_STAGE, &w_map, (int)(c * 128u), (int)out0, &s.full[r.i]);
+                r.next(FEW_STAGES);
+            }
+            if (s.fail.failed) {  // as in linear4_kernel
+                const uint64_t began = tc::nanoseconds();
+                while (tc::nanoseconds() - began < 10000000ull) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {  // scales to tensor memory, products
+            const uint32_t base = tc::smem_u32(smem), sfa = tmem + 128u, sfb = sfa + 8u;
+            const uint32_t id = tc::idesc_mxf4(128, 0, 0) | (n >> 3) << 17, id1 = tc::idesc_mxf4(128, 0, 1) | (n >> 3) << 17;
+            tc::Ring r;
+            bool ok = true;
+            for (uint32_t c = c0; c < c1; ++c) {
+                ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
+                if (!ok) break;
+                tc::fence_after();
+                const uint32_t st = base + r.i * FEW_STAGE, sf = st + 32768u, steps = min(4u, (a.cols - c * L4_K + 63u) / 64u);
+                for (uint32_t g = 0; 2u * g < steps; ++g) {
+                    tc::tmem_copy_scales(sfa + g * 4u, tc::scale_desc(sf + g * 512u));
+                    tc::tmem_copy_scales(sfb + g * 4u, tc::scale_desc(sf + 1024u + g * 512u));
+                }
+                for (uint32_t k = 0; k < steps; ++k)
+                    tc::mma_mxf4(tmem, tc::smem_desc(st + k * 32u, 16, 1024), tc::smem_desc(st + 16384u + k * 32u, 16, 1024),
+                                 k & 1u ? id1 : id, sfa + (k >> 1) * 4u, sfb + (k >> 1) * 4u, c != c0 || k != 0);
+                tc::commit(&s.empty[r.i]);
+                r.next(FEW_STAGES);
+            }
+            tc::commit(&s.acc_full);
+            if (!ok) tc::mbar_wait_slow(&s.acc_full, 0, fail, a.err, true);  // leave no product in flight
+        }
+    } else if (warp >= 4 && warp < 8) {  // the weight's scales, then this CTA's sums to its shared memory
+        const uint32_t quad = warp % 4u, i = quad * 32u + lane;
+        tc::Ring r;
+        bool ok = true;
+        for (uint32_t c = c0; c < c1; ++c) {
+            const uint2 e = out0 + i < a.outs ? load_scales(a.w_exps, out0 + i, a.blocks, c * 8u) : make_uint2(0, 0);
+            ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
+            if (!ok) break;
+            uint8_t *sf = smem + r.i * FEW_STAGE + 32768u + scale_place(i);
+            *reinterpret_cast<uint32_t *>(sf) = e.x;
+            *reinterpret_cast<uint32_t *>(sf + 512u) = e.y;
+            tc::fence_async_shared();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
+            r.next(FEW_STAGES);
+        }
+        if (ok && __all_sync(~0u, tc::mbar_wait(&s.acc_full, 0, fail, a.err))) {
+            tc::fence_after();
+            // all products are done, so the stages are free: [row][output] in binary32
+            float *sum = reinterpret_cast<float *>(smem);
+            for (uint32_t j = 0; j < n; j += 32u) {
+                uint32_t v[32];
+                tc::tmem_load32(tmem + (quad * 32u << 16) + j, v);
+                tc::tmem_wait_load();
+#pragma unroll
+                for (uint32_t k = 0; k < 32; ++k)  // the last splits may have no part of k
+                    if (j + k < rows) sum[(j + k) * 128u + i] = c0 < c1 ? __uint_as_float(v[k]) : 0.0f;
+            }
+        }
+    } else if (warp >= 8) {  // x to 4 bits, a lane a block
+        tc::Ring r;
+        for (uint32_t c = c0; c < c1; ++c) {
+            const bool ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
+            if (!ok) break;
+            uint8_t *st = smem + r.i * FEW_STAGE + 16384u;
+            for (uint32_t i = threadIdx.x - 256u; i < rows * 8u; i += 256u) {
+                const uint32_t row = i / 8u, block = i % 8u, col = c * L4_K + block * 32u;
+                const T *p = (const T *)a.x + (row0 + row) * a.x_stride + col;
+                uint4 w[4];
+                if (a.x_vec && col + 32u <= a.cols) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) w[u] = __ldg(reinterpret_cast<const uint4 *>(p) + u);
+                } else {
+                    uint32_t *h = reinterpret_cast<uint32_t *>(w);
+#pragma unroll
+                    for (uint32_t u = 0; u < 16; ++u) {
+                        const uint32_t lo = col + 2 * u < a.cols ? __ldg(reinterpret_cast<const unsigned short *>(p) + 2 * u) : 0u;
+                        const uint32_t hi = col + 2 * u + 1 < a.cols ? __ldg(reinterpret_cast<const unsigned short *>(p) + 2 * u + 1) : 0u;
+                        h[u] = lo | hi << 16;
+                    }
+                }
+                uint32_t E;
+                const uint4 codes = block_codes<T>(w, E);
+                *reinterpret_cast<uint4 *>(st + row * 128u + ((block ^ (row & 7u)) << 4)) = codes;
+                st[16384u + 1024u + scale_place(row) + (block >> 2) * 512u + (block & 3u)] = (uint8_t)E;
+            }
+            tc::fence_async_shared();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
+            r.next(FEW_STAGES);
+        }
+    }
+    __syncwarp();
+    tc::fence_before();
+    tc::cluster_sync();
+    if (!s.fail.failed) {  // each CTA finishes every splits-th row: the parts in the order of k
+        const uint32_t out = threadIdx.x % 128u;
+        const float b = a.bias && out0 + out < a.outs ? to_f32<T>(__ldg((const T *)a.bias + out0 + out)) : 0.0f;
+        for (uint32_t row = rank + splits * (threadIdx.x / 128u); row < rows; row += splits * (FEW_THREADS / 128u)) {
+            float v = 0.0f;
+            for (uint32_t p = 0; p < splits; ++p) v += tc::load_cluster(reinterpret_cast<float *>(smem) + row * 128u + out, p);
+            if (out0 + out < a.outs)
+                ((T *)a.y)[(row0 + row) * a.outs + out0 + out] = from_f32<T>(unpair(act_value2<ACT>(both(v + b))).x);
+        }
+    }
+    __syncwarp();
+    tc::cluster_sync();  // no CTA leaves while another may still read its sums
+    if (warp == 1) tc::tmem_free<256>(tmem);
 }
 
 // No columns: the activation of the bias alone.
@@ -337,12 +517,53 @@ static vt_status launch_linear4(const void *x, uint64_t x_stride, const uint8_t 
     return check_launch("linear4_kernel");
 }
 
+// Splits of k for few_kernel, a power of two up to 8; 0: there are tiles enough for linear4_kernel.
+// few_kernel's tiles are 128 x 128 and every SM gets at most one CTA of it; with more of them than
+// half the SMs splitting gains nothing and the larger tiles read their operands less often.
+static uint32_t few_splits(uint64_t rows, uint32_t cols, uint32_t outs, uint32_t sms)
+{
+    const uint64_t tiles = (rows + 127u) / 128u * ((outs + 127u) / 128u);
+    if (tiles > sms / 2u) return 0;
+    const uint32_t chunks = (cols + L4_K - 1u) / L4_K;
+    uint32_t n = 1;
+    while (n < 8u && 2u * n <= chunks && tiles * 2u * n <= sms) n *= 2u;
+    return n;
+}
+
+template <typename T, int ACT>
+static vt_status launch_few(const uint8_t *w_codes, FewArgs a, uint32_t splits, cudaStream_t stream)
+{
+    static std::atomic<uint64_t> allowed{0};
+    CUtensorMap w_map;
+    const uint64_t pitch = (uint64_t)a.blocks * 16u;
+    if (vt_status s = tc::make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w_codes, a.outs, pitch, pitch, 128, 128)) return s;
+    if (vt_status s = tc::allow_smem(few_kernel<T, ACT>, FEW_SMEM, allowed)) return s;
+    a.chunks_a_split = (a.chunks + splits - 1u) / splits;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(splits, (a.outs + 127u) / 128u, (unsigned)((a.rows + 127u) / 128u));
+    config.blockDim = dim3(FEW_THREADS);
+    config.dynamicSmemBytes = FEW_SMEM;
+    config.stream = stream;
+    cudaLaunchAttribute cluster = {};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim = {splits, 1, 1};
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&config, few_kernel<T, ACT>, w_map, a);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(VT_ERR_CUDA, "few_kernel: %s", cudaGetErrorString(e));
+    }
+    return VT_OK;
+}
+
 }  // namespace vt
 
 // copies: x's rows do not start on 16 bytes
 extern "C" uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs, int copies)
 {
     const uint64_t blocks = vt::mx_blocks(cols);
+    if (vt::few_splits(rows, cols, outs, (uint32_t)vt::sm_count())) return 0;
     if (outs <= 256u) return copies ? rows * vt::align_up(cols, 8) * 2u : 0;  // x is rounded inside the kernel
     return rows * blocks * 16u + vt::align_up(rows * blocks, 16);
 }
@@ -376,6 +597,22 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
         a.err = err;
         a.y_wide = outs % 16u == 0 && vt::aligned32(y);
         if (cols == 0) return vt::with_act(act, [&](auto f) { return vt::launch_bias<T, decltype(f)::value>(a, st); });
+        if (const uint32_t splits = vt::few_splits(rows, cols, outs, (uint32_t)vt::sm_count())) {
+            vt::FewArgs f = {};
+            f.rows = rows;
+            f.x_stride = x_stride;
+            f.cols = cols;
+            f.outs = outs;
+            f.blocks = a.blocks;
+            f.chunks = a.chunks;
+            f.x = x;
+            f.w_exps = exps;
+            f.bias = bias;
+            f.y = y;
+            f.err = err;
+            f.x_vec = vt::whole_words<T>(x, x_stride);
+            return vt::with_act(act, [&](auto k) { return vt::launch_few<T, decltype(k)::value>(codes, f, splits, st); });
+        }
         if (outs <= 256u) {
             const void *from = x;
             uint64_t stride = x_stride;

@@ -198,6 +198,15 @@ __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// This CTA's shared-memory word, read in the cluster's CTA of that rank
+__device__ __forceinline__ float load_cluster(const float *p, uint32_t rank)
+{
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
 // Address of the leader's copy of a shared-memory object
 __device__ __forceinline__ uint32_t leader_addr(const void *p)
 {
