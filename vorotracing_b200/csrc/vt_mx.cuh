@@ -157,23 +157,28 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// 32 columns of a row from packed pairs.  wide: the row starts on 32 bytes and holds whole
+// 16 columns of a row from packed pairs.  wide: the row starts on 32 bytes and holds whole
 // 32-byte pieces, which are whole sectors of L2.
 template <typename T>
-__device__ __forceinline__ void store_row32(T *row, uint32_t col, uint32_t cols, bool wide, const uint32_t *w)
+__device__ __forceinline__ void store_row16(T *row, uint32_t col, uint32_t cols, bool wide, const uint32_t *w)
 {
     T *p = row + col;
     if (wide) {
         if (col < cols) store32(p, w);
-        if (col + 16u < cols) store32(p + 16, w + 8);
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
+        for (uint32_t i = 0; i < 8; ++i) {
             const float2 v = unpack2<T>(w[i]);
             if (col + 2 * i < cols) p[2 * i] = from_f32<T>(v.x);
             if (col + 2 * i + 1 < cols) p[2 * i + 1] = from_f32<T>(v.y);
         }
     }
+}
+template <typename T>
+__device__ __forceinline__ void store_row32(T *row, uint32_t col, uint32_t cols, bool wide, const uint32_t *w)
+{
+    store_row16<T>(row, col, cols, wide, w);
+    store_row16<T>(row, col + 16u, cols, wide, w + 8);
 }
 
 // ---- formats ----

@@ -7,7 +7,7 @@
 // shared memory (TMA, 128-byte swizzle) and used twice: as the K-major A operand of
 // dH = dy W, and, the same bytes read the other way, as the MN-major A operand of
 // dW += dy^T act(z8), whose accumulator stays in tensor memory over all the CTA's rows.
-// Between the two products eight warps take dH out of tensor memory, read the 8-bit z, evaluate
+// Between the two products sixteen warps take dH out of tensor memory, read the 8-bit z, evaluate
 // act and act' together (one logistic serves both), write dz, and leave act(z8) in shared memory
 // as the second product's B operand, rounded to the operands' 16-bit type as the forward pass's
 // own activations are.  Two more warps add up dy's columns from the staged tile.  At its end a CTA
@@ -24,11 +24,12 @@ namespace vt {
 
 // ---- layers with up to 256 outputs ----
 
-constexpr uint32_t TILE_ROWS = 128, NARROW_OUTS = 256, NARROW_THREADS = 384;
+constexpr uint32_t TILE_ROWS = 128, NARROW_OUTS = 256, NARROW_THREADS = 640;
 
 // OC: dy's columns in chunks of 64; NC: the slab's columns in chunks of 64.
 template <int OC, int NC> struct Narrow {
     static constexpr uint32_t W_BYTES = OC * 8192u * NC, DY_BYTES = OC * 16384u, H_BYTES = NC * 16384u;
+    static constexpr int PIECES = NC;  // of 16 columns an activation warp takes: 4 warps a quadrant
     // as much staging as 227 KB hold
     static constexpr uint32_t STAGES = OC >= 3 ? 2 : OC == 2 ? 3 : 4, H_BUFS = OC == 4 && NC == 2 ? 1 : 2;
     static constexpr uint32_t DY_AT = W_BYTES, H_AT = DY_AT + STAGES * DY_BYTES, CTRL_AT = H_AT + H_BUFS * H_BYTES;
@@ -57,22 +58,28 @@ struct NarrowArgs {
     bool dz_wide;      // dz's rows hold whole 32-byte pieces
 };
 
-// One row's block of 32 columns: g = dH (binary32) in, h and dz out as packed 16-bit pairs.
+// 16 columns of a row: codes (4 words) and their block's scale, g = dH (binary32) in, h and dz out
+// as packed 16-bit pairs.
 template <typename T, int ACT, bool VALUE>
-__device__ __forceinline__ void transform_block(const uint32_t *codes, uint32_t E, const uint32_t *g, uint32_t *h, uint32_t *dz)
+__device__ __forceinline__ void transform16(const uint32_t *codes, f32x2 sc, const uint32_t *g, uint32_t *h, uint32_t *dz)
 {
-    const f32x2 sc = both(mx8_scale(E));
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < 4; ++w) {
         const uint32_t c = codes[w] ^ 0x80808080u;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            f32x2 v, slope;
-            act_pair<ACT, VALUE, true>(mul2(code_pair(c, 2 * i), sc), v, slope);
             const int at = 2 * w + i;
-            if (VALUE) h[at] = pack2<T>(v);
-            const f32x2 gp = pair(__uint_as_float(g[2 * at]), __uint_as_float(g[2 * at + 1]));
-            dz[at] = pack2<T>(ACT == ACT_IDENTITY ? gp : mul2(gp, slope));
+            const f32x2 z = mul2(code_pair(c, 2 * i), sc), gp = pair(__uint_as_float(g[2 * at]), __uint_as_float(g[2 * at + 1]));
+            if constexpr (ACT == ACT_RELU) {
+                const float2 v = unpair(z), d = unpair(gp), zero = unpair(mul2(sc, both(0.0f)));  // NaN in a NaN block
+                if (VALUE) h[at] = pack2<T>(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
+                dz[at] = pack2<T>(v.x > 0.0f ? d.x : zero.x, v.y > 0.0f ? d.y : zero.x);
+            } else {
+                f32x2 v, slope;
+                act_pair<ACT, VALUE, true>(z, v, slope);
+                if (VALUE) h[at] = pack2<T>(v);
+                dz[at] = pack2<T>(ACT == ACT_IDENTITY ? gp : mul2(gp, slope));
+            }
         }
     }
 }
@@ -99,10 +106,10 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         }
         for (uint32_t i = 0; i < 2; ++i) {
             tc::mbar_init(&s.dh_full[i], 1);
-            tc::mbar_init(&s.dh_empty[i], 8);
+            tc::mbar_init(&s.dh_empty[i], 16);
         }
         for (uint32_t i = 0; i < P::H_BUFS; ++i) {
-            tc::mbar_init(&s.h_full[i], 8);
+            tc::mbar_init(&s.h_full[i], 16);
             tc::mbar_init(&s.h_empty[i], 1);
         }
         tc::mbar_init(&s.w_full, 1);
@@ -190,7 +197,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
     } else if (warp < 4) {
         if (sums) {  // column sums: each of the two warps takes half of a tile's rows, a lane two columns
             tc::Ring r;
-            float2 total[OC] = {};
+            f32x2 total[OC] = {};
             bool ok = true;
             const uint32_t row0 = (warp - 2u) * 64u;
             for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
@@ -200,15 +207,13 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 for (int c = 0; c < OC; ++c) {
                     if (c % sharers != slab) continue;
                     const uint8_t *p = smem + P::DY_AT + r.i * P::DY_BYTES + c * 16384 + row0 * 128u;
-                    float2 v = make_float2(0.0f, 0.0f);
+                    f32x2 v = 0;
 #pragma unroll 8
                     for (uint32_t i = 0; i < 64; ++i) {
                         const float2 x = unpack2<T>(*reinterpret_cast<const uint32_t *>(p + i * 128u + ((lane * 4u) ^ (i & 7u) << 4)));
-                        v.x += x.x;
-                        v.y += x.y;
+                        v = add2(v, pair(x.x, x.y));
                     }
-                    total[c].x += v.x;
-                    total[c].y += v.y;
+                    total[c] = add2(total[c], v);
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s.empty[r.i]);
@@ -217,27 +222,30 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
 #pragma unroll
             for (int c = 0; c < OC; ++c)
                 if (c % sharers == slab)
-                    *reinterpret_cast<float2 *>(a.db_parts + ((uint64_t)group * 2u + (warp - 2u)) * (OC * 64u) + c * 64u + lane * 2u) =
+                    *reinterpret_cast<f32x2 *>(a.db_parts + ((uint64_t)group * 2u + (warp - 2u)) * (OC * 64u) + c * 64u + lane * 2u) =
                         total[c];
         }
-    } else {  // activations: warp w reads rows 32 (w % 4).. of the tile and half of the slab's columns
-        const uint32_t quad = warp % 4u, half = (warp - 4u) / 4u;
-        const uint32_t in_tile = quad * 32u + lane, block0 = (slab * NC * 2u) + half * NC;
-        uint32_t codes[NC][8], E[NC];
-        auto fetch = [&](uint32_t t, uint32_t (&c)[NC][8], uint32_t (&e)[NC]) {
+    } else {  // activations: a warp has rows 32 (w % 4).. of the tile and a quarter of the slab's columns
+        constexpr int PIECES = P::PIECES;
+        const uint32_t quad = warp % 4u, part = (warp - 4u) / 4u, in_tile = quad * 32u + lane;
+        const uint32_t col0 = part * PIECES * 16u, col = slab * NC * 64u + col0;  // in the slab, in the row
+        uint32_t codes[PIECES][4], E;
+        auto fetch = [&](uint32_t t, uint32_t (&c)[PIECES][4], uint32_t &e) {
             const uint64_t row = (uint64_t)t * TILE_ROWS + in_tile;
-#pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                const bool in = t < a.tiles && row < a.rows && block0 + j < a.blocks;
-                if (in) {
-                    const uint64_t b = row * a.blocks + block0 + j;
-                    load32(a.codes + b * 32u, c[j]);
-                    e[j] = __ldg(a.exps + b);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) c[j][i] = 0;
-                    e[j] = 127;
+            if (t < a.tiles && row < a.rows && col < a.blocks * 32u) {
+                const uint64_t at = row * a.blocks * 32u + col;
+                if (PIECES == 2) load32(a.codes + at, c[0]);  // c[0] and c[1] are neighbours
+                else {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(a.codes + at));
+                    c[0][0] = v.x; c[0][1] = v.y; c[0][2] = v.z; c[0][3] = v.w;
                 }
+                e = __ldg(a.exps + (at >> 5));
+            } else {
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) c[p][i] = 0;
+                e = 127;
             }
         };
         fetch(group, codes, E);
@@ -245,43 +253,45 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         bool ok = true;
         for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
             const uint64_t row = (uint64_t)t * TILE_ROWS + in_tile;
-            uint32_t next[NC][8], next_E[NC];
+            uint32_t next[PIECES][4], next_E;
             fetch(t + a.groups, next, next_E);
-            ok = tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err) &&
-                 tc::mbar_wait(&s.h_empty[h.i], h.phase ^ 1u, fail, a.err);
-            if (!__all_sync(~0u, ok)) { ok = false; break; }
+            ok = __all_sync(~0u, tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err));
+            if (!ok) break;
             tc::fence_after();
+            const f32x2 sc = both(mx8_scale(E));
+            uint8_t *to = smem + P::H_AT + h.i * P::H_BYTES + (col0 >> 6) * 16384u + in_tile * 128u;
 #pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                uint32_t g[32], hv[16], dz[16];
-                tc::tmem_load32(dh_at + dh.i * P::DH_COLS + (quad * 32u << 16) + (half * NC + j) * 32u, g);
+            for (int p = 0; p < PIECES; ++p) {
+                uint32_t g[16], hv[8], dz[8];
+                tc::tmem_load16(dh_at + dh.i * P::DH_COLS + (quad * 32u << 16) + col0 + p * 16u, g);
                 tc::tmem_wait_load();
-                if (j == NC - 1) {
+                if (p == PIECES - 1) {
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.dh_empty[dh.i]);
                 }
-                transform_block<T, ACT, true>(codes[j], E[j], g, hv, dz);
-                // activations: 64-byte piece of row in_tile in the swizzled chunk
-                uint8_t *p = smem + P::H_AT + h.i * P::H_BYTES + (NC == 2 ? half * 16384u : 0u) + in_tile * 128u;
-                const uint32_t unit = (NC == 2 ? j : half) * 4u;
-#pragma unroll
-                for (uint32_t u = 0; u < 4; ++u)
-                    *reinterpret_cast<uint4 *>(p + (((unit + u) ^ (in_tile & 7u)) << 4)) =
-                        make_uint4(hv[4 * u], hv[4 * u + 1], hv[4 * u + 2], hv[4 * u + 3]);
-                if (a.dz && row < a.rows) store_row32<T>((T *)a.dz + row * a.cols, (block0 + j) * 32u, a.cols, a.dz_wide, dz);
+                transform16<T, ACT, true>(codes[p], sc, g, hv, dz);
+                if (a.dz && row < a.rows) store_row16<T>((T *)a.dz + row * a.cols, col + p * 16u, a.cols, a.dz_wide, dz);
+                // the last product that reads this buffer has had the time of the first piece to end
+                if (p == 0) {
+                    ok = __all_sync(~0u, tc::mbar_wait(&s.h_empty[h.i], h.phase ^ 1u, fail, a.err));
+                    if (!ok) break;
+                }
+                const uint32_t unit = ((col0 & 63u) >> 3) + p * 2u;
+                *reinterpret_cast<uint4 *>(to + ((unit ^ (in_tile & 7u)) << 4)) = make_uint4(hv[0], hv[1], hv[2], hv[3]);
+                *reinterpret_cast<uint4 *>(to + (((unit + 1u) ^ (in_tile & 7u)) << 4)) = make_uint4(hv[4], hv[5], hv[6], hv[7]);
             }
+            if (!ok) break;
             tc::fence_async_shared();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&s.h_full[h.i]);
             dh.next(2);
             h.next(P::H_BUFS);
 #pragma unroll
-            for (int j = 0; j < NC; ++j) {
+            for (int p = 0; p < PIECES; ++p)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) codes[j][i] = next[j][i];
-                E[j] = next_E[j];
-            }
+                for (int i = 0; i < 4; ++i) codes[p][i] = next[p][i];
+            E = next_E;
         }
         if (a.dw_parts) {
             ok = ok && tc::mbar_wait(&s.done, 0, fail, a.err);
@@ -290,13 +300,13 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 float *out = a.dw_parts + ((uint64_t)group * a.slabs + slab) * (NC * 64u) * (P::MT * 128u);
                 for (uint32_t m = 0; m < P::MT; ++m)
 #pragma unroll
-                    for (int j = 0; j < NC; ++j) {
-                        uint32_t v[32];
-                        const uint32_t n0 = (half * NC + j) * 32u;
-                        tc::tmem_load32(tmem + m * P::DH_COLS + (quad * 32u << 16) + n0, v);
+                    for (int p = 0; p < PIECES; ++p) {
+                        uint32_t v[16];
+                        const uint32_t n0 = col0 + p * 16u;
+                        tc::tmem_load16(tmem + m * P::DH_COLS + (quad * 32u << 16) + n0, v);
                         tc::tmem_wait_load();
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; ++i)
+                        for (uint32_t i = 0; i < 16; ++i)
                             out[(n0 + i) * (P::MT * 128u) + m * 128u + in_tile] = __uint_as_float(v[i]);
                     }
             }
@@ -484,7 +494,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
                 }
                 if (row >= a.m) continue;
                 if (DZ) {
-                    transform_block<T, ACT, false>(codes, E, v, nullptr, w);
+                    const f32x2 sc = both(mx8_scale(E));
+                    transform16<T, ACT, false>(codes, sc, v, nullptr, w);
+                    transform16<T, ACT, false>(codes + 4, sc, v + 16, nullptr, w + 8);
                     store_row32<T>((T *)a.out + row * a.n, col, (uint32_t)a.n, a.out_wide, w);
                 } else if (a.splits > 1) {
                     float *p = a.parts + ((uint64_t)split * a.m + row) * a.n + col;
