@@ -480,3 +480,44 @@ def test_entry_points_refuse():
     assert f("vt_mx4_linear")(p, 64, 0, 8, 64, 4, p, p, None, 0, p, p, 1 << 20, None, None) == 1 and "16" in err()
     assert f("vt_mx8_linear_bwd")(p, 4, p, 64, 2, 1 << 32, 64, 4, p, p, 0, p, p, p, p, 1 << 40, None, None) == 1 and "rows" in err()
     assert f("vt_mx8_linear_bwd")(p, 4, None, 64, 2, 8, 64, 4, p, p, 0, p, p, p, p, 1 << 40, None, None) == 1 and "null" in err()
+
+
+@pytest.mark.parametrize("rows,cols,outs", [(1, 64, 3), (65, 40, 16), (129, 64, 64), (161, 200, 256), (300, 96, 300), (1000, 264, 30)])
+def test_linear_backward_writes_its_outputs_only(rows, cols, outs):
+    """dz, dW and db in the middle of larger buffers, whose other bytes keep their value."""
+    from vorotracing_b200 import mx
+
+    z, dy, w = values(rows, cols, torch.bfloat16), values(rows, outs, torch.bfloat16, 1), values(outs, cols, torch.bfloat16, 2)
+    _, ckpt = mx.act_checkpoint(z, "silu")
+    want = mx.linear_backward(dy, w, ckpt)
+    pads = [torch.full((t.numel() + 131072,), 7.0, dtype=torch.bfloat16, device="cuda") for t in want]
+    at = 65536
+    p = [t.data_ptr() + 2 * at for t in pads]
+    copies = mx._unaligned(dy.data_ptr(), outs) + 2 * mx._unaligned(w.data_ptr(), cols)
+    n = mx._call("vt_mx8_linear_bwd_workspace_bytes")(rows, cols, outs, copies)
+    ws = torch.full((n + 131072,), 7, dtype=torch.uint8, device="cuda")
+    assert mx._call("vt_mx8_linear_bwd")(dy.data_ptr(), outs, w.data_ptr(), cols, 2, rows, cols, outs, ckpt.codes.data_ptr(),
+                                         ckpt.exps.data_ptr(), 2, *p, ws.data_ptr() + at, n, None, None) == 0
+    torch.cuda.synchronize()
+    assert (ws[:at] == 7).all() and (ws[at + n:] == 7).all()
+    for t, x in zip(want, pads):
+        assert torch.equal(x[at:at + t.numel()].view(t.shape), t)
+        assert (x[:at] == 7).all() and (x[at + t.numel():] == 7).all()
+
+
+@pytest.mark.parametrize("rows,cols,outs", [(1, 64, 3), (77, 1000, 333), (130, 96, 40), (9601, 40, 24), (9601, 96, 200), (1300, 64, 4000)])
+def test_linear4_writes_its_output_only(rows, cols, outs):
+    from vorotracing_b200 import mx
+
+    x, w = values(rows, cols, torch.float16), mx.quantize4(values(outs, cols, torch.float32, 1))
+    want = mx.linear4(x, w)
+    at = 65536
+    y = torch.full((want.numel() + 2 * at,), 7.0, dtype=torch.float16, device="cuda")
+    n = mx._call("vt_mx4_linear_workspace_bytes")(rows, cols, outs, mx._unaligned(x.data_ptr(), cols))
+    ws = torch.full((n + 2 * at,), 7, dtype=torch.uint8, device="cuda")
+    assert mx._call("vt_mx4_linear")(x.data_ptr(), cols, 1, rows, cols, outs, w.codes.data_ptr(), w.exps.data_ptr(), None, 0,
+                                     y.data_ptr() + 2 * at, ws.data_ptr() + at, n, None, None) == 0
+    torch.cuda.synchronize()
+    assert (ws[:at] == 7).all() and (ws[at + n:] == 7).all()
+    assert torch.equal(y[at:at + want.numel()].view(want.shape), want)
+    assert (y[:at] == 7).all() and (y[at + want.numel():] == 7).all()

@@ -3,16 +3,22 @@
 //
 // Layers with up to 256 outputs (narrow_kernel) make all three in one pass over the rows, so dy
 // and the checkpoint are read from HBM once and act(z8) never reaches memory.  A CTA owns a slab
-// of up to 128 columns of z and every G-th tile of 128 rows.  A tile of dy is staged once in
-// shared memory (TMA, 128-byte swizzle) and used twice: as the K-major A operand of
-// dH = dy W, and, the same bytes read the other way, as the MN-major A operand of
-// dW += dy^T act(z8), whose accumulator stays in tensor memory over all the CTA's rows.
-// Between the two products sixteen warps take dH out of tensor memory, read the 8-bit z, evaluate
-// act and act' together (one logistic serves both), write dz, and leave act(z8) in shared memory
-// as the second product's B operand, rounded to the operands' 16-bit type as the forward pass's
-// own activations are.  Two more warps add up dy's columns from the staged tile.  At its end a CTA
-// writes its part of dW in binary32; a second kernel adds the parts in order, so results do not
-// depend on timing.
+// of 128 columns of z and every G-th tile of 64 rows.  A tile of dy is staged once in shared
+// memory (TMA, 128-byte swizzle) and used twice: as the K-major B operand of dH^T = W^T dy^T,
+// whose result has z's columns in the lanes of tensor memory, and, the same bytes read the other
+// way, as the MN-major B operand of dW^T += act(z8)^T dy, whose accumulator stays in tensor memory
+// over all the CTA's rows.  Between the two products sixteen warps take dH out of tensor memory,
+// read the 8-bit z, evaluate act and act' together (one logistic serves both), write dz, and put
+// act(z8) back into the place of dH as the second product's A operand, rounded to the operands'
+// 16-bit type as the forward pass's own activations are.  Two more warps add up dy's columns from
+// the staged tile.  At its end a CTA writes its part of dW in binary32; a second kernel adds the
+// parts in order, so results do not depend on timing.
+//
+// Shared memory's bandwidth is what is short between HBM and the tensor cores here, which decides
+// the orientation: with z's columns in the lanes the activations need no shared memory at all, a
+// warp's dz is 64 contiguous bytes a row, and the second product reads one operand instead of two.
+// Layers of up to 64 columns would leave half of the lanes empty; they get W twice instead (FOLD),
+// and each half of the lanes takes half of a tile's rows.
 //
 // Wider layers are two matrix products (wide_kernel), both on pairs of CTAs that share a 256 x 256
 // tile: dz = (dy W) * act'(z8), with the slope in the epilogue, and dW = dy^T h with h = act(z8)
@@ -24,26 +30,23 @@ namespace vt {
 
 // ---- layers with up to 256 outputs ----
 
-constexpr uint32_t TILE_ROWS = 128, NARROW_OUTS = 256, NARROW_THREADS = 640;
+constexpr uint32_t TILE_ROWS = 64, NARROW_OUTS = 256, NARROW_THREADS = 672;
 
-// OC: dy's columns in chunks of 64; NC: the slab's columns in chunks of 64.
-template <int OC, int NC> struct Narrow {
-    static constexpr uint32_t W_BYTES = OC * 8192u * NC, DY_BYTES = OC * 16384u, H_BYTES = NC * 16384u;
-    static constexpr int PIECES = NC;  // of 16 columns an activation warp takes: 4 warps a quadrant
-    // as much staging as 227 KB hold
-    static constexpr uint32_t STAGES = OC >= 3 ? 2 : OC == 2 ? 3 : 4, H_BUFS = OC == 4 && NC == 2 ? 1 : 2;
-    static constexpr uint32_t DY_AT = W_BYTES, H_AT = DY_AT + STAGES * DY_BYTES, CTRL_AT = H_AT + H_BUFS * H_BYTES;
-    static constexpr uint32_t MT = (OC + 1) / 2;                 // accumulator tiles of 128 outputs
-    static constexpr uint32_t DW_COLS = MT * NC * 64u, DH_COLS = NC * 64u;
-    static constexpr uint32_t TMEM_USED = DW_COLS + 2u * DH_COLS;
-    static constexpr uint32_t TMEM = TMEM_USED <= 128 ? 128 : TMEM_USED <= 256 ? 256 : 512;
+// OC: dy's columns in chunks of 64.  A slab is 128 columns of z, or all of up to 64 (FOLD).
+template <int OC, bool FOLD> struct Narrow {
+    static constexpr uint32_t W_BYTES = OC * 16384u, CHUNK = TILE_ROWS * 128u, DY_BYTES = OC * CHUNK, CODE_PITCH = FOLD ? 64u : 128u;
+    static constexpr uint32_t STAGE = DY_BYTES + TILE_ROWS * CODE_PITCH;
     struct Ctrl {
-        uint64_t full[STAGES], empty[STAGES], dh_full[2], dh_empty[2], h_full[H_BUFS], h_empty[H_BUFS], w_full, done;
+        float scale[16][32];  // of the blocks in each activation warp's rows
+        uint64_t full[8], empty[8], dh_full[4], dh_empty[4], h_full[4], w_full, done, failed;
         uint32_t tmem;
         tc::Fail fail;
     };
-    static constexpr uint32_t SMEM = CTRL_AT + sizeof(Ctrl);
-    static_assert(TMEM_USED <= 512 && SMEM <= 232448, "does not fit an SM");
+    static constexpr uint32_t FIT = (232448u - W_BYTES - sizeof(Ctrl)) / STAGE, STAGES = FIT < 8u ? FIT : 8u;
+    static constexpr uint32_t CTRL_AT = W_BYTES + STAGES * STAGE, SMEM = CTRL_AT + sizeof(Ctrl);
+    static constexpr uint32_t DH_AT = OC * 64u, TMEM = 512;  // columns: dW, then four of dH
+    static constexpr int ROWS = FOLD ? 16 : 32;  // of a tile an activation warp takes
+    static_assert(STAGES >= 4 && DH_AT + 256u <= TMEM, "does not fit an SM");
 };
 
 struct NarrowArgs {
@@ -52,16 +55,15 @@ struct NarrowArgs {
     const int8_t *codes;
     const uint8_t *exps;
     void *dz;          // null: not wanted
-    float *dw_parts;   // [group][slab][NC * 64][MT * 128]; null: dW not wanted
+    float *dw_parts;   // [group][slab][OC * 64][128]; null: dW not wanted
     float *db_parts;   // [group][2][OC * 64]; null: db not wanted
     uint32_t *err;
-    bool dz_wide;      // dz's rows hold whole 32-byte pieces
 };
 
-// 16 columns of a row: codes (4 words) and their block's scale, g = dH (binary32) in, h and dz out
-// as packed 16-bit pairs.
-template <typename T, int ACT, bool VALUE>
-__device__ __forceinline__ void transform16(const uint32_t *codes, f32x2 sc, const uint32_t *g, uint32_t *h, uint32_t *dz)
+// 16 columns of a row: codes (4 words) and their block's scale, g = dH (binary32) in, dz out as
+// packed 16-bit pairs.
+template <typename T, int ACT>
+__device__ __forceinline__ void slope16(const uint32_t *codes, f32x2 sc, const uint32_t *g, uint32_t *dz)
 {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -69,30 +71,22 @@ __device__ __forceinline__ void transform16(const uint32_t *codes, f32x2 sc, con
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int at = 2 * w + i;
-            const f32x2 z = mul2(code_pair(c, 2 * i), sc), gp = pair(__uint_as_float(g[2 * at]), __uint_as_float(g[2 * at + 1]));
-            if constexpr (ACT == ACT_RELU) {
-                const float2 v = unpair(z), d = unpair(gp), zero = unpair(mul2(sc, both(0.0f)));  // NaN in a NaN block
-                if (VALUE) h[at] = pack2<T>(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
-                dz[at] = pack2<T>(v.x > 0.0f ? d.x : zero.x, v.y > 0.0f ? d.y : zero.x);
-            } else {
-                f32x2 v, slope;
-                act_pair<ACT, VALUE, true>(z, v, slope);
-                if (VALUE) h[at] = pack2<T>(v);
-                dz[at] = pack2<T>(ACT == ACT_IDENTITY ? gp : mul2(gp, slope));
-            }
+            const f32x2 gp = pair(__uint_as_float(g[2 * at]), __uint_as_float(g[2 * at + 1]));
+            dz[at] = pack2<T>(ACT == ACT_IDENTITY ? gp : mul2(gp, act_slope2<ACT>(mul2(code_pair(c, 2 * i), sc))));
         }
     }
 }
 
-template <typename T, int ACT, int OC, int NC>
+template <typename T, int ACT, int OC, bool FOLD>
 __global__ void __launch_bounds__(NARROW_THREADS, 1)
-    narrow_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap w_map, const NarrowArgs a)
+    narrow_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap w_map,
+                  const __grid_constant__ CUtensorMap code_map, const NarrowArgs a)
 {
-    using P = Narrow<OC, NC>;
+    using P = Narrow<OC, FOLD>;
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(1024) uint8_t smem[];
     typename P::Ctrl &s = *reinterpret_cast<typename P::Ctrl *>(smem + P::CTRL_AT);
-    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    const uint32_t warp = tc::warp_number(), lane = threadIdx.x % 32u;
     const uint32_t slab = blockIdx.x % a.slabs, group = blockIdx.x / a.slabs;
     // dy's chunks are shared out among the slabs for the column sums
     const uint32_t sharers = a.slabs < OC ? a.slabs : OC;
@@ -104,40 +98,40 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             tc::mbar_init(&s.full[i], 1);
             tc::mbar_init(&s.empty[i], sums ? 3 : 1);
         }
-        for (uint32_t i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < 4; ++i) {
             tc::mbar_init(&s.dh_full[i], 1);
-            tc::mbar_init(&s.dh_empty[i], 16);
-        }
-        for (uint32_t i = 0; i < P::H_BUFS; ++i) {
-            tc::mbar_init(&s.h_full[i], 16);
-            tc::mbar_init(&s.h_empty[i], 1);
+            tc::mbar_init(&s.dh_empty[i], 1);
+            tc::mbar_init(&s.h_full[i], 8);
         }
         tc::mbar_init(&s.w_full, 1);
         tc::mbar_init(&s.done, 1);
+        tc::mbar_init(&s.failed, 1);
         s.fail.failed = 0;
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&dy_map);
         tc::tma_prefetch_map(&w_map);
+        tc::tma_prefetch_map(&code_map);
     }
     if (warp == 1) tc::tmem_alloc<P::TMEM>(&s.tmem);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = s.tmem, dh_at = tmem + P::DW_COLS;
+    const uint32_t tmem = s.tmem, dh_at = tmem + P::DH_AT;
 
     if (warp == 0) {
         if (lane == 0) {  // TMA
             uint32_t issued = 0;
             tc::mbar_arrive_tx(&s.w_full, P::W_BYTES);
-            for (int n = 0; n < NC; ++n)
-                tc::tma_load_2d(smem + n * (OC * 8192), &w_map, (int)(slab * NC + n) * 64, 0, &s.w_full);
+            for (int n = 0; n < 2; ++n)  // FOLD: the same 64 columns twice
+                tc::tma_load_2d(smem + n * (OC * 8192), &w_map, FOLD ? 0 : (int)(slab * 2 + n) * 64, 0, &s.w_full);
             tc::Ring r;
             for (uint32_t t = group; t < a.tiles; t += a.groups) {
                 if (!tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err)) break;
-                tc::mbar_arrive_tx(&s.full[r.i], P::DY_BYTES);
+                uint8_t *st = smem + P::W_BYTES + r.i * P::STAGE;
+                tc::mbar_arrive_tx(&s.full[r.i], P::STAGE);
                 for (int c = 0; c < OC; ++c)
-                    tc::tma_load_2d(smem + P::DY_AT + r.i * P::DY_BYTES + c * 16384, &dy_map, c * 64, (int)(t * TILE_ROWS),
-                                    &s.full[r.i]);
+                    tc::tma_load_2d(st + c * (TILE_ROWS * 128u), &dy_map, c * 64, (int)(t * TILE_ROWS), &s.full[r.i]);
+                tc::tma_load_2d(st + P::DY_BYTES, &code_map, (int)(slab * 128), (int)(t * TILE_ROWS), &s.full[r.i]);
                 ++issued;
                 r.next(P::STAGES);
             }
@@ -147,69 +141,80 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                     tc::mbar_wait_slow(&s.full[i], ((issued - 1 - i) / P::STAGES) & 1u, fail, a.err, true);
             }
         }
-    } else if (warp == 1) {
-        if (lane == 0) {  // products
-            constexpr uint32_t ID_DH = tc::idesc_f16<BF16>(128, P::DH_COLS, false, true);
-            constexpr uint32_t ID_DW = tc::idesc_f16<BF16>(128, P::DH_COLS, true, true);
-            const uint32_t w_addr = tc::smem_u32(smem), dy_addr = w_addr + P::DY_AT, h_addr = w_addr + P::H_AT;
-            tc::Ring r, dh, h, prev;
-            bool ok = tc::mbar_wait(&s.w_full, 0, fail, a.err), first = true;
-            // dW += dy^T h of the tile before the current one: its activations are ready only now.
-            // For an odd number of chunks the last accumulator tile's upper 64 rows come from
-            // whatever follows in shared memory; they are never read.
-            auto weight_product = [&]() -> bool {
-                if (!tc::mbar_wait(&s.h_full[h.i], h.phase, fail, a.err)) return false;
-                tc::fence_after();
-                if (a.dw_parts) {
-                    for (uint32_t m = 0; m < P::MT; ++m)
-                        for (uint32_t k = 0; k < 8; ++k)
-                            tc::mma_f16(tmem + m * P::DH_COLS,
-                                        tc::smem_desc(dy_addr + prev.i * P::DY_BYTES + m * 32768u + k * 2048u, 16384, 1024),
-                                        tc::smem_desc(h_addr + h.i * P::H_BYTES + k * 2048u, 16384, 1024), ID_DW,
-                                        !(first && k == 0));
-                    first = false;
-                }
-                tc::commit(&s.h_empty[h.i]);
-                tc::commit(&s.empty[prev.i]);
-                h.next(P::H_BUFS);
-                prev.next(P::STAGES);
-                return true;
-            };
-            for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
-                ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err) &&
-                     tc::mbar_wait(&s.dh_empty[dh.i], dh.phase ^ 1u, fail, a.err);
-                if (!ok) break;
-                tc::fence_after();
+    } else if (warp == 1) {  // dH^T = W^T dy^T
+        constexpr uint32_t ID = tc::idesc_f16<BF16>(128, TILE_ROWS, true, false);
+        const uint32_t w_addr = tc::smem_u32(smem), st_addr = w_addr + P::W_BYTES;
+        const uint64_t w_desc = tc::smem_desc(w_addr, OC * 8192u, 1024);
+        const bool mine = tc::elect();
+        tc::Ring r, dh;
+        bool ok = __all_sync(~0u, tc::mbar_wait(&s.w_full, 0, fail, a.err));
+        for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
+            ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err) &&
+                                     tc::mbar_wait(&s.dh_empty[dh.i], dh.phase ^ 1u, fail, a.err));
+            if (!ok) break;
+            tc::fence_after();
+            const uint64_t b = tc::smem_desc(st_addr + r.i * P::STAGE, 16, 1024);
+            if (mine) {
+#pragma unroll
                 for (uint32_t c = 0; c < OC; ++c)
+#pragma unroll
                     for (uint32_t k = 0; k < 4; ++k)
-                        tc::mma_f16(dh_at + dh.i * P::DH_COLS,
-                                    tc::smem_desc(dy_addr + r.i * P::DY_BYTES + c * 16384u + k * 32u, 16, 1024),
-                                    tc::smem_desc(w_addr + c * 8192u + k * 2048u, OC * 8192u, 1024), ID_DH, c + k != 0);
+                        tc::mma_f16(dh_at + dh.i * TILE_ROWS, w_desc + c * 512u + k * 128u, b + c * (P::CHUNK >> 4) + k * 2u, ID, c + k != 0);
                 tc::commit(&s.dh_full[dh.i]);
-                r.next(P::STAGES);
-                dh.next(2);
-                if (t != group) ok = weight_product();
             }
-            if (ok) ok = weight_product();
-            tc::commit(&s.done);
-            if (!ok) tc::mbar_wait_slow(&s.done, 0, fail, a.err, true);  // leave no product in flight
+            __syncwarp();
+            r.next(P::STAGES);
+            dh.next(4);
         }
+        if (!ok) {  // leave no product in flight
+            if (mine) tc::commit(&s.failed);
+            tc::mbar_wait_slow(&s.failed, 0, fail, a.err, true);
+        }
+    } else if (warp == 20) {  // dW^T += h^T dy, behind the activations; in a warp of its own, so that neither product waits
+                              // for what the other one waits for
+        constexpr uint32_t ID = tc::idesc_f16<BF16>(128, OC * 64, false, true);
+        const uint32_t st_addr = tc::smem_u32(smem) + P::W_BYTES;
+        const bool mine = tc::elect();
+        tc::Ring r, h;
+        bool ok = true;
+        for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
+            ok = __all_sync(~0u, tc::mbar_wait(&s.h_full[h.i], h.phase, fail, a.err) &&
+                                     tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
+            if (!ok) break;
+            tc::fence_after();
+            const uint64_t b = tc::smem_desc(st_addr + r.i * P::STAGE, P::CHUNK, 1024);
+            const uint32_t from = dh_at + h.i * TILE_ROWS;
+            if (mine) {
+                if (a.dw_parts) {
+                    tc::mma_f16_tmem(tmem, from, b, ID, t != group);
+#pragma unroll
+                    for (uint32_t k = 1; k < TILE_ROWS / 16u; ++k) tc::mma_f16_tmem(tmem, from + k * 16u, b + k * 128u, ID, true);
+                }
+                tc::commit(&s.empty[r.i]);
+                tc::commit(&s.dh_empty[h.i]);
+            }
+            __syncwarp();
+            r.next(P::STAGES);
+            h.next(4);
+        }
+        if (mine) tc::commit(&s.done);
+        if (!ok) tc::mbar_wait_slow(&s.done, 0, fail, a.err, true);  // leave no product in flight
     } else if (warp < 4) {
         if (sums) {  // column sums: each of the two warps takes half of a tile's rows, a lane two columns
             tc::Ring r;
             f32x2 total[OC] = {};
             bool ok = true;
-            const uint32_t row0 = (warp - 2u) * 64u;
+            const uint32_t row0 = (warp - 2u) * (TILE_ROWS / 2u);
             for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
                 ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
                 if (!ok) break;
 #pragma unroll
                 for (int c = 0; c < OC; ++c) {
                     if (c % sharers != slab) continue;
-                    const uint8_t *p = smem + P::DY_AT + r.i * P::DY_BYTES + c * 16384 + row0 * 128u;
+                    const uint8_t *p = smem + P::W_BYTES + r.i * P::STAGE + c * (TILE_ROWS * 128u) + row0 * 128u;
                     f32x2 v = 0;
 #pragma unroll 8
-                    for (uint32_t i = 0; i < 64; ++i) {
+                    for (uint32_t i = 0; i < TILE_ROWS / 2u; ++i) {
                         const float2 x = unpack2<T>(*reinterpret_cast<const uint32_t *>(p + i * 128u + ((lane * 4u) ^ (i & 7u) << 4)));
                         v = add2(v, pair(x.x, x.y));
                     }
@@ -225,119 +230,149 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                     *reinterpret_cast<f32x2 *>(a.db_parts + ((uint64_t)group * 2u + (warp - 2u)) * (OC * 64u) + c * 64u + lane * 2u) =
                         total[c];
         }
-    } else {  // activations: a warp has rows 32 (w % 4).. of the tile and a quarter of the slab's columns
-        constexpr int PIECES = P::PIECES;
-        const uint32_t quad = warp % 4u, part = (warp - 4u) / 4u, in_tile = quad * 32u + lane;
-        const uint32_t col0 = part * PIECES * 16u, col = slab * NC * 64u + col0;  // in the slab, in the row
-        uint32_t codes[PIECES][4], E;
-        auto fetch = [&](uint32_t t, uint32_t (&c)[PIECES][4], uint32_t &e) {
-            const uint64_t row = (uint64_t)t * TILE_ROWS + in_tile;
-            if (t < a.tiles && row < a.rows && col < a.blocks * 32u) {
-                const uint64_t at = row * a.blocks * 32u + col;
-                if (PIECES == 2) load32(a.codes + at, c[0]);  // c[0] and c[1] are neighbours
-                else {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(a.codes + at));
-                    c[0][0] = v.x; c[0][1] = v.y; c[0][2] = v.z; c[0][3] = v.w;
-                }
-                e = __ldg(a.exps + (at >> 5));
-            } else {
-#pragma unroll
-                for (int p = 0; p < PIECES; ++p)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) c[p][i] = 0;
-                e = 127;
-            }
+    } else {  // activations: two sets of eight warps take tiles in turn; a lane has a column of z (a
+              // warp one block of 32) and ROWS rows of the tile
+        constexpr int ROWS = P::ROWS;
+        const uint32_t quad = warp % 4u, set = (warp - 4u) / 8u, part = (warp - 4u) / 4u % 2u;
+        const uint32_t block = FOLD ? quad & 1u : slab * 4u + quad, n = block * 32u + lane;
+        const uint32_t row0 = FOLD ? (quad >> 1) * 32u + part * 16u : part * 32u;  // in the tile
+        const uint32_t lanes = quad * 32u << 16, code0 = row0 * P::CODE_PITCH + (FOLD ? n : quad * 32u + lane);
+        float *const scale = s.scale[warp - 4u];
+        // exponent byte of this warp's block in row lane of its rows
+        auto exponent = [&](uint32_t t) -> uint32_t {
+            const uint64_t row = (uint64_t)t * TILE_ROWS + row0 + lane;
+            return t < a.tiles && lane < ROWS && row < a.rows && block < a.blocks ? __ldg(a.exps + row * a.blocks + block) : 127u;
         };
-        fetch(group, codes, E);
-        tc::Ring dh, h;
+        const uint32_t first = group + set * a.groups, step = 2u * a.groups;
+        uint32_t E = exponent(first);
+        tc::Ring r, dh;
+        if (set) { r.next(P::STAGES); dh.next(4); }
         bool ok = true;
-        for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
-            const uint64_t row = (uint64_t)t * TILE_ROWS + in_tile;
-            uint32_t next[PIECES][4], next_E;
-            fetch(t + a.groups, next, next_E);
-            ok = __all_sync(~0u, tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err));
+        for (uint32_t t = first; t < a.tiles && ok; t += step) {
+            const uint64_t row = (uint64_t)t * TILE_ROWS + row0;
+            const uint32_t next_E = exponent(t + step);
+            __syncwarp();
+            scale[lane] = mx8_scale(E);
+            __syncwarp();
+            ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err) &&
+                                     tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err));
             if (!ok) break;
             tc::fence_after();
-            const f32x2 sc = both(mx8_scale(E));
-            uint8_t *to = smem + P::H_AT + h.i * P::H_BYTES + (col0 >> 6) * 16384u + in_tile * 128u;
+            const uint8_t *codes = smem + P::W_BYTES + r.i * P::STAGE + P::DY_BYTES + code0;
+            const uint32_t buffer = dh_at + dh.i * TILE_ROWS + lanes, here = buffer + row0;
+            const uint32_t count = row >= a.rows ? 0u : a.rows - row < (uint64_t)ROWS ? (uint32_t)(a.rows - row) : ROWS;
+            unsigned short *out = (unsigned short *)a.dz + row * a.cols + n;
+            const bool write = a.dz && n < a.cols;
 #pragma unroll
-            for (int p = 0; p < PIECES; ++p) {
-                uint32_t g[16], hv[8], dz[8];
-                tc::tmem_load16(dh_at + dh.i * P::DH_COLS + (quad * 32u << 16) + col0 + p * 16u, g);
+            for (int p = 0; p < ROWS; p += 16) {
+                uint32_t g[16], h[8], d[8];
+                tc::tmem_load16(here + p, g);
                 tc::tmem_wait_load();
-                if (p == PIECES - 1) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t c0 = codes[(p + 2 * i) * P::CODE_PITCH], c1 = codes[(p + 2 * i + 1) * P::CODE_PITCH];
+                    // a code's byte with its sign bit turned, under the exponent of 2^23, is 2^23 + 128 + code
+                    const f32x2 sc = *reinterpret_cast<const f32x2 *>(scale + p + 2 * i);
+                    const f32x2 z = mul2(add2(pair(__uint_as_float(c0 ^ 0x4b000080u), __uint_as_float(c1 ^ 0x4b000080u)),
+                                              both(-8388736.0f)), sc);
+                    const f32x2 gp = pair(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+                    if constexpr (ACT == ACT_RELU) {
+                        const float2 v = unpair(z), q = unpair(gp), zero = unpair(mul2(sc, both(0.0f)));  // NaN in a NaN block
+                        h[i] = pack2<T>(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
+                        d[i] = pack2<T>(v.x > 0.0f ? q.x : zero.x, v.y > 0.0f ? q.y : zero.y);
+                    } else {
+                        f32x2 v, slope;
+                        act_pair<ACT, true, true>(z, v, slope);
+                        h[i] = pack2<T>(v);
+                        d[i] = pack2<T>(ACT == ACT_IDENTITY ? gp : mul2(gp, slope));
+                    }
+                }
+                // the activations go where the dH that this warp has read was
+                tc::tmem_store8(here + p, h);
+                if (FOLD) {  // this half of the lanes has no part in the other half's rows
+                    const uint32_t none[8] = {};
+                    tc::tmem_store8(buffer + (row0 ^ 32u), none);
+                }
+                if (p + 16 == ROWS) {
+                    tc::tmem_wait_store();
                     tc::fence_before();
                     __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&s.dh_empty[dh.i]);
+                    if (lane == 0) tc::mbar_arrive(&s.h_full[dh.i]);
                 }
-                transform16<T, ACT, true>(codes[p], sc, g, hv, dz);
-                if (a.dz && row < a.rows) store_row16<T>((T *)a.dz + row * a.cols, col + p * 16u, a.cols, a.dz_wide, dz);
-                // the last product that reads this buffer has had the time of the first piece to end
-                if (p == 0) {
-                    ok = __all_sync(~0u, tc::mbar_wait(&s.h_empty[h.i], h.phase ^ 1u, fail, a.err));
-                    if (!ok) break;
+                if (write) {
+                    if (count == ROWS) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            out[0] = (unsigned short)d[i];
+                            out[a.cols] = (unsigned short)(d[i] >> 16);
+                            out += 2 * a.cols;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            if (p + 2 * i < count) out[0] = (unsigned short)d[i];
+                            if (p + 2 * i + 1 < count) out[a.cols] = (unsigned short)(d[i] >> 16);
+                            out += 2 * a.cols;
+                        }
+                    }
                 }
-                const uint32_t unit = ((col0 & 63u) >> 3) + p * 2u;
-                *reinterpret_cast<uint4 *>(to + ((unit ^ (in_tile & 7u)) << 4)) = make_uint4(hv[0], hv[1], hv[2], hv[3]);
-                *reinterpret_cast<uint4 *>(to + (((unit + 1u) ^ (in_tile & 7u)) << 4)) = make_uint4(hv[4], hv[5], hv[6], hv[7]);
             }
-            if (!ok) break;
-            tc::fence_async_shared();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&s.h_full[h.i]);
-            dh.next(2);
-            h.next(P::H_BUFS);
-#pragma unroll
-            for (int p = 0; p < PIECES; ++p)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) codes[p][i] = next[p][i];
+            dh.next(4);
+            dh.next(4);
+            r.next(P::STAGES);
+            r.next(P::STAGES);
             E = next_E;
         }
         if (a.dw_parts) {
             ok = ok && tc::mbar_wait(&s.done, 0, fail, a.err);
             if (__all_sync(~0u, ok)) {
                 tc::fence_after();
-                float *out = a.dw_parts + ((uint64_t)group * a.slabs + slab) * (NC * 64u) * (P::MT * 128u);
-                for (uint32_t m = 0; m < P::MT; ++m)
+                float *out = a.dw_parts + ((uint64_t)group * a.slabs + slab) * (OC * 64u) * 128u + quad * 32u + lane;
 #pragma unroll
-                    for (int p = 0; p < PIECES; ++p) {
-                        uint32_t v[16];
-                        const uint32_t n0 = col0 + p * 16u;
-                        tc::tmem_load16(tmem + m * P::DH_COLS + (quad * 32u << 16) + n0, v);
-                        tc::tmem_wait_load();
+                for (uint32_t c = 0; c < OC; ++c) {
+                    const uint32_t o0 = ((set * 2u + part) * OC + c) * 16u;
+                    uint32_t v[16];
+                    tc::tmem_load16(tmem + lanes + o0, v);
+                    tc::tmem_wait_load();
 #pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i)
-                            out[(n0 + i) * (P::MT * 128u) + m * 128u + in_tile] = __uint_as_float(v[i]);
-                    }
+                    for (uint32_t i = 0; i < 16; ++i) out[(o0 + i) * 128u] = __uint_as_float(v[i]);
+                }
             }
         }
     }
+    __syncwarp();
     tc::fence_before();
     __syncthreads();
     if (warp == 1) tc::tmem_free<P::TMEM>(tmem);
 }
 
-// Adds the groups' parts in order: dw (outs, cols) and db (outs).
+// Adds the groups' parts in order: dw (outs, cols) and db (outs).  A part has 128 columns a slab;
+// with one slab of up to 64 (fold) its two halves come from different rows and are added.
 template <typename T>
 __global__ void __launch_bounds__(256) narrow_reduce_kernel(const float *__restrict__ dw_parts, const float *__restrict__ db_parts,
-                                                            uint32_t groups, uint32_t slabs, uint32_t slab_cols, uint32_t part_outs,
+                                                            uint32_t groups, uint32_t slabs, uint32_t part_outs, bool fold,
                                                             uint32_t cols, uint32_t outs, T *__restrict__ dw, T *__restrict__ db)
 {
-    const uint64_t per_group = (uint64_t)slabs * slab_cols * part_outs;
+    const uint64_t per_group = (uint64_t)slabs * part_outs * 128u;
     const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
     if (dw && i < per_group) {
-        const uint32_t o = (uint32_t)(i % part_outs), n = (uint32_t)(i / part_outs);
+        const uint32_t o = (uint32_t)(i / 128u % part_outs), n = (uint32_t)(i / 128u / part_outs) * 128u + (uint32_t)(i % 128u);
         if (o < outs && n < cols) {
             float v = 0.0f;
 #pragma unroll 8
             for (uint32_t g = 0; g < groups; ++g) v += __ldg(dw_parts + g * per_group + i);
+            if (fold) {
+                float u = 0.0f;
+#pragma unroll 8
+                for (uint32_t g = 0; g < groups; ++g) u += __ldg(dw_parts + g * per_group + i + 64u);
+                v += u;
+            }
             dw[(uint64_t)o * cols + n] = from_f32<T>(v);
         }
     }
     if (db && i < outs) {
-        const uint32_t pad = (outs + 63u) / 64u * 64u;
         float v = 0.0f;
-        for (uint32_t g = 0; g < 2u * groups; ++g) v += __ldg(db_parts + (uint64_t)g * pad + i);
+        for (uint32_t g = 0; g < 2u * groups; ++g) v += __ldg(db_parts + (uint64_t)g * part_outs + i);
         db[i] = from_f32<T>(v);
     }
 }
@@ -495,8 +530,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
                 if (row >= a.m) continue;
                 if (DZ) {
                     const f32x2 sc = both(mx8_scale(E));
-                    transform16<T, ACT, false>(codes, sc, v, nullptr, w);
-                    transform16<T, ACT, false>(codes + 4, sc, v + 16, nullptr, w + 8);
+                    slope16<T, ACT>(codes, sc, v, w);
+                    slope16<T, ACT>(codes + 4, sc, v + 16, w + 8);
                     store_row32<T>((T *)a.out + row * a.n, col, (uint32_t)a.n, a.out_wide, w);
                 } else if (a.splits > 1) {
                     float *p = a.parts + ((uint64_t)split * a.m + row) * a.n + col;
@@ -612,23 +647,24 @@ enum : int { COPY_DY = 1, COPY_WEIGHT = 2 };
 
 // How a narrow call is cut, and where its workspace parts lie.
 struct NarrowPlan {
-    uint32_t oc, nc, slabs, tiles, groups, part_outs;
+    uint32_t oc, slabs, tiles, groups, part_outs;
+    bool fold;
     uint64_t dw_at, db_at, dy_at, w_at, bytes;
 };
 static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, int copies, uint32_t sms)
 {
     NarrowPlan p;
     p.oc = (outs + 63u) / 64u;
-    p.nc = cols <= 64u ? 1u : 2u;
-    p.slabs = (cols + p.nc * 64u - 1u) / (p.nc * 64u);
+    p.fold = cols <= 64u;
+    p.slabs = (cols + 127u) / 128u;
     p.tiles = (uint32_t)((rows + TILE_ROWS - 1u) / TILE_ROWS);
     // one CTA an SM; a slab more than there are SMs still gets its own
     p.groups = p.slabs < sms ? sms / p.slabs : 1u;
     if (p.groups > p.tiles) p.groups = p.tiles;
-    p.part_outs = (p.oc + 1u) / 2u * 128u;
+    p.part_outs = p.oc * 64u;
     p.dw_at = 0;
-    p.db_at = p.dw_at + align_up((uint64_t)p.groups * p.slabs * p.nc * 64u * p.part_outs * 4u, 256);
-    p.dy_at = p.db_at + align_up((uint64_t)p.groups * 2u * p.oc * 64u * 4u, 256);
+    p.db_at = p.dw_at + align_up((uint64_t)p.groups * p.slabs * 128u * p.part_outs * 4u, 256);
+    p.dy_at = p.db_at + align_up((uint64_t)p.groups * 2u * p.part_outs * 4u, 256);
     p.w_at = p.dy_at + (copies & COPY_DY ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
     p.bytes = p.w_at + (copies & COPY_WEIGHT ? align_up((uint64_t)outs * align_up(cols, 8) * 2u, 256) : 0);
     return p;
@@ -639,13 +675,17 @@ template <typename T> static int copies_of(const void *dy, uint64_t dy_stride, c
     return (whole_words<T>(dy, dy_stride) ? 0 : COPY_DY) | (whole_words<T>(w, w_stride) ? 0 : COPY_WEIGHT);
 }
 
-template <typename T, int ACT, int OC, int NC>
+template <typename T, int ACT, int OC, bool FOLD>
 static vt_status launch_narrow(const CUtensorMap &dy, const CUtensorMap &w, const NarrowArgs &a, cudaStream_t stream)
 {
     static std::atomic<uint64_t> allowed{0};
-    using P = Narrow<OC, NC>;
-    if (vt_status s = tc::allow_smem(narrow_kernel<T, ACT, OC, NC>, P::SMEM, allowed)) return s;
-    narrow_kernel<T, ACT, OC, NC><<<a.groups * a.slabs, NARROW_THREADS, P::SMEM, stream>>>(dy, w, a);
+    using P = Narrow<OC, FOLD>;
+    CUtensorMap codes;
+    const uint64_t width = (uint64_t)a.blocks * 32u;
+    if (vt_status s = tc::make_map(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.rows, width, width, TILE_ROWS, P::CODE_PITCH, false))
+        return s;
+    if (vt_status s = tc::allow_smem(narrow_kernel<T, ACT, OC, FOLD>, P::SMEM, allowed)) return s;
+    narrow_kernel<T, ACT, OC, FOLD><<<a.groups * a.slabs, NARROW_THREADS, P::SMEM, stream>>>(dy, w, codes, a);
     return check_launch("narrow_kernel");
 }
 
@@ -674,22 +714,21 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     a.dw_parts = dw ? (float *)(workspace + p.dw_at) : nullptr;
     a.db_parts = db ? (float *)(workspace + p.db_at) : nullptr;
     a.err = err;
-    a.dz_wide = cols % 16u == 0 && aligned32(dz);
     vt_status s = VT_OK;
-    switch (p.oc * 2u + p.nc) {
-    case 3: s = launch_narrow<T, ACT, 1, 1>(dy_map, w_map, a, stream); break;
-    case 4: s = launch_narrow<T, ACT, 1, 2>(dy_map, w_map, a, stream); break;
-    case 5: s = launch_narrow<T, ACT, 2, 1>(dy_map, w_map, a, stream); break;
-    case 6: s = launch_narrow<T, ACT, 2, 2>(dy_map, w_map, a, stream); break;
-    case 7: s = launch_narrow<T, ACT, 3, 1>(dy_map, w_map, a, stream); break;
-    case 8: s = launch_narrow<T, ACT, 3, 2>(dy_map, w_map, a, stream); break;
-    case 9: s = launch_narrow<T, ACT, 4, 1>(dy_map, w_map, a, stream); break;
-    default: s = launch_narrow<T, ACT, 4, 2>(dy_map, w_map, a, stream); break;
+    switch (p.oc * 2u + p.fold) {
+    case 2: s = launch_narrow<T, ACT, 1, false>(dy_map, w_map, a, stream); break;
+    case 3: s = launch_narrow<T, ACT, 1, true>(dy_map, w_map, a, stream); break;
+    case 4: s = launch_narrow<T, ACT, 2, false>(dy_map, w_map, a, stream); break;
+    case 5: s = launch_narrow<T, ACT, 2, true>(dy_map, w_map, a, stream); break;
+    case 6: s = launch_narrow<T, ACT, 3, false>(dy_map, w_map, a, stream); break;
+    case 7: s = launch_narrow<T, ACT, 3, true>(dy_map, w_map, a, stream); break;
+    case 8: s = launch_narrow<T, ACT, 4, false>(dy_map, w_map, a, stream); break;
+    default: s = launch_narrow<T, ACT, 4, true>(dy_map, w_map, a, stream); break;
     }
     if (s || !(dw || db)) return s;
-    const uint64_t n = (uint64_t)p.slabs * p.nc * 64u * p.part_outs;
-    narrow_reduce_kernel<T><<<(unsigned)((n + 255u) / 256u), 256, 0, stream>>>(a.dw_parts, a.db_parts, p.groups, p.slabs, p.nc * 64u,
-                                                                           p.part_outs, cols, outs, (T *)dw, (T *)db);
+    const uint64_t n = (uint64_t)p.slabs * 128u * p.part_outs;
+    narrow_reduce_kernel<T><<<(unsigned)((n + 255u) / 256u), 256, 0, stream>>>(a.dw_parts, a.db_parts, p.groups, p.slabs, p.part_outs,
+                                                                           p.fold, cols, outs, (T *)dw, (T *)db);
     return check_launch("narrow_reduce_kernel");
 }
 

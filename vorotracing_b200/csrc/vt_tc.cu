@@ -25,7 +25,7 @@ static EncodeTiled encode_tiled()
 }
 
 vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint64_t cols,
-                   uint64_t pitch, uint32_t box_rows, uint32_t box_cols)
+                   uint64_t pitch, uint32_t box_rows, uint32_t box_cols, bool swizzle)
 {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return set_error(VT_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
@@ -33,7 +33,7 @@ vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, ui
     const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
     const auto make = [&] {
         return encode(map, type, 2, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                      swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
     CUresult r = make();
     if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread that has made no runtime call yet, as autograd's

@@ -137,6 +137,25 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t *r)
                  : "r"(addr));
 }
 
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One lane of a converged warp, the same each time.  Roles run with their whole warp and only
+// their asynchronous instructions under it, so that addresses and descriptors stay in uniform
+// registers, where those instructions want them.
+__device__ __forceinline__ bool elect()
+{
+    uint32_t p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p;
+}
+// The warp's number in its block, known to be the same in all its lanes
+__device__ __forceinline__ uint32_t warp_number() { return __shfl_sync(~0u, threadIdx.x / 32u, 0); }
+
 // ---- products ----
 
 // Shared-memory operand in the 128-byte swizzle.  Atoms are 8 rows of 128 bytes (1024-byte
@@ -184,6 +203,13 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
                  "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"((uint32_t)accumulate) : "memory");
+}
+// The same with A (M rows in the lanes, two 16-bit steps of k a column) in tensor memory.
+__device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate)
+{
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
 // The barrier gets one arrival when the products issued so far by this thread are done.
 __device__ __forceinline__ void commit(uint64_t *bar)
@@ -258,9 +284,9 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar)
 // ---- host: tensor maps ----
 
 // A row-major matrix (rows, cols) of `bytes`-wide elements with a row pitch in bytes, read in
-// boxes of (box_rows, box_cols) with 128-byte swizzle; outside of the matrix zeros are read.
+// boxes of (box_rows, box_cols), by default with 128-byte swizzle; outside of the matrix zeros are read.
 vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint64_t cols,
-                   uint64_t pitch, uint32_t box_rows, uint32_t box_cols);
+                   uint64_t pitch, uint32_t box_rows, uint32_t box_cols, bool swizzle = true);
 
 // Lets a kernel have more shared memory than 48 KB, once a device.
 template <typename K> inline vt_status allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done)
