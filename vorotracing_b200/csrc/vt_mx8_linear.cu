@@ -34,7 +34,7 @@ constexpr uint32_t TILE_ROWS = 64, NARROW_OUTS = 256, NARROW_THREADS = 672;
 
 // OC: dy's columns in chunks of 64.  A slab is 128 columns of z, or all of up to 64 (FOLD).
 template <int OC, bool FOLD> struct Narrow {
-    static constexpr uint32_t W_BYTES = OC * 16384u, CHUNK = TILE_ROWS * 128u, DY_BYTES = OC * CHUNK, CODE_PITCH = FOLD ? 64u : 128u;
+    static constexpr uint32_t CHUNK = TILE_ROWS * 128u, DY_BYTES = OC * CHUNK, CODE_PITCH = FOLD ? 64u : 128u;
     static constexpr uint32_t STAGE = DY_BYTES + TILE_ROWS * CODE_PITCH;
     struct Ctrl {
         float scale[16][32];  // of the blocks in each activation warp's rows
@@ -42,16 +42,20 @@ template <int OC, bool FOLD> struct Narrow {
         uint32_t tmem;
         tc::Fail fail;
     };
-    static constexpr uint32_t FIT = (232448u - W_BYTES - sizeof(Ctrl)) / STAGE, STAGES = FIT < 8u ? FIT : 8u;
-    static constexpr uint32_t CTRL_AT = W_BYTES + STAGES * STAGE, SMEM = CTRL_AT + sizeof(Ctrl);
-    static constexpr uint32_t DH_AT = OC * 64u, TMEM = 512;  // columns: dW, then four of dH
+    static constexpr uint32_t FIT = (232448u - sizeof(Ctrl)) / STAGE, STAGES = FIT < 8u ? FIT : 8u;
+    static constexpr uint32_t CTRL_AT = STAGES * STAGE, SMEM = CTRL_AT + sizeof(Ctrl);
+    static constexpr uint32_t TMEM = 512;
+    // columns of tensor memory: dW, W, and as many of dH as there is room for, up to four
+    static constexpr uint32_t W_AT = OC * 64u, DH_AT = W_AT + OC * 32u, BUFS = OC == 4 ? 2 : OC == 3 ? 3 : 4;
     static constexpr int ROWS = FOLD ? 16 : 32;  // of a tile an activation warp takes
-    static_assert(STAGES >= 4 && DH_AT + 256u <= TMEM, "does not fit an SM");
+    static_assert(STAGES >= 4 && DH_AT + BUFS * TILE_ROWS <= TMEM, "does not fit an SM");
 };
 
 struct NarrowArgs {
     uint64_t rows;
     uint32_t cols, outs, blocks, tiles, groups, slabs;
+    const void *weight;
+    uint64_t weight_stride;
     const int8_t *codes;
     const uint8_t *exps;
     void *dz;          // null: not wanted
@@ -79,8 +83,7 @@ __device__ __forceinline__ void slope16(const uint32_t *codes, f32x2 sc, const u
 
 template <typename T, int ACT, int OC, bool FOLD>
 __global__ void __launch_bounds__(NARROW_THREADS, 1)
-    narrow_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap w_map,
-                  const __grid_constant__ CUtensorMap code_map, const NarrowArgs a)
+    narrow_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap code_map, const NarrowArgs a)
 {
     using P = Narrow<OC, FOLD>;
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -98,18 +101,17 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             tc::mbar_init(&s.full[i], 1);
             tc::mbar_init(&s.empty[i], sums ? 3 : 1);
         }
-        for (uint32_t i = 0; i < 4; ++i) {
+        for (uint32_t i = 0; i < P::BUFS; ++i) {
             tc::mbar_init(&s.dh_full[i], 1);
             tc::mbar_init(&s.dh_empty[i], 1);
             tc::mbar_init(&s.h_full[i], 8);
         }
-        tc::mbar_init(&s.w_full, 1);
+        tc::mbar_init(&s.w_full, 16);
         tc::mbar_init(&s.done, 1);
         tc::mbar_init(&s.failed, 1);
         s.fail.failed = 0;
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&dy_map);
-        tc::tma_prefetch_map(&w_map);
         tc::tma_prefetch_map(&code_map);
     }
     if (warp == 1) tc::tmem_alloc<P::TMEM>(&s.tmem);
@@ -121,30 +123,29 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
     if (warp == 0) {
         if (lane == 0) {  // TMA
             uint32_t issued = 0;
-            tc::mbar_arrive_tx(&s.w_full, P::W_BYTES);
-            for (int n = 0; n < 2; ++n)  // FOLD: the same 64 columns twice
-                tc::tma_load_2d(smem + n * (OC * 8192), &w_map, FOLD ? 0 : (int)(slab * 2 + n) * 64, 0, &s.w_full);
             tc::Ring r;
             for (uint32_t t = group; t < a.tiles; t += a.groups) {
                 if (!tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err)) break;
-                uint8_t *st = smem + P::W_BYTES + r.i * P::STAGE;
+                uint8_t *st = smem + r.i * P::STAGE;
                 tc::mbar_arrive_tx(&s.full[r.i], P::STAGE);
                 for (int c = 0; c < OC; ++c)
                     tc::tma_load_2d(st + c * (TILE_ROWS * 128u), &dy_map, c * 64, (int)(t * TILE_ROWS), &s.full[r.i]);
                 tc::tma_load_2d(st + P::DY_BYTES, &code_map, (int)(slab * 128), (int)(t * TILE_ROWS), &s.full[r.i]);
+                const uint32_t ahead = t + P::STAGES * a.groups;
+                if (ahead < a.tiles) {
+                    for (uint32_t c = slab; c < OC; c += a.slabs) tc::tma_prefetch_2d(&dy_map, c * 64, (int)(ahead * TILE_ROWS));
+                    tc::tma_prefetch_2d(&code_map, (int)(slab * 128), (int)(ahead * TILE_ROWS));
+                }
                 ++issued;
                 r.next(P::STAGES);
             }
-            if (s.fail.failed) {  // leave no copy in flight
-                tc::mbar_wait_slow(&s.w_full, 0, fail, a.err, true);
+            if (s.fail.failed)  // leave no copy in flight
                 for (uint32_t i = 0; i < P::STAGES && i < issued; ++i)
                     tc::mbar_wait_slow(&s.full[i], ((issued - 1 - i) / P::STAGES) & 1u, fail, a.err, true);
-            }
         }
     } else if (warp == 1) {  // dH^T = W^T dy^T
-        constexpr uint32_t ID = tc::idesc_f16<BF16>(128, TILE_ROWS, true, false);
-        const uint32_t w_addr = tc::smem_u32(smem), st_addr = w_addr + P::W_BYTES;
-        const uint64_t w_desc = tc::smem_desc(w_addr, OC * 8192u, 1024);
+        constexpr uint32_t ID = tc::idesc_f16<BF16>(128, TILE_ROWS, false, false);
+        const uint32_t st_addr = tc::smem_u32(smem);
         const bool mine = tc::elect();
         tc::Ring r, dh;
         bool ok = __all_sync(~0u, tc::mbar_wait(&s.w_full, 0, fail, a.err));
@@ -159,12 +160,13 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 for (uint32_t c = 0; c < OC; ++c)
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k)
-                        tc::mma_f16(dh_at + dh.i * TILE_ROWS, w_desc + c * 512u + k * 128u, b + c * (P::CHUNK >> 4) + k * 2u, ID, c + k != 0);
+                        tc::mma_f16_tmem(dh_at + dh.i * TILE_ROWS, tmem + P::W_AT + (c * 4u + k) * 8u, b + c * (P::CHUNK >> 4) + k * 2u,
+                                         ID, c + k != 0);
                 tc::commit(&s.dh_full[dh.i]);
             }
             __syncwarp();
             r.next(P::STAGES);
-            dh.next(4);
+            dh.next(P::BUFS);
         }
         if (!ok) {  // leave no product in flight
             if (mine) tc::commit(&s.failed);
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
     } else if (warp == 20) {  // dW^T += h^T dy, behind the activations; in a warp of its own, so that neither product waits
                               // for what the other one waits for
         constexpr uint32_t ID = tc::idesc_f16<BF16>(128, OC * 64, false, true);
-        const uint32_t st_addr = tc::smem_u32(smem) + P::W_BYTES;
+        const uint32_t st_addr = tc::smem_u32(smem);
         const bool mine = tc::elect();
         tc::Ring r, h;
         bool ok = true;
@@ -195,7 +197,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             }
             __syncwarp();
             r.next(P::STAGES);
-            h.next(4);
+            h.next(P::BUFS);
         }
         if (mine) tc::commit(&s.done);
         if (!ok) tc::mbar_wait_slow(&s.done, 0, fail, a.err, true);  // leave no product in flight
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
 #pragma unroll
                 for (int c = 0; c < OC; ++c) {
                     if (c % sharers != slab) continue;
-                    const uint8_t *p = smem + P::W_BYTES + r.i * P::STAGE + c * (TILE_ROWS * 128u) + row0 * 128u;
+                    const uint8_t *p = smem + r.i * P::STAGE + c * (TILE_ROWS * 128u) + row0 * 128u;
                     f32x2 v = 0;
 #pragma unroll 8
                     for (uint32_t i = 0; i < TILE_ROWS / 2u; ++i) {
@@ -245,8 +247,29 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         };
         const uint32_t first = group + set * a.groups, step = 2u * a.groups;
         uint32_t E = exponent(first);
+        {  // W^T, an A operand: a lane has a column, a word two outputs; a warp a quarter of the outputs
+            const T *w = (const T *)a.weight + n;
+            const uint32_t o0 = (warp - 4u) / 4u * OC * 16u;
+#pragma unroll
+            for (uint32_t c = 0; c < OC; ++c) {
+                uint32_t v[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint32_t o = o0 + c * 16u + 2u * i;
+                    const unsigned short *p = (const unsigned short *)(w + o * a.weight_stride);
+                    const uint32_t lo = n < a.cols && o < a.outs ? __ldg(p) : 0u;
+                    const uint32_t hi = n < a.cols && o + 1u < a.outs ? __ldg(p + a.weight_stride) : 0u;
+                    v[i] = lo | hi << 16;
+                }
+                tc::tmem_store8(tmem + P::W_AT + lanes + (o0 + c * 16u) / 2u, v);
+            }
+            tc::tmem_wait_store();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s.w_full);
+        }
         tc::Ring r, dh;
-        if (set) { r.next(P::STAGES); dh.next(4); }
+        if (set) { r.next(P::STAGES); dh.next(P::BUFS); }
         bool ok = true;
         for (uint32_t t = first; t < a.tiles && ok; t += step) {
             const uint64_t row = (uint64_t)t * TILE_ROWS + row0;
@@ -258,7 +281,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                                      tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err));
             if (!ok) break;
             tc::fence_after();
-            const uint8_t *codes = smem + P::W_BYTES + r.i * P::STAGE + P::DY_BYTES + code0;
+            const uint8_t *codes = smem + r.i * P::STAGE + P::DY_BYTES + code0;
             const uint32_t buffer = dh_at + dh.i * TILE_ROWS + lanes, here = buffer + row0;
             const uint32_t count = row >= a.rows ? 0u : a.rows - row < (uint64_t)ROWS ? (uint32_t)(a.rows - row) : ROWS;
             unsigned short *out = (unsigned short *)a.dz + row * a.cols + n;
@@ -317,8 +340,8 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                     }
                 }
             }
-            dh.next(4);
-            dh.next(4);
+            dh.next(P::BUFS);
+            dh.next(P::BUFS);
             r.next(P::STAGES);
             r.next(P::STAGES);
             E = next_E;
@@ -649,7 +672,7 @@ enum : int { COPY_DY = 1, COPY_WEIGHT = 2 };
 struct NarrowPlan {
     uint32_t oc, slabs, tiles, groups, part_outs;
     bool fold;
-    uint64_t dw_at, db_at, dy_at, w_at, bytes;
+    uint64_t dw_at, db_at, dy_at, bytes;
 };
 static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, int copies, uint32_t sms)
 {
@@ -665,8 +688,7 @@ static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, int c
     p.dw_at = 0;
     p.db_at = p.dw_at + align_up((uint64_t)p.groups * p.slabs * 128u * p.part_outs * 4u, 256);
     p.dy_at = p.db_at + align_up((uint64_t)p.groups * 2u * p.part_outs * 4u, 256);
-    p.w_at = p.dy_at + (copies & COPY_DY ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
-    p.bytes = p.w_at + (copies & COPY_WEIGHT ? align_up((uint64_t)outs * align_up(cols, 8) * 2u, 256) : 0);
+    p.bytes = p.dy_at + (copies & COPY_DY ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
     return p;
 }
 
@@ -676,7 +698,7 @@ template <typename T> static int copies_of(const void *dy, uint64_t dy_stride, c
 }
 
 template <typename T, int ACT, int OC, bool FOLD>
-static vt_status launch_narrow(const CUtensorMap &dy, const CUtensorMap &w, const NarrowArgs &a, cudaStream_t stream)
+static vt_status launch_narrow(const CUtensorMap &dy, const NarrowArgs &a, cudaStream_t stream)
 {
     static std::atomic<uint64_t> allowed{0};
     using P = Narrow<OC, FOLD>;
@@ -685,7 +707,7 @@ static vt_status launch_narrow(const CUtensorMap &dy, const CUtensorMap &w, cons
     if (vt_status s = tc::make_map(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.rows, width, width, TILE_ROWS, P::CODE_PITCH, false))
         return s;
     if (vt_status s = tc::allow_smem(narrow_kernel<T, ACT, OC, FOLD>, P::SMEM, allowed)) return s;
-    narrow_kernel<T, ACT, OC, FOLD><<<a.groups * a.slabs, NARROW_THREADS, P::SMEM, stream>>>(dy, w, codes, a);
+    narrow_kernel<T, ACT, OC, FOLD><<<a.groups * a.slabs, NARROW_THREADS, P::SMEM, stream>>>(dy, codes, a);
     return check_launch("narrow_kernel");
 }
 
@@ -695,12 +717,12 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
                             uint8_t *workspace, uint32_t *err, cudaStream_t stream)
 {
     const NarrowPlan p = narrow_plan(rows, cols, outs, copies_of<T>(dy, dy_stride, w, w_stride), (uint32_t)sm_count());
-    CUtensorMap dy_map, w_map;
+    CUtensorMap dy_map;
     if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
-    if (vt_status s = whole_rows<T>(w, w_stride, outs, cols, workspace + p.w_at, stream)) return s;
     if (vt_status s = map_rows<T>(&dy_map, dy, dy_stride, rows, outs, TILE_ROWS)) return s;
-    if (vt_status s = map_rows<T>(&w_map, w, w_stride, outs, cols, p.oc * 64u)) return s;
     NarrowArgs a;
+    a.weight = w;
+    a.weight_stride = w_stride;
     a.rows = rows;
     a.cols = cols;
     a.outs = outs;
@@ -716,14 +738,14 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     a.err = err;
     vt_status s = VT_OK;
     switch (p.oc * 2u + p.fold) {
-    case 2: s = launch_narrow<T, ACT, 1, false>(dy_map, w_map, a, stream); break;
-    case 3: s = launch_narrow<T, ACT, 1, true>(dy_map, w_map, a, stream); break;
-    case 4: s = launch_narrow<T, ACT, 2, false>(dy_map, w_map, a, stream); break;
-    case 5: s = launch_narrow<T, ACT, 2, true>(dy_map, w_map, a, stream); break;
-    case 6: s = launch_narrow<T, ACT, 3, false>(dy_map, w_map, a, stream); break;
-    case 7: s = launch_narrow<T, ACT, 3, true>(dy_map, w_map, a, stream); break;
-    case 8: s = launch_narrow<T, ACT, 4, false>(dy_map, w_map, a, stream); break;
-    default: s = launch_narrow<T, ACT, 4, true>(dy_map, w_map, a, stream); break;
+    case 2: s = launch_narrow<T, ACT, 1, false>(dy_map, a, stream); break;
+    case 3: s = launch_narrow<T, ACT, 1, true>(dy_map, a, stream); break;
+    case 4: s = launch_narrow<T, ACT, 2, false>(dy_map, a, stream); break;
+    case 5: s = launch_narrow<T, ACT, 2, true>(dy_map, a, stream); break;
+    case 6: s = launch_narrow<T, ACT, 3, false>(dy_map, a, stream); break;
+    case 7: s = launch_narrow<T, ACT, 3, true>(dy_map, a, stream); break;
+    case 8: s = launch_narrow<T, ACT, 4, false>(dy_map, a, stream); break;
+    default: s = launch_narrow<T, ACT, 4, true>(dy_map, a, stream); break;
     }
     if (s || !(dw || db)) return s;
     const uint64_t n = (uint64_t)p.slabs * 128u * p.part_outs;
