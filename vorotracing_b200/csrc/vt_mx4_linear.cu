@@ -155,10 +155,7 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             }
             // A stage's barrier also waits for other warps, so a failed launch cannot use it to
             // see that its copies are in: it waits for them by time, far longer than a copy takes.
-            if (s.fail.failed) {
-                const uint64_t began = tc::nanoseconds();
-                while (tc::nanoseconds() - began < 10000000ull) {}
-            }
+            if (s.fail.failed) tc::outlast_copies();
         }
     } else if (warp == 1) {
         if (lane == 0) {  // scales to tensor memory, products
@@ -374,10 +371,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_consta
                 tc::tma_load_2d(smem + r.i * FEW_STAGE, &w_map, (int)(c * 128u), (int)out0, &s.full[r.i]);
                 r.next(FEW_STAGES);
             }
-            if (s.fail.failed) {  // as in linear4_kernel
-                const uint64_t began = tc::nanoseconds();
-                while (tc::nanoseconds() - began < 10000000ull) {}
-            }
+            if (s.fail.failed) tc::outlast_copies();
         }
     } else if (warp == 1) {
         if (lane == 0) {  // scales to tensor memory, products

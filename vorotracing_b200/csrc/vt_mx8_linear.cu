@@ -3,14 +3,14 @@
 //
 // Layers with up to 256 outputs (narrow_kernel) make all three in one pass over the rows, so dy
 // and the checkpoint are read from HBM once and act(z8) never reaches memory.  A CTA owns a slab
-// of 128 columns of z and every G-th tile of 64 rows.  A tile of dy is staged once in shared
+// of 128 columns of z and every G-th tile of 32 rows.  A tile of dy is staged once in shared
 // memory (TMA, 128-byte swizzle) and used twice: as the K-major B operand of dH^T = W^T dy^T,
 // whose result has z's columns in the lanes of tensor memory, and, the same bytes read the other
 // way, as the MN-major B operand of dW^T += act(z8)^T dy, whose accumulator stays in tensor memory
 // over all the CTA's rows.  Between the two products sixteen warps take dH out of tensor memory,
 // read the 8-bit z, evaluate act and act' together (one logistic serves both), write dz, and put
 // act(z8) back into the place of dH as the second product's A operand, rounded to the operands'
-// 16-bit type as the forward pass's own activations are.  Two more warps add up dy's columns from
+// 16-bit type as the forward pass's own activations are.  One more warp adds up dy's columns from
 // the staged tile.  At its end a CTA writes its part of dW in binary32; a second kernel adds the
 // parts in order, so results do not depend on timing.
 //
@@ -30,7 +30,7 @@ namespace vt {
 
 // ---- layers with up to 256 outputs ----
 
-constexpr uint32_t TILE_ROWS = 64, NARROW_OUTS = 256, NARROW_THREADS = 672;
+constexpr uint32_t TILE_ROWS = 32, NARROW_OUTS = 256, NARROW_THREADS = 640;
 
 // OC: dy's columns in chunks of 64.  A slab is 128 columns of z, or all of up to 64 (FOLD).
 template <int OC, bool FOLD> struct Narrow {
@@ -38,15 +38,15 @@ template <int OC, bool FOLD> struct Narrow {
     static constexpr uint32_t STAGE = DY_BYTES + TILE_ROWS * CODE_PITCH;
     struct Ctrl {
         float scale[16][32];  // of the blocks in each activation warp's rows
-        uint64_t full[8], empty[8], dh_full[4], dh_empty[4], h_full[4], w_full, done, failed;
+        uint64_t full[12], empty[12], dh_full[8], dh_empty[8], h_full[8], w_full, done, failed;
         uint32_t tmem;
         tc::Fail fail;
     };
-    static constexpr uint32_t FIT = (232448u - sizeof(Ctrl)) / STAGE, STAGES = FIT < 8u ? FIT : 8u;
+    static constexpr uint32_t FIT = (232448u - sizeof(Ctrl)) / STAGE, STAGES = FIT < 12u ? FIT : 12u;
     static constexpr uint32_t CTRL_AT = STAGES * STAGE, SMEM = CTRL_AT + sizeof(Ctrl);
     static constexpr uint32_t TMEM = 512;
-    // columns of tensor memory: dW, W, and as many of dH as there is room for, up to four
-    static constexpr uint32_t W_AT = OC * 64u, DH_AT = W_AT + OC * 32u, BUFS = OC == 4 ? 2 : OC == 3 ? 3 : 4;
+    // columns of tensor memory: dW, W, and as many of dH as there is room for, up to eight
+    static constexpr uint32_t W_AT = OC * 64u, DH_AT = W_AT + OC * 32u, BUFS = OC == 4 ? 4 : OC == 3 ? 6 : 8;
     static constexpr int ROWS = FOLD ? 16 : 32;  // of a tile an activation warp takes
     static_assert(STAGES >= 4 && DH_AT + BUFS * TILE_ROWS <= TMEM, "does not fit an SM");
 };
@@ -60,8 +60,9 @@ struct NarrowArgs {
     const uint8_t *exps;
     void *dz;          // null: not wanted
     float *dw_parts;   // [group][slab][OC * 64][128]; null: dW not wanted
-    float *db_parts;   // [group][2][OC * 64]; null: db not wanted
+    float *db_parts;   // [group][OC * 64]; null: db not wanted
     uint32_t *err;
+    bool dy_chunked;   // dy's columns are whole chunks of 64: one TMA copy brings all of them in
 };
 
 // 16 columns of a row: codes (4 words) and their block's scale, g = dH (binary32) in, dz out as
@@ -79,6 +80,22 @@ __device__ __forceinline__ void slope16(const uint32_t *codes, f32x2 sc, const u
             dz[at] = pack2<T>(ACT == ACT_IDENTITY ? gp : mul2(gp, act_slope2<ACT>(mul2(code_pair(c, 2 * i), sc))));
         }
     }
+}
+
+// d += (16 columns by 16 rows, read across from shared memory) times ones: each column's sum in
+// d[0] (columns 0..7, a group of four lanes each) and d[2] (columns 8..15).
+template <typename T> __device__ __forceinline__ void add_columns(float *d, uint32_t addr)
+{
+    uint32_t x[4];
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
+    const uint32_t ones = pack2<T>(1.0f, 1.0f);
+    if constexpr (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %8}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(ones));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %8}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(ones));
 }
 
 template <typename T, int ACT, int OC, bool FOLD>
@@ -99,12 +116,12 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < P::STAGES; ++i) {
             tc::mbar_init(&s.full[i], 1);
-            tc::mbar_init(&s.empty[i], sums ? 3 : 1);
+            tc::mbar_init(&s.empty[i], sums ? 2 : 1);
         }
         for (uint32_t i = 0; i < P::BUFS; ++i) {
             tc::mbar_init(&s.dh_full[i], 1);
             tc::mbar_init(&s.dh_empty[i], 1);
-            tc::mbar_init(&s.h_full[i], 8);
+            tc::mbar_init(&s.h_full[i], 4);
         }
         tc::mbar_init(&s.w_full, 16);
         tc::mbar_init(&s.done, 1);
@@ -128,14 +145,13 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 if (!tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err)) break;
                 uint8_t *st = smem + r.i * P::STAGE;
                 tc::mbar_arrive_tx(&s.full[r.i], P::STAGE);
-                for (int c = 0; c < OC; ++c)
-                    tc::tma_load_2d(st + c * (TILE_ROWS * 128u), &dy_map, c * 64, (int)(t * TILE_ROWS), &s.full[r.i]);
-                tc::tma_load_2d(st + P::DY_BYTES, &code_map, (int)(slab * 128), (int)(t * TILE_ROWS), &s.full[r.i]);
-                const uint32_t ahead = t + P::STAGES * a.groups;
-                if (ahead < a.tiles) {
-                    for (uint32_t c = slab; c < OC; c += a.slabs) tc::tma_prefetch_2d(&dy_map, c * 64, (int)(ahead * TILE_ROWS));
-                    tc::tma_prefetch_2d(&code_map, (int)(slab * 128), (int)(ahead * TILE_ROWS));
+                if (OC > 1 && a.dy_chunked) {
+                    tc::tma_load_3d(st, &dy_map, 0, (int)(t * TILE_ROWS), 0, &s.full[r.i]);
+                } else {
+                    for (int c = 0; c < OC; ++c)
+                        tc::tma_load_2d(st + c * P::CHUNK, &dy_map, c * 64, (int)(t * TILE_ROWS), &s.full[r.i]);
                 }
+                tc::tma_load_2d(st + P::DY_BYTES, &code_map, (int)(slab * 128), (int)(t * TILE_ROWS), &s.full[r.i]);
                 ++issued;
                 r.next(P::STAGES);
             }
@@ -172,7 +188,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             if (mine) tc::commit(&s.failed);
             tc::mbar_wait_slow(&s.failed, 0, fail, a.err, true);
         }
-    } else if (warp == 20) {  // dW^T += h^T dy, behind the activations; in a warp of its own, so that neither product waits
+    } else if (warp == 3) {  // dW^T += h^T dy, behind the activations; in a warp of its own, so that neither product waits
                               // for what the other one waits for
         constexpr uint32_t ID = tc::idesc_f16<BF16>(128, OC * 64, false, true);
         const uint32_t st_addr = tc::smem_u32(smem);
@@ -201,26 +217,22 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         }
         if (mine) tc::commit(&s.done);
         if (!ok) tc::mbar_wait_slow(&s.done, 0, fail, a.err, true);  // leave no product in flight
-    } else if (warp < 4) {
-        if (sums) {  // column sums: each of the two warps takes half of a tile's rows, a lane two columns
+    } else if (warp == 2) {
+        if (sums) {  // column sums: products of 16 outputs by 16 rows of dy with ones, which cost an eighth of the adds
             tc::Ring r;
-            f32x2 total[OC] = {};
-            bool ok = true;
-            const uint32_t row0 = (warp - 2u) * (TILE_ROWS / 2u);
-            for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
-                ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
-                if (!ok) break;
+            float total[OC * 4][4] = {};
+            const uint32_t k = (lane & 7u) + (lane >> 4) * 8u, o = (lane >> 3 & 1u) * 16u;  // row and byte of this lane's address
+            for (uint32_t t = group; t < a.tiles; t += a.groups) {
+                if (!__all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err))) break;
+                const uint32_t st = tc::smem_u32(smem) + r.i * P::STAGE + k * 128u;
 #pragma unroll
                 for (int c = 0; c < OC; ++c) {
                     if (c % sharers != slab) continue;
-                    const uint8_t *p = smem + r.i * P::STAGE + c * (TILE_ROWS * 128u) + row0 * 128u;
-                    f32x2 v = 0;
-#pragma unroll 8
-                    for (uint32_t i = 0; i < TILE_ROWS / 2u; ++i) {
-                        const float2 x = unpack2<T>(*reinterpret_cast<const uint32_t *>(p + i * 128u + ((lane * 4u) ^ (i & 7u) << 4)));
-                        v = add2(v, pair(x.x, x.y));
-                    }
-                    total[c] = add2(total[c], v);
+#pragma unroll
+                    for (uint32_t m = 0; m < 4; ++m)
+#pragma unroll
+                        for (uint32_t row = 0; row < TILE_ROWS; row += 16u)
+                            add_columns<T>(total[c * 4 + m], st + c * P::CHUNK + row * 128u + ((m * 32u + o) ^ (k & 7u) << 4));
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s.empty[r.i]);
@@ -228,28 +240,43 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             }
 #pragma unroll
             for (int c = 0; c < OC; ++c)
-                if (c % sharers == slab)
-                    *reinterpret_cast<f32x2 *>(a.db_parts + ((uint64_t)group * 2u + (warp - 2u)) * (OC * 64u) + c * 64u + lane * 2u) =
-                        total[c];
+                if (c % sharers == slab && lane % 4u == 0) {
+                    float *out = a.db_parts + (uint64_t)group * (OC * 64u) + c * 64u + lane / 4u;
+#pragma unroll
+                    for (uint32_t m = 0; m < 4; ++m) {
+                        out[m * 16u] = total[c * 4 + m][0];
+                        out[m * 16u + 8u] = total[c * 4 + m][2];
+                    }
+                }
         }
-    } else {  // activations: two sets of eight warps take tiles in turn; a lane has a column of z (a
+    } else {  // activations: four sets of four warps take tiles in turn; a lane has a column of z (a
               // warp one block of 32) and ROWS rows of the tile
         constexpr int ROWS = P::ROWS;
-        const uint32_t quad = warp % 4u, set = (warp - 4u) / 8u, part = (warp - 4u) / 4u % 2u;
+        const uint32_t quad = warp % 4u, set = (warp - 4u) / 4u;
         const uint32_t block = FOLD ? quad & 1u : slab * 4u + quad, n = block * 32u + lane;
-        const uint32_t row0 = FOLD ? (quad >> 1) * 32u + part * 16u : part * 32u;  // in the tile
+        const uint32_t row0 = FOLD ? (quad >> 1) * 16u : 0u;  // in the tile
         const uint32_t lanes = quad * 32u << 16, code0 = row0 * P::CODE_PITCH + (FOLD ? n : quad * 32u + lane);
         float *const scale = s.scale[warp - 4u];
-        // exponent byte of this warp's block in row lane of its rows
+        const uint32_t first = group + set * a.groups, step = 4u * a.groups;
+        // exponent bytes of this warp's block, a row a lane: this tile's, and the next one's on their way
+        const uint64_t first_row = (uint64_t)first * TILE_ROWS + row0;
+        const uint8_t *exps = a.exps + (first_row + lane) * a.blocks + block;
+        const uint64_t exps_step = (uint64_t)step * TILE_ROWS * a.blocks;
+        const bool scaled = lane < ROWS && block < a.blocks;
+        const uint32_t last = a.tiles - 1u, last_rows = (uint32_t)(a.rows - (uint64_t)last * TILE_ROWS);  // rows of the last tile
+        const uint32_t last_count = last_rows > row0 ? min(last_rows - row0, (uint32_t)ROWS) : 0u;
         auto exponent = [&](uint32_t t) -> uint32_t {
-            const uint64_t row = (uint64_t)t * TILE_ROWS + row0 + lane;
-            return t < a.tiles && lane < ROWS && row < a.rows && block < a.blocks ? __ldg(a.exps + row * a.blocks + block) : 127u;
+            const uint32_t e = scaled && (t < last || (t == last && lane < last_count)) ? __ldg(exps) : 127u;
+            exps += exps_step;
+            return e;
         };
-        const uint32_t first = group + set * a.groups, step = 2u * a.groups;
         uint32_t E = exponent(first);
+        unsigned short *out = (unsigned short *)a.dz + first_row * a.cols + n;
+        const uint64_t out_step = ((uint64_t)step * TILE_ROWS - ROWS) * a.cols;
+        const bool write = a.dz && n < a.cols;
         {  // W^T, an A operand: a lane has a column, a word two outputs; a warp a quarter of the outputs
             const T *w = (const T *)a.weight + n;
-            const uint32_t o0 = (warp - 4u) / 4u * OC * 16u;
+            const uint32_t o0 = set * OC * 16u;
 #pragma unroll
             for (uint32_t c = 0; c < OC; ++c) {
                 uint32_t v[8];
@@ -269,10 +296,10 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             if (lane == 0) tc::mbar_arrive(&s.w_full);
         }
         tc::Ring r, dh;
-        if (set) { r.next(P::STAGES); dh.next(P::BUFS); }
+        r.skip(set, P::STAGES);
+        dh.skip(set, P::BUFS);
         bool ok = true;
         for (uint32_t t = first; t < a.tiles && ok; t += step) {
-            const uint64_t row = (uint64_t)t * TILE_ROWS + row0;
             const uint32_t next_E = exponent(t + step);
             __syncwarp();
             scale[lane] = mx8_scale(E);
@@ -283,9 +310,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             tc::fence_after();
             const uint8_t *codes = smem + r.i * P::STAGE + P::DY_BYTES + code0;
             const uint32_t buffer = dh_at + dh.i * TILE_ROWS + lanes, here = buffer + row0;
-            const uint32_t count = row >= a.rows ? 0u : a.rows - row < (uint64_t)ROWS ? (uint32_t)(a.rows - row) : ROWS;
-            unsigned short *out = (unsigned short *)a.dz + row * a.cols + n;
-            const bool write = a.dz && n < a.cols;
+            const uint32_t count = t == last ? last_count : ROWS;
 #pragma unroll
             for (int p = 0; p < ROWS; p += 16) {
                 uint32_t g[16], h[8], d[8];
@@ -314,7 +339,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 tc::tmem_store8(here + p, h);
                 if (FOLD) {  // this half of the lanes has no part in the other half's rows
                     const uint32_t none[8] = {};
-                    tc::tmem_store8(buffer + (row0 ^ 32u), none);
+                    tc::tmem_store8(buffer + (row0 ^ 16u), none);
                 }
                 if (p + 16 == ROWS) {
                     tc::tmem_wait_store();
@@ -322,28 +347,25 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.h_full[dh.i]);
                 }
-                if (write) {
-                    if (count == ROWS) {
+                if (write && count == ROWS) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            out[0] = (unsigned short)d[i];
-                            out[a.cols] = (unsigned short)(d[i] >> 16);
-                            out += 2 * a.cols;
-                        }
-                    } else {
+                    for (int i = 0; i < 8; ++i) {
+                        out[0] = (unsigned short)d[i];
+                        out[a.cols] = (unsigned short)(d[i] >> 16);
+                        out += 2 * a.cols;
+                    }
+                } else if (write) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            if (p + 2 * i < count) out[0] = (unsigned short)d[i];
-                            if (p + 2 * i + 1 < count) out[a.cols] = (unsigned short)(d[i] >> 16);
-                            out += 2 * a.cols;
-                        }
+                    for (int i = 0; i < 8; ++i) {
+                        if (p + 2 * i < count) out[0] = (unsigned short)d[i];
+                        if (p + 2 * i + 1 < count) out[a.cols] = (unsigned short)(d[i] >> 16);
+                        out += 2 * a.cols;
                     }
                 }
             }
-            dh.next(P::BUFS);
-            dh.next(P::BUFS);
-            r.next(P::STAGES);
-            r.next(P::STAGES);
+            out += out_step;
+            dh.skip(4, P::BUFS);
+            r.skip(4, P::STAGES);
             E = next_E;
         }
         if (a.dw_parts) {
@@ -353,7 +375,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 float *out = a.dw_parts + ((uint64_t)group * a.slabs + slab) * (OC * 64u) * 128u + quad * 32u + lane;
 #pragma unroll
                 for (uint32_t c = 0; c < OC; ++c) {
-                    const uint32_t o0 = ((set * 2u + part) * OC + c) * 16u;
+                    const uint32_t o0 = (set * OC + c) * 16u;
                     uint32_t v[16];
                     tc::tmem_load16(tmem + lanes + o0, v);
                     tc::tmem_wait_load();
@@ -395,7 +417,7 @@ __global__ void __launch_bounds__(256) narrow_reduce_kernel(const float *__restr
     }
     if (db && i < outs) {
         float v = 0.0f;
-        for (uint32_t g = 0; g < 2u * groups; ++g) v += __ldg(db_parts + (uint64_t)g * part_outs + i);
+        for (uint32_t g = 0; g < groups; ++g) v += __ldg(db_parts + (uint64_t)g * part_outs + i);
         db[i] = from_f32<T>(v);
     }
 }
@@ -484,10 +506,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
             }
             // The bytes of both CTAs are counted in the leader alone, so after a failure each CTA
             // waits for its copies by time, far longer than they take.
-            if (s.fail.failed) {
-                const uint64_t began = tc::nanoseconds();
-                while (tc::nanoseconds() - began < 10000000ull) {}
-            }
+            if (s.fail.failed) tc::outlast_copies();
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {  // products, in the leader
@@ -687,7 +706,7 @@ static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, int c
     p.part_outs = p.oc * 64u;
     p.dw_at = 0;
     p.db_at = p.dw_at + align_up((uint64_t)p.groups * p.slabs * 128u * p.part_outs * 4u, 256);
-    p.dy_at = p.db_at + align_up((uint64_t)p.groups * 2u * p.part_outs * 4u, 256);
+    p.dy_at = p.db_at + align_up((uint64_t)p.groups * p.part_outs * 4u, 256);
     p.bytes = p.dy_at + (copies & COPY_DY ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
     return p;
 }
@@ -719,8 +738,12 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     const NarrowPlan p = narrow_plan(rows, cols, outs, copies_of<T>(dy, dy_stride, w, w_stride), (uint32_t)sm_count());
     CUtensorMap dy_map;
     if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
-    if (vt_status s = map_rows<T>(&dy_map, dy, dy_stride, rows, outs, TILE_ROWS)) return s;
+    const bool chunked = outs % 64u == 0 && outs > 64u;
+    if (vt_status s = chunked ? tc::make_chunk_map(&dy_map, tma_type<T>(), dy, rows, p.oc, dy_stride * sizeof(T), TILE_ROWS, 64, sizeof(T))
+                              : map_rows<T>(&dy_map, dy, dy_stride, rows, outs, TILE_ROWS))
+        return s;
     NarrowArgs a;
+    a.dy_chunked = chunked;
     a.weight = w;
     a.weight_stride = w_stride;
     a.rows = rows;

@@ -45,12 +45,14 @@ static vt_status whole_rows(const void *&p, uint64_t &stride, uint64_t rows, uin
     }
     return VT_OK;
 }
+template <typename T> constexpr CUtensorMapDataType tma_type()
+{
+    return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
 template <typename T>
 static vt_status map_rows(CUtensorMap *map, const void *p, uint64_t stride, uint64_t rows, uint64_t cols, uint32_t box_rows)
 {
-    const CUtensorMapDataType type =
-        std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    return tc::make_map(map, type, p, rows, cols, stride * sizeof(T), box_rows, 64);
+    return tc::make_map(map, tma_type<T>(), p, rows, cols, stride * sizeof(T), box_rows, 64);
 }
 
 }  // namespace vt

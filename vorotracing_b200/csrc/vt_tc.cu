@@ -24,16 +24,16 @@ static EncodeTiled encode_tiled()
     return f;
 }
 
-vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint64_t cols,
-                   uint64_t pitch, uint32_t box_rows, uint32_t box_cols, bool swizzle)
+static vt_status encode_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, int rank, const cuuint64_t *dims,
+                            const cuuint64_t *strides, const cuuint32_t *box, bool swizzle)
 {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return set_error(VT_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
-    const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
+    const cuuint32_t one[3] = {1, 1, 1};
     const auto make = [&] {
-        return encode(map, type, 2, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        return encode(map, type, rank, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
     CUresult r = make();
     if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread that has made no runtime call yet, as autograd's
@@ -42,8 +42,24 @@ vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, ui
     }
     if (r != CUDA_SUCCESS)
         return set_error(VT_ERR_CUDA, "cuTensorMapEncodeTiled: error %d (%llu x %llu, pitch %llu)", (int)r,
-                         (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)pitch);
+                         (unsigned long long)dims[1], (unsigned long long)dims[0], (unsigned long long)strides[0]);
     return VT_OK;
+}
+
+vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint64_t cols,
+                   uint64_t pitch, uint32_t box_rows, uint32_t box_cols, bool swizzle)
+{
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+    const cuuint32_t box[2] = {box_cols, box_rows};
+    return encode_map(map, type, p, 2, dims, strides, box, swizzle);
+}
+
+vt_status make_chunk_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint32_t chunks,
+                         uint64_t pitch, uint32_t box_rows, uint32_t box_cols, uint32_t bytes)
+{
+    const cuuint64_t dims[3] = {box_cols, rows, chunks}, strides[2] = {pitch, (cuuint64_t)box_cols * bytes};
+    const cuuint32_t box[3] = {box_cols, box_rows, chunks};
+    return encode_map(map, type, p, 3, dims, strides, box, true);
 }
 
 }  // namespace tc

@@ -46,22 +46,18 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
                  : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return ok;
 }
-__device__ __forceinline__ uint64_t nanoseconds()
-{
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-constexpr uint64_t WAIT_LIMIT_NS = 1000000000ull;
+// About a second of the SM's clock.  (Reading %globaltimer instead takes about a microsecond, which
+// every wait that is not over at once would pay.)
+constexpr long long WAIT_LIMIT = 2000000000ll;
 
 static __device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, Fail *fail, uint32_t *err, bool last)
 {
-    const uint64_t began = nanoseconds();
+    const long long began = clock64();
     for (;;) {
         for (int i = 0; i < 64; ++i)
             if (mbar_try(bar, parity)) return true;
         if (fail->failed && !last) return false;
-        if (nanoseconds() - began > WAIT_LIMIT_NS) {
+        if (clock64() - began > WAIT_LIMIT) {
             fail->failed = 1;
             report(err, VT_ERR_CUDA);
             return false;
@@ -76,12 +72,24 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, Fail *
     return mbar_wait_slow(bar, parity, fail, err, false);
 }
 
+// Far longer than a copy takes: for copies in flight that no barrier tells of.
+__device__ __forceinline__ void outlast_copies()
+{
+    const long long began = clock64();
+    while (clock64() - began < WAIT_LIMIT / 100) {}
+}
+
 // Counts through the stages of a ring: index and the parity of its current use.
 struct Ring {
     uint32_t i = 0, phase = 0;
     __device__ __forceinline__ void next(uint32_t stages)
     {
         if (++i == stages) { i = 0; phase ^= 1u; }
+    }
+    __device__ __forceinline__ void skip(uint32_t n, uint32_t stages)  // n at most stages
+    {
+        i += n;
+        if (i >= stages) { i -= stages; phase ^= 1u; }
     }
 };
 
@@ -92,10 +100,10 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, i
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
-// A tile to L2 alone, ahead of its load
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int x, int y)
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar)
 {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map)
 {
@@ -292,6 +300,11 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar)
 // boxes of (box_rows, box_cols), by default with 128-byte swizzle; outside of the matrix zeros are read.
 vt_status make_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint64_t cols,
                    uint64_t pitch, uint32_t box_rows, uint32_t box_cols, bool swizzle = true);
+
+// The same matrix as column chunks of `box_cols` side by side, all of them in one box, which
+// lie one behind the other in shared memory.  The chunks have to make up whole rows.
+vt_status make_chunk_map(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t rows, uint32_t chunks,
+                         uint64_t pitch, uint32_t box_rows, uint32_t box_cols, uint32_t bytes);
 
 // Lets a kernel have more shared memory than 48 KB, once a device.
 template <typename K> inline vt_status allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done)
