@@ -10,8 +10,8 @@
 // over all the CTA's rows.  Between the two products sixteen warps take dH out of tensor memory,
 // read the 8-bit z, evaluate act and act' together (one logistic serves both), write dz, and put
 // act(z8) back into the place of dH as the second product's A operand, rounded to the operands'
-// 16-bit type as the forward pass's own activations are.  One more warp adds up dy's columns from
-// the staged tile.  At its end a CTA writes its part of dW in binary32; a second kernel adds the
+// 16-bit type as the forward pass's own activations are.  The column sums of
+// dy are one more, narrow product of the staged tile.  At its end a CTA writes its part of dW in binary32; a second kernel adds the
 // parts in order, so results do not depend on timing.
 //
 // Shared memory's bandwidth is what is short between HBM and the tensor cores here, which decides
@@ -42,11 +42,11 @@ template <int OC, bool FOLD> struct Narrow {
         uint32_t tmem;
         tc::Fail fail;
     };
-    static constexpr uint32_t FIT = (232448u - sizeof(Ctrl)) / STAGE, STAGES = FIT < 12u ? FIT : 12u;
-    static constexpr uint32_t CTRL_AT = STAGES * STAGE, SMEM = CTRL_AT + sizeof(Ctrl);
+    static constexpr uint32_t ONES = 2048u, FIT = (232448u - ONES - sizeof(Ctrl)) / STAGE, STAGES = FIT < 12u ? FIT : 12u;
+    static constexpr uint32_t ONES_AT = STAGES * STAGE, CTRL_AT = ONES_AT + ONES, SMEM = CTRL_AT + sizeof(Ctrl);
     static constexpr uint32_t TMEM = 512;
-    // columns of tensor memory: dW, W, and as many of dH as there is room for, up to eight
-    static constexpr uint32_t W_AT = OC * 64u, DH_AT = W_AT + OC * 32u, BUFS = OC == 4 ? 4 : OC == 3 ? 6 : 8;
+    // columns of tensor memory: dW, W, db (16 for 128 outputs), and as many of dH as there is room for, up to eight
+    static constexpr uint32_t W_AT = OC * 64u, MT = (OC + 1) / 2, DB_AT = W_AT + OC * 32u, DH_AT = DB_AT + MT * 16u, BUFS = OC == 4 ? 3 : OC == 3 ? 6 : 8;
     static constexpr int ROWS = FOLD ? 16 : 32;  // of a tile an activation warp takes
     static_assert(STAGES >= 4 && DH_AT + BUFS * TILE_ROWS <= TMEM, "does not fit an SM");
 };
@@ -82,22 +82,6 @@ __device__ __forceinline__ void slope16(const uint32_t *codes, f32x2 sc, const u
     }
 }
 
-// d += (16 columns by 16 rows, read across from shared memory) times ones: each column's sum in
-// d[0] (columns 0..7, a group of four lanes each) and d[2] (columns 8..15).
-template <typename T> __device__ __forceinline__ void add_columns(float *d, uint32_t addr)
-{
-    uint32_t x[4];
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
-    const uint32_t ones = pack2<T>(1.0f, 1.0f);
-    if constexpr (std::is_same<T, __half>::value)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %8}, {%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(ones));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %8}, {%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(ones));
-}
-
 template <typename T, int ACT, int OC, bool FOLD>
 __global__ void __launch_bounds__(NARROW_THREADS, 1)
     narrow_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap code_map, const NarrowArgs a)
@@ -108,15 +92,15 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
     typename P::Ctrl &s = *reinterpret_cast<typename P::Ctrl *>(smem + P::CTRL_AT);
     const uint32_t warp = tc::warp_number(), lane = threadIdx.x % 32u;
     const uint32_t slab = blockIdx.x % a.slabs, group = blockIdx.x / a.slabs;
-    // dy's chunks are shared out among the slabs for the column sums
-    const uint32_t sharers = a.slabs < OC ? a.slabs : OC;
+    // the column sums of dy, 128 outputs at a time, are shared out among the slabs
+    const uint32_t sharers = a.slabs < P::MT ? a.slabs : P::MT;
     const bool sums = a.db_parts && slab < sharers;
     tc::Fail *const fail = &s.fail;
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < P::STAGES; ++i) {
             tc::mbar_init(&s.full[i], 1);
-            tc::mbar_init(&s.empty[i], sums ? 2 : 1);
+            tc::mbar_init(&s.empty[i], 1);
         }
         for (uint32_t i = 0; i < P::BUFS; ++i) {
             tc::mbar_init(&s.dh_full[i], 1);
@@ -131,6 +115,9 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         tc::tma_prefetch_map(&dy_map);
         tc::tma_prefetch_map(&code_map);
     }
+    for (uint32_t i = threadIdx.x; i < P::ONES / 4u; i += NARROW_THREADS)
+        reinterpret_cast<uint32_t *>(smem + P::ONES_AT)[i] = pack2<T>(1.0f, 1.0f);
+    tc::fence_async_shared();
     if (warp == 1) tc::tmem_alloc<P::TMEM>(&s.tmem);
     tc::fence_before();
     __syncthreads();
@@ -190,8 +177,9 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         }
     } else if (warp == 3) {  // dW^T += h^T dy, behind the activations; in a warp of its own, so that neither product waits
                               // for what the other one waits for
-        constexpr uint32_t ID = tc::idesc_f16<BF16>(128, OC * 64, false, true);
+        constexpr uint32_t ID = tc::idesc_f16<BF16>(128, OC * 64, false, true), ID_DB = tc::idesc_f16<BF16>(128, 16, true, false);
         const uint32_t st_addr = tc::smem_u32(smem);
+        const uint64_t ones = tc::smem_desc(st_addr + P::ONES_AT, 16, 1024);
         const bool mine = tc::elect();
         tc::Ring r, h;
         bool ok = true;
@@ -208,6 +196,16 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
 #pragma unroll
                     for (uint32_t k = 1; k < TILE_ROWS / 16u; ++k) tc::mma_f16_tmem(tmem, from + k * 16u, b + k * 128u, ID, true);
                 }
+                // db += dy^T ones.  Of an odd number of chunks the last tile's upper 64 outputs are whatever
+                // follows in shared memory; they are not read.
+                if (sums)
+#pragma unroll
+                    for (uint32_t m = 0; m < P::MT; ++m)
+                        if (m % sharers == slab)
+#pragma unroll
+                            for (uint32_t k = 0; k < TILE_ROWS / 16u; ++k)
+                                tc::mma_f16(tmem + P::DB_AT + m * 16u, b + m * (2u * P::CHUNK >> 4) + k * 128u, ones, ID_DB,
+                                            t != group || k != 0);
                 tc::commit(&s.empty[r.i]);
                 tc::commit(&s.dh_empty[h.i]);
             }
@@ -217,39 +215,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         }
         if (mine) tc::commit(&s.done);
         if (!ok) tc::mbar_wait_slow(&s.done, 0, fail, a.err, true);  // leave no product in flight
-    } else if (warp == 2) {
-        if (sums) {  // column sums: products of 16 outputs by 16 rows of dy with ones, which cost an eighth of the adds
-            tc::Ring r;
-            float total[OC * 4][4] = {};
-            const uint32_t k = (lane & 7u) + (lane >> 4) * 8u, o = (lane >> 3 & 1u) * 16u;  // row and byte of this lane's address
-            for (uint32_t t = group; t < a.tiles; t += a.groups) {
-                if (!__all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err))) break;
-                const uint32_t st = tc::smem_u32(smem) + r.i * P::STAGE + k * 128u;
-#pragma unroll
-                for (int c = 0; c < OC; ++c) {
-                    if (c % sharers != slab) continue;
-#pragma unroll
-                    for (uint32_t m = 0; m < 4; ++m)
-#pragma unroll
-                        for (uint32_t row = 0; row < TILE_ROWS; row += 16u)
-                            add_columns<T>(total[c * 4 + m], st + c * P::CHUNK + row * 128u + ((m * 32u + o) ^ (k & 7u) << 4));
-                }
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&s.empty[r.i]);
-                r.next(P::STAGES);
-            }
-#pragma unroll
-            for (int c = 0; c < OC; ++c)
-                if (c % sharers == slab && lane % 4u == 0) {
-                    float *out = a.db_parts + (uint64_t)group * (OC * 64u) + c * 64u + lane / 4u;
-#pragma unroll
-                    for (uint32_t m = 0; m < 4; ++m) {
-                        out[m * 16u] = total[c * 4 + m][0];
-                        out[m * 16u + 8u] = total[c * 4 + m][2];
-                    }
-                }
-        }
-    } else {  // activations: four sets of four warps take tiles in turn; a lane has a column of z (a
+    } else if (warp >= 4) {  // activations: four sets of four warps take tiles in turn; a lane has a column of z (a
               // warp one block of 32) and ROWS rows of the tile
         constexpr int ROWS = P::ROWS;
         const uint32_t quad = warp % 4u, set = (warp - 4u) / 4u;
@@ -304,8 +270,12 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             __syncwarp();
             scale[lane] = mx8_scale(E);
             __syncwarp();
-            ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err) &&
-                                     tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err));
+            ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
+            // A parity tells a phase from the one before it only.  Of a buffer's last use this set knows
+            // that it is over when that was four tiles ago or earlier; with fewer buffers it asks.
+            if (P::BUFS < 4u && t >= group + P::BUFS * a.groups)
+                ok = ok && __all_sync(~0u, tc::mbar_wait(&s.dh_full[dh.i], dh.phase ^ 1u, fail, a.err));
+            ok = ok && __all_sync(~0u, tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err));
             if (!ok) break;
             tc::fence_after();
             const uint8_t *codes = smem + r.i * P::STAGE + P::DY_BYTES + code0;
@@ -364,25 +334,31 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 }
             }
             out += out_step;
-            dh.skip(4, P::BUFS);
+            dh.skip(P::BUFS < 4u ? P::BUFS : 4u, P::BUFS);
+            if (P::BUFS < 4u) dh.skip(4u - P::BUFS, P::BUFS);
             r.skip(4, P::STAGES);
             E = next_E;
         }
-        if (a.dw_parts) {
-            ok = ok && tc::mbar_wait(&s.done, 0, fail, a.err);
-            if (__all_sync(~0u, ok)) {
-                tc::fence_after();
-                float *out = a.dw_parts + ((uint64_t)group * a.slabs + slab) * (OC * 64u) * 128u + quad * 32u + lane;
+        ok = __all_sync(~0u, ok && tc::mbar_wait(&s.done, 0, fail, a.err));
+        tc::fence_after();
+        if (ok && a.dw_parts) {
+            float *out = a.dw_parts + ((uint64_t)group * a.slabs + slab) * (OC * 64u) * 128u + quad * 32u + lane;
 #pragma unroll
-                for (uint32_t c = 0; c < OC; ++c) {
-                    const uint32_t o0 = (set * OC + c) * 16u;
-                    uint32_t v[16];
-                    tc::tmem_load16(tmem + lanes + o0, v);
-                    tc::tmem_wait_load();
+            for (uint32_t c = 0; c < OC; ++c) {
+                const uint32_t o0 = (set * OC + c) * 16u;
+                uint32_t v[16];
+                tc::tmem_load16(tmem + lanes + o0, v);
+                tc::tmem_wait_load();
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) out[(o0 + i) * 128u] = __uint_as_float(v[i]);
-                }
+                for (uint32_t i = 0; i < 16; ++i) out[(o0 + i) * 128u] = __uint_as_float(v[i]);
             }
+        }
+        if (ok && sums && set < P::MT && set % sharers == slab) {  // a lane has an output; its 16 columns are equal
+            uint32_t v[16];
+            tc::tmem_load16(tmem + P::DB_AT + set * 16u + lanes, v);
+            tc::tmem_wait_load();
+            const uint32_t o = set * 128u + quad * 32u + lane;
+            if (o < OC * 64u) a.db_parts[(uint64_t)group * (OC * 64u) + o] = __uint_as_float(v[0]);
         }
     }
     __syncwarp();
