@@ -170,6 +170,11 @@ def check_linear(got, dy, w, z8, act):
     R.assert_within(got[2], v, u * v.abs() + rows * 2.0 ** -23 * size + tiny, "db")
 
 
+# several tiles for every SM
+LINEAR += [(60001, 64, 3), (60001, 40, 64), (60000, 56, 250), (30011, 256, 256), (30011, 200, 130), (30000, 136, 70), (30000, 96, 192),
+           (20011, 520, 300), (3001, 96, 5000)]
+
+
 @pytest.mark.parametrize("dtype", TYPES16)
 @pytest.mark.parametrize("rows,cols,outs", LINEAR)
 def test_linear_backward(rows, cols, outs, dtype):
@@ -279,6 +284,10 @@ def test_linear_backward_is_reproducible():
 LINEAR4 = [(1, 1, 1), (1, 64, 8), (1, 4096, 512), (2, 33, 3), (16, 1000, 333), (17, 256, 128), (64, 96, 130),
            (77, 1000, 77), (130, 520, 264), (300, 192, 64), (1000, 75, 48), (513, 1024, 640), (128, 4100, 200),
            (9600, 96, 40), (10000, 75, 8), (9999, 200, 128), (9700, 520, 200), (2000, 333, 1300), (5000, 256, 512)]
+
+
+# several tiles for every SM, so that stages, accumulators and buffers are used again
+LINEAR4 += [(60001, 192, 64), (60001, 96, 48), (41000, 300, 100), (41000, 600, 256), (40960, 40, 130), (20001, 520, 600)]
 
 
 @pytest.mark.parametrize("dtype", TYPES16)

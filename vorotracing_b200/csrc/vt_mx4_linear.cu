@@ -35,10 +35,12 @@ template <int TN, bool QUANT> struct L4 {
     static constexpr uint32_t ACCS = TN == 256 ? 1 : 2;
     static constexpr uint32_t SF_AT = ACCS * TN, SF_COLS = 8u + 8u * B_PARTS;
     static constexpr uint32_t TMEM = SF_AT + SF_COLS <= 256 ? 256 : 512;
-    static constexpr uint32_t SCALE_WARPS = 4, QUANT_WARPS = QUANT ? 8 : 0;
+    // The warps that bring scales take stages in turn.  A parity tells a phase from the one before it only, and
+    // what a warp knows of a stage is from its last turn: there may be no more turns than stages.
+    static constexpr uint32_t SCALE_WARPS = 4, TURNS = STAGES < SCALE_WARPS ? STAGES : SCALE_WARPS, QUANT_WARPS = QUANT ? 8 : 0;
     // warps: 0 TMA, 1 products, 2 TMA of x, 3 none, 4..7 results, 8..11 scales, 12.. x to 4 bits
     static constexpr uint32_t THREADS = 32u * (8u + SCALE_WARPS + QUANT_WARPS);
-    static constexpr uint32_t FULL_COUNT = 1u + SCALE_WARPS + QUANT_WARPS;
+    static constexpr uint32_t FULL_COUNT = 1u + 1u + QUANT_WARPS;
     struct Ctrl {
         uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS], x_full[X_STAGES], x_empty[X_STAGES];
         uint32_t tmem;
@@ -228,32 +230,35 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             }
             acc.next(P::ACCS);
         }
-    } else if (warp >= 8 && warp < 12) {  // scales: a row of each operand's 128 a lane
-        const uint32_t i = (warp - 8u) * 32u + lane;
+    } else if (warp >= 8 && warp < 12) {  // scales: the four warps take stages in turn, which hides the loads' latency
+        constexpr int A_ROWS = QUANT ? 0 : L4_ROWS / 32, B_ROWS = TN / 32;
         tc::Ring r;
-        bool ok = true;
+        bool ok = warp - 8u < P::TURNS;
+        uint32_t turn = warp - 8u;  // stages until this warp's
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const uint64_t row = (uint64_t)(t / a.out_tiles) * L4_ROWS + i;
-            const uint32_t out = t % a.out_tiles * TN + i;
-            for (uint32_t c = 0; c < a.chunks; ++c) {
-                uint2 e[1 + P::B_PARTS];
-                if (!QUANT) e[0] = row < a.rows ? load_scales(a.x_exps, row, a.blocks, c * 8u) : make_uint2(0, 0);
+            const uint64_t row = (uint64_t)(t / a.out_tiles) * L4_ROWS + lane;
+            const uint32_t out = t % a.out_tiles * TN + lane;
+            for (uint32_t c = 0; c < a.chunks; ++c, r.next(P::STAGES), turn = turn ? turn - 1u : P::TURNS - 1u) {
+                if (turn != 0) continue;
+                uint2 e[A_ROWS + B_ROWS];
 #pragma unroll
-                for (uint32_t p = 0; p < P::B_PARTS; ++p)
-                    e[1 + p] = i + p * 128u < TN && out + p * 128u < a.outs ? load_scales(a.w_exps, out + p * 128u, a.blocks, c * 8u)
-                                                                            : make_uint2(0, 0);
+                for (int i = 0; i < A_ROWS; ++i)
+                    e[i] = row + i * 32u < a.rows ? load_scales(a.x_exps, row + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
+#pragma unroll
+                for (int i = 0; i < B_ROWS; ++i)
+                    e[A_ROWS + i] = out + i * 32u < a.outs ? load_scales(a.w_exps, out + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
                 ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
                 if (!ok) break;
-                uint8_t *sf = smem + r.i * P::STAGE + P::A_BYTES + P::B_BYTES + scale_place(i);
+                uint8_t *sf = smem + r.i * P::STAGE + P::A_BYTES + P::B_BYTES;
 #pragma unroll
-                for (uint32_t p = QUANT ? 1 : 0; p < 1 + P::B_PARTS; ++p) {
-                    *reinterpret_cast<uint32_t *>(sf + p * 1024u) = e[p].x;
-                    *reinterpret_cast<uint32_t *>(sf + p * 1024u + 512u) = e[p].y;
+                for (int i = 0; i < A_ROWS + B_ROWS; ++i) {
+                    uint8_t *to = sf + (i < A_ROWS ? scale_place(i * 32u + lane) : 1024u + scale_place((i - A_ROWS) * 32u + lane));
+                    *reinterpret_cast<uint32_t *>(to) = e[i].x;
+                    *reinterpret_cast<uint32_t *>(to + 512u) = e[i].y;
                 }
                 tc::fence_async_shared();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
-                r.next(P::STAGES);
             }
         }
     } else if (QUANT && warp == 2) {
@@ -348,7 +353,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_consta
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < FEW_STAGES; ++i) {
-            tc::mbar_init(&s.full[i], 1 + 4 + 8);
+            tc::mbar_init(&s.full[i], 1 + 1 + 8);
             tc::mbar_init(&s.empty[i], 1);
         }
         tc::mbar_init(&s.acc_full, 1);
@@ -401,17 +406,23 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_consta
         const uint32_t quad = warp % 4u, i = quad * 32u + lane;
         tc::Ring r;
         bool ok = true;
-        for (uint32_t c = c0; c < c1; ++c) {
-            const uint2 e = out0 + i < a.outs ? load_scales(a.w_exps, out0 + i, a.blocks, c * 8u) : make_uint2(0, 0);
+        for (uint32_t c = c0; c < c1; ++c, r.next(FEW_STAGES)) {
+            if ((c - c0) % 4u != quad) continue;  // the warps take stages in turn
+            uint2 e[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                e[k] = out0 + k * 32u + lane < a.outs ? load_scales(a.w_exps, out0 + k * 32u + lane, a.blocks, c * 8u) : make_uint2(0, 0);
             ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
             if (!ok) break;
-            uint8_t *sf = smem + r.i * FEW_STAGE + 32768u + scale_place(i);
-            *reinterpret_cast<uint32_t *>(sf) = e.x;
-            *reinterpret_cast<uint32_t *>(sf + 512u) = e.y;
+            uint8_t *sf = smem + r.i * FEW_STAGE + 32768u;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                *reinterpret_cast<uint32_t *>(sf + scale_place(k * 32u + lane)) = e[k].x;
+                *reinterpret_cast<uint32_t *>(sf + scale_place(k * 32u + lane) + 512u) = e[k].y;
+            }
             tc::fence_async_shared();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
-            r.next(FEW_STAGES);
         }
         if (ok && __all_sync(~0u, tc::mbar_wait(&s.acc_full, 0, fail, a.err))) {
             tc::fence_after();
@@ -432,7 +443,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_consta
             const bool ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
             if (!ok) break;
             uint8_t *st = smem + r.i * FEW_STAGE + 16384u;
-            for (uint32_t i = threadIdx.x - 256u; i < rows * 8u; i += 256u) {
+            // with few blocks a stage the warps' shares turn with the stages, so that all warps have loads in flight
+            for (uint32_t i = (warp - c * ((rows + 3u) / 4u)) % 8u * 32u + lane; i < rows * 8u; i += 256u) {
                 const uint32_t row = i / 8u, block = i % 8u, col = c * L4_K + block * 32u;
                 const T *p = (const T *)a.x + (row0 + row) * a.x_stride + col;
                 uint4 w[4];
