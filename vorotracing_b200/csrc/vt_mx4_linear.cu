@@ -26,15 +26,17 @@ constexpr uint32_t L4_ROWS = 128, L4_K = 256;
 
 template <int TN, bool QUANT> struct L4 {
     static constexpr uint32_t A_BYTES = L4_ROWS * 128u, B_BYTES = TN * 128u;
-    static constexpr uint32_t B_PARTS = TN > 128 ? TN / 128 : 1;  // groups of 128 rows of scales
+    static constexpr uint32_t B_PARTS = TN > 128 ? 2 : 1;  // groups of 128 rows of scales
     static constexpr uint32_t SF_BYTES = (1u + B_PARTS) * 1024u;
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SF_BYTES;
     static constexpr uint32_t STAGES = QUANT ? (TN == 256 ? 2 : 3) : 4;
     static constexpr uint32_t X_BYTES = L4_ROWS * 128u, X_STAGES = TN == 64 ? 8 : 7;  // QUANT: 64 columns of x each
     // two accumulators when they leave room for the scales
-    static constexpr uint32_t ACCS = TN == 256 ? 1 : 2;
-    static constexpr uint32_t SF_AT = ACCS * TN, SF_COLS = 8u + 8u * B_PARTS;
-    static constexpr uint32_t TMEM = SF_AT + SF_COLS <= 256 ? 256 : 512;
+    static constexpr uint32_t ACCS = TN > 224 ? 1 : 2;
+    // Scales in tensor memory have a place for every stage, or two in turn: nothing says that a copy waits
+    // for the products before it that still read what it overwrites.
+    static constexpr uint32_t SF_AT = ACCS * TN, SF_COLS = 8u + 8u * B_PARTS, SF_BUFS = QUANT ? STAGES : 2;
+    static constexpr uint32_t TMEM_USED = SF_AT + SF_BUFS * SF_COLS, TMEM = TMEM_USED <= 256 ? 256 : 512;
     // The warps that bring scales take stages in turn.  A parity tells a phase from the one before it only, and
     // what a warp knows of a stage is from its last turn: there may be no more turns than stages.
     static constexpr uint32_t SCALE_WARPS = 4, TURNS = STAGES < SCALE_WARPS ? STAGES : SCALE_WARPS, QUANT_WARPS = QUANT ? 8 : 0;
@@ -42,18 +44,18 @@ template <int TN, bool QUANT> struct L4 {
     static constexpr uint32_t THREADS = 32u * (8u + SCALE_WARPS + QUANT_WARPS);
     static constexpr uint32_t FULL_COUNT = 1u + 1u + QUANT_WARPS;
     struct Ctrl {
-        uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS], x_full[X_STAGES], x_empty[X_STAGES];
+        uint64_t full[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS], x_full[X_STAGES], x_empty[X_STAGES], failed;
         uint32_t tmem;
         tc::Fail fail;
         alignas(8) float bias[TN];
     };
     static constexpr uint32_t X_AT = STAGES * STAGE, CTRL_AT = X_AT + (QUANT ? X_STAGES * X_BYTES : 0u), SMEM = CTRL_AT + sizeof(Ctrl);
-    static_assert(SMEM <= 232448 && SF_AT + SF_COLS <= 512, "does not fit an SM");
+    static_assert(SMEM <= 232448 && TMEM_USED <= 512, "does not fit an SM");
 };
 
 struct L4Args {
     uint64_t rows;
-    uint32_t cols, outs, blocks, chunks, row_tiles, out_tiles;
+    uint32_t cols, outs, blocks, chunks, last_steps, row_tiles, out_tiles;  // last_steps: of 64, in a row's last chunk
     const uint8_t *x_exps;  // not QUANT
     const uint8_t *w_exps;
     const void *bias;
@@ -104,6 +106,27 @@ template <typename T> __device__ __forceinline__ uint4 block_codes(const uint4 *
     return make_uint4(codes[0], codes[1], codes[2], codes[3]);
 }
 
+// A stage's scales to tensor memory and its products, by one lane: `steps` of 64 steps of k, 4 but
+// for a row's last stage.  Descriptors of the operands at the stage's start; the scales of A
+// (1 group of 128 rows) and of B (PARTS groups) at sf, going to sfa and sfb.
+template <int PARTS>
+__device__ __forceinline__ void stage_products(uint32_t d, uint64_t a, uint64_t b, uint64_t sf, uint32_t sfa, uint32_t sfb, uint32_t id0,
+                                               uint32_t id1, uint32_t steps, bool accumulate)
+{
+#pragma unroll
+    for (uint32_t g = 0; g < 2; ++g)
+        if (2u * g < steps) {
+            tc::tmem_copy_scales(sfa + g * 4u, sf + g * 32u);
+#pragma unroll
+            for (uint32_t p = 0; p < PARTS; ++p) tc::tmem_copy_scales(sfb + (g * PARTS + p) * 4u, sf + 64u + p * 64u + g * 32u);
+        }
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+        if (k < steps)
+            tc::mma_mxf4(d, a + k * 2u, b + k * 2u, k & 1u ? id1 : id0, sfa + (k >> 1) * 4u, sfb + (k >> 1) * PARTS * 4u,
+                         accumulate || k != 0);
+}
+
 template <typename T, int ACT, int TN, bool QUANT>
 __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
     linear4_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const L4Args a)
@@ -111,7 +134,7 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
     using P = L4<TN, QUANT>;
     extern __shared__ __align__(1024) uint8_t smem[];
     typename P::Ctrl &s = *reinterpret_cast<typename P::Ctrl *>(smem + P::CTRL_AT);
-    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    const uint32_t warp = tc::warp_number(), lane = threadIdx.x % 32u;
     const uint32_t tiles = a.row_tiles * a.out_tiles;
     tc::Fail *const fail = &s.fail;
 
@@ -128,6 +151,7 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             tc::mbar_init(&s.x_full[i], 1);
             tc::mbar_init(&s.x_empty[i], P::QUANT_WARPS);
         }
+        tc::mbar_init(&s.failed, 1);
         s.fail.failed = 0;
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&w_map);
@@ -159,41 +183,42 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             // see that its copies are in: it waits for them by time, far longer than a copy takes.
             if (s.fail.failed) tc::outlast_copies();
         }
-    } else if (warp == 1) {
-        if (lane == 0) {  // scales to tensor memory, products
-            const uint32_t base = tc::smem_u32(smem);
-            tc::Ring r, acc;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                ok = tc::mbar_wait(&s.acc_empty[acc.i], acc.phase ^ 1u, fail, a.err);
+    } else if (warp == 1) {  // scales to tensor memory, products
+        const uint32_t base = tc::smem_u32(smem);
+        constexpr uint32_t ID0 = tc::idesc_mxf4(128, TN, 0), ID1 = tc::idesc_mxf4(128, TN, 1);
+        const bool mine = tc::elect();
+        tc::Ring r, acc, old, sf;  // old: the stage whose scales' place comes next
+        uint32_t ahead = 0;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            ok = __all_sync(~0u, tc::mbar_wait(&s.acc_empty[acc.i], acc.phase ^ 1u, fail, a.err));
+            if (!ok) break;
+            tc::fence_after();
+            for (uint32_t c = 0; c < a.chunks; ++c) {
+                ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
+                if (P::SF_BUFS < P::STAGES && ++ahead > P::SF_BUFS) {
+                    ok = ok && __all_sync(~0u, tc::mbar_wait(&s.empty[old.i], old.phase, fail, a.err));
+                    old.next(P::STAGES);
+                }
                 if (!ok) break;
-                const uint32_t d = tmem + acc.i * TN, sfa = tmem + P::SF_AT, sfb = sfa + 8u;
-                for (uint32_t c = 0; c < a.chunks; ++c) {
-                    ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
-                    if (!ok) break;
-                    tc::fence_after();
-                    const uint32_t st = base + r.i * P::STAGE, sf = st + P::A_BYTES + P::B_BYTES;
-                    const uint32_t steps = min(4u, (a.cols - c * L4_K + 63u) / 64u);
-                    for (uint32_t g = 0; 2u * g < steps; ++g) {
-                        tc::tmem_copy_scales(sfa + g * 4u, tc::scale_desc(sf + g * 512u));
-                        for (uint32_t p = 0; p < P::B_PARTS; ++p)
-                            tc::tmem_copy_scales(sfb + (g * P::B_PARTS + p) * 4u, tc::scale_desc(sf + 1024u + p * 1024u + g * 512u));
-                    }
-                    for (uint32_t k = 0; k < steps; ++k) {
-                        constexpr uint32_t ID0 = tc::idesc_mxf4(128, TN, 0), ID1 = tc::idesc_mxf4(128, TN, 1);
-                        tc::mma_mxf4(d, tc::smem_desc(st + k * 32u, 16, 1024), tc::smem_desc(st + P::A_BYTES + k * 32u, 16, 1024),
-                                     k & 1u ? ID1 : ID0, sfa + (k >> 1) * 4u, sfb + (k >> 1) * P::B_PARTS * 4u, c + k != 0);
-                    }
+                tc::fence_after();
+                const uint32_t st = base + r.i * P::STAGE, sfa = tmem + P::SF_AT + sf.i * P::SF_COLS, sfb = sfa + 8u;
+                sf.next(P::SF_BUFS);
+                if (mine) {
+                    stage_products<P::B_PARTS>(tmem + acc.i * TN, tc::smem_desc(st, 16, 1024), tc::smem_desc(st + P::A_BYTES, 16, 1024),
+                                               tc::scale_desc(st + P::A_BYTES + P::B_BYTES), sfa, sfb, ID0, ID1,
+                                               c + 1u == a.chunks ? a.last_steps : 4u, c != 0);
                     tc::commit(&s.empty[r.i]);
-                    r.next(P::STAGES);
+                    if (c + 1u == a.chunks) tc::commit(&s.acc_full[acc.i]);
                 }
-                tc::commit(&s.acc_full[acc.i]);
-                if (!ok) {  // leave no product in flight
-                    tc::mbar_wait_slow(&s.acc_full[acc.i], acc.phase, fail, a.err, true);
-                    break;
-                }
-                acc.next(P::ACCS);
+                __syncwarp();
+                r.next(P::STAGES);
             }
+            acc.next(P::ACCS);
+        }
+        if (!ok) {  // leave no product in flight
+            if (mine) tc::commit(&s.failed);
+            tc::mbar_wait_slow(&s.failed, 0, fail, a.err, true);
         }
     } else if (warp >= 4 && warp < 8) {  // results
         const uint32_t quad = warp % 4u, in_tile = quad * 32u + lane;
@@ -216,7 +241,6 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             for (uint32_t n0 = 0; n0 < TN; n0 += 32u) {
                 uint32_t v[32], w[16];
                 tc::tmem_load32(tmem + acc.i * TN + (quad * 32u << 16) + n0, v);
-                tc::tmem_wait_load();
                 if (n0 + 32u == TN) {
                     tc::fence_before();
                     __syncwarp();
@@ -297,14 +321,16 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
                     uint4 w[4];
 #pragma unroll
                     for (uint32_t u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const uint4 *>(from + (((part * 4u + u) ^ (row & 7u)) << 4));
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&s.x_empty[x.i]);
-                    x.next(P::X_STAGES);
                     uint32_t E;
                     const uint4 codes = block_codes<T>(w, E);
                     const uint32_t block = k * 2u + part;
                     *reinterpret_cast<uint4 *>(st + row * 128u + ((block ^ (row & 7u)) << 4)) = codes;
                     sf[(block >> 2) * 512u + (block & 3u)] = (uint8_t)E;
+                    // x's place is free once its values have arrived in registers, which the stores above, made
+                    // of them, have seen; an arrival right behind the loads may overtake them
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s.x_empty[x.i]);
+                    x.next(P::X_STAGES);
                 }
                 tc::fence_async_shared();
                 __syncwarp();
@@ -313,6 +339,7 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             }
         }
     }
+    __syncwarp();
     tc::fence_before();
     __syncthreads();
     if (warp == 1) tc::tmem_free<P::TMEM>(tmem);
@@ -330,7 +357,7 @@ constexpr uint32_t FEW_SMEM = FEW_STAGES * FEW_STAGE + sizeof(FewCtrl);
 
 struct FewArgs {
     uint64_t rows, x_stride;
-    uint32_t cols, outs, blocks, chunks, chunks_a_split;
+    uint32_t cols, outs, blocks, chunks, last_steps, chunks_a_split;
     const void *x;
     const uint8_t *w_exps;
     const void *bias;
@@ -345,7 +372,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_consta
 {
     extern __shared__ __align__(1024) uint8_t smem[];
     FewCtrl &s = *reinterpret_cast<FewCtrl *>(smem + FEW_STAGES * FEW_STAGE);
-    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, splits = gridDim.x, rank = blockIdx.x;
+    const uint32_t warp = tc::warp_number(), lane = threadIdx.x % 32u, splits = gridDim.x, rank = blockIdx.x;
     const uint32_t out0 = blockIdx.y * 128u, c0 = rank * a.chunks_a_split, c1 = min(a.chunks, c0 + a.chunks_a_split);
     const uint64_t row0 = (uint64_t)blockIdx.z * 128u;
     const uint32_t rows = (uint32_t)(a.rows - row0 < 128u ? a.rows - row0 : 128u), n = (rows + 15u) / 16u * 16u;
@@ -378,30 +405,27 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_consta
             }
             if (s.fail.failed) tc::outlast_copies();
         }
-    } else if (warp == 1) {
-        if (lane == 0) {  // scales to tensor memory, products
-            const uint32_t base = tc::smem_u32(smem), sfa = tmem + 128u, sfb = sfa + 8u;
-            const uint32_t id = tc::idesc_mxf4(128, 0, 0) | (n >> 3) << 17, id1 = tc::idesc_mxf4(128, 0, 1) | (n >> 3) << 17;
-            tc::Ring r;
-            bool ok = true;
-            for (uint32_t c = c0; c < c1; ++c) {
-                ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
-                if (!ok) break;
-                tc::fence_after();
-                const uint32_t st = base + r.i * FEW_STAGE, sf = st + 32768u, steps = min(4u, (a.cols - c * L4_K + 63u) / 64u);
-                for (uint32_t g = 0; 2u * g < steps; ++g) {
-                    tc::tmem_copy_scales(sfa + g * 4u, tc::scale_desc(sf + g * 512u));
-                    tc::tmem_copy_scales(sfb + g * 4u, tc::scale_desc(sf + 1024u + g * 512u));
-                }
-                for (uint32_t k = 0; k < steps; ++k)
-                    tc::mma_mxf4(tmem, tc::smem_desc(st + k * 32u, 16, 1024), tc::smem_desc(st + 16384u + k * 32u, 16, 1024),
-                                 k & 1u ? id1 : id, sfa + (k >> 1) * 4u, sfb + (k >> 1) * 4u, c != c0 || k != 0);
+    } else if (warp == 1) {  // scales to tensor memory, products
+        const uint32_t base = tc::smem_u32(smem);
+        const uint32_t id0 = tc::idesc_mxf4(128, 0, 0) | (n >> 3) << 17, id1 = tc::idesc_mxf4(128, 0, 1) | (n >> 3) << 17;
+        const bool mine = tc::elect();
+        tc::Ring r;
+        bool ok = true;
+        for (uint32_t c = c0; c < c1; ++c) {
+            ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
+            if (!ok) break;
+            tc::fence_after();
+            const uint32_t st = base + r.i * FEW_STAGE, sfa = tmem + 128u + r.i * 16u, sfb = sfa + 8u;  // a place for every stage
+            if (mine) {
+                stage_products<1>(tmem, tc::smem_desc(st, 16, 1024), tc::smem_desc(st + 16384u, 16, 1024), tc::scale_desc(st + 32768u), sfa,
+                                  sfb, id0, id1, c + 1u == a.chunks ? a.last_steps : 4u, c != c0);
                 tc::commit(&s.empty[r.i]);
-                r.next(FEW_STAGES);
             }
-            tc::commit(&s.acc_full);
-            if (!ok) tc::mbar_wait_slow(&s.acc_full, 0, fail, a.err, true);  // leave no product in flight
+            __syncwarp();
+            r.next(FEW_STAGES);
         }
+        if (mine) tc::commit(&s.acc_full);
+        if (!ok) tc::mbar_wait_slow(&s.acc_full, 0, fail, a.err, true);  // leave no product in flight
     } else if (warp >= 4 && warp < 8) {  // the weight's scales, then this CTA's sums to its shared memory
         const uint32_t quad = warp % 4u, i = quad * 32u + lane;
         tc::Ring r;
@@ -431,7 +455,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_consta
             for (uint32_t j = 0; j < n; j += 32u) {
                 uint32_t v[32];
                 tc::tmem_load32(tmem + (quad * 32u << 16) + j, v);
-                tc::tmem_wait_load();
 #pragma unroll
                 for (uint32_t k = 0; k < 32; ++k)  // the last splits may have no part of k
                     if (j + k < rows) sum[(j + k) * 128u + i] = c0 < c1 ? __uint_as_float(v[k]) : 0.0f;
@@ -597,6 +620,7 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
         a.outs = outs;
         a.blocks = vt::mx_blocks(cols);
         a.chunks = (cols + vt::L4_K - 1u) / vt::L4_K;
+        a.last_steps = ((cols - 1u) % vt::L4_K + 64u) / 64u;
         a.w_exps = exps;
         a.bias = bias;
         a.y = y;
@@ -611,6 +635,7 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
             f.outs = outs;
             f.blocks = a.blocks;
             f.chunks = a.chunks;
+            f.last_steps = a.last_steps;
             f.x = x;
             f.w_exps = exps;
             f.bias = bias;
@@ -634,7 +659,7 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
         if (vt_status s = vt_mx4_quantize(x, dtype, rows, cols, x_stride, x_codes, x_exps, stream)) return s;
         a.x_exps = x_exps;
         return vt::with_act(act, [&](auto f) -> vt_status {
-            return vt::launch_linear4<T, decltype(f)::value, 256, false>(x_codes, 0, codes, a, st);
+            return vt::launch_linear4<T, decltype(f)::value, 224, false>(x_codes, 0, codes, a, st);
         });
     });
 }

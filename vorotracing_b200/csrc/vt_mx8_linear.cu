@@ -285,7 +285,6 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             for (int p = 0; p < ROWS; p += 16) {
                 uint32_t g[16], h[8], d[8];
                 tc::tmem_load16(here + p, g);
-                tc::tmem_wait_load();
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t c0 = codes[(p + 2 * i) * P::CODE_PITCH], c1 = codes[(p + 2 * i + 1) * P::CODE_PITCH];
@@ -348,7 +347,6 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 const uint32_t o0 = (set * OC + c) * 16u;
                 uint32_t v[16];
                 tc::tmem_load16(tmem + lanes + o0, v);
-                tc::tmem_wait_load();
 #pragma unroll
                 for (uint32_t i = 0; i < 16; ++i) out[(o0 + i) * 128u] = __uint_as_float(v[i]);
             }
@@ -356,7 +354,6 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         if (ok && sums && set < P::MT && set % sharers == slab) {  // a lane has an output; its 16 columns are equal
             uint32_t v[16];
             tc::tmem_load16(tmem + P::DB_AT + set * 16u + lanes, v);
-            tc::tmem_wait_load();
             const uint32_t o = set * 128u + quad * 32u + lane;
             if (o < OC * 64u) a.db_parts[(uint64_t)group * (OC * 64u) + o] = __uint_as_float(v[0]);
         }
@@ -402,7 +399,7 @@ __global__ void __launch_bounds__(256) narrow_reduce_kernel(const float *__restr
 
 constexpr uint32_t WIDE_STAGES = 6, WIDE_STAGE_BYTES = 32768, WIDE_THREADS = 256;
 struct WideCtrl {
-    uint64_t full[WIDE_STAGES], empty[WIDE_STAGES], acc_full[2], acc_empty[2];
+    uint64_t full[WIDE_STAGES], empty[WIDE_STAGES], acc_full[2], acc_empty[2], failed;
     uint32_t tmem;
     tc::Fail fail;
 };
@@ -430,7 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(1024) uint8_t smem[];
     WideCtrl &s = *reinterpret_cast<WideCtrl *>(smem + WIDE_STAGES * WIDE_STAGE_BYTES);
-    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = tc::cluster_rank();
+    const uint32_t warp = tc::warp_number(), lane = threadIdx.x % 32u, rank = tc::cluster_rank();
     const uint32_t units = a.m_tiles * a.n_tiles * a.splits, first = blockIdx.x / 2u, step = gridDim.x / 2u;
     const uint32_t half_n = a.tile_n / 2u, b_boxes = half_n > 64u ? 2u : 1u;
     tc::Fail *const fail = &s.fail;
@@ -444,6 +441,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
             tc::mbar_init(&s.acc_full[i], 1);
             tc::mbar_init(&s.acc_empty[i], 8);
         }
+        tc::mbar_init(&s.failed, 1);
         s.fail.failed = 0;
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&a_map);
@@ -485,33 +483,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
             if (s.fail.failed) tc::outlast_copies();
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {  // products, in the leader
+        if (rank == 0) {  // products, in the leader
             const uint32_t base = tc::smem_u32(smem), id = tc::idesc_f16<BF16>(256, 0, !DZ, true) | (a.tile_n >> 3) << 17;
+            const bool mine = tc::elect();
             tc::Ring r, acc;
             bool ok = true;
             for (uint32_t u = first; u < units && ok; u += step) {
                 const uint32_t c0 = u / (a.m_tiles * a.n_tiles) * a.chunks_a_split, c1 = min(a.chunks, c0 + a.chunks_a_split);
-                ok = tc::mbar_wait(&s.acc_empty[acc.i], acc.phase ^ 1u, fail, a.err);
+                ok = __all_sync(~0u, tc::mbar_wait(&s.acc_empty[acc.i], acc.phase ^ 1u, fail, a.err));
                 if (!ok) break;
+                tc::fence_after();
                 for (uint32_t c = c0; c < c1; ++c) {
-                    ok = tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err);
+                    ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
                     if (!ok) break;
                     tc::fence_after();
                     const uint32_t st = base + r.i * WIDE_STAGE_BYTES;
+                    const uint64_t da = DZ ? tc::smem_desc(st, 16, 1024) : tc::smem_desc(st, 8192, 1024), db = tc::smem_desc(st + 16384u, 8192, 1024);
+                    if (mine) {
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)
-                        tc::mma_f16_pair(tmem + acc.i * 256u,
-                                         DZ ? tc::smem_desc(st + k * 32u, 16, 1024) : tc::smem_desc(st + k * 2048u, 8192, 1024),
-                                         tc::smem_desc(st + 16384u + k * 2048u, 8192, 1024), id, c != c0 || k != 0);
-                    tc::commit_pair(&s.empty[r.i]);
+                        for (uint32_t k = 0; k < 4; ++k)
+                            tc::mma_f16_pair(tmem + acc.i * 256u, da + k * (DZ ? 2u : 128u), db + k * 128u, id, c != c0 || k != 0);
+                        tc::commit_pair(&s.empty[r.i]);
+                        if (c + 1u == c1) tc::commit_pair(&s.acc_full[acc.i]);
+                    }
+                    __syncwarp();
                     r.next(WIDE_STAGES);
                 }
-                tc::commit_pair(&s.acc_full[acc.i]);
-                if (!ok) {  // leave no product in flight
-                    tc::mbar_wait_slow(&s.acc_full[acc.i], acc.phase, fail, a.err, true);
-                    break;
-                }
                 acc.next(2);
+            }
+            if (!ok) {  // leave no product in flight
+                if (mine) tc::commit_pair(&s.failed);
+                tc::mbar_wait_slow(&s.failed, 0, fail, a.err, true);
             }
         }
     } else if (warp >= 4) {  // results: a lane has a row of this CTA's 128
@@ -539,7 +541,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
                     }
                 }
                 tc::tmem_load32(tmem + acc.i * 256u + (quad * 32u << 16) + j, v);
-                tc::tmem_wait_load();
                 if (j + 32u >= a.tile_n) {
                     tc::fence_before();
                     __syncwarp();
