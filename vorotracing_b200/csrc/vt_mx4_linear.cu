@@ -6,40 +6,41 @@
 // thread issues copies and products; four warps take finished accumulators out of tensor memory,
 // add the bias, apply the activation and round once.
 //
-// x is rounded to 4 bits inside the same kernel while one tile spans all outputs (QUANT): TMA
+// x is rounded to 4 bits inside the same kernel while one tile spans all outputs (linear4_kernel): TMA
 // brings x in as it is, deep enough ahead to keep HBM busy (112 to 128 KB), and eight warps round
 // it, a lane a block of 32 columns, into the operand's place.  x is then read from HBM once and
 // nothing of its 4-bit form is written.
 // With more outputs the same rows would be rounded again for every tile of outputs, so a pass of
-// its own writes codes and scales first, 17/32 byte a value, and TMA brings them in.
-#include "vt_mx_rows.cuh"
-
+// its own writes codes and scales first, 17/32 byte a value, and pairs of CTAs multiply
+// (pair4_kernel).
+//
 // Too few tiles to occupy the GPU (few rows, as in serving one token at a time) go the other way
 // round (few_kernel): 128 outputs are the product's rows and up to 128 rows of x its columns, k is
 // split over a cluster of up to 8 CTAs, each CTA rounds its part of x itself, and the parts of the
 // sums meet in distributed shared memory, where they are added in the order of k.  One launch; the
 // weight is spread over as many SMs as there are.
+#include "vt_mx_rows.cuh"
 
 namespace vt {
 
 constexpr uint32_t L4_ROWS = 128, L4_K = 256;
 
-template <int TN, bool QUANT> struct L4 {
+template <int TN> struct L4 {
     static constexpr uint32_t A_BYTES = L4_ROWS * 128u, B_BYTES = TN * 128u;
     static constexpr uint32_t B_PARTS = TN > 128 ? 2 : 1;  // groups of 128 rows of scales
     static constexpr uint32_t SF_BYTES = (1u + B_PARTS) * 1024u;
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SF_BYTES;
-    static constexpr uint32_t STAGES = QUANT ? (TN == 256 ? 2 : 3) : 4;
-    static constexpr uint32_t X_BYTES = L4_ROWS * 128u, X_STAGES = TN == 64 ? 8 : 7;  // QUANT: 64 columns of x each
+    static constexpr uint32_t STAGES = TN == 256 ? 2 : 3;
+    static constexpr uint32_t X_BYTES = L4_ROWS * 128u, X_STAGES = TN == 64 ? 8 : 7;  // 64 columns of x each
     // two accumulators when they leave room for the scales
-    static constexpr uint32_t ACCS = TN > 224 ? 1 : 2;
-    // Scales in tensor memory have a place for every stage, or two in turn: nothing says that a copy waits
-    // for the products before it that still read what it overwrites.
-    static constexpr uint32_t SF_AT = ACCS * TN, SF_COLS = 8u + 8u * B_PARTS, SF_BUFS = QUANT ? STAGES : 2;
-    static constexpr uint32_t TMEM_USED = SF_AT + SF_BUFS * SF_COLS, TMEM = TMEM_USED <= 256 ? 256 : 512;
+    static constexpr uint32_t ACCS = TN == 256 ? 1 : 2;
+    // Scales in tensor memory have a place for every stage: nothing says that a copy waits for the products
+    // before it that still read what it overwrites.
+    static constexpr uint32_t SF_AT = ACCS * TN, SF_COLS = 8u + 8u * B_PARTS;
+    static constexpr uint32_t TMEM_USED = SF_AT + STAGES * SF_COLS, TMEM = TMEM_USED <= 256 ? 256 : 512;
     // The warps that bring scales take stages in turn.  A parity tells a phase from the one before it only, and
     // what a warp knows of a stage is from its last turn: there may be no more turns than stages.
-    static constexpr uint32_t SCALE_WARPS = 4, TURNS = STAGES < SCALE_WARPS ? STAGES : SCALE_WARPS, QUANT_WARPS = QUANT ? 8 : 0;
+    static constexpr uint32_t SCALE_WARPS = 4, TURNS = STAGES < SCALE_WARPS ? STAGES : SCALE_WARPS, QUANT_WARPS = 8;
     // warps: 0 TMA, 1 products, 2 TMA of x, 3 none, 4..7 results, 8..11 scales, 12.. x to 4 bits
     static constexpr uint32_t THREADS = 32u * (8u + SCALE_WARPS + QUANT_WARPS);
     static constexpr uint32_t FULL_COUNT = 1u + 1u + QUANT_WARPS;
@@ -49,14 +50,14 @@ template <int TN, bool QUANT> struct L4 {
         tc::Fail fail;
         alignas(8) float bias[TN];
     };
-    static constexpr uint32_t X_AT = STAGES * STAGE, CTRL_AT = X_AT + (QUANT ? X_STAGES * X_BYTES : 0u), SMEM = CTRL_AT + sizeof(Ctrl);
+    static constexpr uint32_t X_AT = STAGES * STAGE, CTRL_AT = X_AT + X_STAGES * X_BYTES, SMEM = CTRL_AT + sizeof(Ctrl);
     static_assert(SMEM <= 232448 && TMEM_USED <= 512, "does not fit an SM");
 };
 
 struct L4Args {
     uint64_t rows;
     uint32_t cols, outs, blocks, chunks, last_steps, row_tiles, out_tiles;  // last_steps: of 64, in a row's last chunk
-    const uint8_t *x_exps;  // not QUANT
+    const uint8_t *x_exps;  // pair4_kernel
     const uint8_t *w_exps;
     const void *bias;
     void *y;
@@ -77,6 +78,12 @@ __device__ __forceinline__ uint2 load_scales(const uint8_t *exps, uint64_t row, 
 }
 // Place of a row's scales in a stage: 16 bytes for each of 32 rows, a word a group of 32.
 __device__ __forceinline__ uint32_t scale_place(uint32_t row) { return (row >> 7) * 1024u + (row & 31u) * 16u + ((row >> 5) & 3u) * 4u; }
+
+__device__ __forceinline__ void store_scales(uint8_t *sf, uint32_t row, uint2 e)
+{
+    *reinterpret_cast<uint32_t *>(sf + scale_place(row)) = e.x;
+    *reinterpret_cast<uint32_t *>(sf + scale_place(row) + 512u) = e.y;
+}
 
 // A block of 32 16-bit numbers to 4 bits: codes and exponent byte
 template <typename T> __device__ __forceinline__ uint4 block_codes(const uint4 *w, uint32_t &E)
@@ -106,36 +113,53 @@ template <typename T> __device__ __forceinline__ uint4 block_codes(const uint4 *
     return make_uint4(codes[0], codes[1], codes[2], codes[3]);
 }
 
+// Columns col..col + 31 of a row of y from sums and bias.
+template <typename T, int ACT>
+__device__ __forceinline__ void store_results(T *row, uint32_t col, uint32_t cols, bool wide, const uint32_t *v, const float *bias)
+{
+    uint32_t w[16];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i)
+        w[i] = pack2<T>(act_value2<ACT>(add2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])),
+                                             *reinterpret_cast<const f32x2 *>(bias + 2 * i))));
+    store_row32<T>(row, col, cols, wide, w);
+}
+
 // A stage's scales to tensor memory and its products, by one lane: `steps` of 64 steps of k, 4 but
 // for a row's last stage.  Descriptors of the operands at the stage's start; the scales of A
 // (1 group of 128 rows) and of B (PARTS groups) at sf, going to sfa and sfb.
-template <int PARTS>
+template <int PARTS, bool PAIR = false>
 __device__ __forceinline__ void stage_products(uint32_t d, uint64_t a, uint64_t b, uint64_t sf, uint32_t sfa, uint32_t sfb, uint32_t id0,
                                                uint32_t id1, uint32_t steps, bool accumulate)
 {
+    const auto copy = [](uint32_t to, uint64_t from) {
+        if (PAIR) tc::tmem_copy_scales_pair(to, from); else tc::tmem_copy_scales(to, from);
+    };
 #pragma unroll
     for (uint32_t g = 0; g < 2; ++g)
         if (2u * g < steps) {
-            tc::tmem_copy_scales(sfa + g * 4u, sf + g * 32u);
+            copy(sfa + g * 4u, sf + g * 32u);
 #pragma unroll
-            for (uint32_t p = 0; p < PARTS; ++p) tc::tmem_copy_scales(sfb + (g * PARTS + p) * 4u, sf + 64u + p * 64u + g * 32u);
+            for (uint32_t p = 0; p < PARTS; ++p) copy(sfb + (g * PARTS + p) * 4u, sf + 64u + p * 64u + g * 32u);
         }
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k)
-        if (k < steps)
-            tc::mma_mxf4(d, a + k * 2u, b + k * 2u, k & 1u ? id1 : id0, sfa + (k >> 1) * 4u, sfb + (k >> 1) * PARTS * 4u,
-                         accumulate || k != 0);
+        if (k < steps) {
+            const uint32_t id = k & 1u ? id1 : id0, ta = sfa + (k >> 1) * 4u, tb = sfb + (k >> 1) * PARTS * 4u;
+            if (PAIR) tc::mma_mxf4_pair(d, a + k * 2u, b + k * 2u, id, ta, tb, accumulate || k != 0);
+            else tc::mma_mxf4(d, a + k * 2u, b + k * 2u, id, ta, tb, accumulate || k != 0);
+        }
 }
 
-template <typename T, int ACT, int TN, bool QUANT>
-__global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
+template <typename T, int ACT, int TN>
+__global__ void __launch_bounds__(L4<TN>::THREADS, 1)
     linear4_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const L4Args a)
 {
-    using P = L4<TN, QUANT>;
+    using P = L4<TN>;
     extern __shared__ __align__(1024) uint8_t smem[];
     typename P::Ctrl &s = *reinterpret_cast<typename P::Ctrl *>(smem + P::CTRL_AT);
     const uint32_t warp = tc::warp_number(), lane = threadIdx.x % 32u;
-    const uint32_t tiles = a.row_tiles * a.out_tiles;
+    const uint32_t tiles = a.row_tiles;  // one tile spans all outputs
     tc::Fail *const fail = &s.fail;
 
     if (threadIdx.x == 0) {
@@ -168,14 +192,12 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             tc::Ring r;
             bool ok = true;
             for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                const int row0 = (int)(t / a.out_tiles * L4_ROWS), out0 = (int)(t % a.out_tiles * TN);
                 for (uint32_t c = 0; c < a.chunks; ++c) {
                     ok = tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err);
                     if (!ok) break;
                     uint8_t *st = smem + r.i * P::STAGE;
-                    tc::mbar_arrive_tx(&s.full[r.i], P::B_BYTES + (QUANT ? 0u : P::A_BYTES));
-                    if (!QUANT) tc::tma_load_2d(st, &x_map, (int)(c * 128u), row0, &s.full[r.i]);
-                    tc::tma_load_2d(st + P::A_BYTES, &w_map, (int)(c * 128u), out0, &s.full[r.i]);
+                    tc::mbar_arrive_tx(&s.full[r.i], P::B_BYTES);
+                    tc::tma_load_2d(st + P::A_BYTES, &w_map, (int)(c * 128u), 0, &s.full[r.i]);
                     r.next(P::STAGES);
                 }
             }
@@ -187,8 +209,7 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
         const uint32_t base = tc::smem_u32(smem);
         constexpr uint32_t ID0 = tc::idesc_mxf4(128, TN, 0), ID1 = tc::idesc_mxf4(128, TN, 1);
         const bool mine = tc::elect();
-        tc::Ring r, acc, old, sf;  // old: the stage whose scales' place comes next
-        uint32_t ahead = 0;
+        tc::Ring r, acc;
         bool ok = true;
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
             ok = __all_sync(~0u, tc::mbar_wait(&s.acc_empty[acc.i], acc.phase ^ 1u, fail, a.err));
@@ -196,14 +217,9 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
             tc::fence_after();
             for (uint32_t c = 0; c < a.chunks; ++c) {
                 ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
-                if (P::SF_BUFS < P::STAGES && ++ahead > P::SF_BUFS) {
-                    ok = ok && __all_sync(~0u, tc::mbar_wait(&s.empty[old.i], old.phase, fail, a.err));
-                    old.next(P::STAGES);
-                }
                 if (!ok) break;
                 tc::fence_after();
-                const uint32_t st = base + r.i * P::STAGE, sfa = tmem + P::SF_AT + sf.i * P::SF_COLS, sfb = sfa + 8u;
-                sf.next(P::SF_BUFS);
+                const uint32_t st = base + r.i * P::STAGE, sfa = tmem + P::SF_AT + r.i * P::SF_COLS, sfb = sfa + 8u;
                 if (mine) {
                     stage_products<P::B_PARTS>(tmem + acc.i * TN, tc::smem_desc(st, 16, 1024), tc::smem_desc(st + P::A_BYTES, 16, 1024),
                                                tc::scale_desc(st + P::A_BYTES + P::B_BYTES), sfa, sfb, ID0, ID1,
@@ -222,70 +238,50 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
         }
     } else if (warp >= 4 && warp < 8) {  // results
         const uint32_t quad = warp % 4u, in_tile = quad * 32u + lane;
+        for (uint32_t i = in_tile; i < TN; i += 128u) s.bias[i] = a.bias && i < a.outs ? to_f32<T>(__ldg((const T *)a.bias + i)) : 0.0f;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
         tc::Ring acc;
         for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-            const uint64_t row = (uint64_t)(t / a.out_tiles) * L4_ROWS + in_tile;
-            const uint32_t out0 = t % a.out_tiles * TN;
-            // the bias of the tile's outputs; the first barrier keeps the last tile's until it is used
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            for (uint32_t i = in_tile; i < TN; i += 128u)
-                s.bias[i] = a.bias && out0 + i < a.outs ? to_f32<T>(__ldg((const T *)a.bias + out0 + i)) : 0.0f;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const uint64_t row = (uint64_t)t * L4_ROWS + in_tile;
             const bool ok = tc::mbar_wait(&s.acc_full[acc.i], acc.phase, fail, a.err);
-            if (!__all_sync(~0u, ok)) {  // failed: on to the next barrier with the other warps
-                acc.next(P::ACCS);
-                continue;
-            }
+            if (!__all_sync(~0u, ok)) break;
             tc::fence_after();
 #pragma unroll 1
             for (uint32_t n0 = 0; n0 < TN; n0 += 32u) {
-                uint32_t v[32], w[16];
+                uint32_t v[32];
                 tc::tmem_load32(tmem + acc.i * TN + (quad * 32u << 16) + n0, v);
                 if (n0 + 32u == TN) {
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.acc_empty[acc.i]);
                 }
-#pragma unroll
-                for (uint32_t i = 0; i < 16; ++i)
-                    w[i] = pack2<T>(act_value2<ACT>(add2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])),
-                                                         *reinterpret_cast<const f32x2 *>(&s.bias[n0 + 2 * i]))));
-                if (row < a.rows) store_row32<T>((T *)a.y + row * a.outs, out0 + n0, a.outs, a.y_wide, w);
+                if (row < a.rows) store_results<T, ACT>((T *)a.y + row * a.outs, n0, a.outs, a.y_wide, v, s.bias + n0);
             }
             acc.next(P::ACCS);
         }
     } else if (warp >= 8 && warp < 12) {  // scales: the four warps take stages in turn, which hides the loads' latency
-        constexpr int A_ROWS = QUANT ? 0 : L4_ROWS / 32, B_ROWS = TN / 32;
+        constexpr int ROWS = TN / 32;
         tc::Ring r;
         bool ok = warp - 8u < P::TURNS;
         uint32_t turn = warp - 8u;  // stages until this warp's
         for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const uint64_t row = (uint64_t)(t / a.out_tiles) * L4_ROWS + lane;
-            const uint32_t out = t % a.out_tiles * TN + lane;
             for (uint32_t c = 0; c < a.chunks; ++c, r.next(P::STAGES), turn = turn ? turn - 1u : P::TURNS - 1u) {
                 if (turn != 0) continue;
-                uint2 e[A_ROWS + B_ROWS];
+                uint2 e[ROWS];
 #pragma unroll
-                for (int i = 0; i < A_ROWS; ++i)
-                    e[i] = row + i * 32u < a.rows ? load_scales(a.x_exps, row + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
-#pragma unroll
-                for (int i = 0; i < B_ROWS; ++i)
-                    e[A_ROWS + i] = out + i * 32u < a.outs ? load_scales(a.w_exps, out + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
+                for (int i = 0; i < ROWS; ++i)
+                    e[i] = lane + i * 32u < a.outs ? load_scales(a.w_exps, lane + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
                 ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
                 if (!ok) break;
-                uint8_t *sf = smem + r.i * P::STAGE + P::A_BYTES + P::B_BYTES;
+                uint8_t *sf = smem + r.i * P::STAGE + P::A_BYTES + P::B_BYTES + 1024u;
 #pragma unroll
-                for (int i = 0; i < A_ROWS + B_ROWS; ++i) {
-                    uint8_t *to = sf + (i < A_ROWS ? scale_place(i * 32u + lane) : 1024u + scale_place((i - A_ROWS) * 32u + lane));
-                    *reinterpret_cast<uint32_t *>(to) = e[i].x;
-                    *reinterpret_cast<uint32_t *>(to + 512u) = e[i].y;
-                }
+                for (int i = 0; i < ROWS; ++i) store_scales(sf, i * 32u + lane, e[i]);
                 tc::fence_async_shared();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
             }
         }
-    } else if (QUANT && warp == 2) {
+    } else if (warp == 2) {
         if (lane == 0) {  // TMA of x, 64 columns at a time
             tc::Ring r;
             uint32_t issued = 0;
@@ -295,7 +291,7 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
                     ok = tc::mbar_wait(&s.x_empty[r.i], r.phase ^ 1u, fail, a.err);
                     if (!ok) break;
                     tc::mbar_arrive_tx(&s.x_full[r.i], P::X_BYTES);
-                    tc::tma_load_2d(smem + P::X_AT + r.i * P::X_BYTES, &x_map, (int)col, (int)(t / a.out_tiles * L4_ROWS),
+                    tc::tma_load_2d(smem + P::X_AT + r.i * P::X_BYTES, &x_map, (int)col, (int)(t * L4_ROWS),
                                     &s.x_full[r.i]);
                     ++issued;
                     r.next(P::X_STAGES);
@@ -304,7 +300,7 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
                 for (uint32_t i = 0; i < P::X_STAGES && i < issued; ++i)
                     tc::mbar_wait_slow(&s.x_full[i], ((issued - 1 - i) / P::X_STAGES) & 1u, fail, a.err, true);
         }
-    } else if (QUANT && warp >= 12) {  // x to 4 bits: a lane has a row, each half of the warps one of a chunk's two blocks
+    } else if (warp >= 12) {  // x to 4 bits: a lane has a row, each half of the warps one of a chunk's two blocks
         const uint32_t row = warp % 4u * 32u + lane, part = (warp - 12u) / 4u;
         tc::Ring r, x;
         bool ok = true;
@@ -343,6 +339,176 @@ __global__ void __launch_bounds__(L4<TN, QUANT>::THREADS, 1)
     tc::fence_before();
     __syncthreads();
     if (warp == 1) tc::tmem_free<P::TMEM>(tmem);
+}
+
+// ---- many outputs ----
+//
+// Both operands come in 4 bits.  A pair of CTAs shares a tile of 256 rows by 224 outputs: each stages its
+// 128 rows of x and half of the outputs' weights, so a byte of shared memory serves twice the products of
+// a CTA alone, whose shared memory's bandwidth and room for stages bound it (182 us for 4096 x 8192 x 8192).
+// 224 outputs leave room in tensor memory for two accumulators and two places of scales.
+
+constexpr uint32_t PAIR_N = 224, PAIR_A = 16384, PAIR_B = PAIR_N / 2 * 128, PAIR_STAGE = PAIR_A + PAIR_B + 3072, PAIR_STAGES = 6,
+                   PAIR_THREADS = 384, PAIR_SF_AT = 2 * PAIR_N, PAIR_SF_COLS = 24;
+struct PairCtrl {
+    uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], failed;
+    uint32_t tmem;
+    tc::Fail fail;
+    alignas(8) float bias[PAIR_N];
+};
+constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + sizeof(PairCtrl);
+static_assert(PAIR_SMEM <= 232448 && PAIR_SF_AT + 2 * PAIR_SF_COLS <= 512, "does not fit an SM");
+
+template <typename T, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    pair4_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const L4Args a)
+{
+    extern __shared__ __align__(1024) uint8_t smem[];
+    PairCtrl &s = *reinterpret_cast<PairCtrl *>(smem + PAIR_STAGES * PAIR_STAGE);
+    const uint32_t warp = tc::warp_number(), lane = threadIdx.x % 32u, rank = tc::cluster_rank();
+    const uint32_t tiles = a.row_tiles * a.out_tiles, first = blockIdx.x / 2u, step = gridDim.x / 2u;
+    tc::Fail *const fail = &s.fail;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < PAIR_STAGES; ++i) {
+            tc::mbar_init(&s.full[i], 3);  // the leader's: the bytes of both CTAs, a warp of scales of each
+            tc::mbar_init(&s.empty[i], 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            tc::mbar_init(&s.acc_full[i], 1);
+            tc::mbar_init(&s.acc_empty[i], 8);
+        }
+        tc::mbar_init(&s.failed, 1);
+        s.fail.failed = 0;
+        tc::mbar_init_fence();
+        tc::tma_prefetch_map(&x_map);
+        tc::tma_prefetch_map(&w_map);
+    }
+    if (warp == 1) tc::tmem_alloc_pair<512>(&s.tmem);
+    tc::fence_before();
+    tc::cluster_sync();
+    tc::fence_after();
+    const uint32_t tmem = s.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {  // TMA
+            tc::Ring r;
+            bool ok = true;
+            for (uint32_t t = first; t < tiles && ok; t += step) {
+                const int row0 = (int)(t / a.out_tiles * 256u + rank * 128u), out0 = (int)(t % a.out_tiles * PAIR_N + rank * (PAIR_N / 2u));
+                for (uint32_t c = 0; c < a.chunks; ++c) {
+                    ok = tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err);
+                    if (!ok) break;
+                    uint8_t *st = smem + r.i * PAIR_STAGE;
+                    const uint32_t bar = tc::leader_addr(&s.full[r.i]);
+                    if (rank == 0) tc::mbar_arrive_tx(&s.full[r.i], 2u * (PAIR_A + PAIR_B));
+                    tc::tma_load_2d_pair(st, &x_map, (int)(c * 128u), row0, bar);
+                    tc::tma_load_2d_pair(st + PAIR_A, &w_map, (int)(c * 128u), out0, bar);
+                    r.next(PAIR_STAGES);
+                }
+            }
+            if (s.fail.failed) tc::outlast_copies();  // their bytes are counted in the leader alone
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {  // scales to tensor memory and products, in the leader for both
+            const uint32_t base = tc::smem_u32(smem);
+            constexpr uint32_t ID0 = tc::idesc_mxf4(256, PAIR_N, 0), ID1 = tc::idesc_mxf4(256, PAIR_N, 1);
+            const bool mine = tc::elect();
+            tc::Ring r, acc, old, sf;  // old: the stage whose scales' place comes next
+            uint32_t ahead = 0;
+            bool ok = true;
+            for (uint32_t t = first; t < tiles && ok; t += step) {
+                ok = __all_sync(~0u, tc::mbar_wait(&s.acc_empty[acc.i], acc.phase ^ 1u, fail, a.err));
+                if (!ok) break;
+                tc::fence_after();
+                for (uint32_t c = 0; c < a.chunks; ++c) {
+                    ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
+                    if (++ahead > 2u) {
+                        ok = ok && __all_sync(~0u, tc::mbar_wait(&s.empty[old.i], old.phase, fail, a.err));
+                        old.next(PAIR_STAGES);
+                    }
+                    if (!ok) break;
+                    tc::fence_after();
+                    const uint32_t st = base + r.i * PAIR_STAGE, sfa = tmem + PAIR_SF_AT + sf.i * PAIR_SF_COLS;
+                    if (mine) {
+                        stage_products<2, true>(tmem + acc.i * PAIR_N, tc::smem_desc(st, 16, 1024), tc::smem_desc(st + PAIR_A, 16, 1024),
+                                                tc::scale_desc(st + PAIR_A + PAIR_B), sfa, sfa + 8u, ID0, ID1,
+                                                c + 1u == a.chunks ? a.last_steps : 4u, c != 0);
+                        tc::commit_pair(&s.empty[r.i]);
+                        if (c + 1u == a.chunks) tc::commit_pair(&s.acc_full[acc.i]);
+                    }
+                    __syncwarp();
+                    sf.next(2);
+                    r.next(PAIR_STAGES);
+                }
+                acc.next(2);
+            }
+            if (!ok) {  // leave no product in flight
+                if (mine) tc::commit_pair(&s.failed);
+                tc::mbar_wait_slow(&s.failed, 0, fail, a.err, true);
+            }
+        }
+    } else if (warp >= 4 && warp < 8) {  // results: a lane has a row of this CTA's 128
+        const uint32_t quad = warp % 4u, in_tile = quad * 32u + lane;
+        tc::Ring acc;
+        for (uint32_t t = first; t < tiles; t += step) {
+            const uint64_t row = (uint64_t)(t / a.out_tiles) * 256u + rank * 128u + in_tile;
+            const uint32_t out0 = t % a.out_tiles * PAIR_N;
+            // the bias of the tile's outputs; the first barrier keeps the last tile's until it is used
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            for (uint32_t i = in_tile; i < PAIR_N; i += 128u)
+                s.bias[i] = a.bias && out0 + i < a.outs ? to_f32<T>(__ldg((const T *)a.bias + out0 + i)) : 0.0f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const bool ok = tc::mbar_wait(&s.acc_full[acc.i], acc.phase, fail, a.err);
+            if (__all_sync(~0u, ok)) {  // else on to the next barrier with the other warps
+                tc::fence_after();
+#pragma unroll 1
+                for (uint32_t n0 = 0; n0 < PAIR_N; n0 += 32u) {
+                    uint32_t v[32];
+                    tc::tmem_load32(tmem + acc.i * PAIR_N + (quad * 32u << 16) + n0, v);
+                    if (n0 + 32u == PAIR_N) {
+                        tc::fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive_cluster(tc::leader_addr(&s.acc_empty[acc.i]));
+                    }
+                    if (row < a.rows) store_results<T, ACT>((T *)a.y + row * a.outs, out0 + n0, a.outs, a.y_wide, v, s.bias + n0);
+                }
+            }
+            acc.next(2);
+        }
+    } else if (warp >= 8) {  // scales: the four warps take stages in turn
+        tc::Ring r;
+        bool ok = true;
+        uint32_t turn = warp - 8u;
+        for (uint32_t t = first; t < tiles && ok; t += step) {
+            const uint64_t row = (uint64_t)(t / a.out_tiles) * 256u + rank * 128u + lane;
+            const uint32_t out = t % a.out_tiles * PAIR_N + lane;
+            for (uint32_t c = 0; c < a.chunks; ++c, r.next(PAIR_STAGES), turn = (turn - 1u) & 3u) {
+                if (turn != 0) continue;
+                uint2 e[4 + PAIR_N / 32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    e[i] = row + i * 32u < a.rows ? load_scales(a.x_exps, row + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
+#pragma unroll
+                for (int i = 0; i < (int)PAIR_N / 32; ++i)
+                    e[4 + i] = out + i * 32u < a.outs ? load_scales(a.w_exps, out + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
+                ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
+                if (!ok) break;
+                uint8_t *sf = smem + r.i * PAIR_STAGE + PAIR_A + PAIR_B;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) store_scales(sf, i * 32u + lane, e[i]);
+#pragma unroll
+                for (int i = 0; i < (int)PAIR_N / 32; ++i) store_scales(sf + 1024u, i * 32u + lane, e[4 + i]);
+                tc::fence_async_shared();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive_cluster(tc::leader_addr(&s.full[r.i]));
+            }
+        }
+    }
+    __syncwarp();
+    tc::fence_before();
+    tc::cluster_sync();  // no CTA leaves while the other may still reach its barriers
+    if (warp == 1) tc::tmem_free_pair<512>(tmem);
 }
 
 // ---- few tiles ----
@@ -440,10 +606,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_kernel(const __grid_consta
             if (!ok) break;
             uint8_t *sf = smem + r.i * FEW_STAGE + 32768u;
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-                *reinterpret_cast<uint32_t *>(sf + scale_place(k * 32u + lane)) = e[k].x;
-                *reinterpret_cast<uint32_t *>(sf + scale_place(k * 32u + lane) + 512u) = e[k].y;
-            }
+            for (uint32_t k = 0; k < 4; ++k) store_scales(sf, k * 32u + lane, e[k]);
             tc::fence_async_shared();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
@@ -524,26 +687,37 @@ template <typename T, int ACT> static vt_status launch_bias(const L4Args &a, cud
     return check_launch("bias_rows_kernel");
 }
 
-template <typename T, int ACT, int TN, bool QUANT>
+template <typename T, int ACT, int TN>
 static vt_status launch_linear4(const void *x, uint64_t x_stride, const uint8_t *w_codes, L4Args a, cudaStream_t stream)
 {
     static std::atomic<uint64_t> allowed{0};
-    using P = L4<TN, QUANT>;
+    using P = L4<TN>;
     CUtensorMap x_map, w_map;
     const uint64_t pitch = (uint64_t)a.blocks * 16u;
-    if (QUANT) {  // x itself
-        if (vt_status s = map_rows<T>(&x_map, x, x_stride, a.rows, a.cols, L4_ROWS)) return s;
-    } else {  // its codes
-        if (vt_status s = tc::make_map(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, a.rows, pitch, pitch, L4_ROWS, 128)) return s;
-    }
+    if (vt_status s = map_rows<T>(&x_map, x, x_stride, a.rows, a.cols, L4_ROWS)) return s;
     if (vt_status s = tc::make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w_codes, a.outs, pitch, pitch, TN, 128)) return s;
-    if (vt_status s = tc::allow_smem(linear4_kernel<T, ACT, TN, QUANT>, P::SMEM, allowed)) return s;
+    if (vt_status s = tc::allow_smem(linear4_kernel<T, ACT, TN>, P::SMEM, allowed)) return s;
     a.row_tiles = (uint32_t)((a.rows + L4_ROWS - 1u) / L4_ROWS);
-    a.out_tiles = (a.outs + TN - 1u) / TN;
-    const uint64_t tiles = (uint64_t)a.row_tiles * a.out_tiles;
     const uint32_t sms = (uint32_t)sm_count();
-    linear4_kernel<T, ACT, TN, QUANT><<<(unsigned)(tiles < sms ? tiles : sms), P::THREADS, P::SMEM, stream>>>(x_map, w_map, a);
+    linear4_kernel<T, ACT, TN><<<a.row_tiles < sms ? a.row_tiles : sms, P::THREADS, P::SMEM, stream>>>(x_map, w_map, a);
     return check_launch("linear4_kernel");
+}
+
+template <typename T, int ACT>
+static vt_status launch_pair4(const uint8_t *x_codes, const uint8_t *w_codes, L4Args a, cudaStream_t stream)
+{
+    static std::atomic<uint64_t> allowed{0};
+    CUtensorMap x_map, w_map;
+    const uint64_t pitch = (uint64_t)a.blocks * 16u;
+    if (vt_status s = tc::make_map(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, x_codes, a.rows, pitch, pitch, 128, 128)) return s;
+    if (vt_status s = tc::make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w_codes, a.outs, pitch, pitch, PAIR_N / 2, 128)) return s;
+    if (vt_status s = tc::allow_smem(pair4_kernel<T, ACT>, PAIR_SMEM, allowed)) return s;
+    a.row_tiles = (uint32_t)((a.rows + 255u) / 256u);
+    a.out_tiles = (a.outs + PAIR_N - 1u) / PAIR_N;
+    const uint64_t tiles = (uint64_t)a.row_tiles * a.out_tiles;
+    const uint32_t pairs = (uint32_t)sm_count() / 2u;
+    pair4_kernel<T, ACT><<<(unsigned)(tiles < pairs ? tiles : pairs) * 2u, PAIR_THREADS, PAIR_SMEM, stream>>>(x_map, w_map, a);
+    return check_launch("pair4_kernel");
 }
 
 // Splits of k for few_kernel, a power of two up to 8; 0: there are tiles enough for linear4_kernel.
@@ -650,16 +824,16 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
             if (vt_status s = vt::whole_rows<T>(from, stride, rows, cols, workspace, st)) return s;
             return vt::with_act(act, [&](auto f) -> vt_status {
                 constexpr int ACT = decltype(f)::value;
-                if (outs <= 64u) return vt::launch_linear4<T, ACT, 64, true>(from, stride, codes, a, st);
-                if (outs <= 128u) return vt::launch_linear4<T, ACT, 128, true>(from, stride, codes, a, st);
-                return vt::launch_linear4<T, ACT, 256, true>(from, stride, codes, a, st);
+                if (outs <= 64u) return vt::launch_linear4<T, ACT, 64>(from, stride, codes, a, st);
+                if (outs <= 128u) return vt::launch_linear4<T, ACT, 128>(from, stride, codes, a, st);
+                return vt::launch_linear4<T, ACT, 256>(from, stride, codes, a, st);
             });
         }
         uint8_t *x_codes = (uint8_t *)workspace, *x_exps = x_codes + rows * a.blocks * 16u;
         if (vt_status s = vt_mx4_quantize(x, dtype, rows, cols, x_stride, x_codes, x_exps, stream)) return s;
         a.x_exps = x_exps;
         return vt::with_act(act, [&](auto f) -> vt_status {
-            return vt::launch_linear4<T, decltype(f)::value, 224, false>(x_codes, 0, codes, a, st);
+            return vt::launch_pair4<T, decltype(f)::value>(x_codes, codes, a, st);
         });
     });
 }

@@ -289,6 +289,19 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b,
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
+// Block-scaled 4-bit products of a pair: each CTA's tensor memory has the scales of its own 128 rows of A
+// and of all of B's columns.  The copy runs in both CTAs, from and to the same places of each.
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t d, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(d), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void mma_mxf4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b,
+                                              bool accumulate)
+{
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"((uint32_t)accumulate) : "memory");
+}
 // One arrival at the barrier of this offset in both CTAs when the leader's products so far are done.
 __device__ __forceinline__ void commit_pair(uint64_t *bar)
 {
