@@ -57,7 +57,6 @@ template <int TN> struct L4 {
 struct L4Args {
     uint64_t rows;
     uint32_t cols, outs, blocks, chunks, last_steps, row_tiles, out_tiles;  // last_steps: of 64, in a row's last chunk
-    const uint8_t *x_exps;  // pair4_kernel
     const uint8_t *w_exps;
     const void *bias;
     void *y;
@@ -343,13 +342,16 @@ __global__ void __launch_bounds__(L4<TN>::THREADS, 1)
 
 // ---- many outputs ----
 //
-// Both operands come in 4 bits.  A pair of CTAs shares a tile of 256 rows by 224 outputs: each stages its
+// Both operands come in 4 bits, their scales in the order of the stages: for 128 rows and 256 columns 1 KB as it
+// is copied to tensor memory, so that TMA brings everything in.  (Warps that gathered the scales from their rows
+// kept up with half the speed: each stage takes 8 bytes of 352 rows.)  stage4_kernel writes them, and x's codes.
+// A pair of CTAs shares a tile of 256 rows by 224 outputs: each stages its
 // 128 rows of x and half of the outputs' weights, so a byte of shared memory serves twice the products of
 // a CTA alone, whose shared memory's bandwidth and room for stages bound it (182 us for 4096 x 8192 x 8192).
 // 224 outputs leave room in tensor memory for two accumulators and two places of scales.
 
 constexpr uint32_t PAIR_N = 224, PAIR_A = 16384, PAIR_B = PAIR_N / 2 * 128, PAIR_STAGE = PAIR_A + PAIR_B + 3072, PAIR_STAGES = 6,
-                   PAIR_THREADS = 384, PAIR_SF_AT = 2 * PAIR_N, PAIR_SF_COLS = 24;
+                   PAIR_THREADS = 256, PAIR_SF_AT = 2 * PAIR_N, PAIR_SF_COLS = 24;
 struct PairCtrl {
     uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], failed;
     uint32_t tmem;
@@ -359,9 +361,82 @@ struct PairCtrl {
 constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + sizeof(PairCtrl);
 static_assert(PAIR_SMEM <= 232448 && PAIR_SF_AT + 2 * PAIR_SF_COLS <= 512, "does not fit an SM");
 
+// Workspace of a call: x's codes, x's scales in order (1 KB for 128 rows and a chunk), w's (2 KB for 224 outputs).
+struct PairPlan {
+    uint32_t row_tiles, out_tiles, chunks;  // tiles of 256 rows and of 224 outputs
+    uint64_t x_scales_at, w_scales_at, bytes;
+};
+static PairPlan pair_plan(uint64_t rows, uint32_t cols, uint32_t outs)
+{
+    PairPlan p;
+    p.row_tiles = (uint32_t)((rows + 255u) / 256u);
+    p.out_tiles = (outs + PAIR_N - 1u) / PAIR_N;
+    p.chunks = (cols + L4_K - 1u) / L4_K;
+    p.x_scales_at = align_up(rows * mx_blocks(cols) * 16u, 1024);
+    p.w_scales_at = p.x_scales_at + (uint64_t)p.row_tiles * 2u * p.chunks * 1024u;
+    p.bytes = p.w_scales_at + (uint64_t)p.out_tiles * p.chunks * 2048u;
+    return p;
+}
+
+// x (rows, cols) to 4 bits, four lanes a block; scales of x and of the weight in order.  Places behind the
+// operands' rows and columns get zeros, which multiply zero codes.
+template <typename T>
+__global__ void __launch_bounds__(256) stage4_kernel(const T *__restrict__ x, uint64_t x_stride, uint64_t rows, uint32_t cols, uint32_t blocks,
+                                                     bool vec, uint32_t chunks, uint64_t x_items, uint32_t *__restrict__ codes,
+                                                     uint8_t *__restrict__ x_scales, const uint8_t *__restrict__ w_exps, uint32_t outs,
+                                                     uint64_t w_items, uint32_t *__restrict__ w_scales)
+{
+    const uint64_t step = (uint64_t)gridDim.x * 256u, start = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    const uint32_t per_row = chunks * 32u;  // lanes of a row, its padding included
+    for (uint64_t t = start; t < x_items; t += step) {
+        const uint64_t row = t >> 32 ? t / per_row : (uint32_t)t / per_row;
+        const uint32_t in_row = (uint32_t)(t - row * per_row), block = in_row >> 2, col = in_row * 8u;
+        Vec8<T> w;
+        w.zero();
+        if (row < rows && col < cols) {
+            const T *p = x + row * x_stride + col;
+            if (vec) w.load(p);
+            else
+                for (uint32_t i = 0; i < 8u && col + i < cols; ++i) reinterpret_cast<T *>(w.w)[i] = p[i];
+        }
+        float v[8];
+        w.unpack(v);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        const uint32_t lanes = 0xfu << (threadIdx.x & 28u);
+        top = max(top, __shfl_xor_sync(lanes, top, 1));
+        top = max(top, __shfl_xor_sync(lanes, top, 2));
+        const uint32_t E = mx4_exponent(top);
+        const f32x2 inv = both(mx4_inverse(E == 255u ? 1u : E));
+        const bool in = row < rows && block < blocks;
+        if (in) {
+            f32x2 q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = mul2(pair(v[2 * i], v[2 * i + 1]), inv);
+            codes[(row * blocks + block) * 4u + (in_row & 3u)] = E == 255u ? 0u : mx4_word(q);
+        }
+        if ((in_row & 3u) == 0)
+            x_scales[((row >> 7) * chunks + (block >> 3)) * 1024u + (block >> 2 & 1u) * 512u + scale_place((uint32_t)row & 127u) + (block & 3u)] =
+                in ? (uint8_t)E : 0;
+    }
+    for (uint64_t t = start; t < w_items; t += step) {  // a word: 4 blocks of an output
+        const uint32_t slot = (uint32_t)t & 255u, half = (uint32_t)(t >> 8) & 1u;
+        const uint64_t at = t >> 9;  // tile, chunk
+        const uint32_t tile = (uint32_t)(at / chunks), c = (uint32_t)(at % chunks), out = tile * PAIR_N + slot, b0 = c * 8u + half * 4u;
+        uint32_t w = 0;
+        if (slot < PAIR_N && out < outs)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+                if (b0 + i < blocks) w |= (uint32_t)__ldg(w_exps + (uint64_t)out * blocks + b0 + i) << (8u * i);
+        w_scales[at * 512u + (slot >> 7) * 256u + half * 128u + (slot & 31u) * 4u + (slot >> 5 & 3u)] = w;
+    }
+}
+
 template <typename T, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
-    pair4_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const L4Args a)
+    pair4_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
+                 const __grid_constant__ CUtensorMap x_scale_map, const __grid_constant__ CUtensorMap w_scale_map, const L4Args a)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
     PairCtrl &s = *reinterpret_cast<PairCtrl *>(smem + PAIR_STAGES * PAIR_STAGE);
@@ -371,7 +446,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < PAIR_STAGES; ++i) {
-            tc::mbar_init(&s.full[i], 3);  // the leader's: the bytes of both CTAs, a warp of scales of each
+            tc::mbar_init(&s.full[i], 1);  // the leader's counts the bytes of both CTAs
             tc::mbar_init(&s.empty[i], 1);
         }
         for (uint32_t i = 0; i < 2; ++i) {
@@ -383,6 +458,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&x_map);
         tc::tma_prefetch_map(&w_map);
+        tc::tma_prefetch_map(&x_scale_map);
+        tc::tma_prefetch_map(&w_scale_map);
     }
     if (warp == 1) tc::tmem_alloc_pair<512>(&s.tmem);
     tc::fence_before();
@@ -396,14 +473,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             bool ok = true;
             for (uint32_t t = first; t < tiles && ok; t += step) {
                 const int row0 = (int)(t / a.out_tiles * 256u + rank * 128u), out0 = (int)(t % a.out_tiles * PAIR_N + rank * (PAIR_N / 2u));
+                const uint32_t x_scales = (t / a.out_tiles * 2u + rank) * a.chunks * 8u, w_scales = t % a.out_tiles * a.chunks * 16u;
                 for (uint32_t c = 0; c < a.chunks; ++c) {
                     ok = tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err);
                     if (!ok) break;
                     uint8_t *st = smem + r.i * PAIR_STAGE;
                     const uint32_t bar = tc::leader_addr(&s.full[r.i]);
-                    if (rank == 0) tc::mbar_arrive_tx(&s.full[r.i], 2u * (PAIR_A + PAIR_B));
+                    if (rank == 0) tc::mbar_arrive_tx(&s.full[r.i], 2u * PAIR_STAGE);
                     tc::tma_load_2d_pair(st, &x_map, (int)(c * 128u), row0, bar);
                     tc::tma_load_2d_pair(st + PAIR_A, &w_map, (int)(c * 128u), out0, bar);
+                    tc::tma_load_2d_pair(st + PAIR_A + PAIR_B, &x_scale_map, 0, (int)(x_scales + c * 8u), bar);
+                    tc::tma_load_2d_pair(st + PAIR_A + PAIR_B + 1024, &w_scale_map, 0, (int)(w_scales + c * 16u), bar);
                     r.next(PAIR_STAGES);
                 }
             }
@@ -475,34 +555,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 }
             }
             acc.next(2);
-        }
-    } else if (warp >= 8) {  // scales: the four warps take stages in turn
-        tc::Ring r;
-        bool ok = true;
-        uint32_t turn = warp - 8u;
-        for (uint32_t t = first; t < tiles && ok; t += step) {
-            const uint64_t row = (uint64_t)(t / a.out_tiles) * 256u + rank * 128u + lane;
-            const uint32_t out = t % a.out_tiles * PAIR_N + lane;
-            for (uint32_t c = 0; c < a.chunks; ++c, r.next(PAIR_STAGES), turn = (turn - 1u) & 3u) {
-                if (turn != 0) continue;
-                uint2 e[4 + PAIR_N / 32];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    e[i] = row + i * 32u < a.rows ? load_scales(a.x_exps, row + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
-#pragma unroll
-                for (int i = 0; i < (int)PAIR_N / 32; ++i)
-                    e[4 + i] = out + i * 32u < a.outs ? load_scales(a.w_exps, out + i * 32u, a.blocks, c * 8u) : make_uint2(0, 0);
-                ok = __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
-                if (!ok) break;
-                uint8_t *sf = smem + r.i * PAIR_STAGE + PAIR_A + PAIR_B;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) store_scales(sf, i * 32u + lane, e[i]);
-#pragma unroll
-                for (int i = 0; i < (int)PAIR_N / 32; ++i) store_scales(sf + 1024u, i * 32u + lane, e[4 + i]);
-                tc::fence_async_shared();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive_cluster(tc::leader_addr(&s.full[r.i]));
-            }
         }
     }
     __syncwarp();
@@ -704,19 +756,32 @@ static vt_status launch_linear4(const void *x, uint64_t x_stride, const uint8_t 
 }
 
 template <typename T, int ACT>
-static vt_status launch_pair4(const uint8_t *x_codes, const uint8_t *w_codes, L4Args a, cudaStream_t stream)
+static vt_status launch_pair4(const void *x, uint64_t x_stride, const uint8_t *w_codes, L4Args a, uint8_t *workspace, cudaStream_t stream)
 {
     static std::atomic<uint64_t> allowed{0};
-    CUtensorMap x_map, w_map;
+    const PairPlan p = pair_plan(a.rows, a.cols, a.outs);
+    VT_REQUIRE((uint64_t)p.row_tiles * p.chunks < (1u << 26) && (uint64_t)p.out_tiles * p.chunks < (1u << 26), "vt_mx4_linear: too large");
+    uint8_t *codes = workspace, *x_scales = workspace + p.x_scales_at, *w_scales = workspace + p.w_scales_at;
+    const uint32_t sms = (uint32_t)sm_count(), pairs = sms / 2u;
+    const uint64_t x_items = (uint64_t)p.row_tiles * 256u * p.chunks * 32u, w_items = (uint64_t)p.out_tiles * p.chunks * 512u;
+    const uint64_t want = ((x_items > w_items ? x_items : w_items) + 255u) / 256u;
+    const bool vec = a.cols % 8u == 0 && x_stride % 8u == 0 && aligned16(x);
+    stage4_kernel<T><<<(unsigned)(want < sms * 32u ? want : sms * 32u), 256, 0, stream>>>((const T *)x, x_stride, a.rows, a.cols, a.blocks, vec,
+                                                                                      p.chunks, x_items, (uint32_t *)codes, x_scales, a.w_exps,
+                                                                                      a.outs, w_items, (uint32_t *)w_scales);
+    if (vt_status s = check_launch("stage4_kernel")) return s;
+    CUtensorMap x_map, w_map, x_scale_map, w_scale_map;
     const uint64_t pitch = (uint64_t)a.blocks * 16u;
-    if (vt_status s = tc::make_map(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, x_codes, a.rows, pitch, pitch, 128, 128)) return s;
-    if (vt_status s = tc::make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w_codes, a.outs, pitch, pitch, PAIR_N / 2, 128)) return s;
+    const CUtensorMapDataType bytes = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    if (vt_status s = tc::make_map(&x_map, bytes, codes, a.rows, pitch, pitch, 128, 128)) return s;
+    if (vt_status s = tc::make_map(&w_map, bytes, w_codes, a.outs, pitch, pitch, PAIR_N / 2, 128)) return s;
+    if (vt_status s = tc::make_map(&x_scale_map, bytes, x_scales, (uint64_t)p.row_tiles * 2u * p.chunks * 8u, 128, 128, 8, 128, false)) return s;
+    if (vt_status s = tc::make_map(&w_scale_map, bytes, w_scales, (uint64_t)p.out_tiles * p.chunks * 16u, 128, 128, 16, 128, false)) return s;
     if (vt_status s = tc::allow_smem(pair4_kernel<T, ACT>, PAIR_SMEM, allowed)) return s;
-    a.row_tiles = (uint32_t)((a.rows + 255u) / 256u);
-    a.out_tiles = (a.outs + PAIR_N - 1u) / PAIR_N;
+    a.row_tiles = p.row_tiles;
+    a.out_tiles = p.out_tiles;
     const uint64_t tiles = (uint64_t)a.row_tiles * a.out_tiles;
-    const uint32_t pairs = (uint32_t)sm_count() / 2u;
-    pair4_kernel<T, ACT><<<(unsigned)(tiles < pairs ? tiles : pairs) * 2u, PAIR_THREADS, PAIR_SMEM, stream>>>(x_map, w_map, a);
+    pair4_kernel<T, ACT><<<(unsigned)(tiles < pairs ? tiles : pairs) * 2u, PAIR_THREADS, PAIR_SMEM, stream>>>(x_map, w_map, x_scale_map, w_scale_map, a);
     return check_launch("pair4_kernel");
 }
 
@@ -765,10 +830,9 @@ static vt_status launch_few(const uint8_t *w_codes, FewArgs a, uint32_t splits, 
 // copies: x's rows do not start on 16 bytes
 extern "C" uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs, int copies)
 {
-    const uint64_t blocks = vt::mx_blocks(cols);
     if (vt::few_splits(rows, cols, outs, (uint32_t)vt::sm_count())) return 0;
     if (outs <= 256u) return copies ? rows * vt::align_up(cols, 8) * 2u : 0;  // x is rounded inside the kernel
-    return rows * blocks * 16u + vt::align_up(rows * blocks, 16);
+    return vt::pair_plan(rows, cols, outs).bytes;
 }
 
 extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, uint64_t rows, uint32_t cols,
@@ -829,11 +893,8 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
                 return vt::launch_linear4<T, ACT, 256>(from, stride, codes, a, st);
             });
         }
-        uint8_t *x_codes = (uint8_t *)workspace, *x_exps = x_codes + rows * a.blocks * 16u;
-        if (vt_status s = vt_mx4_quantize(x, dtype, rows, cols, x_stride, x_codes, x_exps, stream)) return s;
-        a.x_exps = x_exps;
         return vt::with_act(act, [&](auto f) -> vt_status {
-            return vt::launch_pair4<T, decltype(f)::value>(x_codes, codes, a, st);
+            return vt::launch_pair4<T, decltype(f)::value>(x, x_stride, codes, a, (uint8_t *)workspace, st);
         });
     });
 }
