@@ -97,18 +97,18 @@ __global__ void __launch_bounds__(256) mx8_checkpoint_kernel(MxShape s, const T 
         float v[8];
         mx_load(s, it, z, s.in_stride, v);
         const uint32_t E = mx8_exponent(block_top(v));
-        const float inv = mx8_inverse(E);
-        uint32_t c[8];
+        const f32x2 inv = both(mx8_inverse(E));
+        f32x2 p[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = E == 255u ? 0u : (uint32_t)mx8_code(v[i], inv) & 255u;
-        reinterpret_cast<uint2 *>(codes)[t] =
-            make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+        for (int i = 0; i < 4; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
+        const uint2 c = make_uint2(mx8_codes(p[0], p[1], inv), mx8_codes(p[2], p[3], inv));
+        reinterpret_cast<uint2 *>(codes)[t] = E == 255u ? make_uint2(0, 0) : c;
         if ((t & 3u) == 0) exps[t >> 2] = (uint8_t)E;
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const float2 a = unpair(act_value2<ACT>(pair(v[i], v[i + 1])));
-            v[i] = a.x;
-            v[i + 1] = a.y;
+        for (int i = 0; i < 4; ++i) {
+            const float2 a = unpair(act_value2<ACT>(p[i]));
+            v[2 * i] = a.x;
+            v[2 * i + 1] = a.y;
         }
         mx_store(s, it, h, v);
     }

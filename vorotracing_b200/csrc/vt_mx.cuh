@@ -206,9 +206,17 @@ __device__ __forceinline__ float mx4_scale(uint32_t E)
 {
     return __uint_as_float(E == 255u ? 0x7fc00000u : E << 23);
 }
-__device__ __forceinline__ int mx8_code(float x, float inverse)
+// Four 8-bit codes in a word.  Adding 1.5 2^23 rounds to the nearest whole number, ties to even, and leaves
+// it in the low byte: two instructions a pair, where conversions would share the pipe of the activations'
+// exponentials and reciprocals, which bounds these kernels next to HBM.
+__device__ __forceinline__ uint32_t mx8_codes(f32x2 a, f32x2 b, f32x2 inverse)
 {
-    return __float2int_rn(fminf(fmaxf(x * inverse, -127.0f), 127.0f));
+    const float2 x = unpair(mul2(a, inverse)), y = unpair(mul2(b, inverse));
+    const f32x2 magic = both(12582912.0f);
+    const float2 u = unpair(add2(pair(fminf(fmaxf(x.x, -127.0f), 127.0f), fminf(fmaxf(x.y, -127.0f), 127.0f)), magic));
+    const float2 v = unpair(add2(pair(fminf(fmaxf(y.x, -127.0f), 127.0f), fminf(fmaxf(y.y, -127.0f), 127.0f)), magic));
+    return __byte_perm(__byte_perm(__float_as_uint(u.x), __float_as_uint(u.y), 0x0040),
+                       __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x0040), 0x5410);
 }
 // Eight e2m1 codes in a word, the first in the lowest nibble; rounds to nearest even and saturates.
 __device__ __forceinline__ uint32_t mx4_word(const f32x2 *v)
