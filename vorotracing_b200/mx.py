@@ -50,12 +50,12 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 _error_words = {}
 
 
-def _error_word(device) -> torch.Tensor:
-    """The device word where a product's kernel reports that one of its waits has run out."""
-    t = _error_words.get(device.index)
+def _error_word(index: int) -> int:
+    """Address of the device word where a product's kernel reports that one of its waits has run out."""
+    t = _error_words.get(index)
     if t is None:
-        t = _error_words[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-    return t
+        t = _error_words[index] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{index}")
+    return t.data_ptr()
 
 
 def raise_errors(device=None):
@@ -94,30 +94,30 @@ def _act_code(act: str) -> int:
 
 
 def _matrix(t, name: str, types=_DTYPES):
-    """A tensor as rows of its last dimension with unit column stride: (tensor, rows, cols, row stride)."""
-    if not t.is_cuda:
-        _fail(f"{name} must be on CUDA device")
-    if t.dtype not in types:
+    """A tensor as rows of its last dimension with unit column stride: (tensor, rows, cols, row
+    stride, type code)."""
+    code = types.get(t.dtype)
+    if code is None or not t.is_cuda:
+        if not t.is_cuda:
+            _fail(f"{name} must be on CUDA device")
         _fail(f"{name} had dtype {str(t.dtype).replace('torch.', '')}, expected one of "
               + ", ".join(str(d).replace("torch.", "") for d in types))
-    if t.dim() == 0:
+    shape = t.shape
+    if len(shape) == 2:
+        rows, cols = shape
+        stride, unit = t.stride()
+        if (unit == 1 or cols <= 1) and (stride >= cols or rows <= 1):
+            return t, rows, cols, stride if rows > 1 else cols, code
+    elif not shape:
         _fail(f"{name} must have at least one dimension")
-    cols = t.size(-1)
-    if t.dim() == 2 and (t.stride(1) == 1 or cols <= 1) and (t.stride(0) >= cols or t.size(0) <= 1):
-        return t, t.size(0), cols, t.stride(0) if t.size(0) > 1 else cols
     t = t.contiguous()
-    rows = 1
-    for n in t.shape[:-1]:
+    rows, cols = 1, shape[-1]
+    for n in shape[:-1]:
         rows *= n
-    return t, rows, cols, cols
+    return t, rows, cols, cols, code
 
 
 _PRODUCT_TYPES = {torch.float16: 1, torch.bfloat16: 2}
-
-
-def _same(a, b, name: str, other: str):
-    if a.device != b.device:
-        _fail(f"{name} must be on the same device as {other}")
 
 
 def _launch(name: str, index: int, *args):
@@ -137,98 +137,120 @@ def _unaligned(ptr: int, stride: int) -> bool:
     return bool(ptr % 16 or stride % 8)
 
 
-def _check_parts(codes, exps, cols, code_dtype, per_block, what):
-    if codes.dim() != 2 or exps.dim() != 2:
-        _fail(f"{what}: codes and exponents are matrices")
-    blocks = -(-cols // BLOCK)
-    if codes.dtype != code_dtype or exps.dtype != torch.uint8:
-        _fail(f"{what}: codes must be {str(code_dtype).replace('torch.', '')} and exponents uint8")
-    if codes.size(1) != blocks * per_block or exps.size(1) != blocks or codes.size(0) != exps.size(0):
-        _fail(f"{what}: {cols} columns take codes (rows, {blocks * per_block}) and exponents "
-              f"(rows, {blocks}), got {tuple(codes.shape)} and {tuple(exps.shape)}")
-    if not codes.is_cuda or codes.device != exps.device:
-        _fail(f"{what}: codes and exponents must be on the same CUDA device")
-    if not codes.is_contiguous() or not exps.is_contiguous():
-        _fail(f"{what}: codes and exponents must be contiguous")
-    align = 32 if code_dtype == torch.int8 else 16
-    if codes.data_ptr() % align:
-        _fail(f"{what}: codes must be {align}-byte aligned")
+class _Blocks:
+    """Codes and exponent bytes of a matrix, as two tensors or as one buffer that holds both."""
+
+    __slots__ = ("cols", "rows", "device_index", "_codes", "_exps", "_buf", "_pc", "_pe")
+    _dtype: torch.dtype
+    _per_block: int
+    _align: int
+
+    def _take(self, codes, exps, cols: int):
+        what, per, blocks = type(self).__name__, self._per_block, -(-cols // BLOCK)
+        if codes.dtype is not self._dtype or exps.dtype is not torch.uint8:
+            _fail(f"{what}: codes must be {str(self._dtype).replace('torch.', '')} and exponents uint8")
+        shape = codes.shape
+        if len(shape) != 2 or shape[1] != blocks * per or exps.shape != (shape[0], blocks):
+            _fail(f"{what}: {cols} columns take codes (rows, {blocks * per}) and exponents "
+                  f"(rows, {blocks}), got {tuple(shape)} and {tuple(exps.shape)}")
+        if not codes.is_cuda or codes.get_device() != exps.get_device():
+            _fail(f"{what}: codes and exponents must be on the same CUDA device")
+        if not codes.is_contiguous() or not exps.is_contiguous():
+            _fail(f"{what}: codes and exponents must be contiguous")
+        self._pc, self._pe = codes.data_ptr(), exps.data_ptr()
+        if self._pc % self._align:
+            _fail(f"{what}: codes must be {self._align}-byte aligned")
+        self._codes, self._exps, self._buf = codes, exps, None
+        self.cols, self.rows, self.device_index = cols, shape[0], codes.get_device()
+
+    def _new(self, like, rows: int, cols: int):
+        blocks = -(-cols // BLOCK)
+        n = rows * blocks
+        self._buf = like.new_empty(n * (self._per_block + 1), dtype=torch.uint8)
+        self._pc = self._buf.data_ptr()
+        self._pe = self._pc + n * self._per_block
+        self._codes = self._exps = None
+        self.cols, self.rows, self.device_index = cols, rows, like.get_device()
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            n = self.rows * -(-self.cols // BLOCK) * self._per_block
+            self._codes = self._buf[:n].view(self._dtype).view(self.rows, -(-self.cols // BLOCK) * self._per_block)
+        return self._codes
+
+    @property
+    def exps(self) -> torch.Tensor:
+        if self._exps is None:
+            n = self.rows * -(-self.cols // BLOCK) * self._per_block
+            self._exps = self._buf[n:].view(self.rows, -(-self.cols // BLOCK))
+        return self._exps
+
+    def _dequantize(self, entry: str, dtype) -> torch.Tensor:
+        code = _DTYPES.get(dtype)
+        if code is None:
+            _fail(f"cannot dequantise to {str(dtype).replace('torch.', '')}")
+        out = (self._buf if self._codes is None else self._codes).new_empty((self.rows, self.cols), dtype=dtype)
+        _launch(entry, self.device_index, self._pc, self._pe, self.rows, self.cols, code, out.data_ptr())
+        return out
 
 
-class Checkpoint:
+class Checkpoint(_Blocks):
     """A matrix of pre-activations in 8 bits and the activation it goes through.
 
     codes (rows, 32 B) int8, exps (rows, B) uint8, B = ceil(cols / 32)."""
 
-    __slots__ = ("codes", "exps", "cols", "act", "_act")
+    __slots__ = ("act", "_act")
+    _dtype, _per_block, _align = torch.int8, BLOCK, 32
 
     def __init__(self, codes, exps, cols: int, act: str):
         self._act = _act_code(act)
-        _check_parts(codes, exps, cols, torch.int8, BLOCK, "Checkpoint")
-        self.codes, self.exps, self.cols, self.act = codes, exps, cols, act
-
-    @property
-    def rows(self) -> int:
-        return self.codes.size(0)
+        self.act = act
+        self._take(codes, exps, cols)
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """The 8-bit values, (rows, cols)."""
-        if dtype not in _DTYPES:
-            _fail(f"cannot dequantise to {str(dtype).replace('torch.', '')}")
-        out = self.codes.new_empty((self.rows, self.cols), dtype=dtype)
-        _launch("vt_mx8_dequantize", out.device.index, self.codes.data_ptr(), self.exps.data_ptr(),
-                self.rows, self.cols, _DTYPES[dtype], out.data_ptr())
-        return out
+        return self._dequantize("vt_mx8_dequantize", dtype)
 
 
-class MX4:
+class MX4(_Blocks):
     """A matrix in 4-bit microscaled blocks: codes (rows, 16 B) uint8, two columns a
     byte with the even one in the low nibble, exps (rows, B) uint8."""
 
-    __slots__ = ("codes", "exps", "cols")
+    __slots__ = ()
+    _dtype, _per_block, _align = torch.uint8, BLOCK // 2, 16
 
     def __init__(self, codes, exps, cols: int):
-        _check_parts(codes, exps, cols, torch.uint8, BLOCK // 2, "MX4")
-        self.codes, self.exps, self.cols = codes, exps, cols
-
-    @property
-    def rows(self) -> int:
-        return self.codes.size(0)
+        self._take(codes, exps, cols)
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """The 4-bit values, (rows, cols)."""
-        if dtype not in _DTYPES:
-            _fail(f"cannot dequantise to {str(dtype).replace('torch.', '')}")
-        out = self.codes.new_empty((self.rows, self.cols), dtype=dtype)
-        _launch("vt_mx4_dequantize", out.device.index, self.codes.data_ptr(), self.exps.data_ptr(),
-                self.rows, self.cols, _DTYPES[dtype], out.data_ptr())
-        return out
+        return self._dequantize("vt_mx4_dequantize", dtype)
 
 
 def act_checkpoint(z: torch.Tensor, act: str = "silu"):
     """(act(z), 8-bit checkpoint of z) for z (..., cols), in one pass."""
     code = _act_code(act)
-    m, rows, cols, stride = _matrix(z, "z")
-    blocks = -(-cols // BLOCK)
+    m, rows, cols, stride, dtype = _matrix(z, "z")
     h = m.new_empty(z.shape)
-    codes = m.new_empty((rows, blocks * BLOCK), dtype=torch.int8)
-    exps = m.new_empty((rows, blocks), dtype=torch.uint8)
-    _launch("vt_mx8_checkpoint", z.device.index, m.data_ptr(), _DTYPES[z.dtype], rows, cols, stride,
-            code, h.data_ptr(), codes.data_ptr(), exps.data_ptr())
     ckpt = Checkpoint.__new__(Checkpoint)
-    ckpt.codes, ckpt.exps, ckpt.cols, ckpt.act, ckpt._act = codes, exps, cols, act, code
+    ckpt.act, ckpt._act = act, code
+    ckpt._new(m, rows, cols)
+    _launch("vt_mx8_checkpoint", ckpt.device_index, m.data_ptr(), dtype, rows, cols, stride, code,
+            h.data_ptr(), ckpt._pc, ckpt._pe)
     return h, ckpt
 
 
 def act_backward(dh: torch.Tensor, ckpt: Checkpoint) -> torch.Tensor:
     """dz = dh * act'(z8), in dh's type and shape."""
-    m, rows, cols, stride = _matrix(dh, "dh")
+    m, rows, cols, stride, dtype = _matrix(dh, "dh")
     if rows != ckpt.rows or cols != ckpt.cols:
         _fail(f"dh had {rows} rows of {cols}, the checkpoint has {ckpt.rows} of {ckpt.cols}")
-    _same(dh, ckpt.codes, "dh", "the checkpoint")
+    if m.get_device() != ckpt.device_index:
+        _fail("dh must be on the same device as the checkpoint")
     dz = m.new_empty(dh.shape)
-    _launch("vt_mx8_act_bwd", dh.device.index, m.data_ptr(), _DTYPES[dh.dtype], rows, cols, stride,
-            ckpt.codes.data_ptr(), ckpt.exps.data_ptr(), ckpt._act, dz.data_ptr())
+    _launch("vt_mx8_act_bwd", ckpt.device_index, m.data_ptr(), dtype, rows, cols, stride, ckpt._pc,
+            ckpt._pe, ckpt._act, dz.data_ptr())
     return dz
 
 
@@ -240,18 +262,18 @@ def linear_backward(dy: torch.Tensor, weight: torch.Tensor, ckpt: Checkpoint, bi
     (dz, dw, db) in that type: dz (..., cols) = (dy W) * act'(z8), dw (outs,
     cols) = dy^T act(z8) and db (outs) = column sums of dy; None for those not
     asked for."""
-    m, rows, outs, dy_stride = _matrix(dy, "dy", _PRODUCT_TYPES)
-    w, w_rows, cols, w_stride = _matrix(weight, "weight", _PRODUCT_TYPES)
-    if weight.dim() != 2 or w_rows != outs:
+    m, rows, outs, dy_stride, dtype = _matrix(dy, "dy", _PRODUCT_TYPES)
+    w, w_rows, cols, w_stride, w_type = _matrix(weight, "weight", _PRODUCT_TYPES)
+    if w_rows != outs or weight.dim() != 2:
         _fail(f"weight had shape {tuple(weight.shape)}, expected ({outs}, columns)")
-    if weight.dtype != dy.dtype:
+    if w_type != dtype:
         _fail("weight must have the dtype of dy")
     if rows != ckpt.rows or cols != ckpt.cols:
         _fail(f"dy has {rows} rows and weight {cols} columns, the checkpoint has {ckpt.rows} "
               f"rows of {ckpt.cols}")
-    _same(weight, dy, "weight", "dy")
-    _same(ckpt.codes, dy, "the checkpoint", "dy")
-    dev, dt = dy.device, dy.dtype
+    index = m.get_device()
+    if w.get_device() != index or ckpt.device_index != index:
+        _fail("weight and the checkpoint must be on the same device as dy")
     dz = m.new_empty((*dy.shape[:-1], cols)) if need_dz else None
     dw = m.new_empty((outs, cols)) if need_dw else None
     db = m.new_empty(outs) if bias else None
@@ -259,10 +281,10 @@ def linear_backward(dy: torch.Tensor, weight: torch.Tensor, ckpt: Checkpoint, bi
     n = _call("vt_mx8_linear_bwd_workspace_bytes")(
         rows, cols, outs, _unaligned(m_ptr, dy_stride) + 2 * _unaligned(w_ptr, w_stride))
     ws = m.new_empty(n, dtype=torch.uint8) if n else None
-    _launch("vt_mx8_linear_bwd", dev.index, m_ptr, dy_stride, w_ptr, w_stride,
-            _DTYPES[dt], rows, cols, outs, ckpt.codes.data_ptr(), ckpt.exps.data_ptr(), ckpt._act,
-            dz.data_ptr() if need_dz else None, dw.data_ptr() if need_dw else None,
-            db.data_ptr() if bias else None, ws.data_ptr() if n else None, n, _error_word(dev).data_ptr())
+    _launch("vt_mx8_linear_bwd", index, m_ptr, dy_stride, w_ptr, w_stride, dtype, rows, cols, outs,
+            ckpt._pc, ckpt._pe, ckpt._act, dz.data_ptr() if need_dz else None,
+            dw.data_ptr() if need_dw else None, db.data_ptr() if bias else None,
+            ws.data_ptr() if n else None, n, _error_word(index))
     return dz, dw, db
 
 
@@ -291,14 +313,10 @@ def act_linear(z: torch.Tensor, weight: torch.Tensor, bias=None, act: str = "sil
 
 def quantize4(x: torch.Tensor) -> MX4:
     """x (..., cols) in 4-bit microscaled blocks, as (rows, cols)."""
-    m, rows, cols, stride = _matrix(x, "x")
-    blocks = -(-cols // BLOCK)
+    m, rows, cols, stride, dtype = _matrix(x, "x")
     q = MX4.__new__(MX4)
-    q.codes = m.new_empty((rows, blocks * BLOCK // 2), dtype=torch.uint8)
-    q.exps = m.new_empty((rows, blocks), dtype=torch.uint8)
-    q.cols = cols
-    _launch("vt_mx4_quantize", x.device.index, m.data_ptr(), _DTYPES[x.dtype], rows, cols, stride,
-            q.codes.data_ptr(), q.exps.data_ptr())
+    q._new(m, rows, cols)
+    _launch("vt_mx4_quantize", q.device_index, m.data_ptr(), dtype, rows, cols, stride, q._pc, q._pe)
     return q
 
 
@@ -307,21 +325,24 @@ def linear4(x: torch.Tensor, w: MX4, bias=None, act: str = "identity") -> torch.
     4 bits on the way, w is the weight (outs, cols) in 4 bits, bias (outs) has
     x's type.  y (..., outs) has x's type."""
     code = _act_code(act)
-    m, rows, cols, stride = _matrix(x, "x", _PRODUCT_TYPES)
-    outs = w.rows
+    m, rows, cols, stride, dtype = _matrix(x, "x", _PRODUCT_TYPES)
+    outs, index = w.rows, w.device_index
     if cols != w.cols:
         _fail(f"x had {cols} columns, the weight has {w.cols}")
-    _same(w.codes, x, "the weight", "x")
+    if m.get_device() != index:
+        _fail("the weight must be on the same device as x")
+    b_ptr = None
     if bias is not None:
-        if bias.dtype != x.dtype or bias.dim() != 1 or bias.size(0) != outs:
+        if bias.dtype is not x.dtype or bias.shape != (outs,):
             _fail(f"bias must have the dtype of x and shape ({outs},)")
-        _same(bias, x, "bias", "x")
+        if bias.get_device() != index:
+            _fail("bias must be on the same device as x")
         bias = bias.contiguous()
+        b_ptr = bias.data_ptr()
     y = m.new_empty((*x.shape[:-1], outs))
     m_ptr = m.data_ptr()
     n = _call("vt_mx4_linear_workspace_bytes")(rows, cols, outs, _unaligned(m_ptr, stride))
     ws = m.new_empty(n, dtype=torch.uint8) if n else None
-    _launch("vt_mx4_linear", x.device.index, m_ptr, stride, _DTYPES[x.dtype], rows, cols, outs,
-            w.codes.data_ptr(), w.exps.data_ptr(), bias.data_ptr() if bias is not None else None,
-            code, y.data_ptr(), ws.data_ptr() if n else None, n, _error_word(x.device).data_ptr())
+    _launch("vt_mx4_linear", index, m_ptr, stride, dtype, rows, cols, outs, w._pc, w._pe, b_ptr, code,
+            y.data_ptr(), ws.data_ptr() if n else None, n, _error_word(index))
     return y
