@@ -54,6 +54,6 @@ def test_workspace_sizes_cover_the_layout():
         assert n(rows, cols, 8, 0) == 0 and n(rows, cols, 8, 1) >= rows * cols * 2
     n = mx._call("vt_mx8_linear_bwd_workspace_bytes")
     for rows, cols, outs in ((1, 1, 1), (1000, 200, 77), (1000, 200, 777)):
-        assert n(rows, cols, outs, 1) - n(rows, cols, outs, 0) >= rows * outs * 2
+        assert n(rows, cols, outs, 1) - n(rows, cols, outs, 0) >= (rows * outs * 2 if outs > 8 else 0)
         if outs > 256:
             assert n(rows, cols, outs, 2) - n(rows, cols, outs, 0) >= cols * outs * 2

@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "vt_abi.cuh"
 
 namespace vt {
@@ -361,11 +363,16 @@ template <typename F> inline vt_status with_type16(int dtype, F f)
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned32(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 inline uint32_t mx_blocks(uint32_t cols) { return cols / MX_BLOCK + (cols % MX_BLOCK != 0); }
-inline int sm_count()
+inline int sm_count()  // of the current device, asked for once
 {
-    int dev = 0, sms = 148;
+    static std::atomic<int> known[64];
+    int dev = 0, sms = 0;
     cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    std::atomic<int> &k = known[dev & 63];
+    if ((sms = k.load(std::memory_order_relaxed)) == 0) {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+        else k.store(sms, std::memory_order_relaxed);
+    }
     return sms;
 }
 

@@ -17,6 +17,9 @@
 // Shared memory's bandwidth is what is short between HBM and the tensor cores here, which decides
 // the orientation: with z's columns in the lanes the activations need no shared memory at all, a
 // warp's dz is 64 contiguous bytes a row, and the second product reads one operand instead of two.
+// Up to 8 outputs (a colour) are rows of 16 bytes or less, whose TMA copies would take as long as
+// eight times the bytes; one warp brings them in instead, without a copy to whole words before.
+//
 // Layers of up to 64 columns would leave half of the lanes empty; they get W twice instead (FOLD),
 // and each half of the lanes takes half of a tile's rows.
 //
@@ -30,7 +33,7 @@ namespace vt {
 
 // ---- layers with up to 256 outputs ----
 
-constexpr uint32_t TILE_ROWS = 32, NARROW_OUTS = 256, NARROW_THREADS = 640;
+constexpr uint32_t TILE_ROWS = 32, NARROW_OUTS = 256, NARROW_THREADS = 640, TINY_OUTS = 8;
 
 // OC: dy's columns in chunks of 64.  A slab is 128 columns of z, or all of up to 64 (FOLD).
 template <int OC, bool FOLD> struct Narrow {
@@ -62,6 +65,9 @@ struct NarrowArgs {
     float *dw_parts;   // [group][slab][OC * 64][128]; null: dW not wanted
     float *db_parts;   // [group][OC * 64]; null: db not wanted
     uint32_t *err;
+    const void *dy;    // read by a warp instead of TMA: up to TINY_OUTS outputs; else null
+    uint64_t dy_stride;
+    bool codes_whole;  // a tile's codes are one piece of memory
     bool dy_chunked;   // dy's columns are whole chunks of 64: one TMA copy brings all of them in
 };
 
@@ -82,6 +88,15 @@ __device__ __forceinline__ void slope16(const uint32_t *codes, f32x2 sc, const u
     }
 }
 
+// 16 bits, or 0; without a branch, so that many are under way at once
+__device__ __forceinline__ uint32_t load16_if(const unsigned short *p, bool wanted)
+{
+    unsigned short v;
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %2, 0;\nmov.u16 %0, 0;\n@p ld.global.nc.u16 %0, [%1];\n}"
+                 : "=h"(v) : "l"(p), "r"((uint32_t)wanted));
+    return v;
+}
+
 template <typename T, int ACT, int OC, bool FOLD>
 __global__ void __launch_bounds__(NARROW_THREADS, 1)
     narrow_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap code_map, const NarrowArgs a)
@@ -94,12 +109,12 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
     const uint32_t slab = blockIdx.x % a.slabs, group = blockIdx.x / a.slabs;
     // the column sums of dy, 128 outputs at a time, are shared out among the slabs
     const uint32_t sharers = a.slabs < P::MT ? a.slabs : P::MT;
-    const bool sums = a.db_parts && slab < sharers;
+    const bool sums = a.db_parts && slab < sharers, tiny = OC == 1 && a.dy;
     tc::Fail *const fail = &s.fail;
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < P::STAGES; ++i) {
-            tc::mbar_init(&s.full[i], 1);
+            tc::mbar_init(&s.full[i], tiny ? 2 : 1);
             tc::mbar_init(&s.empty[i], 1);
         }
         for (uint32_t i = 0; i < P::BUFS; ++i) {
@@ -112,11 +127,14 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         tc::mbar_init(&s.failed, 1);
         s.fail.failed = 0;
         tc::mbar_init_fence();
-        tc::tma_prefetch_map(&dy_map);
-        tc::tma_prefetch_map(&code_map);
+        if (!tiny) tc::tma_prefetch_map(&dy_map);
+        if (!a.codes_whole) tc::tma_prefetch_map(&code_map);
     }
     for (uint32_t i = threadIdx.x; i < P::ONES / 4u; i += NARROW_THREADS)
         reinterpret_cast<uint32_t *>(smem + P::ONES_AT)[i] = pack2<T>(1.0f, 1.0f);
+    if (tiny)  // all but the first 16 bytes of dy's rows stay zero
+        for (uint32_t i = threadIdx.x; i < P::STAGES * (P::CHUNK / 16u); i += NARROW_THREADS)
+            *reinterpret_cast<uint4 *>(smem + i / (P::CHUNK / 16u) * P::STAGE + i % (P::CHUNK / 16u) * 16u) = make_uint4(0, 0, 0, 0);
     tc::fence_async_shared();
     if (warp == 1) tc::tmem_alloc<P::TMEM>(&s.tmem);
     tc::fence_before();
@@ -131,14 +149,21 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             for (uint32_t t = group; t < a.tiles; t += a.groups) {
                 if (!tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err)) break;
                 uint8_t *st = smem + r.i * P::STAGE;
-                tc::mbar_arrive_tx(&s.full[r.i], P::STAGE);
-                if (OC > 1 && a.dy_chunked) {
+                // a last tile's missing rows of whole codes keep those of an older tile: their dy is zero
+                const uint32_t code_bytes = !a.codes_whole || t + 1u < a.tiles ? TILE_ROWS * P::CODE_PITCH
+                                                                              : (uint32_t)(a.rows - (uint64_t)t * TILE_ROWS) * P::CODE_PITCH;
+                tc::mbar_arrive_tx(&s.full[r.i], (tiny ? 0u : P::DY_BYTES) + code_bytes);
+                if (tiny) {
+                } else if (OC > 1 && a.dy_chunked) {
                     tc::tma_load_3d(st, &dy_map, 0, (int)(t * TILE_ROWS), 0, &s.full[r.i]);
                 } else {
                     for (int c = 0; c < OC; ++c)
                         tc::tma_load_2d(st + c * P::CHUNK, &dy_map, c * 64, (int)(t * TILE_ROWS), &s.full[r.i]);
                 }
-                tc::tma_load_2d(st + P::DY_BYTES, &code_map, (int)(slab * 128), (int)(t * TILE_ROWS), &s.full[r.i]);
+                if (a.codes_whole)
+                    tc::bulk_load(st + P::DY_BYTES, a.codes + (uint64_t)t * (TILE_ROWS * P::CODE_PITCH), code_bytes, &s.full[r.i]);
+                else
+                    tc::tma_load_2d(st + P::DY_BYTES, &code_map, (int)(slab * 128), (int)(t * TILE_ROWS), &s.full[r.i]);
                 ++issued;
                 r.next(P::STAGES);
             }
@@ -215,6 +240,34 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         }
         if (mine) tc::commit(&s.done);
         if (!ok) tc::mbar_wait_slow(&s.done, 0, fail, a.err, true);  // leave no product in flight
+    } else if (warp == 2) {
+        if (tiny) {  // dy of few outputs, a row a lane, eight tiles in flight
+            tc::Ring r;
+            bool ok = true;
+            const unsigned short *dy = (const unsigned short *)a.dy;
+            for (uint32_t t0 = group; t0 < a.tiles && ok; t0 += 8u * a.groups) {
+                uint32_t v[8][TINY_OUTS];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint64_t row = (uint64_t)(t0 + i * a.groups) * TILE_ROWS + lane;
+                    const unsigned short *p = dy + row * a.dy_stride;
+#pragma unroll
+                    for (uint32_t o = 0; o < TINY_OUTS; ++o) v[i][o] = load16_if(p + o, row < a.rows && o < a.outs);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    if (t0 + i * a.groups >= a.tiles) break;
+                    ok = ok && __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
+                    if (!ok) break;
+                    *reinterpret_cast<uint4 *>(smem + r.i * P::STAGE + lane * 128u + ((lane & 7u) << 4)) =
+                        make_uint4(v[i][0] | v[i][1] << 16, v[i][2] | v[i][3] << 16, v[i][4] | v[i][5] << 16, v[i][6] | v[i][7] << 16);
+                    tc::fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
+                    r.next(P::STAGES);
+                }
+            }
+        }
     } else if (warp >= 4) {  // activations: four sets of four warps take tiles in turn; a lane has a column of z (a
               // warp one block of 32) and ROWS rows of the tile
         constexpr int ROWS = P::ROWS;
@@ -684,7 +737,7 @@ static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, int c
     p.dw_at = 0;
     p.db_at = p.dw_at + align_up((uint64_t)p.groups * p.slabs * 128u * p.part_outs * 4u, 256);
     p.dy_at = p.db_at + align_up((uint64_t)p.groups * p.part_outs * 4u, 256);
-    p.bytes = p.dy_at + (copies & COPY_DY ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
+    p.bytes = p.dy_at + (copies & COPY_DY && outs > TINY_OUTS ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
     return p;
 }
 
@@ -713,13 +766,18 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
                             uint8_t *workspace, uint32_t *err, cudaStream_t stream)
 {
     const NarrowPlan p = narrow_plan(rows, cols, outs, copies_of<T>(dy, dy_stride, w, w_stride), (uint32_t)sm_count());
-    CUtensorMap dy_map;
-    if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
+    CUtensorMap dy_map = {};
+    const bool tiny = outs <= TINY_OUTS;
+    if (!tiny)
+        if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
     const bool chunked = outs % 64u == 0 && outs > 64u;
-    if (vt_status s = chunked ? tc::make_chunk_map(&dy_map, tma_type<T>(), dy, rows, p.oc, dy_stride * sizeof(T), TILE_ROWS, 64, sizeof(T))
+    if (vt_status s = tiny ? VT_OK : chunked ? tc::make_chunk_map(&dy_map, tma_type<T>(), dy, rows, p.oc, dy_stride * sizeof(T), TILE_ROWS, 64, sizeof(T))
                               : map_rows<T>(&dy_map, dy, dy_stride, rows, outs, TILE_ROWS))
         return s;
     NarrowArgs a;
+    a.dy = tiny ? dy : nullptr;
+    a.dy_stride = dy_stride;
+    a.codes_whole = mx_blocks(cols) * 32u == (p.fold ? 64u : 128u);
     a.dy_chunked = chunked;
     a.weight = w;
     a.weight_stride = w_stride;
