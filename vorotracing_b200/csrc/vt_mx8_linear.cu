@@ -3,7 +3,7 @@
 //
 // Layers with up to 256 outputs (narrow_kernel) make all three in one pass over the rows, so dy
 // and the checkpoint are read from HBM once and act(z8) never reaches memory.  A CTA owns a slab
-// of 128 columns of z and every G-th tile of 32 rows.  A tile of dy is staged once in shared
+// of 128 columns of z and every G-th tile of 32 or 64 rows.  A tile of dy is staged once in shared
 // memory (TMA, 128-byte swizzle) and used twice: as the K-major B operand of dH^T = W^T dy^T,
 // whose result has z's columns in the lanes of tensor memory, and, the same bytes read the other
 // way, as the MN-major B operand of dW^T += act(z8)^T dy, whose accumulator stays in tensor memory
@@ -33,25 +33,29 @@ namespace vt {
 
 // ---- layers with up to 256 outputs ----
 
-constexpr uint32_t TILE_ROWS = 32, NARROW_OUTS = 256, NARROW_THREADS = 640, TINY_OUTS = 8;
+constexpr uint32_t NARROW_OUTS = 256, NARROW_THREADS = 640, TINY_OUTS = 8;
 
 // OC: dy's columns in chunks of 64.  A slab is 128 columns of z, or all of up to 64 (FOLD).
+// Rows of a tile: fewer barriers a row against smaller stages, of which four are the least.
+constexpr uint32_t narrow_rows(uint32_t oc) { return oc <= 2 ? 64 : 32; }
+
 template <int OC, bool FOLD> struct Narrow {
+    static constexpr uint32_t TILE_ROWS = narrow_rows(OC);
     static constexpr uint32_t CHUNK = TILE_ROWS * 128u, DY_BYTES = OC * CHUNK, CODE_PITCH = FOLD ? 64u : 128u;
     static constexpr uint32_t STAGE = DY_BYTES + TILE_ROWS * CODE_PITCH;
     struct Ctrl {
-        float scale[16][32];  // of the blocks in each activation warp's rows
-        uint64_t full[12], empty[12], dh_full[8], dh_empty[8], h_full[8], w_full, done, failed;
+        float scale[16][TILE_ROWS];  // of the blocks in each activation warp's rows
+        uint64_t full[12], empty[12], dh_full[8], h_full[8], w_full, done, failed;
         uint32_t tmem;
         tc::Fail fail;
     };
     static constexpr uint32_t ONES = 2048u, FIT = (232448u - ONES - sizeof(Ctrl)) / STAGE, STAGES = FIT < 12u ? FIT : 12u;
     static constexpr uint32_t ONES_AT = STAGES * STAGE, CTRL_AT = ONES_AT + ONES, SMEM = CTRL_AT + sizeof(Ctrl);
     static constexpr uint32_t TMEM = 512;
-    // columns of tensor memory: dW, W, db (16 for 128 outputs), and as many of dH as there is room for, up to eight
-    static constexpr uint32_t W_AT = OC * 64u, MT = (OC + 1) / 2, DB_AT = W_AT + OC * 32u, DH_AT = DB_AT + MT * 16u, BUFS = OC == 4 ? 3 : OC == 3 ? 6 : 8;
-    static constexpr int ROWS = FOLD ? 16 : 32;  // of a tile an activation warp takes
-    static_assert(STAGES >= 4 && DH_AT + BUFS * TILE_ROWS <= TMEM, "does not fit an SM");
+    // columns of tensor memory: dW, W, db (16 for 128 outputs), and as many of dH as there is room for, up to six
+    static constexpr uint32_t W_AT = OC * 64u, MT = (OC + 1) / 2, DB_AT = W_AT + OC * 32u, DH_AT = DB_AT + MT * 16u, BUFS = OC == 4 ? 3 : OC == 3 ? 6 : 4;
+    static constexpr int ROWS = FOLD ? TILE_ROWS / 2 : TILE_ROWS;  // of a tile an activation warp takes
+    static_assert(STAGES >= 4 && STAGES > BUFS && DH_AT + BUFS * TILE_ROWS <= TMEM, "does not fit an SM");
 };
 
 struct NarrowArgs {
@@ -103,6 +107,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
 {
     using P = Narrow<OC, FOLD>;
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr uint32_t TILE_ROWS = P::TILE_ROWS;
     extern __shared__ __align__(1024) uint8_t smem[];
     typename P::Ctrl &s = *reinterpret_cast<typename P::Ctrl *>(smem + P::CTRL_AT);
     const uint32_t warp = tc::warp_number(), lane = threadIdx.x % 32u;
@@ -119,7 +124,6 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         }
         for (uint32_t i = 0; i < P::BUFS; ++i) {
             tc::mbar_init(&s.dh_full[i], 1);
-            tc::mbar_init(&s.dh_empty[i], 1);
             tc::mbar_init(&s.h_full[i], 4);
         }
         tc::mbar_init(&s.w_full, 16);
@@ -175,11 +179,14 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         constexpr uint32_t ID = tc::idesc_f16<BF16>(128, TILE_ROWS, false, false);
         const uint32_t st_addr = tc::smem_u32(smem);
         const bool mine = tc::elect();
-        tc::Ring r, dh;
+        tc::Ring r, dh, old;  // old: the stage of the tile that had this one's buffer of dH
         bool ok = __all_sync(~0u, tc::mbar_wait(&s.w_full, 0, fail, a.err));
         for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
-            ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err) &&
-                                     tc::mbar_wait(&s.dh_empty[dh.i], dh.phase ^ 1u, fail, a.err));
+            ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
+            if (t >= group + P::BUFS * a.groups) {  // its second product has left both
+                ok = ok && __all_sync(~0u, tc::mbar_wait(&s.empty[old.i], old.phase, fail, a.err));
+                old.next(P::STAGES);
+            }
             if (!ok) break;
             tc::fence_after();
             const uint64_t b = tc::smem_desc(st_addr + r.i * P::STAGE, 16, 1024);
@@ -232,7 +239,6 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                                 tc::mma_f16(tmem + P::DB_AT + m * 16u, b + m * (2u * P::CHUNK >> 4) + k * 128u, ones, ID_DB,
                                             t != group || k != 0);
                 tc::commit(&s.empty[r.i]);
-                tc::commit(&s.dh_empty[h.i]);
             }
             __syncwarp();
             r.next(P::STAGES);
@@ -241,26 +247,31 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         if (mine) tc::commit(&s.done);
         if (!ok) tc::mbar_wait_slow(&s.done, 0, fail, a.err, true);  // leave no product in flight
     } else if (warp == 2) {
-        if (tiny) {  // dy of few outputs, a row a lane, eight tiles in flight
+        if (tiny) {  // dy of few outputs, eight rows a lane in flight
+            constexpr uint32_t PARTS = TILE_ROWS / 32u, AHEAD = 8u / PARTS;
             tc::Ring r;
             bool ok = true;
             const unsigned short *dy = (const unsigned short *)a.dy;
-            for (uint32_t t0 = group; t0 < a.tiles && ok; t0 += 8u * a.groups) {
+            for (uint32_t t0 = group; t0 < a.tiles && ok; t0 += AHEAD * a.groups) {
                 uint32_t v[8][TINY_OUTS];
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {
-                    const uint64_t row = (uint64_t)(t0 + i * a.groups) * TILE_ROWS + lane;
+                    const uint64_t row = (uint64_t)(t0 + i / PARTS * a.groups) * TILE_ROWS + i % PARTS * 32u + lane;
                     const unsigned short *p = dy + row * a.dy_stride;
 #pragma unroll
                     for (uint32_t o = 0; o < TINY_OUTS; ++o) v[i][o] = load16_if(p + o, row < a.rows && o < a.outs);
                 }
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
+                for (uint32_t i = 0; i < AHEAD; ++i) {
                     if (t0 + i * a.groups >= a.tiles) break;
                     ok = ok && __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
                     if (!ok) break;
-                    *reinterpret_cast<uint4 *>(smem + r.i * P::STAGE + lane * 128u + ((lane & 7u) << 4)) =
-                        make_uint4(v[i][0] | v[i][1] << 16, v[i][2] | v[i][3] << 16, v[i][4] | v[i][5] << 16, v[i][6] | v[i][7] << 16);
+#pragma unroll
+                    for (uint32_t j = 0; j < PARTS; ++j) {
+                        const uint32_t *w = v[i * PARTS + j];
+                        *reinterpret_cast<uint4 *>(smem + r.i * P::STAGE + (j * 32u + lane) * 128u + ((lane & 7u) << 4)) =
+                            make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+                    }
                     tc::fence_async_shared();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
@@ -273,7 +284,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         constexpr int ROWS = P::ROWS;
         const uint32_t quad = warp % 4u, set = (warp - 4u) / 4u;
         const uint32_t block = FOLD ? quad & 1u : slab * 4u + quad, n = block * 32u + lane;
-        const uint32_t row0 = FOLD ? (quad >> 1) * 16u : 0u;  // in the tile
+        const uint32_t row0 = FOLD ? (quad >> 1) * (TILE_ROWS / 2u) : 0u;  // in the tile
         const uint32_t lanes = quad * 32u << 16, code0 = row0 * P::CODE_PITCH + (FOLD ? n : quad * 32u + lane);
         float *const scale = s.scale[warp - 4u];
         const uint32_t first = group + set * a.groups, step = 4u * a.groups;
@@ -281,15 +292,20 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         const uint64_t first_row = (uint64_t)first * TILE_ROWS + row0;
         const uint8_t *exps = a.exps + (first_row + lane) * a.blocks + block;
         const uint64_t exps_step = (uint64_t)step * TILE_ROWS * a.blocks;
-        const bool scaled = lane < ROWS && block < a.blocks;
+        constexpr int EXPS = (ROWS + 31) / 32;  // rows a lane has the scales of
         const uint32_t last = a.tiles - 1u, last_rows = (uint32_t)(a.rows - (uint64_t)last * TILE_ROWS);  // rows of the last tile
         const uint32_t last_count = last_rows > row0 ? min(last_rows - row0, (uint32_t)ROWS) : 0u;
-        auto exponent = [&](uint32_t t) -> uint32_t {
-            const uint32_t e = scaled && (t < last || (t == last && lane < last_count)) ? __ldg(exps) : 127u;
+        auto exponent = [&](uint32_t t, uint32_t (&e)[EXPS]) {
+#pragma unroll
+            for (int i = 0; i < EXPS; ++i) {
+                const uint32_t row = i * 32u + lane;
+                const bool in = row < ROWS && block < a.blocks && (t < last || (t == last && row < last_count));
+                e[i] = in ? __ldg(exps + (uint64_t)i * 32u * a.blocks) : 127u;
+            }
             exps += exps_step;
-            return e;
         };
-        uint32_t E = exponent(first);
+        uint32_t E[EXPS];
+        exponent(first, E);
         unsigned short *out = (unsigned short *)a.dz + first_row * a.cols + n;
         const uint64_t out_step = ((uint64_t)step * TILE_ROWS - ROWS) * a.cols;
         const bool write = a.dz && n < a.cols;
@@ -319,9 +335,11 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         dh.skip(set, P::BUFS);
         bool ok = true;
         for (uint32_t t = first; t < a.tiles && ok; t += step) {
-            const uint32_t next_E = exponent(t + step);
+            uint32_t next_E[EXPS];
+            exponent(t + step, next_E);
             __syncwarp();
-            scale[lane] = mx8_scale(E);
+#pragma unroll
+            for (int i = 0; i < EXPS; ++i) scale[i * 32 + lane] = mx8_scale(E[i]);
             __syncwarp();
             ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
             // A parity tells a phase from the one before it only.  Of a buffer's last use this set knows
@@ -361,7 +379,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 tc::tmem_store8(here + p, h);
                 if (FOLD) {  // this half of the lanes has no part in the other half's rows
                     const uint32_t none[8] = {};
-                    tc::tmem_store8(buffer + (row0 ^ 16u), none);
+                    tc::tmem_store8(buffer + (row0 ^ (TILE_ROWS / 2u)) + p, none);
                 }
                 if (p + 16 == ROWS) {
                     tc::tmem_wait_store();
@@ -389,7 +407,8 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             dh.skip(P::BUFS < 4u ? P::BUFS : 4u, P::BUFS);
             if (P::BUFS < 4u) dh.skip(4u - P::BUFS, P::BUFS);
             r.skip(4, P::STAGES);
-            E = next_E;
+#pragma unroll
+            for (int i = 0; i < EXPS; ++i) E[i] = next_E[i];
         }
         ok = __all_sync(~0u, ok && tc::mbar_wait(&s.done, 0, fail, a.err));
         tc::fence_after();
@@ -729,7 +748,8 @@ static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, int c
     p.oc = (outs + 63u) / 64u;
     p.fold = cols <= 64u;
     p.slabs = (cols + 127u) / 128u;
-    p.tiles = (uint32_t)((rows + TILE_ROWS - 1u) / TILE_ROWS);
+    const uint32_t tile_rows = narrow_rows(p.oc);
+    p.tiles = (uint32_t)((rows + tile_rows - 1u) / tile_rows);
     // one CTA an SM; a slab more than there are SMs still gets its own
     p.groups = p.slabs < sms ? sms / p.slabs : 1u;
     if (p.groups > p.tiles) p.groups = p.tiles;
@@ -753,7 +773,7 @@ static vt_status launch_narrow(const CUtensorMap &dy, const NarrowArgs &a, cudaS
     using P = Narrow<OC, FOLD>;
     CUtensorMap codes;
     const uint64_t width = (uint64_t)a.blocks * 32u;
-    if (vt_status s = tc::make_map(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.rows, width, width, TILE_ROWS, P::CODE_PITCH, false))
+    if (vt_status s = tc::make_map(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.rows, width, width, P::TILE_ROWS, P::CODE_PITCH, false))
         return s;
     if (vt_status s = tc::allow_smem(narrow_kernel<T, ACT, OC, FOLD>, P::SMEM, allowed)) return s;
     narrow_kernel<T, ACT, OC, FOLD><<<a.groups * a.slabs, NARROW_THREADS, P::SMEM, stream>>>(dy, codes, a);
@@ -771,8 +791,8 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     if (!tiny)
         if (vt_status s = whole_rows<T>(dy, dy_stride, rows, outs, workspace + p.dy_at, stream)) return s;
     const bool chunked = outs % 64u == 0 && outs > 64u;
-    if (vt_status s = tiny ? VT_OK : chunked ? tc::make_chunk_map(&dy_map, tma_type<T>(), dy, rows, p.oc, dy_stride * sizeof(T), TILE_ROWS, 64, sizeof(T))
-                              : map_rows<T>(&dy_map, dy, dy_stride, rows, outs, TILE_ROWS))
+    if (vt_status s = tiny ? VT_OK : chunked ? tc::make_chunk_map(&dy_map, tma_type<T>(), dy, rows, p.oc, dy_stride * sizeof(T), narrow_rows(p.oc), 64, sizeof(T))
+                              : map_rows<T>(&dy_map, dy, dy_stride, rows, outs, narrow_rows(p.oc)))
         return s;
     NarrowArgs a;
     a.dy = tiny ? dy : nullptr;
