@@ -78,8 +78,10 @@ struct NarrowArgs {
     const int8_t *codes;
     const uint8_t *exps;
     void *dz;          // null: not wanted
-    float *dw_parts;   // [group][slab][OC * 64][128]; null: dW not wanted
-    float *db_parts;   // [group][OC * 64]; null: db not wanted
+    // where dW and db go, null if not wanted: parts for a second kernel, [group][slab][OC * 64][128] and
+    // [group][OC * 64], or with one group the results themselves
+    float *dw_parts, *db_parts;
+    void *dw, *db;
     uint32_t *err;
     const void *dy;    // read by a warp instead of TMA: up to TINY_OUTS outputs; else null
     uint64_t dy_stride;
@@ -104,15 +106,6 @@ __device__ __forceinline__ void slope16(const uint32_t *codes, f32x2 sc, const u
     }
 }
 
-// 16 bits, or 0; without a branch, so that many are under way at once
-__device__ __forceinline__ uint32_t load16_if(const unsigned short *p, bool wanted)
-{
-    unsigned short v;
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %2, 0;\nmov.u16 %0, 0;\n@p ld.global.nc.u16 %0, [%1];\n}"
-                 : "=h"(v) : "l"(p), "r"((uint32_t)wanted));
-    return v;
-}
-
 template <typename T, int ACT, int OC, bool FOLD>
 __global__ void __launch_bounds__(NARROW_THREADS, 1)
     narrow_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap code_map, const NarrowArgs a)
@@ -126,7 +119,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
     const uint32_t slab = blockIdx.x % a.slabs, group = blockIdx.x / a.slabs;
     // the column sums of dy, 128 outputs at a time, are shared out among the slabs
     const uint32_t sharers = a.slabs < P::MT ? a.slabs : P::MT;
-    const bool sums = a.db_parts && slab < sharers, tiny = OC == 1 && a.dy;
+    const bool sums = (a.db_parts || a.db) && slab < sharers, tiny = OC == 1 && a.dy;
     tc::Fail *const fail = &s.fail;
 
     if (threadIdx.x == 0) {
@@ -235,11 +228,10 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             const uint64_t b = tc::smem_desc(st_addr + r.i * P::STAGE, P::CHUNK, 1024);
             const uint32_t from = dh_at + h.i * TILE_ROWS;
             if (mine) {
-                if (a.dw_parts) {
-                    tc::mma_f16_tmem(tmem, from, b, ID, t != group);
+                if (a.dw_parts || a.dw)
 #pragma unroll
-                    for (uint32_t k = 1; k < TILE_ROWS / 16u; ++k) tc::mma_f16_tmem(tmem, from + k * 16u, b + k * 128u, ID, true);
-                }
+                    for (uint32_t k = 0; k < TILE_ROWS / 16u; ++k)
+                        tc::mma_f16_tmem(tmem, from + k * 16u, b + k * 128u, ID, k != 0 || t != group);
                 // db += dy^T ones.  Of an odd number of chunks the last tile's upper 64 outputs are whatever
                 // follows in shared memory; they are not read.
                 if (sums)
@@ -249,7 +241,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
 #pragma unroll
                             for (uint32_t k = 0; k < TILE_ROWS / 16u; ++k)
                                 tc::mma_f16(tmem + P::DB_AT + m * 16u, b + m * (2u * P::CHUNK >> 4) + k * 128u, ones, ID_DB,
-                                            t != group || k != 0);
+                                            k != 0 || t != group);
                 tc::commit(&s.empty[r.i]);
             }
             __syncwarp();
@@ -263,33 +255,41 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             constexpr uint32_t PARTS = TILE_ROWS / 32u, AHEAD = 8u / PARTS;
             tc::Ring r;
             bool ok = true;
-            const unsigned short *dy = (const unsigned short *)a.dy;
-            for (uint32_t t0 = group; t0 < a.tiles && ok; t0 += AHEAD * a.groups) {
-                uint32_t v[8][TINY_OUTS];
+            unsigned short v[8][TINY_OUTS] = {};
+            // a tile; rows behind the end repeat the last one here and become zero below
+            const auto load = [&](uint32_t t, unsigned short (*w)[TINY_OUTS]) {
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    const uint64_t row = (uint64_t)(t0 + i / PARTS * a.groups) * TILE_ROWS + i % PARTS * 32u + lane;
-                    const unsigned short *p = dy + row * a.dy_stride;
+                for (uint32_t j = 0; j < PARTS; ++j) {
+                    const uint64_t row = (uint64_t)t * TILE_ROWS + j * 32u + lane;
+                    const unsigned short *p = (const unsigned short *)a.dy + (row < a.rows ? row : a.rows - 1u) * a.dy_stride;
 #pragma unroll
-                    for (uint32_t o = 0; o < TINY_OUTS; ++o) v[i][o] = load16_if(p + o, row < a.rows && o < a.outs);
+                    for (uint32_t o = 0; o < TINY_OUTS; ++o)
+                        if (o < a.outs) w[j][o] = __ldg(p + o);
                 }
+            };
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; ++i) load(group + i * a.groups, v + i * PARTS);
+            for (uint32_t t0 = group; t0 < a.tiles && ok; t0 += AHEAD * a.groups)
 #pragma unroll
                 for (uint32_t i = 0; i < AHEAD; ++i) {
-                    if (t0 + i * a.groups >= a.tiles) break;
+                    const uint32_t t = t0 + i * a.groups;
+                    if (t >= a.tiles) break;
                     ok = ok && __all_sync(~0u, tc::mbar_wait(&s.empty[r.i], r.phase ^ 1u, fail, a.err));
                     if (!ok) break;
 #pragma unroll
                     for (uint32_t j = 0; j < PARTS; ++j) {
-                        const uint32_t *w = v[i * PARTS + j];
-                        *reinterpret_cast<uint4 *>(smem + r.i * P::STAGE + (j * 32u + lane) * 128u + ((lane & 7u) << 4)) =
-                            make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+                        const unsigned short *w = v[i * PARTS + j];
+                        const bool in = t + 1u < a.tiles || (uint64_t)t * TILE_ROWS + j * 32u + lane < a.rows;
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        if (in) x = make_uint4(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16, w[4] | (uint32_t)w[5] << 16, w[6] | (uint32_t)w[7] << 16);
+                        *reinterpret_cast<uint4 *>(smem + r.i * P::STAGE + (j * 32u + lane) * 128u + ((lane & 7u) << 4)) = x;
                     }
                     tc::fence_async_shared();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.full[r.i]);
                     r.next(P::STAGES);
+                    load(t + AHEAD * a.groups, v + i * PARTS);
                 }
-            }
         }
     } else if (warp >= 4) {  // activations: four sets of four warps take tiles in turn; a lane has a column of z (a
               // warp one block of 32) and ROWS rows of the tile
@@ -424,22 +424,38 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         }
         ok = __all_sync(~0u, ok && tc::mbar_wait(&s.done, 0, fail, a.err));
         tc::fence_after();
-        if (ok && a.dw_parts) {
-            float *out = a.dw_parts + ((uint64_t)group * a.slabs + slab) * (OC * 64u) * 128u + quad * 32u + lane;
+        // dW^T, 16 outputs at a time, to its part in memory or, of the only group, to dW
+        float *const fold = reinterpret_cast<float *>(smem) + (quad & 1u) * 32u + lane;  // the upper lanes' half: [output][64]
 #pragma unroll
-            for (uint32_t c = 0; c < OC; ++c) {
-                const uint32_t o0 = (set * OC + c) * 16u;
-                uint32_t v[16];
-                tc::tmem_load16(tmem + lanes + o0, v);
+        for (uint32_t c = 0; c < OC; ++c) {
+            const uint32_t o0 = (set * OC + c) * 16u;
+            uint32_t v[16];
+            if (ok && (a.dw_parts || a.dw)) tc::tmem_load16(tmem + lanes + o0, v);
+            if (ok && a.dw_parts) {
+                float *out = a.dw_parts + (((uint64_t)group * a.slabs + slab) * (OC * 64u) + o0) * 128u + quad * 32u + lane;
 #pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) out[(o0 + i) * 128u] = __uint_as_float(v[i]);
+                for (uint32_t i = 0; i < 16; ++i) out[i * 128u] = __uint_as_float(v[i]);
+            }
+            if (a.dw) {
+                if (FOLD) {
+                    if (ok && quad >= 2u)
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) fold[(o0 + i) * 64u] = __uint_as_float(v[i]);
+                    asm volatile("bar.sync 1, 512;" ::: "memory");  // the sixteen warps, failed or not
+                }
+                if (ok && n < a.cols && (!FOLD || quad < 2u))
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i)
+                        if (o0 + i < a.outs)
+                            ((T *)a.dw)[(uint64_t)(o0 + i) * a.cols + n] = from_f32<T>(__uint_as_float(v[i]) + (FOLD ? fold[(o0 + i) * 64u] : 0.0f));
             }
         }
         if (ok && sums && set < P::MT && set % sharers == slab) {  // a lane has an output; its 16 columns are equal
             uint32_t v[16];
             tc::tmem_load16(tmem + P::DB_AT + set * 16u + lanes, v);
             const uint32_t o = set * 128u + quad * 32u + lane;
-            if (o < OC * 64u) a.db_parts[(uint64_t)group * (OC * 64u) + o] = __uint_as_float(v[0]);
+            if (a.db_parts && o < OC * 64u) a.db_parts[(uint64_t)group * (OC * 64u) + o] = __uint_as_float(v[0]);
+            if (a.db && o < a.outs) ((T *)a.db)[o] = from_f32<T>(__uint_as_float(v[0]));
         }
     }
     __syncwarp();
@@ -685,10 +701,11 @@ __global__ void __launch_bounds__(256) activate_kernel(const int8_t *__restrict_
     }
 }
 
-// Column sums of dy in parts: a block takes 256 columns, 8 a lane, and every gridDim.y-th group of 8 rows.
+// Column sums of dy in parts: a block takes 256 columns, 8 a lane, and every gridDim.y-th group of 8 rows;
+// one part is the result.
 template <typename T>
 __global__ void __launch_bounds__(256) column_parts_kernel(const T *__restrict__ dy, uint64_t rows, uint32_t cols, uint64_t pitch,
-                                                           float *__restrict__ parts)
+                                                           float *__restrict__ parts, T *__restrict__ out)
 {
     __shared__ float sum[8][257];
     const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, col = blockIdx.x * 256u + lane * 8u;
@@ -714,7 +731,9 @@ __global__ void __launch_bounds__(256) column_parts_kernel(const T *__restrict__
     const uint32_t c = blockIdx.x * 256u + threadIdx.x;
     float total = 0.0f;
     for (int w = 0; w < 8; ++w) total += sum[w][threadIdx.x];
-    if (c < cols) parts[(uint64_t)blockIdx.y * cols + c] = total;
+    if (c >= cols) return;
+    if (gridDim.y == 1) out[c] = from_f32<T>(total);
+    else parts[(uint64_t)blockIdx.y * cols + c] = total;
 }
 
 // Column sums in one launch, for the rare matrix that no other kernel reads.
@@ -763,12 +782,14 @@ static NarrowPlan narrow_plan(uint64_t rows, uint32_t cols, uint32_t outs, int c
     const uint32_t tile_rows = narrow_rows(p.oc);
     p.tiles = (uint32_t)((rows + tile_rows - 1u) / tile_rows);
     // one CTA an SM; a slab more than there are SMs still gets its own
-    p.groups = p.slabs < sms ? sms / p.slabs : 1u;
+    // and few tiles are one group's: a CTA takes a tile every 0.4 us, less in all than a second kernel
+    p.groups = p.slabs < sms && p.tiles > 16u ? sms / p.slabs : 1u;
     if (p.groups > p.tiles) p.groups = p.tiles;
+    const bool parts = p.groups > 1u;
     p.part_outs = p.oc * 64u;
     p.dw_at = 0;
-    p.db_at = p.dw_at + align_up((uint64_t)p.groups * p.slabs * 128u * p.part_outs * 4u, 256);
-    p.dy_at = p.db_at + align_up((uint64_t)p.groups * p.part_outs * 4u, 256);
+    p.db_at = p.dw_at + (parts ? align_up((uint64_t)p.groups * p.slabs * 128u * p.part_outs * 4u, 256) : 0);
+    p.dy_at = p.db_at + (parts ? align_up((uint64_t)p.groups * p.part_outs * 4u, 256) : 0);
     p.bytes = p.dy_at + (copies & COPY_DY && outs > TINY_OUTS ? align_up(rows * align_up(outs, 8) * 2u, 256) : 0);
     return p;
 }
@@ -823,8 +844,11 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     a.codes = codes;
     a.exps = exps;
     a.dz = dz;
-    a.dw_parts = dw ? (float *)(workspace + p.dw_at) : nullptr;
-    a.db_parts = db ? (float *)(workspace + p.db_at) : nullptr;
+    const bool parts = p.groups > 1u;
+    a.dw_parts = dw && parts ? (float *)(workspace + p.dw_at) : nullptr;
+    a.db_parts = db && parts ? (float *)(workspace + p.db_at) : nullptr;
+    a.dw = parts ? nullptr : dw;
+    a.db = parts ? nullptr : db;
     a.err = err;
     vt_status s = VT_OK;
     switch (p.oc * 2u + p.fold) {
@@ -837,7 +861,7 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     case 8: s = launch_narrow<T, ACT, 4, false>(dy_map, a, stream); break;
     default: s = launch_narrow<T, ACT, 4, true>(dy_map, a, stream); break;
     }
-    if (s || !(dw || db)) return s;
+    if (s || !parts || !(dw || db)) return s;
     const uint64_t n = (uint64_t)p.slabs * 128u * p.part_outs;
     narrow_reduce_kernel<T><<<(unsigned)((n + 255u) / 256u), 256, 0, stream>>>(a.dw_parts, a.db_parts, p.groups, p.slabs, p.part_outs,
                                                                            p.fold, cols, outs, (T *)dw, (T *)db);
@@ -936,8 +960,9 @@ static vt_status run_wide(const void *dy, uint64_t dy_stride, const void *w, uin
     }
     if (db) {
         float *parts = (float *)(workspace + p.db_at);
-        column_parts_kernel<T><<<dim3((outs + 255u) / 256u, p.sum_parts), 256, 0, stream>>>((const T *)dy, rows, outs, dy_stride, parts);
-        add_parts_kernel<T><<<(outs + 255u) / 256u, 256, 0, stream>>>(parts, p.sum_parts, outs, (T *)db);
+        column_parts_kernel<T><<<dim3((outs + 255u) / 256u, p.sum_parts), 256, 0, stream>>>((const T *)dy, rows, outs, dy_stride, parts,
+                                                                                                  (T *)db);
+        if (p.sum_parts > 1) add_parts_kernel<T><<<(outs + 255u) / 256u, 256, 0, stream>>>(parts, p.sum_parts, outs, (T *)db);
         if (vt_status s = check_launch("column_parts_kernel")) return s;
     }
     return VT_OK;
