@@ -159,28 +159,35 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// 16 columns of a row from packed pairs.  wide: the row starts on 32 bytes and holds whole
-// 32-byte pieces, which are whole sectors of L2.
-template <typename T>
-__device__ __forceinline__ void store_row16(T *row, uint32_t col, uint32_t cols, bool wide, const uint32_t *w)
+// 32 columns of a row from packed pairs, for rows that start on 32 bytes and hold whole 32-byte pieces,
+// which are whole sectors of L2.
+template <typename T> __device__ __forceinline__ void store_row32(T *row, uint32_t col, uint32_t cols, const uint32_t *w)
 {
-    T *p = row + col;
-    if (wide) {
-        if (col < cols) store32(p, w);
-    } else {
+    if (col < cols) store32(row + col, w);
+    if (col + 16u < cols) store32(row + col + 16u, w + 8);
+}
+// The same for any rows: a warp's 32 rows by 32 columns (a lane a row of packed pairs) turned in shared memory, so
+// that a row's 32 columns are one access.  (A lane storing its own row's columns touches 32 rows an access: 277867 x 195
+// in bfloat16 took 557 us that way.)  `rows` of the 32 exist; out is the first one, a matrix of `cols` columns.
+constexpr uint32_t TURN_WORDS = 32u * 17u;
+template <typename T>
+__device__ __forceinline__ void store_turned(T *out, uint32_t rows, uint32_t col, uint32_t cols, const uint32_t *w, uint32_t *turn)
+{
+    const uint32_t lane = threadIdx.x & 31u;
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            const float2 v = unpack2<T>(w[i]);
-            if (col + 2 * i < cols) p[2 * i] = from_f32<T>(v.x);
-            if (col + 2 * i + 1 < cols) p[2 * i + 1] = from_f32<T>(v.y);
+    for (uint32_t i = 0; i < 16; ++i) turn[lane * 17u + i] = w[i];
+    __syncwarp();
+    const unsigned short *from = reinterpret_cast<const unsigned short *>(turn) + lane;
+    unsigned short *to = reinterpret_cast<unsigned short *>(out) + col + lane;
+    if (col + lane < cols) {
+        if (rows == 32u) {
+#pragma unroll 8
+            for (uint32_t r = 0; r < 32; ++r) to[(uint64_t)r * cols] = from[r * 34u];
+        } else {
+            for (uint32_t r = 0; r < rows; ++r) to[(uint64_t)r * cols] = from[r * 34u];
         }
     }
-}
-template <typename T>
-__device__ __forceinline__ void store_row32(T *row, uint32_t col, uint32_t cols, bool wide, const uint32_t *w)
-{
-    store_row16<T>(row, col, cols, wide, w);
-    store_row16<T>(row, col + 16u, cols, wide, w + 8);
+    __syncwarp();
 }
 
 // ---- formats ----

@@ -53,6 +53,7 @@ template <int TN> struct L4 {
         uint32_t tmem;
         tc::Fail fail;
         alignas(8) float bias[TN];
+        uint32_t turn[4][TURN_WORDS];
     };
     static constexpr uint32_t X_AT = STAGES * STAGE, CTRL_AT = X_AT + X_STAGES * X_BYTES, SMEM = CTRL_AT + sizeof(Ctrl);
     static_assert(SMEM <= 232448 && TMEM_USED <= 512, "does not fit an SM");
@@ -116,16 +117,25 @@ template <typename T> __device__ __forceinline__ uint4 block_codes(const uint4 *
     return make_uint4(codes[0], codes[1], codes[2], codes[3]);
 }
 
-// Columns col..col + 31 of a row of y from sums and bias.
+// Columns col..col + 31 of a warp's 32 rows of y, a lane a row, from sums and bias.  y: the warp's first row, of which
+// `rows` of the 32 exist.
 template <typename T, int ACT>
-__device__ __forceinline__ void store_results(T *row, uint32_t col, uint32_t cols, bool wide, const uint32_t *v, const float *bias)
+__device__ __forceinline__ void store_results(T *y, uint32_t rows, uint32_t col, uint32_t cols, bool wide, const uint32_t *v, const float *bias,
+                                              uint32_t *turn)
 {
     uint32_t w[16];
 #pragma unroll
     for (uint32_t i = 0; i < 16; ++i)
         w[i] = pack2<T>(act_value2<ACT>(add2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])),
                                              *reinterpret_cast<const f32x2 *>(bias + 2 * i))));
-    store_row32<T>(row, col, cols, wide, w);
+    const uint32_t lane = threadIdx.x & 31u;
+    if (!wide) store_turned<T>(y, rows, col, cols, w, turn);
+    else if (lane < rows) store_row32<T>(y + (uint64_t)lane * cols, col, cols, w);
+}
+// Rows of 32 from `row` on
+__device__ __forceinline__ uint32_t rows_left(uint64_t row, uint64_t rows)
+{
+    return row >= rows ? 0u : rows - row < 32u ? (uint32_t)(rows - row) : 32u;
 }
 
 // A stage's scales to tensor memory and its products, by one lane: `steps` of 64 steps of k, 4 but
@@ -245,7 +255,7 @@ __global__ void __launch_bounds__(L4<TN>::THREADS, 1)
         asm volatile("bar.sync 1, 128;" ::: "memory");
         tc::Ring acc;
         for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-            const uint64_t row = (uint64_t)t * L4_ROWS + in_tile;
+            const uint64_t row = (uint64_t)t * L4_ROWS + quad * 32u;  // the warp's first
             const bool ok = tc::mbar_wait(&s.acc_full[acc.i], acc.phase, fail, a.err);
             if (!__all_sync(~0u, ok)) break;
             tc::fence_after();
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(L4<TN>::THREADS, 1)
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.acc_empty[acc.i]);
                 }
-                if (row < a.rows) store_results<T, ACT>((T *)a.y + row * a.outs, n0, a.outs, a.y_wide, v, s.bias + n0);
+                store_results<T, ACT>((T *)a.y + row * a.outs, rows_left(row, a.rows), n0, a.outs, a.y_wide, v, s.bias + n0, s.turn[quad]);
             }
             acc.next(P::ACCS);
         }
@@ -363,6 +373,7 @@ struct PairCtrl {
     uint32_t tmem;
     tc::Fail fail;
     alignas(8) float bias[PAIR_N];
+    uint32_t turn[4][TURN_WORDS];
 };
 constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + sizeof(PairCtrl);
 static_assert(PAIR_SMEM <= 232448 && PAIR_SF_AT + 2 * PAIR_SF_COLS <= 512, "does not fit an SM");
@@ -538,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         const uint32_t quad = warp % 4u, in_tile = quad * 32u + lane;
         tc::Ring acc;
         for (uint32_t t = first; t < tiles; t += step) {
-            const uint64_t row = (uint64_t)(t / a.out_tiles) * 256u + rank * 128u + in_tile;
+            const uint64_t row = (uint64_t)(t / a.out_tiles) * 256u + rank * 128u + quad * 32u;  // the warp's first
             const uint32_t out0 = t % a.out_tiles * PAIR_N;
             // the bias of the tile's outputs; the first barrier keeps the last tile's until it is used
             asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -557,7 +568,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                         __syncwarp();
                         if (lane == 0) tc::mbar_arrive_cluster(tc::leader_addr(&s.acc_empty[acc.i]));
                     }
-                    if (row < a.rows) store_results<T, ACT>((T *)a.y + row * a.outs, out0 + n0, a.outs, a.y_wide, v, s.bias + n0);
+                    store_results<T, ACT>((T *)a.y + row * a.outs, rows_left(row, a.rows), out0 + n0, a.outs, a.y_wide, v, s.bias + n0,
+                                          s.turn[quad]);
                 }
             }
             acc.next(2);

@@ -502,6 +502,7 @@ struct WideCtrl {
     uint64_t full[WIDE_STAGES], empty[WIDE_STAGES], acc_full[2], acc_empty[2], failed;
     uint32_t tmem;
     tc::Fail fail;
+    uint32_t turn[4][TURN_WORDS];
 };
 constexpr uint32_t WIDE_SMEM = WIDE_STAGES * WIDE_STAGE_BYTES + sizeof(WideCtrl);
 
@@ -646,15 +647,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive_cluster(tc::leader_addr(&s.acc_empty[acc.i]));
                 }
-                if (row >= a.m) continue;
-                if (DZ) {
-                    const f32x2 sc = both(mx8_scale(E));
-                    slope16<T, ACT>(codes, sc, v, w);
-                    slope16<T, ACT>(codes + 4, sc, v + 16, w + 8);
-                    store_row32<T>((T *)a.out + row * a.n, col, (uint32_t)a.n, a.out_wide, w);
-                } else if (a.splits > 1) {
+                if (!DZ && a.splits > 1) {  // parts: 8 columns at a time if the rows allow it
                     float *p = a.parts + ((uint64_t)split * a.m + row) * a.n + col;
-                    if (a.n % 8u == 0) {
+                    if (row >= a.m) {
+                    } else if (a.n % 8u == 0) {
 #pragma unroll
                         for (uint32_t i = 0; i < 4; ++i)
                             if (col + 8u * i < a.n) store32(p + 8u * i, v + 8 * i);
@@ -663,10 +659,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1)
                         for (uint32_t i = 0; i < 32; ++i)
                             if (col + i < a.n) p[i] = __uint_as_float(v[i]);
                     }
+                    continue;
+                }
+                if (DZ) {
+                    const f32x2 sc = both(mx8_scale(E));
+                    slope16<T, ACT>(codes, sc, v, w);
+                    slope16<T, ACT>(codes + 4, sc, v + 16, w + 8);
                 } else {
 #pragma unroll
                     for (uint32_t i = 0; i < 16; ++i) w[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                    store_row32<T>((T *)a.out + row * a.n, col, (uint32_t)a.n, a.out_wide, w);
+                }
+                const uint64_t row0 = row - lane;  // the warp's first
+                if (a.out_wide) {
+                    if (row < a.m) store_row32<T>((T *)a.out + row * a.n, col, (uint32_t)a.n, w);
+                } else {
+                    store_turned<T>((T *)a.out + row0 * a.n, row0 >= a.m ? 0u : (uint32_t)min((unsigned long long)(a.m - row0), 32ull), col,
+                                    (uint32_t)a.n, w, s.turn[quad]);
                 }
             }
             acc.next(2);
@@ -884,7 +892,8 @@ static WidePlan wide_plan(uint64_t rows, uint32_t cols, uint32_t outs, int copie
     p.splits = (uint32_t)(room < most ? room : most);
     p.chunks_a_split = (chunks + p.splits - 1u) / p.splits;
     p.splits = (chunks + p.chunks_a_split - 1u) / p.chunks_a_split;
-    p.sum_parts = (uint32_t)((rows + 255u) / 256u < 32u ? (rows + 255u) / 256u : 32u);
+    const uint64_t most_parts = 2u * sms / ((outs + 255u) / 256u) + 1u;  // two blocks an SM
+    p.sum_parts = (uint32_t)((rows + 255u) / 256u < most_parts ? (rows + 255u) / 256u : most_parts);
     p.h_at = 0;
     p.dw_at = p.h_at + align_up(rows * align_up(cols, 8) * 2u, 256);
     p.db_at = p.dw_at + (p.splits > 1 ? align_up((uint64_t)p.splits * outs * cols * 4u, 256) : 0);
