@@ -710,29 +710,48 @@ __global__ void __launch_bounds__(256) activate_kernel(const int8_t *__restrict_
 }
 
 // Column sums of dy in parts: a block takes 256 columns, 8 a lane, and every gridDim.y-th group of 8 rows;
-// one part is the result.
+// one part is the result.  `readable` of a row's columns may be loaded: a copy's zeros make its last word whole.
 template <typename T>
-__global__ void __launch_bounds__(256) column_parts_kernel(const T *__restrict__ dy, uint64_t rows, uint32_t cols, uint64_t pitch,
-                                                           float *__restrict__ parts, T *__restrict__ out)
+__global__ void __launch_bounds__(256) column_parts_kernel(const T *__restrict__ dy, uint64_t rows, uint32_t cols, uint32_t readable,
+                                                           uint64_t pitch, float *__restrict__ parts, T *__restrict__ out)
 {
     __shared__ float sum[8][257];
     const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, col = blockIdx.x * 256u + lane * 8u;
     float v[8] = {};
-    if (col < cols)
-        for (uint64_t row = blockIdx.y * 8u + warp; row < rows; row += gridDim.y * 8u) {
-            Vec8<T> x;
-            float f[8];
-            const T *p = dy + row * pitch + col;
-            if (col + 8u <= cols) {
-                x.load(p);
-            } else {
-                x.zero();
-                for (uint32_t i = 0; i < cols - col; ++i) reinterpret_cast<T *>(x.w)[i] = p[i];
-            }
-            x.unpack(f);
+    const uint32_t step = gridDim.y * 8u, have = col >= readable ? 0u : readable - col < 8u ? readable - col : 8u;
+    const auto add = [&](const Vec8<T> &x) {
+        float f[8];
+        x.unpack(f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += f[i];
+        for (int i = 0; i < 8; ++i) v[i] += f[i];
+    };
+    const auto load = [&](Vec8<T> &x, const T *p) {
+        if (have == 8u) {
+            x.load(p);
+        } else {
+            x.zero();
+#pragma unroll
+            for (uint32_t i = 0; i < 7; ++i)
+                if (i < have) reinterpret_cast<T *>(x.w)[i] = p[i];
         }
+    };
+    uint64_t row = blockIdx.y * 8u + warp;
+    const T *p = dy + row * pitch + col;
+    if (have) {
+        // four rows' loads before the first sum
+        for (; row + 3ull * step < rows; row += 4ull * step, p += 4ull * step * pitch) {
+            Vec8<T> x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load(x[i], p + (uint64_t)i * step * pitch);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) add(x[i]);
+        }
+        for (; row < rows; row += step, p += (uint64_t)step * pitch) {
+            Vec8<T> x;
+            load(x, p);
+            add(x);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[warp][lane * 8u + i] = v[i];
     __syncthreads();
@@ -766,7 +785,7 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float *__restrict_
 {
     for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256u) {
         float v = 0.0f;
-#pragma unroll 4
+#pragma unroll 16  // loads under way at once: few threads, many parts
         for (uint32_t p = 0; p < count; ++p) v += __ldg(parts + p * n + i);
         out[i] = from_f32<T>(v);
     }
@@ -931,6 +950,7 @@ static vt_status run_wide(const void *dy, uint64_t dy_stride, const void *w, uin
     a.codes = codes;
     a.exps = exps;
     a.err = err;
+    const uint32_t readable = dy == workspace + p.dy_at ? (uint32_t)dy_stride : outs;
     CUtensorMap ma, mb;
     if (dz) {
         if (vt_status s = whole_rows<T>(w, w_stride, outs, cols, workspace + p.w_at, stream)) return s;
@@ -969,8 +989,8 @@ static vt_status run_wide(const void *dy, uint64_t dy_stride, const void *w, uin
     }
     if (db) {
         float *parts = (float *)(workspace + p.db_at);
-        column_parts_kernel<T><<<dim3((outs + 255u) / 256u, p.sum_parts), 256, 0, stream>>>((const T *)dy, rows, outs, dy_stride, parts,
-                                                                                                  (T *)db);
+        column_parts_kernel<T><<<dim3((outs + 255u) / 256u, p.sum_parts), 256, 0, stream>>>((const T *)dy, rows, outs, readable, dy_stride, parts,
+                                                                                             (T *)db);
         if (p.sum_parts > 1) add_parts_kernel<T><<<(outs + 255u) / 256u, 256, 0, stream>>>(parts, p.sum_parts, outs, (T *)db);
         if (vt_status s = check_launch("column_parts_kernel")) return s;
     }

@@ -16,8 +16,8 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const T *__restrict__ src
     const uint32_t words = pitch / 8u;
     const uint64_t n = rows * words;
     for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256u) {
-        const uint64_t row = i / words;
-        const uint32_t col = (uint32_t)(i % words) * 8u;
+        const uint64_t row = n >> 32 ? i / words : (uint32_t)i / words;  // a 64-bit division takes some hundred instructions
+        const uint32_t col = (uint32_t)(i - row * words) * 8u;
         const T *p = src + row * stride + col;
         Vec8<T> v;
         T *e = reinterpret_cast<T *>(v.w);
