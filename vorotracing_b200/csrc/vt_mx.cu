@@ -12,8 +12,6 @@
 // of 6.45; 4 bits and back on 1000000 x 192 binary32: 310 us, 5.6 TB/s.  The exponential and the reciprocal
 // of an activation share a pipe of 16 lanes an SM, which is half busy: conversions are kept off it.  Two
 // items a thread in flight cost registers and were slower (186 us); so was a grid without a loop (151 us).
-// Rows of odd widths are read and written a column at a time: 25842 x 1929 in binary16 245 us a step, three
-// times the floor (a block a warp, a column a lane, measured 255 us).
 #include "vt_mx.cuh"
 
 namespace vt {
@@ -23,61 +21,141 @@ struct MxShape {
     uint64_t rows;
     uint32_t cols, blocks;  // blocks a row
     uint64_t in_stride, out_stride;
-    bool vec;  // rows start on 16 bytes and hold whole groups of 8 columns
+    int word;  // bytes of the words that rows start on and hold whole (16, 8, 4 or an element's), or TURNED
     __host__ __device__ uint64_t items() const { return rows * blocks * 4u; }
 };
 
-struct MxItem {
+// The row and the block in it that count blocks into the matrix lie at
+__device__ __forceinline__ void mx_place(const MxShape &s, uint64_t block, uint64_t &row, uint32_t &in_row)
+{
+    row = block >> 32 ? block / s.blocks : (uint32_t)block / s.blocks;
+    in_row = (uint32_t)(block - row * s.blocks);
+}
+
+// The 8 columns of an item, for a lane: as words of WORD bytes, as many as the row has.  Rows that only single elements
+// divide are TURNED in shared memory if they are long: the warp's 8 blocks of 32 columns are read and written a block an
+// access, a column a lane, where a lane that touched its own 8 columns would have every access cover 16 to 32 sectors
+// (checkpoint and gradient of 25842 x 1929 in binary16: 156 us turned, 247 by elements).  In rows of few blocks the steps
+// from row to row cost more than that saves (1500000 x 3 in binary32: 191 us turned, 85 by elements; 100000 x 257 in
+// bfloat16, nine blocks: 129 either way).
+constexpr int TURNED = 0;
+constexpr uint32_t TURN_BLOCKS = 9;
+template <int WORD> struct MxTurn { float4 w[WORD == TURNED ? 8 : 1][64]; };
+template <int WORD> struct MxWord;
+template <> struct MxWord<16> { using type = uint4; };
+template <> struct MxWord<8> { using type = uint2; };
+template <> struct MxWord<4> { using type = uint32_t; };
+template <> struct MxWord<2> { using type = unsigned short; };
+
+// Whether whole items are told from ragged ones, or each word has its condition: measured, checkpoint and gradient then 4 bits
+// and back, 200000 x 65 in binary32 63 and 42 us against 62 and 71, 500000 x 100 in bfloat16 133 and 89 against 125 and 84.
+template <int WORD, typename T> constexpr bool mx_whole_first = WORD == 16 || sizeof(T) == 4;
+
+// Calls f(i, offset, whether it exists) for the warp's 8 blocks, a column a lane, with offsets into a matrix of that row
+// stride.  Steps instead of products, and none inside a row: instructions bound the rows read this way.
+template <typename F>
+__device__ __forceinline__ void mx_blocks_of_warp(const MxShape &s, uint64_t t, uint64_t stride, const F &f)
+{
+    const uint32_t lane = threadIdx.x & 31u, last = s.blocks - 1u, tail = s.cols - last * 32u;
+    const uint64_t first = t >> 5 << 3;
     uint64_t row;
-    uint32_t col, n;  // first column, columns inside the row (0..8)
-};
-
-__device__ __forceinline__ MxItem mx_item(const MxShape &s, uint64_t t)
-{
-    const uint32_t per_row = s.blocks * 4u;
-    MxItem it;
     uint32_t in_row;
-    if (t >> 32) {
-        it.row = t / per_row;
-        in_row = (uint32_t)(t % per_row);
-    } else {
-        it.row = (uint32_t)t / per_row;
-        in_row = (uint32_t)t % per_row;
-    }
-    it.col = in_row * 8u;
-    it.n = it.col >= s.cols ? 0u : min(8u, s.cols - it.col);
-    return it;
-}
-
-template <typename T>
-__device__ __forceinline__ void mx_load(const MxShape &s, const MxItem &it, const T *p, uint64_t stride,
-                                        float *v)
-{
-    p += it.row * stride + it.col;
-    if (s.vec) {
-        Vec8<T> w;
-        if (it.n) w.load(p); else w.zero();
-        w.unpack(v);
-    } else {
+    mx_place(s, first, row, in_row);
+    uint64_t at = row * stride + in_row * 32u + lane;
+    if (in_row + 8u <= last) {
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) v[i] = i < it.n ? to_f32<T>(__ldg(p + i)) : 0.0f;
+        for (uint32_t i = 0; i < 8; ++i) f(i, at + i * 32u, true);
+    } else {
+        const uint64_t after = s.rows * s.blocks - first, to_next = stride - last * 32u;
+        const uint32_t left = after < 8u ? (uint32_t)after : 8u;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const bool ends = in_row == last;
+            f(i, at, i < left && (!ends || lane < tail));
+            at += ends ? to_next : 32u;
+            in_row = ends ? 0u : in_row + 1u;
+        }
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void mx_store(const MxShape &s, const MxItem &it, T *p, const float *v)
+// Zeros for columns that do not exist.  Called by whole warps if TURNED.
+template <int WORD, typename T>
+__device__ __forceinline__ void mx_load(const MxShape &s, uint64_t t, const T *p, float *v, MxTurn<WORD> &turn)
 {
-    p += it.row * s.out_stride + it.col;
-    if (s.vec) {
-        if (!it.n) return;
-        Vec8<T> w;
-        w.pack(v);
-        w.store(p);
-    } else {
+    if constexpr (WORD == TURNED) {
+        const uint32_t lane = threadIdx.x & 31u;
+        float x[8];
+        mx_blocks_of_warp(s, t, s.in_stride, [&](uint32_t i, uint64_t at, bool is) { x[i] = is ? to_f32<T>(__ldg(p + at)) : 0.0f; });
+        float4 *w = turn.w[threadIdx.x / 32u];
+        __syncwarp();
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i)
-            if (i < it.n) p[i] = from_f32<T>(v[i]);
+        for (uint32_t i = 0; i < 8; ++i) reinterpret_cast<float *>(w)[i * 32u + lane] = x[i];
+        __syncwarp();
+        *reinterpret_cast<float4 *>(v) = w[lane * 2u];
+        *reinterpret_cast<float4 *>(v + 4) = w[lane * 2u + 1u];
+    } else {
+        using W = typename MxWord<WORD>::type;
+        constexpr uint32_t EACH = WORD / sizeof(T);
+        constexpr bool WHOLE_FIRST = mx_whole_first<WORD, T>;
+        uint64_t row;
+        uint32_t in_row;
+        mx_place(s, t >> 2, row, in_row);
+        const uint32_t col = in_row * 32u + (uint32_t)(t & 3u) * 8u, have = col < s.cols ? s.cols - col : 0u;
+        const W *q = reinterpret_cast<const W *>(p + row * s.in_stride + col);
+        alignas(16) W w[8u / EACH];
+        if (WHOLE_FIRST && have >= 8u) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u / EACH; ++i) w[i] = __ldg(q + i);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u / EACH; ++i) w[i] = i * EACH < have ? __ldg(q + i) : W();
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) v[i] = to_f32<T>(reinterpret_cast<const T *>(w)[i]);
     }
+}
+
+// Called by whole warps if TURNED
+template <int WORD, typename T>
+__device__ __forceinline__ void mx_store(const MxShape &s, uint64_t t, T *p, const float *v, MxTurn<WORD> &turn)
+{
+    if constexpr (WORD == TURNED) {
+        const uint32_t lane = threadIdx.x & 31u;
+        float4 *w = turn.w[threadIdx.x / 32u];
+        __syncwarp();
+        w[lane * 2u] = make_float4(v[0], v[1], v[2], v[3]);
+        w[lane * 2u + 1u] = make_float4(v[4], v[5], v[6], v[7]);
+        __syncwarp();
+        mx_blocks_of_warp(s, t, s.out_stride, [&](uint32_t i, uint64_t at, bool is) {
+            if (is) p[at] = from_f32<T>(reinterpret_cast<const float *>(w)[i * 32u + lane]);
+        });
+    } else {
+        using W = typename MxWord<WORD>::type;
+        constexpr uint32_t EACH = WORD / sizeof(T);
+        constexpr bool WHOLE_FIRST = mx_whole_first<WORD, T>;
+        uint64_t row;
+        uint32_t in_row;
+        mx_place(s, t >> 2, row, in_row);
+        const uint32_t col = in_row * 32u + (uint32_t)(t & 3u) * 8u, have = col < s.cols ? s.cols - col : 0u;
+        W *q = reinterpret_cast<W *>(p + row * s.out_stride + col);
+        alignas(16) W w[8u / EACH];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) reinterpret_cast<T *>(w)[i] = from_f32<T>(v[i]);
+        if (WHOLE_FIRST && have >= 8u) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u / EACH; ++i) q[i] = w[i];
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u / EACH; ++i)
+                if (i * EACH < have) q[i] = w[i];
+        }
+    }
+}
+
+// Whether a thread's loop goes on at item t.  A warp that turns goes on as one, past the last item with it.
+template <int WORD> __device__ __forceinline__ bool mx_goes_on(uint64_t t, uint64_t items)
+{
+    return (WORD == TURNED ? t & ~31ull : t) < items;
 }
 
 // Bits of the largest magnitude of the block that this lane and its three neighbours share.
@@ -93,31 +171,33 @@ __device__ __forceinline__ uint32_t block_top(const float *v)
     return max(top, __shfl_xor_sync(lanes, top, 2));
 }
 
-template <typename T, int ACT>
+template <int WORD, typename T, int ACT>
 __global__ void __launch_bounds__(256) mx8_checkpoint_kernel(MxShape s, const T *__restrict__ z,
                                                              T *__restrict__ h, int8_t *__restrict__ codes,
                                                              uint8_t *__restrict__ exps)
 {
+    __shared__ MxTurn<WORD> turn;
     const uint64_t items = s.items();
-    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; t < items; t += (uint64_t)gridDim.x * 256u) {
-        const MxItem it = mx_item(s, t);
-        float v[8];
-        mx_load(s, it, z, s.in_stride, v);
+    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; mx_goes_on<WORD>(t, items); t += (uint64_t)gridDim.x * 256u) {
+        alignas(16) float v[8];
+        mx_load<WORD>(s, t, z, v, turn);
         const uint32_t E = mx8_exponent(block_top(v));
         const f32x2 inv = both(mx8_inverse(E));
         f32x2 p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
         const uint2 c = make_uint2(mx8_codes(p[0], p[1], inv), mx8_codes(p[2], p[3], inv));
-        reinterpret_cast<uint2 *>(codes)[t] = E == 255u ? make_uint2(0, 0) : c;
-        if ((t & 3u) == 0) exps[t >> 2] = (uint8_t)E;
+        if (WORD != TURNED || t < items) {
+            reinterpret_cast<uint2 *>(codes)[t] = E == 255u ? make_uint2(0, 0) : c;
+            if ((t & 3u) == 0) exps[t >> 2] = (uint8_t)E;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 a = unpair(act_value2<ACT>(p[i]));
             v[2 * i] = a.x;
             v[2 * i + 1] = a.y;
         }
-        mx_store(s, it, h, v);
+        mx_store<WORD>(s, t, h, v, turn);
     }
 }
 
@@ -130,77 +210,83 @@ __device__ __forceinline__ void mx8_values(const int8_t *codes, const uint8_t *e
     for (int i = 0; i < 4; ++i) v[i] = mul2(code_pair((i < 2 ? c.x : c.y) ^ 0x80808080u, i % 2 * 2), sc);
 }
 
-template <typename T, int ACT>
+template <int WORD, typename T, int ACT>
 __global__ void __launch_bounds__(256) mx8_act_bwd_kernel(MxShape s, const T *__restrict__ dh,
                                                           const int8_t *__restrict__ codes,
                                                           const uint8_t *__restrict__ exps, T *__restrict__ dz)
 {
+    __shared__ MxTurn<WORD> turn;
     const uint64_t items = s.items();
-    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; t < items; t += (uint64_t)gridDim.x * 256u) {
-        const MxItem it = mx_item(s, t);
-        float g[8];
+    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; mx_goes_on<WORD>(t, items); t += (uint64_t)gridDim.x * 256u) {
+        alignas(16) float g[8];
         f32x2 v[4];
-        mx_load(s, it, dh, s.in_stride, g);
-        mx8_values(codes, exps, t, v);
+        mx_load<WORD>(s, t, dh, g, turn);
+        mx8_values(codes, exps, WORD != TURNED || t < items ? t : 0u, v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 a = unpair(mul2(pair(g[2 * i], g[2 * i + 1]), act_slope2<ACT>(v[i])));
             g[2 * i] = a.x;
             g[2 * i + 1] = a.y;
         }
-        mx_store(s, it, dz, g);
+        mx_store<WORD>(s, t, dz, g, turn);
     }
 }
 
-template <typename T>
+template <int WORD, typename T>
 __global__ void __launch_bounds__(256) mx8_dequantize_kernel(MxShape s, const int8_t *__restrict__ codes,
                                                              const uint8_t *__restrict__ exps, T *__restrict__ out)
 {
+    __shared__ MxTurn<WORD> turn;
     const uint64_t items = s.items();
-    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; t < items; t += (uint64_t)gridDim.x * 256u) {
+    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; mx_goes_on<WORD>(t, items); t += (uint64_t)gridDim.x * 256u) {
         f32x2 p[4];
         float v[8];
-        mx8_values(codes, exps, t, p);
+        mx8_values(codes, exps, WORD != TURNED || t < items ? t : 0u, p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 a = unpair(p[i]);
             v[2 * i] = a.x;
             v[2 * i + 1] = a.y;
         }
-        mx_store(s, mx_item(s, t), out, v);
+        mx_store<WORD>(s, t, out, v, turn);
     }
 }
 
-template <typename T>
+template <int WORD, typename T>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(MxShape s, const T *__restrict__ x,
                                                            uint32_t *__restrict__ codes, uint8_t *__restrict__ exps)
 {
+    __shared__ MxTurn<WORD> turn;
     const uint64_t items = s.items();
-    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; t < items; t += (uint64_t)gridDim.x * 256u) {
-        float v[8];
-        mx_load(s, mx_item(s, t), x, s.in_stride, v);
+    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; mx_goes_on<WORD>(t, items); t += (uint64_t)gridDim.x * 256u) {
+        alignas(16) float v[8];
+        mx_load<WORD>(s, t, x, v, turn);
         const uint32_t E = mx4_exponent(block_top(v));
         const float inv = mx4_inverse(E == 255u ? 1u : E);
         f32x2 p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = mul2(pair(v[2 * i], v[2 * i + 1]), both(inv));
-        codes[t] = E == 255u ? 0u : mx4_word(p);
-        if ((t & 3u) == 0) exps[t >> 2] = (uint8_t)E;
+        if (WORD != TURNED || t < items) {
+            codes[t] = E == 255u ? 0u : mx4_word(p);
+            if ((t & 3u) == 0) exps[t >> 2] = (uint8_t)E;
+        }
     }
 }
 
-template <typename T>
+template <int WORD, typename T>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(MxShape s, const uint32_t *__restrict__ codes,
                                                              const uint8_t *__restrict__ exps, T *__restrict__ out)
 {
+    __shared__ MxTurn<WORD> turn;
     const uint64_t items = s.items();
-    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; t < items; t += (uint64_t)gridDim.x * 256u) {
-        const uint32_t c = __ldg(codes + t);
-        const float sc = mx4_scale(__ldg(exps + (t >> 2)));
+    for (uint64_t t = (uint64_t)blockIdx.x * 256u + threadIdx.x; mx_goes_on<WORD>(t, items); t += (uint64_t)gridDim.x * 256u) {
+        const uint64_t at = WORD != TURNED || t < items ? t : 0u;
+        const uint32_t c = __ldg(codes + at);
+        const float sc = mx4_scale(__ldg(exps + (at >> 2)));
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = mx4_value(c >> (4 * i) & 15u) * sc;
-        mx_store(s, mx_item(s, t), out, v);
+        mx_store<WORD>(s, t, out, v, turn);
     }
 }
 
@@ -214,10 +300,22 @@ static MxShape mx_shape(uint64_t rows, uint32_t cols, const void *in, uint64_t i
     s.blocks = mx_blocks(cols);
     s.in_stride = in_stride;
     s.out_stride = out_stride;
-    const uint32_t group = 16u / sizeof(T);
-    s.vec = cols % 8u == 0 && in_stride % group == 0 && out_stride % group == 0 && aligned16(in) &&
-            aligned16(out);
+    const uint64_t all = cols * sizeof(T) | in_stride * sizeof(T) | out_stride * sizeof(T) | (uintptr_t)in | (uintptr_t)out;
+    s.word = all % 16u == 0 ? 16 : all % 8u == 0 ? 8 : all % 4u == 0 ? 4 : 2;
+    if (s.word == (int)sizeof(T) && s.blocks >= TURN_BLOCKS) s.word = TURNED;
     return s;
+}
+
+// f with the word's size as a type
+template <typename T, typename F> static vt_status with_word(const MxShape &s, F &&f)
+{
+    if (s.word == 16) return f(std::integral_constant<int, 16>());
+    if (s.word == 8) return f(std::integral_constant<int, 8>());
+    if (s.word == TURNED) return f(std::integral_constant<int, TURNED>());
+    if constexpr (sizeof(T) == 2) {
+        if (s.word == 2) return f(std::integral_constant<int, 2>());
+    }
+    return f(std::integral_constant<int, 4>());
 }
 
 static unsigned mx_grid(const MxShape &s)
@@ -245,9 +343,11 @@ extern "C" vt_status vt_mx8_checkpoint(const void *z, int dtype, uint64_t rows, 
         using T = typename decltype(ty)::type;
         return vt::with_act(act, [&](auto a) {
             const vt::MxShape s = vt::mx_shape<T>(rows, cols, z, z_stride, h, cols);
-            vt::mx8_checkpoint_kernel<T, decltype(a)::value><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
-                s, (const T *)z, (T *)h, codes, exps);
-            return vt::check_launch("mx8_checkpoint_kernel");
+            return vt::with_word<T>(s, [&](auto word) {
+                vt::mx8_checkpoint_kernel<decltype(word)::value, T, decltype(a)::value><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
+                    s, (const T *)z, (T *)h, codes, exps);
+                return vt::check_launch("mx8_checkpoint_kernel");
+            });
         });
     });
 }
@@ -263,9 +363,11 @@ extern "C" vt_status vt_mx8_act_bwd(const void *dh, int dtype, uint64_t rows, ui
         using T = typename decltype(ty)::type;
         return vt::with_act(act, [&](auto a) {
             const vt::MxShape s = vt::mx_shape<T>(rows, cols, dh, dh_stride, dz, cols);
-            vt::mx8_act_bwd_kernel<T, decltype(a)::value><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
-                s, (const T *)dh, codes, exps, (T *)dz);
-            return vt::check_launch("mx8_act_bwd_kernel");
+            return vt::with_word<T>(s, [&](auto word) {
+                vt::mx8_act_bwd_kernel<decltype(word)::value, T, decltype(a)::value><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
+                    s, (const T *)dh, codes, exps, (T *)dz);
+                return vt::check_launch("mx8_act_bwd_kernel");
+            });
         });
     });
 }
@@ -279,8 +381,11 @@ extern "C" vt_status vt_mx8_dequantize(const int8_t *codes, const uint8_t *exps,
     return vt::with_type(dtype, [&](auto ty) {
         using T = typename decltype(ty)::type;
         const vt::MxShape s = vt::mx_shape<T>(rows, cols, out, cols, out, cols);
-        vt::mx8_dequantize_kernel<T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(s, codes, exps, (T *)out);
-        return vt::check_launch("mx8_dequantize_kernel");
+        return vt::with_word<T>(s, [&](auto word) {
+            vt::mx8_dequantize_kernel<decltype(word)::value, T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
+                s, codes, exps, (T *)out);
+            return vt::check_launch("mx8_dequantize_kernel");
+        });
     });
 }
 
@@ -294,9 +399,11 @@ extern "C" vt_status vt_mx4_quantize(const void *x, int dtype, uint64_t rows, ui
     return vt::with_type(dtype, [&](auto ty) {
         using T = typename decltype(ty)::type;
         const vt::MxShape s = vt::mx_shape<T>(rows, cols, x, x_stride, x, x_stride);
-        vt::mx4_quantize_kernel<T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
-            s, (const T *)x, (uint32_t *)codes, exps);
-        return vt::check_launch("mx4_quantize_kernel");
+        return vt::with_word<T>(s, [&](auto word) {
+            vt::mx4_quantize_kernel<decltype(word)::value, T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
+                s, (const T *)x, (uint32_t *)codes, exps);
+            return vt::check_launch("mx4_quantize_kernel");
+        });
     });
 }
 
@@ -309,8 +416,10 @@ extern "C" vt_status vt_mx4_dequantize(const uint8_t *codes, const uint8_t *exps
     return vt::with_type(dtype, [&](auto ty) {
         using T = typename decltype(ty)::type;
         const vt::MxShape s = vt::mx_shape<T>(rows, cols, out, cols, out, cols);
-        vt::mx4_dequantize_kernel<T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
-            s, (const uint32_t *)codes, exps, (T *)out);
-        return vt::check_launch("mx4_dequantize_kernel");
+        return vt::with_word<T>(s, [&](auto word) {
+            vt::mx4_dequantize_kernel<decltype(word)::value, T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
+                s, (const uint32_t *)codes, exps, (T *)out);
+            return vt::check_launch("mx4_dequantize_kernel");
+        });
     });
 }
