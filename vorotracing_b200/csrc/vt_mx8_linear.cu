@@ -464,35 +464,47 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
     if (warp == 1) tc::tmem_free<P::TMEM>(tmem);
 }
 
-// Adds the groups' parts in order: dw (outs, cols) and db (outs).  A part has 128 columns a slab;
-// with one slab of up to 64 (fold) its two halves come from different rows and are added.
-template <typename T>
+// Adds the groups' parts: dw (outs, cols) and db (outs).  A part has 128 columns a slab;
+// with one slab of up to 64 (fold) its two halves come from different rows and are added, always in
+// the same order.  The blocks after dw's take db.  With many groups (SPLIT 8) a block takes 32 numbers and each of its
+// warps every eighth group of them: a thread that added all 148 groups of a number waited 20 us for its loads, now 5
+// (177137 x 16 -> 16).  With few, a thread takes a number's groups (3652 x 2311 -> 197, 8 groups: 7 us, split 27).
+template <typename T, uint32_t SPLIT>
 __global__ void __launch_bounds__(256) narrow_reduce_kernel(const float *__restrict__ dw_parts, const float *__restrict__ db_parts,
                                                             uint32_t groups, uint32_t slabs, uint32_t part_outs, bool fold,
                                                             uint32_t cols, uint32_t outs, T *__restrict__ dw, T *__restrict__ db)
 {
-    const uint64_t per_group = (uint64_t)slabs * part_outs * 128u;
-    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-    if (dw && i < per_group) {
-        const uint32_t o = (uint32_t)(i / 128u % part_outs), n = (uint32_t)(i / 128u / part_outs) * 128u + (uint32_t)(i % 128u);
-        if (o < outs && n < cols) {
-            float v = 0.0f;
+    static_assert(SPLIT == 1 || SPLIT == 8, "a block has eight warps");
+    __shared__ float sum[8][32];
+    const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u;
+    const uint32_t first = SPLIT == 1u ? 0u : warp, in_block = SPLIT == 1u ? threadIdx.x : lane;
+    const uint64_t per_group = (uint64_t)slabs * part_outs * 128u, at = (uint64_t)blockIdx.x * (256u / SPLIT) + in_block;
+    const bool bias = at >= per_group;  // of the whole block
+    const uint64_t i = bias ? at - per_group : at, step = bias ? part_outs : per_group;
+    const uint32_t o = bias ? (uint32_t)i : (uint32_t)(i / 128u % part_outs);
+    const uint32_t n = bias ? 0u : (uint32_t)(i / 128u / part_outs) * 128u + (uint32_t)(i % 128u);
+    T *out = bias ? db : dw;
+    const bool is = out && o < outs && n < cols;
+    const float *p = (bias ? db_parts : dw_parts) + i;
+    float v = 0.0f, u = 0.0f;
+    if (is) {
 #pragma unroll 8
-            for (uint32_t g = 0; g < groups; ++g) v += __ldg(dw_parts + g * per_group + i);
-            if (fold) {
-                float u = 0.0f;
+        for (uint32_t g = first; g < groups; g += SPLIT) v += __ldg(p + g * step);
+        if (fold && !bias) {
 #pragma unroll 8
-                for (uint32_t g = 0; g < groups; ++g) u += __ldg(dw_parts + g * per_group + i + 64u);
-                v += u;
-            }
-            dw[(uint64_t)o * cols + n] = from_f32<T>(v);
+            for (uint32_t g = first; g < groups; g += SPLIT) u += __ldg(p + g * step + 64u);
         }
     }
-    if (db && i < outs) {
-        float v = 0.0f;
-        for (uint32_t g = 0; g < groups; ++g) v += __ldg(db_parts + (uint64_t)g * part_outs + i);
-        db[i] = from_f32<T>(v);
+    float total = v + u;
+    if constexpr (SPLIT > 1u) {
+        sum[warp][lane] = total;
+        __syncthreads();
+        if (warp) return;
+        total = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < 8; ++w) total += sum[w][lane];
     }
+    if (is) out[bias ? i : (uint64_t)o * cols + n] = from_f32<T>(total);
 }
 
 // ---- wider layers ----
@@ -889,9 +901,13 @@ static vt_status run_narrow(const void *dy, uint64_t dy_stride, const void *w, u
     default: s = launch_narrow<T, ACT, 4, true>(dy_map, a, stream); break;
     }
     if (s || !parts || !(dw || db)) return s;
-    const uint64_t n = (uint64_t)p.slabs * 128u * p.part_outs;
-    narrow_reduce_kernel<T><<<(unsigned)((n + 255u) / 256u), 256, 0, stream>>>(a.dw_parts, a.db_parts, p.groups, p.slabs, p.part_outs,
-                                                                           p.fold, cols, outs, (T *)dw, (T *)db);
+    const uint64_t n = (uint64_t)p.slabs * 128u * p.part_outs + p.part_outs;
+    if (p.groups >= 32u)
+        narrow_reduce_kernel<T, 8><<<(unsigned)((n + 31u) / 32u), 256, 0, stream>>>(a.dw_parts, a.db_parts, p.groups, p.slabs, p.part_outs,
+                                                                                   p.fold, cols, outs, (T *)dw, (T *)db);
+    else
+        narrow_reduce_kernel<T, 1><<<(unsigned)((n + 255u) / 256u), 256, 0, stream>>>(a.dw_parts, a.db_parts, p.groups, p.slabs,
+                                                                                     p.part_outs, p.fold, cols, outs, (T *)dw, (T *)db);
     return check_launch("narrow_reduce_kernel");
 }
 
@@ -911,7 +927,7 @@ static WidePlan wide_plan(uint64_t rows, uint32_t cols, uint32_t outs, int copie
     p.splits = (uint32_t)(room < most ? room : most);
     p.chunks_a_split = (chunks + p.splits - 1u) / p.splits;
     p.splits = (chunks + p.chunks_a_split - 1u) / p.chunks_a_split;
-    const uint64_t most_parts = 2u * sms / ((outs + 255u) / 256u) + 1u;  // two blocks an SM
+    const uint64_t most_parts = 6u * sms / ((outs + 255u) / 256u) + 1u;  // six blocks an SM
     p.sum_parts = (uint32_t)((rows + 255u) / 256u < most_parts ? (rows + 255u) / 256u : most_parts);
     p.h_at = 0;
     p.dw_at = p.h_at + align_up(rows * align_up(cols, 8) * 2u, 256);
