@@ -8,8 +8,8 @@
 // are compared as integers: the bits of |x| order like |x|, with infinities and
 // NaN on top, which is what the exponent rule wants.
 //
-// Measured (1088640 x 64, binary16, SiLU): checkpoint and gradient together 134 to 141 us, 5.0 to 5.2 TB/s
-// of 6.45; 4 bits and back on 1000000 x 192 binary32: 310 us, 5.6 TB/s.  The exponential and the reciprocal
+// Measured (1088640 x 64, binary16, SiLU): checkpoint and gradient together 134 to 149 us, 4.7 to 5.2 TB/s
+// of 6.45; 4 bits and back on 1000000 x 192 binary32: 306 to 317 us, 5.5 TB/s.  The exponential and the reciprocal
 // of an activation share a pipe of 16 lanes an SM, which is half busy: conversions are kept off it.  Two
 // items a thread in flight cost registers and were slower (186 us); so was a grid without a loop (151 us).
 #include "vt_mx.cuh"

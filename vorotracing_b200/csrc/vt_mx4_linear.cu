@@ -23,6 +23,8 @@
 // Measured (bfloat16): 1088640 rows, 192 -> 64, SiLU: 115 to 123 us, 4.5 to 4.9 TB/s (floor 86 us), bound by
 // HBM; with x read by the rounding warps themselves 597 us.  One row, 4096 -> 4096: 12.5 us a call, of which
 // the host takes 10; 77 rows, 1000 -> 333: 12.6 us (33 us in the large tiles).
+// 4096 rows, 8192 -> 8192: 161 us, 3.4 PFLOP/s, bound by waits and issue between stages (floor 83 us; tiles of 192
+// outputs with more places for scales 179 us).  277867 rows, 91 -> 195: 138 us, of which copying x to whole words 24.
 #include "vt_mx_rows.cuh"
 
 namespace vt {

@@ -26,11 +26,12 @@
 // Measured (bfloat16, a B200, in a loop of calls): 1088640 rows, 256 -> 256, SiLU: 404 us, 3.5 TB/s of
 // what it has to read and write (floor at 6.45 TB/s: 218 us).  What bounds it: with 256 outputs dW, W and
 // the column sums leave room for three buffers of dH, so one of the four sets of activation warps always
-// waits; a tile of 32 rows takes 1030 cycles where its bytes would take 700.  Steps on the way: rows in the
+// waits; a tile of 32 rows takes 1030 cycles where its bytes would take 700 (399 to 429 us by the GPU).  Steps on the way: rows in the
 // lanes, activations through shared memory 479 us; columns in the lanes 439; W in tensor memory instead of
 // shared memory 424; column sums on the tensor cores (a warp that added took as long as all else) 404.
-// 1614080 rows, 64 -> 3, ReLU: 139 us (floor 50 us), bound by the second product's warp: its wait, issue
-// and commit take 690 cycles a tile.
+// 1614080 rows, 64 -> 3, ReLU: 98 us (floor 50 us), bound by the second product's warp: its wait, issue
+// and commit take most of the 1000 cycles of a tile of 64 rows.  Steps: tiles of 32 rows 150 us; of 64 139;
+// dy's rows loaded ahead in registers 115; parts added by blocks 98.  Two tiles a turn of that warp: no gain.
 //
 // Wider layers are two matrix products (wide_kernel), both on pairs of CTAs that share a 256 x 256
 // tile: dz = (dy W) * act'(z8), with the slope in the epilogue, and dW = dy^T h with h = act(z8)
@@ -47,7 +48,7 @@ namespace vt {
 constexpr uint32_t NARROW_OUTS = 256, NARROW_THREADS = 640, TINY_OUTS = 8;
 
 // Rows of a tile.  64 halve the barriers and commits a row, which bound layers of few outputs (64 -> 3:
-// 150 us with 32, 139 with 64); more than 128 outputs leave tensor memory for buffers of 32 only.
+// 150 us with 32, 139 with 64, before the steps above); more than 128 outputs leave tensor memory for buffers of 32 only.
 constexpr uint32_t narrow_rows(uint32_t oc) { return oc <= 2 ? 64 : 32; }
 
 // OC: dy's columns in chunks of 64.  A slab is 128 columns of z, or all of up to 64 (FOLD).
