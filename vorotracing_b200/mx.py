@@ -123,6 +123,8 @@ _PRODUCT_TYPES = {torch.float16: 1, torch.bfloat16: 2}
 def _launch(name: str, index: int, *args):
     """Calls an entry point on the tensors' device and torch's current stream there."""
     f = _fn.get(name) or _call(name)
+    if index < 0:  # as what was loaded to the host is
+        _fail("the operand must be on CUDA device")
     if index == _get_device():
         status = f(*args, _raw_stream(index))
     else:
@@ -138,9 +140,12 @@ def _unaligned(ptr: int, stride: int) -> bool:
 
 
 class _Blocks:
-    """Codes and exponent bytes of a matrix, as two tensors or as one buffer that holds both."""
+    """Codes and exponent bytes of a matrix, as two tensors or as one buffer that holds both.
 
-    __slots__ = ("cols", "rows", "device_index", "_codes", "_exps", "_buf", "_pc", "_pe")
+    Only tensors and sizes are kept, and addresses are taken from the tensors at each call, so that an
+    object's copies, and what is loaded of it elsewhere, have memory of their own."""
+
+    __slots__ = ("cols", "rows", "_codes", "_exps", "_buf")
     _dtype: torch.dtype
     _per_block: int
     _align: int
@@ -157,41 +162,48 @@ class _Blocks:
             _fail(f"{what}: codes and exponents must be on the same CUDA device")
         if not codes.is_contiguous() or not exps.is_contiguous():
             _fail(f"{what}: codes and exponents must be contiguous")
-        self._pc, self._pe = codes.data_ptr(), exps.data_ptr()
-        if self._pc % self._align:
+        if codes.data_ptr() % self._align:
             _fail(f"{what}: codes must be {self._align}-byte aligned")
         self._codes, self._exps, self._buf = codes, exps, None
-        self.cols, self.rows, self.device_index = cols, shape[0], codes.get_device()
+        self.cols, self.rows = cols, shape[0]
 
     def _new(self, like, rows: int, cols: int):
-        blocks = -(-cols // BLOCK)
-        n = rows * blocks
-        self._buf = like.new_empty(n * (self._per_block + 1), dtype=torch.uint8)
-        self._pc = self._buf.data_ptr()
-        self._pe = self._pc + n * self._per_block
-        self._codes = self._exps = None
-        self.cols, self.rows, self.device_index = cols, rows, like.get_device()
+        self.cols, self.rows, self._codes, self._exps = cols, rows, None, None
+        self._buf = like.new_empty(rows * -(-cols // BLOCK) * (self._per_block + 1), dtype=torch.uint8)
+
+    def _place(self):
+        """(device index, address of the codes, address of the exponents)"""
+        buf = self._buf
+        if buf is not None:
+            p = buf.data_ptr()
+            return buf.get_device(), p, p + self.rows * -(-self.cols // BLOCK) * self._per_block
+        return self._codes.get_device(), self._codes.data_ptr(), self._exps.data_ptr()
+
+    @property
+    def device_index(self) -> int:
+        return (self._codes if self._buf is None else self._buf).get_device()
 
     @property
     def codes(self) -> torch.Tensor:
-        if self._codes is None:
-            n = self.rows * -(-self.cols // BLOCK) * self._per_block
-            self._codes = self._buf[:n].view(self._dtype).view(self.rows, -(-self.cols // BLOCK) * self._per_block)
-        return self._codes
+        if self._buf is None:
+            return self._codes
+        width = -(-self.cols // BLOCK) * self._per_block
+        return self._buf[:self.rows * width].view(self._dtype).view(self.rows, width)
 
     @property
     def exps(self) -> torch.Tensor:
-        if self._exps is None:
-            n = self.rows * -(-self.cols // BLOCK) * self._per_block
-            self._exps = self._buf[n:].view(self.rows, -(-self.cols // BLOCK))
-        return self._exps
+        if self._buf is None:
+            return self._exps
+        blocks = -(-self.cols // BLOCK)
+        return self._buf[self.rows * blocks * self._per_block:].view(self.rows, blocks)
 
     def _dequantize(self, entry: str, dtype) -> torch.Tensor:
         code = _DTYPES.get(dtype)
         if code is None:
             _fail(f"cannot dequantise to {str(dtype).replace('torch.', '')}")
-        out = (self._buf if self._codes is None else self._codes).new_empty((self.rows, self.cols), dtype=dtype)
-        _launch(entry, self.device_index, self._pc, self._pe, self.rows, self.cols, code, out.data_ptr())
+        index, codes, exps = self._place()
+        out = (self._codes if self._buf is None else self._buf).new_empty((self.rows, self.cols), dtype=dtype)
+        _launch(entry, index, codes, exps, self.rows, self.cols, code, out.data_ptr())
         return out
 
 
@@ -236,8 +248,8 @@ def act_checkpoint(z: torch.Tensor, act: str = "silu"):
     ckpt = Checkpoint.__new__(Checkpoint)
     ckpt.act, ckpt._act = act, code
     ckpt._new(m, rows, cols)
-    _launch("vt_mx8_checkpoint", ckpt.device_index, m.data_ptr(), dtype, rows, cols, stride, code,
-            h.data_ptr(), ckpt._pc, ckpt._pe)
+    index, codes, exps = ckpt._place()
+    _launch("vt_mx8_checkpoint", index, m.data_ptr(), dtype, rows, cols, stride, code, h.data_ptr(), codes, exps)
     return h, ckpt
 
 
@@ -246,11 +258,11 @@ def act_backward(dh: torch.Tensor, ckpt: Checkpoint) -> torch.Tensor:
     m, rows, cols, stride, dtype = _matrix(dh, "dh")
     if rows != ckpt.rows or cols != ckpt.cols:
         _fail(f"dh had {rows} rows of {cols}, the checkpoint has {ckpt.rows} of {ckpt.cols}")
-    if m.get_device() != ckpt.device_index:
+    index, codes, exps = ckpt._place()
+    if m.get_device() != index:
         _fail("dh must be on the same device as the checkpoint")
     dz = m.new_empty(dh.shape)
-    _launch("vt_mx8_act_bwd", ckpt.device_index, m.data_ptr(), dtype, rows, cols, stride, ckpt._pc,
-            ckpt._pe, ckpt._act, dz.data_ptr())
+    _launch("vt_mx8_act_bwd", index, m.data_ptr(), dtype, rows, cols, stride, codes, exps, ckpt._act, dz.data_ptr())
     return dz
 
 
@@ -271,8 +283,8 @@ def linear_backward(dy: torch.Tensor, weight: torch.Tensor, ckpt: Checkpoint, bi
     if rows != ckpt.rows or cols != ckpt.cols:
         _fail(f"dy has {rows} rows and weight {cols} columns, the checkpoint has {ckpt.rows} "
               f"rows of {ckpt.cols}")
-    index = m.get_device()
-    if w.get_device() != index or ckpt.device_index != index:
+    index, codes, exps = ckpt._place()
+    if m.get_device() != index or w.get_device() != index:
         _fail("weight and the checkpoint must be on the same device as dy")
     dz = m.new_empty((*dy.shape[:-1], cols)) if need_dz else None
     dw = m.new_empty((outs, cols)) if need_dw else None
@@ -282,7 +294,7 @@ def linear_backward(dy: torch.Tensor, weight: torch.Tensor, ckpt: Checkpoint, bi
         rows, cols, outs, _unaligned(m_ptr, dy_stride) + 2 * _unaligned(w_ptr, w_stride))
     ws = m.new_empty(n, dtype=torch.uint8) if n else None
     _launch("vt_mx8_linear_bwd", index, m_ptr, dy_stride, w_ptr, w_stride, dtype, rows, cols, outs,
-            ckpt._pc, ckpt._pe, ckpt._act, dz.data_ptr() if need_dz else None,
+            codes, exps, ckpt._act, dz.data_ptr() if need_dz else None,
             dw.data_ptr() if need_dw else None, db.data_ptr() if bias else None,
             ws.data_ptr() if n else None, n, _error_word(index))
     return dz, dw, db
@@ -316,7 +328,8 @@ def quantize4(x: torch.Tensor) -> MX4:
     m, rows, cols, stride, dtype = _matrix(x, "x")
     q = MX4.__new__(MX4)
     q._new(m, rows, cols)
-    _launch("vt_mx4_quantize", q.device_index, m.data_ptr(), dtype, rows, cols, stride, q._pc, q._pe)
+    index, codes, exps = q._place()
+    _launch("vt_mx4_quantize", index, m.data_ptr(), dtype, rows, cols, stride, codes, exps)
     return q
 
 
@@ -326,7 +339,8 @@ def linear4(x: torch.Tensor, w: MX4, bias=None, act: str = "identity") -> torch.
     x's type.  y (..., outs) has x's type."""
     code = _act_code(act)
     m, rows, cols, stride, dtype = _matrix(x, "x", _PRODUCT_TYPES)
-    outs, index = w.rows, w.device_index
+    outs = w.rows
+    index, codes, exps = w._place()
     if cols != w.cols:
         _fail(f"x had {cols} columns, the weight has {w.cols}")
     if m.get_device() != index:
@@ -343,6 +357,6 @@ def linear4(x: torch.Tensor, w: MX4, bias=None, act: str = "identity") -> torch.
     m_ptr = m.data_ptr()
     n = _call("vt_mx4_linear_workspace_bytes")(rows, cols, outs, _unaligned(m_ptr, stride))
     ws = m.new_empty(n, dtype=torch.uint8) if n else None
-    _launch("vt_mx4_linear", index, m_ptr, stride, dtype, rows, cols, outs, w._pc, w._pe, b_ptr, code,
+    _launch("vt_mx4_linear", index, m_ptr, stride, dtype, rows, cols, outs, codes, exps, b_ptr, code,
             y.data_ptr(), ws.data_ptr() if n else None, n, _error_word(index))
     return y
