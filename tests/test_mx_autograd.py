@@ -1,0 +1,55 @@
+"""act_linear's autograd function on the host, the kernels behind it replaced by torch operations."""
+import pytest
+import torch
+
+import mx_reference as R
+
+
+@pytest.fixture
+def mx(monkeypatch):
+    from vorotracing_b200 import mx
+
+    def act_checkpoint(z, act="silu"):
+        """A checkpoint as the operator makes it, one buffer of codes and exponents, on the host."""
+        ckpt = mx.Checkpoint.__new__(mx.Checkpoint)
+        ckpt.act, ckpt._act = act, mx.ACTS[act]
+        ckpt._new(z, *z.shape)
+        _, codes, exps = R.round8(z.detach())
+        ckpt.codes.copy_(codes)
+        ckpt.exps.copy_(exps)
+        return R.act(z, act).to(z.dtype), ckpt
+
+    def linear_backward(dy, weight, ckpt, bias=True, need_dz=True, need_dw=True):
+        unit = torch.exp2(ckpt.exps.double() - 133).repeat_interleave(32, dim=1)
+        z8 = (ckpt.codes.double() * unit)[:, :ckpt.cols]
+        g, t = dy.double(), dy.dtype
+        return (((g @ weight.double()) * R.slope(z8, ckpt.act)).to(t) if need_dz else None,
+                (g.t() @ R.act(z8, ckpt.act)).to(t) if need_dw else None, g.sum(0).to(t) if bias else None)
+
+    monkeypatch.setattr(mx, "act_checkpoint", act_checkpoint)
+    monkeypatch.setattr(mx, "linear_backward", linear_backward)
+    return mx
+
+
+def layer(dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(0)
+    return [torch.randn(s, generator=g).to(dtype).requires_grad_() for s in ((6, 32), (5, 32), (5,))]
+
+
+def test_gradients_of_the_first_order(mx):
+    z, w, b = layer()
+    y = mx.act_linear(z, w, b, "silu")
+    g = torch.ones_like(y)
+    got = torch.autograd.grad(y, (z, w, b), g)
+    want = torch.autograd.grad(torch.nn.functional.linear(torch.nn.functional.silu(z), w, b), (z, w, b), g)
+    for a, c in zip(got, want):
+        torch.testing.assert_close(a, c, rtol=0.05, atol=0.05)  # z in 8 bits, a few roundings to bfloat16
+
+
+def test_second_order_is_refused(mx):
+    """A gradient penalty: its second-order terms must not be dropped without a word."""
+    z, w, b = layer()
+    y = mx.act_linear(z, w, b, "silu")
+    (dz,) = torch.autograd.grad(y.float().square().sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (dz.float().square().sum() + y.float().sum()).backward()

@@ -309,6 +309,7 @@ class _ActLinear(torch.autograd.Function):
         return torch.nn.functional.linear(h, weight, bias)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable  # the kernels record no graph: second derivatives are refused
     def backward(ctx, dy):
         need = ctx.needs_input_grad
         dz, dw, db = linear_backward(dy, ctx.saved_tensors[0], ctx.ckpt,
@@ -319,7 +320,7 @@ class _ActLinear(torch.autograd.Function):
 
 def act_linear(z: torch.Tensor, weight: torch.Tensor, bias=None, act: str = "silu"):
     """y = act(z) W^T + b for training: between forward and backward only the
-    8-bit form of z is kept (33/32 byte a value), neither z nor act(z)."""
+    8-bit form of z is kept (33/32 byte a value), neither z nor act(z).  First derivatives only."""
     return _ActLinear.apply(z, weight, bias, act)
 
 
