@@ -1,4 +1,5 @@
-"""The microscaled operators as programs use them: copies and files of their objects."""
+"""The microscaled operators as programs use them: copies and files of their objects, memory between
+steps."""
 import copy
 import io
 
@@ -43,3 +44,23 @@ def test_a_copied_checkpoint_has_codes_of_its_own(how):
     got = (mx.act_backward(z, other), *mx.linear_backward(dy, w, other), other.dequantize())
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_backward_frees_the_checkpoints():
+    """A training step keeps 33/32 byte a value between its passes, and nothing of it when it is over, with the
+    loss still held."""
+    from vorotracing_b200 import mx
+
+    rows, cols = 4096, 256
+    z = values(rows, cols, torch.bfloat16, scale=1.0).requires_grad_()
+    w = values(64, cols, torch.bfloat16, 1, 0.1).requires_grad_()
+    mx.act_linear(z, w, None, "silu").float().square().sum().backward()  # what libraries keep from their first call on
+    z.grad = w.grad = None
+    before = torch.cuda.memory_allocated()
+    y = mx.act_linear(z, w, None, "silu")
+    kept = torch.cuda.memory_allocated() - before - y.numel() * 2
+    assert rows * cols * 33 // 32 <= kept < rows * cols * 33 // 32 + 1024
+    loss = y.float().square().sum()
+    del y
+    loss.backward()
+    assert torch.cuda.memory_allocated() - before < (rows * cols + 64 * cols) * 2 + 4096 and loss.isfinite()

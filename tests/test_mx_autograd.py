@@ -1,4 +1,7 @@
 """act_linear's autograd function on the host, the kernels behind it replaced by torch operations."""
+import weakref
+
+import numpy as np
 import pytest
 import torch
 
@@ -14,6 +17,9 @@ def mx(monkeypatch):
         ckpt = mx.Checkpoint.__new__(mx.Checkpoint)
         ckpt.act, ckpt._act = act, mx.ACTS[act]
         ckpt._new(z, *z.shape)
+        memory = np.zeros(ckpt._buf.numel(), np.uint8)
+        ckpt._buf = torch.from_numpy(memory)
+        mx.kept.append(weakref.ref(memory))
         _, codes, exps = R.round8(z.detach())
         ckpt.codes.copy_(codes)
         ckpt.exps.copy_(exps)
@@ -26,6 +32,7 @@ def mx(monkeypatch):
         return (((g @ weight.double()) * R.slope(z8, ckpt.act)).to(t) if need_dz else None,
                 (g.t() @ R.act(z8, ckpt.act)).to(t) if need_dw else None, g.sum(0).to(t) if bias else None)
 
+    monkeypatch.setattr(mx, "kept", [], raising=False)  # memory of the checkpoints made
     monkeypatch.setattr(mx, "act_checkpoint", act_checkpoint)
     monkeypatch.setattr(mx, "linear_backward", linear_backward)
     return mx
@@ -53,3 +60,24 @@ def test_second_order_is_refused(mx):
     (dz,) = torch.autograd.grad(y.float().square().sum(), z, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         (dz.float().square().sum() + y.float().sum()).backward()
+
+
+def test_backward_frees_the_checkpoint(mx):
+    z, w, b = layer()
+    loss = mx.act_linear(z, w, b, "silu").float().square().sum()
+    (kept,) = mx.kept
+    assert kept() is not None
+    loss.backward()
+    assert kept() is None and loss.isfinite()
+
+
+def test_saved_tensor_hooks_see_the_checkpoint(mx):
+    z, w, b = layer()
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (seen.append(t.dtype), t.clone())[1], lambda t: t):
+        y = mx.act_linear(z, w, b, "silu")
+    assert torch.uint8 in seen and mx.kept[0]() is None  # what the hook made stands in for it
+    got = torch.autograd.grad(y, (z, w, b), torch.ones_like(y))
+    y = mx.act_linear(z, w, b, "silu")
+    for a, c in zip(got, torch.autograd.grad(y, (z, w, b), torch.ones_like(y))):
+        assert torch.equal(a, c)

@@ -220,6 +220,14 @@ class Checkpoint(_Blocks):
         self.act = act
         self._take(codes, exps, cols)
 
+    @classmethod
+    def _of(cls, buf, rows: int, cols: int, act: str):
+        """A checkpoint from its buffer."""
+        ckpt = cls.__new__(cls)
+        ckpt.act, ckpt._act, ckpt._codes, ckpt._exps = act, _act_code(act), None, None
+        ckpt._buf, ckpt.rows, ckpt.cols = buf, rows, cols
+        return ckpt
+
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """The 8-bit values, (rows, cols)."""
         return self._dequantize("vt_mx8_dequantize", dtype)
@@ -304,15 +312,16 @@ class _ActLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, weight, bias, act):
         h, ckpt = act_checkpoint(z, act)
-        ctx.ckpt, ctx.has_bias = ckpt, bias is not None
-        ctx.save_for_backward(weight)
+        ctx.shape, ctx.has_bias = (ckpt.rows, ckpt.cols, act), bias is not None
+        ctx.save_for_backward(weight, ckpt._buf)  # freed by the backward pass, seen by saved-tensor hooks
         return torch.nn.functional.linear(h, weight, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable  # the kernels record no graph: second derivatives are refused
     def backward(ctx, dy):
         need = ctx.needs_input_grad
-        dz, dw, db = linear_backward(dy, ctx.saved_tensors[0], ctx.ckpt,
+        weight, buf = ctx.saved_tensors
+        dz, dw, db = linear_backward(dy, weight, Checkpoint._of(buf, *ctx.shape),
                                      bias=ctx.has_bias and need[2], need_dz=need[0],
                                      need_dw=need[1])
         return dz, dw, db, None
