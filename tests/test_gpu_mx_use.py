@@ -1,5 +1,5 @@
 """The microscaled operators as programs use them: copies and files of their objects, memory between
-steps."""
+steps, 32-bit parameters."""
 import copy
 import io
 
@@ -64,3 +64,48 @@ def test_backward_frees_the_checkpoints():
     del y
     loss.backward()
     assert torch.cuda.memory_allocated() - before < (rows * cols + 64 * cols) * 2 + 4096 and loss.isfinite()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_autocast_trains_32_bit_parameters(dtype):
+    """As with any layer: operands in autocast's type, gradients in the parameters' own."""
+    from vorotracing_b200 import mx
+
+    z, w, b = values(300, 96, torch.float32, scale=1.0), values(40, 96, torch.float32, 1, 0.2), values(1, 40, torch.float32, 2)[0]
+    g = values(300, 40, dtype, 3)
+    for t in (z, w, b):
+        t.requires_grad_()
+    with pytest.raises(RuntimeError, match="z had dtype float32, expected one of float16, bfloat16"):
+        mx.act_linear(z, w, b)
+    with torch.autocast("cuda", dtype):
+        y = mx.act_linear(z, w, b)
+    assert y.dtype is dtype
+    cast = [t.detach().to(dtype).requires_grad_() for t in (z, w, b)]
+    same = mx.act_linear(*cast)
+    assert torch.equal(y, same)
+    for a, c in zip(torch.autograd.grad(y, (z, w, b), g), torch.autograd.grad(same, cast, g)):
+        assert a.dtype is torch.float32 and torch.equal(a, c.float())
+
+
+def test_a_decoder_of_32_bit_parameters():
+    """Trained under autocast, run in 4 bits."""
+    from vorotracing_b200.decoder import RayDecoder
+
+    torch.manual_seed(4)
+    decoder = RayDecoder(features=16, hidden=32, layers=1, dtype=torch.float32)
+    x = values(500, 16, torch.bfloat16, scale=1.0)
+    target = torch.sin(x[:, :3].float())
+    opt = torch.optim.Adam(decoder.parameters(), lr=1e-2)
+    losses = []
+    for _ in range(40):
+        with torch.autocast("cuda", torch.bfloat16):
+            y = decoder(x)
+        loss = (y.float() - target).square().mean()
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+        losses.append(float(loss.detach()))
+    assert all(p.dtype is torch.float32 and p.grad.dtype is torch.float32 for p in decoder.parameters())
+    assert losses[-1] < 0.5 * losses[0]
+    y = decoder.quantized()(x)
+    assert y.dtype is torch.bfloat16 and y.isfinite().all()

@@ -81,3 +81,14 @@ def test_saved_tensor_hooks_see_the_checkpoint(mx):
     y = mx.act_linear(z, w, b, "silu")
     for a, c in zip(got, torch.autograd.grad(y, (z, w, b), torch.ones_like(y))):
         assert torch.equal(a, c)
+
+
+def test_what_the_backward_pass_cannot_take_is_refused_in_the_forward(mx):
+    z, w, b = layer(torch.float32)
+    with pytest.raises(RuntimeError, match="z had dtype float32, expected one of float16, bfloat16"):
+        mx.act_linear(z, w, b)
+    h = lambda t: t.detach().half()
+    for args in ((h(z), w, None), (h(z), h(w), b), (h(z), h(w).bfloat16(), None)):
+        with pytest.raises(RuntimeError, match="the dtype of z"):
+            mx.act_linear(*args)
+    assert not mx.kept

@@ -35,7 +35,9 @@ def ray_features(rgba: torch.Tensor, rays: torch.Tensor, extra=None, dtype=torch
 
 
 class RayDecoder(torch.nn.Module):
-    """features -> hidden (x layers) -> outs, SiLU between the layers."""
+    """features -> hidden (x layers) -> outs, SiLU between the layers.
+
+    Parameters in a 16-bit type train as they are, those in float32 under torch.autocast."""
 
     def __init__(self, features: int, hidden: int = 64, layers: int = 2, outs: int = 3, act: str = "silu",
                  device="cuda", dtype=torch.bfloat16):
@@ -69,6 +71,6 @@ class QuantizedRayDecoder:
     @torch.no_grad()
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         for w, b in self.layers[:-1]:
-            x = mx.linear4(x, w, b, self.act)
+            x = mx.linear4(x, w, b.to(x.dtype), self.act)
         w, b = self.layers[-1]
-        return mx.linear4(x, w, b)
+        return mx.linear4(x, w, b.to(x.dtype))

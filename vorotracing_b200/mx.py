@@ -329,7 +329,21 @@ class _ActLinear(torch.autograd.Function):
 
 def act_linear(z: torch.Tensor, weight: torch.Tensor, bias=None, act: str = "silu"):
     """y = act(z) W^T + b for training: between forward and backward only the
-    8-bit form of z is kept (33/32 byte a value), neither z nor act(z).  First derivatives only."""
+    8-bit form of z is kept (33/32 byte a value), neither z nor act(z).  First derivatives only.
+
+    z, weight and bias have one 16-bit type; under torch.autocast they may have
+    any and are brought to its type, with gradients in their own."""
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        z, weight, bias = (t if t is None or t.dtype is torch.float64 else t.to(dtype) for t in (z, weight, bias))
+        with torch.autocast("cuda", enabled=False):
+            return act_linear(z, weight, bias, act)
+    # what linear_backward would refuse is refused here, before anything is computed
+    if z.dtype not in _PRODUCT_TYPES:
+        _fail(f"z had dtype {str(z.dtype).replace('torch.', '')}, expected one of "
+              + ", ".join(str(d).replace("torch.", "") for d in _PRODUCT_TYPES) + " (or torch.autocast)")
+    if weight.dtype is not z.dtype or (bias is not None and bias.dtype is not z.dtype):
+        _fail("weight and bias must have the dtype of z")
     return _ActLinear.apply(z, weight, bias, act)
 
 
