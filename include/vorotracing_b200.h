@@ -436,7 +436,8 @@ VT_API vt_status vt_mx8_dequantize(const int8_t *codes, const uint8_t *exps, uin
  * dz (rows, cols) = (dy W) * act'(z8), dw (outs, cols) = dy^T act(z8),
  * db (outs) = column sums of dy.  Any output may be null.  copies: 1 if dy's
  * rows do not start on 16 bytes (pointer or stride), plus 2 if the weight's do
- * not; the workspace then has room for copies that do.  err gets VT_ERR_CUDA
+ * not; the workspace then has room for copies that do.  The workspace is
+ * 32-byte aligned.  err gets VT_ERR_CUDA
  * if a wait inside a kernel has run out (a second); the outputs are then not
  * valid. */
 VT_API uint64_t vt_mx8_linear_bwd_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs,
@@ -454,8 +455,8 @@ VT_API vt_status vt_mx4_dequantize(const uint8_t *codes, const uint8_t *exps, ui
                                    uint32_t cols, int dtype, void *out, vt_stream stream);
 /* y (rows, outs) = act(q4(x) w4^T + bias): x (rows, cols) is rounded to 4 bits
  * on the way, codes / exps are the weight (outs, cols) in 4 bits, bias (outs)
- * may be null.  copies: 1 if x's rows do not start on 16 bytes.  err as for
- * vt_mx8_linear_bwd. */
+ * may be null.  copies: 1 if x's rows do not start on 16 bytes.  The workspace
+ * is 16-byte aligned.  err as for vt_mx8_linear_bwd. */
 VT_API uint64_t vt_mx4_linear_workspace_bytes(uint64_t rows, uint32_t cols, uint32_t outs,
                                               int copies);
 VT_API vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, uint64_t rows,

@@ -1,0 +1,37 @@
+"""What the C entry points of the microscaled operators refuse, on the host: an address that a kernel could
+not use never reaches one."""
+import pytest
+
+P = 1 << 20  # an address; nothing is read there
+
+
+@pytest.fixture
+def call():
+    from vorotracing_b200 import mx
+    from vorotracing_b200._lib import lib
+
+    def f(name, *args):
+        status = mx._call(name)(*args)
+        return status, lib().vt_last_error().decode()
+
+    return f
+
+
+@pytest.mark.parametrize("outs", [40, 300])
+def test_workspace_alignment_of_the_gradients(call, outs):
+    n = call("vt_mx8_linear_bwd_workspace_bytes", 4096, 64, outs, 0)[0]
+
+    def bwd(workspace):
+        return call("vt_mx8_linear_bwd", P, outs, P, 64, 2, 4096, 64, outs, P, P, 0, P, P, P, workspace, n, None, None)
+
+    for at in (1, 8, 16, 48):
+        status, text = bwd(P + at)
+        assert status == 1 and "32-byte aligned" in text
+
+
+def test_workspace_alignment_of_the_4_bit_product(call):
+    n = call("vt_mx4_linear_workspace_bytes", 20000, 64, 300, 0)[0]
+    assert n
+    for at in (1, 8, 24):
+        status, text = call("vt_mx4_linear", P, 64, 2, 20000, 64, 300, P, P, None, 0, P, P + at, n, None, None)
+        assert status == 1 and "16-byte aligned" in text

@@ -1074,8 +1074,8 @@ extern "C" vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const
                    "vt_mx8_linear_bwd: a row stride is less than a row");
         VT_REQUIRE(vt::aligned32(codes), "vt_mx8_linear_bwd: codes must be 32-byte aligned");
         VT_REQUIRE(workspace_bytes >= vt_mx8_linear_bwd_workspace_bytes(rows, cols, outs, vt::copies_of<T>(dy, dy_stride, weight, weight_stride)) &&
-                       vt::aligned16(workspace),
-                   "vt_mx8_linear_bwd: workspace too small or not 16-byte aligned");
+                       vt::aligned32(workspace),
+                   "vt_mx8_linear_bwd: workspace too small or not 32-byte aligned");  // parts are stored 32 bytes at a time
         if (cols == 0) {  // a layer without inputs has the bias alone
             vt::column_sum_kernel<T><<<outs, 256, 0, st>>>((const T *)dy, rows, outs, dy_stride, (T *)db);
             return vt::check_launch("column_sum_kernel");
