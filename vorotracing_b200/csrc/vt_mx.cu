@@ -331,6 +331,8 @@ static unsigned mx_grid(const MxShape &s)
     VT_REQUIRE(rows <= (1ull << 40), name ": too many rows");                                      \
     VT_REQUIRE(cols <= (1u << 30), name ": too many columns");                                     \
     if (rows == 0 || cols == 0) return VT_OK
+#define MX_ELEMENTS(name, ...)                                                                     \
+    VT_REQUIRE(vt::on_elements<T>(__VA_ARGS__), name ": a matrix does not start on an element")
 
 extern "C" vt_status vt_mx8_checkpoint(const void *z, int dtype, uint64_t rows, uint32_t cols, uint64_t z_stride,
                                        int act, void *h, int8_t *codes, uint8_t *exps, vt_stream stream)
@@ -339,8 +341,9 @@ extern "C" vt_status vt_mx8_checkpoint(const void *z, int dtype, uint64_t rows, 
     VT_REQUIRE(z && h && codes && exps, "vt_mx8_checkpoint: null pointer");
     VT_REQUIRE(z_stride >= cols, "vt_mx8_checkpoint: the row stride is less than a row");
     VT_REQUIRE(vt::aligned32(codes), "vt_mx8_checkpoint: codes must be 32-byte aligned");
-    return vt::with_type(dtype, [&](auto ty) {
+    return vt::with_type(dtype, [&](auto ty) -> vt_status {
         using T = typename decltype(ty)::type;
+        MX_ELEMENTS("vt_mx8_checkpoint", z, h);
         return vt::with_act(act, [&](auto a) {
             const vt::MxShape s = vt::mx_shape<T>(rows, cols, z, z_stride, h, cols);
             return vt::with_word<T>(s, [&](auto word) {
@@ -359,8 +362,9 @@ extern "C" vt_status vt_mx8_act_bwd(const void *dh, int dtype, uint64_t rows, ui
     VT_REQUIRE(dh && codes && exps && dz, "vt_mx8_act_bwd: null pointer");
     VT_REQUIRE(dh_stride >= cols, "vt_mx8_act_bwd: the row stride is less than a row");
     VT_REQUIRE(vt::aligned32(codes), "vt_mx8_act_bwd: codes must be 32-byte aligned");
-    return vt::with_type(dtype, [&](auto ty) {
+    return vt::with_type(dtype, [&](auto ty) -> vt_status {
         using T = typename decltype(ty)::type;
+        MX_ELEMENTS("vt_mx8_act_bwd", dh, dz);
         return vt::with_act(act, [&](auto a) {
             const vt::MxShape s = vt::mx_shape<T>(rows, cols, dh, dh_stride, dz, cols);
             return vt::with_word<T>(s, [&](auto word) {
@@ -378,8 +382,9 @@ extern "C" vt_status vt_mx8_dequantize(const int8_t *codes, const uint8_t *exps,
     MX_COMMON("vt_mx8_dequantize");
     VT_REQUIRE(codes && exps && out, "vt_mx8_dequantize: null pointer");
     VT_REQUIRE(vt::aligned32(codes), "vt_mx8_dequantize: codes must be 32-byte aligned");
-    return vt::with_type(dtype, [&](auto ty) {
+    return vt::with_type(dtype, [&](auto ty) -> vt_status {
         using T = typename decltype(ty)::type;
+        MX_ELEMENTS("vt_mx8_dequantize", out);
         const vt::MxShape s = vt::mx_shape<T>(rows, cols, out, cols, out, cols);
         return vt::with_word<T>(s, [&](auto word) {
             vt::mx8_dequantize_kernel<decltype(word)::value, T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
@@ -396,8 +401,9 @@ extern "C" vt_status vt_mx4_quantize(const void *x, int dtype, uint64_t rows, ui
     VT_REQUIRE(x && codes && exps, "vt_mx4_quantize: null pointer");
     VT_REQUIRE(x_stride >= cols, "vt_mx4_quantize: the row stride is less than a row");
     VT_REQUIRE(vt::aligned16(codes), "vt_mx4_quantize: codes must be 16-byte aligned");
-    return vt::with_type(dtype, [&](auto ty) {
+    return vt::with_type(dtype, [&](auto ty) -> vt_status {
         using T = typename decltype(ty)::type;
+        MX_ELEMENTS("vt_mx4_quantize", x);
         const vt::MxShape s = vt::mx_shape<T>(rows, cols, x, x_stride, x, x_stride);
         return vt::with_word<T>(s, [&](auto word) {
             vt::mx4_quantize_kernel<decltype(word)::value, T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(
@@ -413,8 +419,9 @@ extern "C" vt_status vt_mx4_dequantize(const uint8_t *codes, const uint8_t *exps
     MX_COMMON("vt_mx4_dequantize");
     VT_REQUIRE(codes && exps && out, "vt_mx4_dequantize: null pointer");
     VT_REQUIRE(vt::aligned16(codes), "vt_mx4_dequantize: codes must be 16-byte aligned");
-    return vt::with_type(dtype, [&](auto ty) {
+    return vt::with_type(dtype, [&](auto ty) -> vt_status {
         using T = typename decltype(ty)::type;
+        MX_ELEMENTS("vt_mx4_dequantize", out);
         const vt::MxShape s = vt::mx_shape<T>(rows, cols, out, cols, out, cols);
         return vt::with_word<T>(s, [&](auto word) {
             vt::mx4_dequantize_kernel<decltype(word)::value, T><<<vt::mx_grid(s), 256, 0, (cudaStream_t)stream>>>(

@@ -369,6 +369,11 @@ template <typename F> inline vt_status with_type16(int dtype, F f)
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned32(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
+// Whether all addresses (nulls among them) are a T's: the kernels touch nothing narrower
+template <typename T, typename... P> inline bool on_elements(const P *...p)
+{
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & (sizeof(T) - 1u)) == 0;
+}
 inline uint32_t mx_blocks(uint32_t cols) { return cols / MX_BLOCK + (cols % MX_BLOCK != 0); }
 inline int sm_count()  // of the current device, asked for once
 {

@@ -869,6 +869,7 @@ extern "C" vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, 
     cudaStream_t st = (cudaStream_t)stream;
     return vt::with_type16(dtype, [&](auto ty) -> vt_status {
         using T = typename decltype(ty)::type;
+        VT_REQUIRE(vt::on_elements<T>(x, bias, y), "vt_mx4_linear: a matrix does not start on an element");
         VT_REQUIRE(workspace_bytes >= vt_mx4_linear_workspace_bytes(rows, cols, outs, !vt::whole_words<T>(x, x_stride)) &&
                        vt::aligned16(workspace),
                    "vt_mx4_linear: workspace too small or not 16-byte aligned");

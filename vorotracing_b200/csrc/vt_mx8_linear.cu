@@ -1070,6 +1070,7 @@ extern "C" vt_status vt_mx8_linear_bwd(const void *dy, uint64_t dy_stride, const
             if (!db) return VT_OK;
         }
         VT_REQUIRE(dy && (cols == 0 || (weight && codes && exps)), "vt_mx8_linear_bwd: null pointer");
+        VT_REQUIRE(vt::on_elements<T>(dy, weight, dz, dw, db), "vt_mx8_linear_bwd: a matrix does not start on an element");
         VT_REQUIRE(dy_stride >= outs && weight_stride >= cols,
                    "vt_mx8_linear_bwd: a row stride is less than a row");
         VT_REQUIRE(vt::aligned32(codes), "vt_mx8_linear_bwd: codes must be 32-byte aligned");
