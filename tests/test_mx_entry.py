@@ -55,3 +55,12 @@ def test_matrices_start_on_an_element(call, dtype, off):
     for args in wrong:
         status, text = call(*args)
         assert status == 1 and "does not start on an element" in text, args
+
+
+def test_matrices_whose_blocks_no_count_holds(call):
+    for rows, cols in (((1 << 40) + 1, 1), (1 << 40, 33), (1 << 36, 1 << 10), (1 << 39, 1 << 30)):
+        for args in (("vt_mx8_checkpoint", P, 2, rows, cols, cols, 0, P, P, P, None), ("vt_mx8_act_bwd", P, 2, rows, cols, cols, P, P, 0, P, None),
+                     ("vt_mx8_dequantize", P, P, rows, cols, 2, P, None), ("vt_mx4_quantize", P, 2, rows, cols, cols, P, P, None),
+                     ("vt_mx4_dequantize", P, P, rows, cols, 2, P, None)):
+            status, text = call(*args)
+            assert status == 1 and "too many rows" in text, args

@@ -326,11 +326,11 @@ static unsigned mx_grid(const MxShape &s)
 
 }  // namespace vt
 
-// rows * (blocks a row) has to leave room for item counts in 64 bits; cols fits 32 bits by type
+// rows * (blocks a row) has to leave room for item counts and offsets in 64 bits
 #define MX_COMMON(name)                                                                            \
-    VT_REQUIRE(rows <= (1ull << 40), name ": too many rows");                                      \
     VT_REQUIRE(cols <= (1u << 30), name ": too many columns");                                     \
-    if (rows == 0 || cols == 0) return VT_OK
+    if (rows == 0 || cols == 0) return VT_OK;                                                      \
+    VT_REQUIRE(rows <= (1ull << 40) / vt::mx_blocks(cols), name ": too many rows")
 #define MX_ELEMENTS(name, ...)                                                                     \
     VT_REQUIRE(vt::on_elements<T>(__VA_ARGS__), name ": a matrix does not start on an element")
 
