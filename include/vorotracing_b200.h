@@ -464,6 +464,10 @@ VT_API vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, uint
                                const uint8_t *exps, const void *bias, int act, void *y,
                                void *workspace, uint64_t workspace_bytes, uint32_t *err,
                                vt_stream stream);
+/* Launches a kernel whose one wait nothing ends: after about a second it reports
+ * VT_ERR_CUDA to err and ends, as a product whose wait has run out does.  For
+ * programs that test what they do then. */
+VT_API vt_status vt_wait_check(uint32_t *err, vt_stream stream);
 
 #ifdef __cplusplus
 }

@@ -1,5 +1,5 @@
 """The microscaled operators as programs use them: copies and files of their objects, memory between
-steps, 32-bit parameters."""
+steps, 32-bit parameters, a wait that runs out."""
 import copy
 import io
 
@@ -109,3 +109,21 @@ def test_a_decoder_of_32_bit_parameters():
     assert losses[-1] < 0.5 * losses[0]
     y = decoder.quantized()(x)
     assert y.dtype is torch.bfloat16 and y.isfinite().all()
+
+
+def test_a_wait_that_runs_out_is_reported():
+    """A kernel that waits for what never comes ends by itself, says so, and leaves the GPU as usable as before."""
+    from vorotracing_b200 import mx
+
+    z, w = values(300, 96, torch.bfloat16), mx.quantize4(values(40, 96, torch.bfloat16, 1))
+    want = mx.linear4(z, w)
+    mx.raise_errors()
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    mx._launch("vt_wait_check", 0, mx._error_word(0))
+    end.record()
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        mx.raise_errors()
+    assert 500 < begin.elapsed_time(end) < 10000  # 2e9 clocks of at most 1965 MHz, looked at in steps
+    mx.raise_errors()
+    assert torch.equal(mx.linear4(z, w), want)

@@ -1,4 +1,4 @@
-// vt_tc.cu -- host side of the tensor-core plumbing: TMA tensor maps.
+// vt_tc.cu -- host side of the tensor-core plumbing: TMA tensor maps; a wait that runs out.
 #include "vt_tc.cuh"
 
 namespace vt {
@@ -62,5 +62,22 @@ vt_status make_chunk_map(CUtensorMap *map, CUtensorMapDataType type, const void 
     return encode_map(map, type, p, 3, dims, strides, box, true);
 }
 
+// One wait for a barrier that has no arrivals to come: it gives up as any wait does, and the kernel ends.
+__global__ void wait_check_kernel(uint32_t *err)
+{
+    __shared__ uint64_t bar;
+    __shared__ Fail fail;
+    mbar_init(&bar, 1);
+    fail.failed = 0;
+    mbar_wait(&bar, 0, &fail, err);
+}
+
 }  // namespace tc
 }  // namespace vt
+
+extern "C" vt_status vt_wait_check(uint32_t *err, vt_stream stream)
+{
+    VT_REQUIRE(err, "vt_wait_check: null pointer");
+    vt::tc::wait_check_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(err);
+    return vt::check_launch("wait_check_kernel");
+}

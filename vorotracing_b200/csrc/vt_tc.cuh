@@ -14,6 +14,7 @@
 #include <atomic>
 
 #include "vt_abi.cuh"
+#include "vt_wait.cuh"
 
 namespace vt {
 namespace tc {
@@ -46,18 +47,16 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
                  : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return ok;
 }
-// About a second of the SM's clock.  (Reading %globaltimer instead takes about a microsecond, which
-// every wait that is not over at once would pay.)
-constexpr long long WAIT_LIMIT = 2000000000ll;
-
+// Waits are timed by the SM's clock (vt_wait.cuh).  Reading %globaltimer instead takes about a microsecond, which
+// every wait that is not over at once would pay.
 static __device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, Fail *fail, uint32_t *err, bool last)
 {
-    const long long began = clock64();
+    WaitTime time(clock64());
     for (;;) {
         for (int i = 0; i < 64; ++i)
             if (mbar_try(bar, parity)) return true;
         if (fail->failed && !last) return false;
-        if (clock64() - began > WAIT_LIMIT) {
+        if (time.over(clock64())) {
             fail->failed = 1;
             report(err, VT_ERR_CUDA);
             return false;

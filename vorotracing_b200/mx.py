@@ -42,6 +42,7 @@ _ARGS = {
     "vt_mx4_dequantize": (_P, _P, _U64, _U32, _I, _P, _P),
     "vt_mx4_linear_workspace_bytes": (_U64, _U32, _U32, _I),
     "vt_mx4_linear": (_P, _U64, _I, _U64, _U32, _U32, _P, _P, _P, _I, _P, _P, _U64, _P, _P),
+    "vt_wait_check": (_P, _P),
 }
 _fn = {}
 _get_device = torch.cuda.current_device
