@@ -468,6 +468,12 @@ VT_API vt_status vt_mx4_linear(const void *x, uint64_t x_stride, int dtype, uint
  * VT_ERR_CUDA to err and ends, as a product whose wait has run out does.  For
  * programs that test what they do then. */
 VT_API vt_status vt_wait_check(uint32_t *err, vt_stream stream);
+/* An error word in page-locked host memory, zero: kernels of every device can
+ * write it, the host reads it without waiting for them, and a stream capture
+ * that is under way takes no part in its making.  Any word of device memory
+ * serves as err too. */
+VT_API vt_status vt_error_word_create(uint32_t **word);
+VT_API vt_status vt_error_word_free(uint32_t *word);
 
 #ifdef __cplusplus
 }

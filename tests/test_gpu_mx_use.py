@@ -2,6 +2,9 @@
 steps, 32-bit parameters, a wait that runs out."""
 import copy
 import io
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -127,3 +130,33 @@ def test_a_wait_that_runs_out_is_reported():
     assert 500 < begin.elapsed_time(end) < 10000  # 2e9 clocks of at most 1965 MHz, looked at in steps
     mx.raise_errors()
     assert torch.equal(mx.linear4(z, w), want)
+
+
+FIRST_CALL_IN_A_GRAPH = """
+import torch
+from vorotracing_b200 import mx
+
+x = torch.randn(300, 96, device="cuda").bfloat16()
+w = mx.quantize4(torch.randn(40, 96, device="cuda"))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = mx.linear4(x, w)      # this process's first product
+mx.raise_errors()             # nothing has run, so nothing has failed
+g.replay()
+mx.raise_errors()
+assert torch.equal(y, mx.linear4(x, w))
+mx._launch("vt_wait_check", 0, mx._error_word(0))
+g.replay()                    # must not hide what was reported before it
+try:
+    mx.raise_errors()
+except RuntimeError as e:
+    assert "gave up waiting" in str(e)
+    print("reported")
+mx.raise_errors()
+"""
+
+
+def test_the_first_product_may_be_captured():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_GRAPH], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "reported" in r.stdout, r.stdout + r.stderr

@@ -1,4 +1,4 @@
-// vt_tc.cu -- host side of the tensor-core plumbing: TMA tensor maps; a wait that runs out.
+// vt_tc.cu -- host side of the tensor-core plumbing: TMA tensor maps; a wait that runs out; error words.
 #include "vt_tc.cuh"
 
 namespace vt {
@@ -80,4 +80,33 @@ extern "C" vt_status vt_wait_check(uint32_t *err, vt_stream stream)
     VT_REQUIRE(err, "vt_wait_check: null pointer");
     vt::tc::wait_check_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(err);
     return vt::check_launch("wait_check_kernel");
+}
+
+extern "C" vt_status vt_error_word_create(uint32_t **word)
+{
+    VT_REQUIRE(word, "vt_error_word_create: null pointer");
+    // An allocation is no part of a graph that this thread may be capturing.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    void *p = nullptr;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) {
+        e = cudaHostAlloc(&p, sizeof(uint32_t), cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return vt::set_error(VT_ERR_CUDA, "vt_error_word_create: %s", cudaGetErrorString(e));
+    }
+    *word = (uint32_t *)p;
+    **word = 0;
+    return VT_OK;
+}
+
+extern "C" vt_status vt_error_word_free(uint32_t *word)
+{
+    if (!word) return VT_OK;
+    const cudaError_t e = cudaFreeHost(word);
+    if (e == cudaSuccess) return VT_OK;
+    cudaGetLastError();
+    return vt::set_error(VT_ERR_CUDA, "vt_error_word_free: %s", cudaGetErrorString(e));
 }

@@ -58,7 +58,7 @@ static __device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parit
         if (fail->failed && !last) return false;
         if (time.over(clock64())) {
             fail->failed = 1;
-            report(err, VT_ERR_CUDA);
+            if (err) *(volatile uint32_t *)err = VT_ERR_CUDA;  // a plain store: the word may be the host's
             return false;
         }
     }

@@ -43,6 +43,7 @@ _ARGS = {
     "vt_mx4_linear_workspace_bytes": (_U64, _U32, _U32, _I),
     "vt_mx4_linear": (_P, _U64, _I, _U64, _U32, _U32, _P, _P, _P, _I, _P, _P, _U64, _P, _P),
     "vt_wait_check": (_P, _P),
+    "vt_error_word_create": (_P,),
 }
 _fn = {}
 _get_device = torch.cuda.current_device
@@ -52,22 +53,27 @@ _error_words = {}
 
 
 def _error_word(index: int) -> int:
-    """Address of the device word where a product's kernel reports that one of its waits has run out."""
-    t = _error_words.get(index)
-    if t is None:
-        t = _error_words[index] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{index}")
-    return t.data_ptr()
+    """Address of the word where a product's kernel on that device reports that one of its waits has run out: host
+    memory, which is not a graph's even if the first product is captured."""
+    word = _error_words.get(index)
+    if word is None:
+        p = _P()
+        check(_call("vt_error_word_create")(C.addressof(p)), "vt_error_word_create")
+        word = _error_words.setdefault(index, C.c_uint32.from_address(p.value))
+    return C.addressof(word)
 
 
 def raise_errors(device=None):
     """Waits for the device and raises if a product's kernel gave up there since the last call."""
     i = torch.cuda.current_device() if device is None else torch.device(device).index
-    t = _error_words.get(torch.cuda.current_device() if i is None else i)
-    if t is not None:
-        torch.cuda.synchronize(t.device)
-        code = int(t.item())
+    if i is None:
+        i = torch.cuda.current_device()
+    word = _error_words.get(i)
+    if word is not None:
+        torch.cuda.synchronize(i)
+        code = word.value
         if code:
-            t.zero_()
+            word.value = 0
             _fail(f"a microscaled product's kernel gave up waiting (status {code}); its outputs "
                   "are not valid")
 
