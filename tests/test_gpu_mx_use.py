@@ -132,6 +132,24 @@ def test_a_wait_that_runs_out_is_reported():
     assert torch.equal(mx.linear4(z, w), want)
 
 
+@pytest.mark.parametrize("call", ["linear4", "linear_backward", "act_linear"])
+def test_the_next_product_tells_of_a_kernel_that_gave_up(call):
+    from vorotracing_b200 import mx
+
+    z, w = values(300, 96, torch.bfloat16).requires_grad_(), values(40, 96, torch.bfloat16, 1).requires_grad_()
+    w4, g = mx.quantize4(w.detach()), values(300, 40, torch.bfloat16, 2)
+    _, ckpt = mx.act_checkpoint(z.detach())
+    f = {"linear4": lambda: mx.linear4(z.detach(), w4), "linear_backward": lambda: mx.linear_backward(g, w.detach(), ckpt)[0],
+         "act_linear": lambda: torch.autograd.grad(mx.act_linear(z, w), z, g)[0]}[call]
+    want = f()
+    mx._launch("vt_wait_check", 0, mx._error_word(0))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        f()
+    assert torch.equal(f(), want)
+    mx.raise_errors()
+
+
 FIRST_CALL_IN_A_GRAPH = """
 import torch
 from vorotracing_b200 import mx

@@ -14,6 +14,7 @@ row, activations outnumber weights by far, so they decide both of its forms:
     colours = decoder(ray_features(rgba, rays))     # trains as any module
     fast = decoder.quantized()
     colours = fast(ray_features(rgba, rays))
+    mx.raise_errors()   # waits; raises if a kernel gave up (else the next call of a layer does)
 """
 from __future__ import annotations
 

@@ -17,6 +17,12 @@ a CUDA device, kernels run on torch's current stream, outputs are new tensors
 there; matrices may have any row stride.  Elementwise operators take float32,
 float16 and bfloat16, products the 16-bit types.  A block of 32 columns that
 holds a NaN or an infinity is NaN in either format.
+
+Every wait inside a product's kernel ends after about a second.  A kernel that
+gave up has outputs that are not valid: the next product called after it has
+ended raises, as an asynchronous error of CUDA does, and ``raise_errors`` waits
+for the device and tells at once.  A loop of training steps learns of it in the
+step after; what must not use such outputs calls ``raise_errors`` first.
 """
 from __future__ import annotations
 
@@ -60,7 +66,15 @@ def _error_word(index: int) -> int:
         p = _P()
         check(_call("vt_error_word_create")(C.addressof(p)), "vt_error_word_create")
         word = _error_words.setdefault(index, C.c_uint32.from_address(p.value))
+    if word.value:
+        _gave_up(word)
     return C.addressof(word)
+
+
+def _gave_up(word):
+    code, word.value = word.value, 0
+    _fail(f"a microscaled product's kernel gave up waiting (status {code}); its outputs "
+          "are not valid")
 
 
 def raise_errors(device=None):
@@ -71,11 +85,8 @@ def raise_errors(device=None):
     word = _error_words.get(i)
     if word is not None:
         torch.cuda.synchronize(i)
-        code = word.value
-        if code:
-            word.value = 0
-            _fail(f"a microscaled product's kernel gave up waiting (status {code}); its outputs "
-                  "are not valid")
+        if word.value:
+            _gave_up(word)
 
 
 def _call(name):
