@@ -434,7 +434,8 @@ VT_API vt_status vt_mx8_dequantize(const int8_t *codes, const uint8_t *exps, uin
                                    uint32_t cols, int dtype, void *out, vt_stream stream);
 /* Gradients of y = act(z) W^T + b, weight (outs, cols), from the 8-bit z:
  * dz (rows, cols) = (dy W) * act'(z8), dw (outs, cols) = dy^T act(z8),
- * db (outs) = column sums of dy.  Any output may be null.  copies: 1 if dy's
+ * db (outs) = column sums of dy.  act(z8) enters dw rounded to the matrices'
+ * type, in whose range it has to lie.  Any output may be null.  copies: 1 if dy's
  * rows do not start on 16 bytes (pointer or stride), plus 2 if the weight's do
  * not; the workspace then has room for copies that do.  The workspace is
  * 32-byte aligned.  err gets VT_ERR_CUDA

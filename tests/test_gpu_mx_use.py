@@ -1,5 +1,5 @@
 """The microscaled operators as programs use them: copies and files of their objects, memory between
-steps, 32-bit parameters, a wait that runs out."""
+steps, 32-bit parameters, a wait that runs out, types that do not fit."""
 import copy
 import io
 import os
@@ -178,3 +178,22 @@ def test_the_first_product_may_be_captured():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_GRAPH], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "reported" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("outs", [16, 300])
+def test_activations_beyond_float16(outs):
+    """z has values that float16 does not hold: bfloat16 products take them, float16 ones have to refuse, since
+    act(z8) is rounded to the products' type (and an infinity times a masked ray's zero is a NaN)."""
+    from vorotracing_b200 import mx
+
+    z, dy, w = values(100, 64, torch.float32, scale=1.0), values(100, outs, torch.bfloat16, 1), values(outs, 64, torch.bfloat16, 2)
+    z[3, 5] = 3e5
+    dy[7] = 0
+    for t in (torch.float32, torch.bfloat16):
+        _, ckpt = mx.act_checkpoint(z.to(t), "relu")
+        assert all(g.isfinite().all() for g in mx.linear_backward(dy, w, ckpt))
+        with pytest.raises(RuntimeError, match="checkpoint of float16 values"):
+            mx.linear_backward(dy.half(), w.half(), ckpt)
+    z = z.clamp(max=65504).half()
+    _, ckpt = mx.act_checkpoint(z, "relu")
+    assert all(g.isfinite().all() for g in mx.linear_backward(dy.half() / 1024, w.half(), ckpt))

@@ -230,19 +230,19 @@ class Checkpoint(_Blocks):
 
     codes (rows, 32 B) int8, exps (rows, B) uint8, B = ceil(cols / 32)."""
 
-    __slots__ = ("act", "_act")
+    __slots__ = ("act", "_act", "dtype")  # dtype: z's, None if unknown
     _dtype, _per_block, _align = torch.int8, BLOCK, 32
 
     def __init__(self, codes, exps, cols: int, act: str):
         self._act = _act_code(act)
-        self.act = act
+        self.act, self.dtype = act, None
         self._take(codes, exps, cols)
 
     @classmethod
     def _of(cls, buf, rows: int, cols: int, act: str):
         """A checkpoint from its buffer."""
         ckpt = cls.__new__(cls)
-        ckpt.act, ckpt._act, ckpt._codes, ckpt._exps = act, _act_code(act), None, None
+        ckpt.act, ckpt._act, ckpt.dtype, ckpt._codes, ckpt._exps = act, _act_code(act), None, None, None
         ckpt._buf, ckpt.rows, ckpt.cols = buf, rows, cols
         return ckpt
 
@@ -272,7 +272,7 @@ def act_checkpoint(z: torch.Tensor, act: str = "silu"):
     m, rows, cols, stride, dtype = _matrix(z, "z")
     h = m.new_empty(z.shape)
     ckpt = Checkpoint.__new__(Checkpoint)
-    ckpt.act, ckpt._act = act, code
+    ckpt.act, ckpt._act, ckpt.dtype = act, code, m.dtype
     ckpt._new(m, rows, cols)
     index, codes, exps = ckpt._place()
     _launch("vt_mx8_checkpoint", index, m.data_ptr(), dtype, rows, cols, stride, code, h.data_ptr(), codes, exps)
@@ -299,13 +299,18 @@ def linear_backward(dy: torch.Tensor, weight: torch.Tensor, ckpt: Checkpoint, bi
     dy (..., outs) and weight (outs, cols) in the same 16-bit type.  Returns
     (dz, dw, db) in that type: dz (..., cols) = (dy W) * act'(z8), dw (outs,
     cols) = dy^T act(z8) and db (outs) = column sums of dy; None for those not
-    asked for."""
+    asked for.  act(z8) enters dw rounded to that type, as the forward pass's
+    own activations do; a checkpoint of values beyond float16's range takes
+    bfloat16 products."""
     m, rows, outs, dy_stride, dtype = _matrix(dy, "dy", _PRODUCT_TYPES)
     w, w_rows, cols, w_stride, w_type = _matrix(weight, "weight", _PRODUCT_TYPES)
     if w_rows != outs or weight.dim() != 2:
         _fail(f"weight had shape {tuple(weight.shape)}, expected ({outs}, columns)")
     if w_type != dtype:
         _fail("weight must have the dtype of dy")
+    if dtype == 1 and ckpt.dtype not in (torch.float16, None):
+        _fail("float16 products take a checkpoint of float16 values, which have its range; this one was made of "
+              + str(ckpt.dtype).replace("torch.", ""))
     if rows != ckpt.rows or cols != ckpt.cols:
         _fail(f"dy has {rows} rows and weight {cols} columns, the checkpoint has {ckpt.rows} "
               f"rows of {ckpt.cols}")
