@@ -21,7 +21,8 @@
 // eight times the bytes; one warp brings them in instead, without a copy to whole words before.
 //
 // Layers of up to 64 columns would leave half of the lanes empty; they get W twice instead (FOLD),
-// and each half of the lanes takes half of a tile's rows.
+// and each half of the lanes takes half of a tile's rows: the second product of a half's rows leaves the other
+// half's lanes as they are.  (Zeros in their place would make an infinity in dy a NaN of every column.)
 //
 // Measured (bfloat16, a B200, in a loop of calls): 1088640 rows, 256 -> 256, SiLU: 404 us, 3.5 TB/s of
 // what it has to read and write (floor at 6.45 TB/s: 218 us).  What bounds it: with 256 outputs dW, W and
@@ -231,8 +232,13 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             if (mine) {
                 if (a.dw_parts || a.dw)
 #pragma unroll
-                    for (uint32_t k = 0; k < TILE_ROWS / 16u; ++k)
-                        tc::mma_f16_tmem(tmem, from + k * 16u, b + k * 128u, ID, k != 0 || t != group);
+                    for (uint32_t k = 0; k < TILE_ROWS / 16u; ++k) {
+                        if (FOLD)  // each half of the lanes adds its own half of the tile's rows
+                            tc::mma_f16_tmem_half(tmem, from + k * 16u, b + k * 128u, ID, k >= TILE_ROWS / 32u,
+                                                  k % (TILE_ROWS / 32u) != 0 || t != group);
+                        else
+                            tc::mma_f16_tmem(tmem, from + k * 16u, b + k * 128u, ID, k != 0 || t != group);
+                    }
                 // db += dy^T ones.  Of an odd number of chunks the last tile's upper 64 outputs are whatever
                 // follows in shared memory; they are not read.
                 if (sums)
@@ -363,7 +369,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             if (!ok) break;
             tc::fence_after();
             const uint8_t *codes = smem + r.i * P::STAGE + P::DY_BYTES + code0;
-            const uint32_t buffer = dh_at + dh.i * TILE_ROWS + lanes, here = buffer + row0;
+            const uint32_t here = dh_at + dh.i * TILE_ROWS + lanes + row0;
             const uint32_t count = t == last ? last_count : ROWS;
 #pragma unroll
             for (int p = 0; p < ROWS; p += 16) {
@@ -390,10 +396,6 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                 }
                 // the activations go where the dH that this warp has read was
                 tc::tmem_store8(here + p, h);
-                if (FOLD) {  // this half of the lanes has no part in the other half's rows
-                    const uint32_t none[8] = {};
-                    tc::tmem_store8(buffer + (row0 ^ (TILE_ROWS / 2u)) + p, none);
-                }
                 if (p + 16 == ROWS) {
                     tc::tmem_wait_store();
                     tc::fence_before();

@@ -231,6 +231,14 @@ __device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b,
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
+// The same for one half of the lanes of D (0..63 or 64..127); the other half keeps its values.
+__device__ __forceinline__ void mma_f16_tmem_half(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool upper, bool accumulate)
+{
+    const uint32_t off01 = upper ? ~0u : 0u, off23 = ~off01;  // a set bit: this lane is not written
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %6, %6}, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(off01), "r"(off23) : "memory");
+}
 // The barrier gets one arrival when the products issued so far by this thread are done.
 __device__ __forceinline__ void commit(uint64_t *bar)
 {
