@@ -1,0 +1,57 @@
+"""Products of whole numbers, whose sums are exact in binary32 whatever their order: results are the exact sums
+rounded once, so that one lost or repeated tile, stage or part of k shows in thousands of elements.
+
+Sums stay below 2^24: rows (or columns) times the largest product.  8-bit blocks hold whole numbers up to 127, 4-bit
+blocks -3 to 3."""
+import pytest
+import torch
+
+from test_gpu_mx import TYPES16, no_kernel_gave_up  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def whole(rows, cols, most, seed, dtype=torch.float64):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-most, most + 1, (rows, cols), generator=g, device="cuda").to(dtype)
+
+
+LINEAR = [(60001, 64, 3), (60001, 40, 64), (60000, 16, 16), (60000, 56, 250), (30011, 256, 256), (30011, 200, 130), (30000, 136, 70), (30000, 96, 192),
+          (177, 64, 64), (20011, 520, 300), (30001, 48, 427), (3001, 96, 5000), (9001, 777, 1301), (100000, 8, 8), (200000, 130, 1), (150001, 24, 260)]
+
+
+@pytest.mark.parametrize("act", ["identity", "relu"])
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("rows,cols,outs", LINEAR)
+def test_gradients_of_whole_numbers(rows, cols, outs, dtype, act):
+    from vorotracing_b200 import mx
+
+    z, dy, w = whole(rows, cols, 2, 0), whole(rows, outs, 1, 1), whole(outs, cols, 2, 2)
+    z[:, 0] = 2  # no block is all zeros
+    dy[rows // 3] = 0
+    _, ckpt = mx.act_checkpoint(z.to(dtype), act)
+    assert torch.equal(ckpt.dequantize().double(), z)
+    h, slope = (z.clamp(min=0), (z > 0).double()) if act == "relu" else (z, 1.0)
+    got = mx.linear_backward(dy.to(dtype), w.to(dtype), ckpt)
+    for name, a, b in zip(("dz", "dw", "db"), got, ((dy @ w) * slope, dy.t() @ h, dy.sum(0))):
+        b = b.to(dtype)
+        assert torch.equal(a, b), f"{name}: {int((a != b).sum())} of {b.numel()} differ"
+
+
+LINEAR4 = [(1, 4096, 4096), (77, 1000, 333), (500, 2000, 1000), (60001, 192, 64), (60001, 96, 48), (41000, 300, 100), (41000, 600, 256), (40961, 40, 130),
+           (20001, 520, 600), (9601, 91, 195), (2049, 4100, 1300), (100000, 64, 3), (5000, 2056, 449)]
+
+
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("rows,cols,outs", LINEAR4)
+def test_4_bit_products_of_whole_numbers(rows, cols, outs, dtype):
+    from vorotracing_b200 import mx
+
+    x, w, b = whole(rows, cols, 3, 0), whole(outs, cols, 3, 1), whole(1, outs, 3, 2)[0]
+    w4 = mx.quantize4(w.float())
+    assert torch.equal(w4.dequantize().double(), w) and torch.equal(mx.quantize4(x.to(dtype)).dequantize().double(), x)
+    for act in ("identity", "relu"):
+        got = mx.linear4(x.to(dtype), w4, b.to(dtype), act)
+        want = x @ w.t() + b
+        want = (want.clamp(min=0) if act == "relu" else want).to(dtype)
+        assert torch.equal(got, want), f"{int((got != want).sum())} of {want.numel()} differ"
