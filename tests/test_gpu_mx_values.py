@@ -1,10 +1,10 @@
-"""Infinities in upstream gradients, as a loss scale that is too large makes them: they spread as far as the
-formulas say and no further."""
+"""Infinities and NaN in every kernel, and rows with gaps: they spread as far as the
+formulas say and no further, and what lies between the rows is not read."""
 import pytest
 import torch
 
 import mx_reference as R
-from test_gpu_mx import TYPES16, no_kernel_gave_up  # noqa: F401
+from test_gpu_mx import TYPES16, no_kernel_gave_up, values  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,76 @@ def test_infinite_gradients(rows, cols, outs, dtype):
         for got, want in zip(mx.linear_backward(dy, w, ckpt), (d @ w.double(), d.t() @ z8, d.sum(0))):
             assert not want.isnan().any() and want.isinf().any()
             same_kind(got, want)
+
+
+# linear4: one CTA a tile with x as it is and as a copy, pairs of CTAs with x read in whole words and not, k split
+LINEAR4 = [(9700, 90, 48), (9700, 96, 48), (9700, 91, 200), (9700, 96, 256), (5000, 96, 512), (5000, 91, 512), (5000, 300, 449), (100, 600, 200)]
+
+
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("rows,cols,outs", LINEAR4)
+def test_nan_and_infinite_blocks_of_4_bits(rows, cols, outs, dtype):
+    """A block of x that holds one makes its row NaN, a block of the weight its output; all else keeps its value."""
+    from vorotracing_b200 import mx
+
+    x, wide = values(rows, cols, dtype, scale=1.0), values(outs, cols, torch.float32, 1, 0.3)
+    w = mx.quantize4(wide)
+    want = mx.linear4(x, w)
+    assert want.isfinite().all()
+    bad = x.clone()
+    hit = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for row, col, v in ((0, 0, "nan"), (rows // 2, cols - 1, "inf"), (rows - 1, cols // 2, "-inf"), (rows // 2 + 1, 33, "nan")):
+        bad[row, col] = float(v)
+        hit[row] = True
+    y = mx.linear4(bad, w)
+    assert y[hit].isnan().all() and torch.equal(y[~hit], want[~hit])
+    out = torch.zeros(outs, dtype=torch.bool, device="cuda")
+    for o, col, v in ((0, 1, "inf"), (outs // 2, cols - 1, "nan"), (outs - 1, 32, "-inf")):
+        wide[o, col] = float(v)
+        out[o] = True
+    y = mx.linear4(x, mx.quantize4(wide))
+    assert y[:, out].isnan().all() and torch.equal(y[:, ~out], want[:, ~out])
+
+
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("rows,cols,outs", LINEAR4)
+def test_4_bit_products_of_rows_with_gaps(rows, cols, outs, dtype):
+    from vorotracing_b200 import mx
+
+    x, w = values(rows, cols, dtype, scale=1.0), mx.quantize4(values(outs, cols, torch.float32, 1, 0.3))
+    want = mx.linear4(x, w)
+    for gap, shift in ((8 + -cols % 8, 0), (8 + -cols % 8, 8), (3, 0), (2, 5), (-cols % 2 + 2, 2)):
+        m = torch.full((rows * (cols + gap) + shift,), float("nan"), dtype=dtype, device="cuda")
+        v = m[shift:].view(rows, cols + gap)[:, :cols]
+        v.copy_(x)
+        assert torch.equal(mx.linear4(v, w), want)
+
+
+LINEAR = [(3000, 96, 300), (3001, 48, 427), (5000, 300, 1000), (3000, 64, 70), (3001, 40, 5), (3000, 200, 256)]
+
+
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("rows,cols,outs", LINEAR)
+def test_nan_blocks_of_8_bits(rows, cols, outs, dtype):
+    """dz is NaN in the block's own row and columns, dW in its columns; all else keeps its value."""
+    from vorotracing_b200 import mx
+
+    for act in ("identity", "relu", "silu", "gelu_tanh"):
+        z, dy, w = values(rows, cols, dtype, scale=1.0), values(rows, outs, dtype, 1, 0.5), values(outs, cols, dtype, 2, 0.3)
+        _, ckpt = mx.act_checkpoint(z, act)
+        want = mx.linear_backward(dy, w, ckpt)
+        column = torch.zeros(cols, dtype=torch.bool, device="cuda")
+        element = torch.zeros((rows, cols), dtype=torch.bool, device="cuda")
+        for row, col, v in ((0, 0, "nan"), (rows - 1, cols - 1, "inf"), (rows // 2, 1, "-inf")):
+            z[row, col] = float(v)
+            first = col // 32 * 32
+            column[first:first + 32] = True
+            element[row, first:first + 32] = True
+        _, ckpt = mx.act_checkpoint(z, act)
+        dz, dw, db = mx.linear_backward(dy, w, ckpt)
+        # the slope of the identity is 1 whatever the value
+        if act == "identity":
+            assert torch.equal(dz[~element], want[0][~element])
+        else:
+            assert dz[element].isnan().all() and torch.equal(dz[~element], want[0][~element])
+        assert dw[:, column].isnan().all() and torch.equal(dw[:, ~column], want[1][:, ~column]) and torch.equal(db, want[2])
