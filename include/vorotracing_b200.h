@@ -408,7 +408,7 @@ VT_API vt_status vt_quantize_u8(const float *src, uint64_t count, float scale, f
  *   8 bits: codes (rows, 32 B) i8, exps (rows, B) u8, B = ceil(cols / 32);
  *           value = code * 2^(E - 133), E >= 7
  *   4 bits: codes (rows, 16 B) u8, the even column in the low nibble, exps
- *           (rows, B) u8; value = e2m1 * 2^(E - 127), E >= 1
+ *           (rows, B) u8; value = e2m1 * 2^(E - 127); written with E >= 1
  * E = 255 marks a block that held a NaN or an infinity: its values are NaN.
  * 8-bit codes are 32-byte aligned, 4-bit codes 16-byte.  Other matrices are row-major with a row stride
  * in elements; outputs are dense.  An element type is VT_F32, VT_F16 or

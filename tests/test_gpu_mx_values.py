@@ -108,3 +108,24 @@ def test_nan_blocks_of_8_bits(rows, cols, outs, dtype):
         else:
             assert dz[element].isnan().all() and torch.equal(dz[~element], want[0][~element])
         assert dw[:, column].isnan().all() and torch.equal(dw[:, ~column], want[1][:, ~column]) and torch.equal(db, want[2])
+
+
+def test_every_exponent_of_4_bits():
+    """Matrices that were quantised elsewhere: all of a byte's scales, 2^-127 to 2^127."""
+    from vorotracing_b200 import mx
+
+    exps = torch.arange(255, device="cuda").to(torch.uint8).view(255, 1)
+    codes = torch.arange(16, device="cuda").to(torch.uint8).expand(255, 16).contiguous()  # the even columns: every code
+    q = mx.MX4(codes, exps, 32)
+    table = torch.tensor([s * v for s in (1, -1) for v in R.E2M1], dtype=torch.float64, device="cuda")
+    want = torch.zeros((255, 32), dtype=torch.float64, device="cuda")
+    want[:, ::2] = table * torch.exp2(exps.double() - 127)
+    got = q.dequantize()
+    assert torch.equal(got, want.float()) and got[0, 2] == 2.0 ** -128
+    # products of the smallest scales with large values: sums of exact products, 16 terms
+    x = torch.full((3, 32), 2.0 ** 100, dtype=torch.bfloat16, device="cuda")
+    x[1] = -x[1]
+    low = mx.MX4(codes[:4, :].contiguous(), exps[:4].contiguous(), 32)
+    low.codes[:, 8:] = 0  # no negatives: 21 units in a row
+    want = x.double() @ low.dequantize().double().t()
+    assert torch.equal(mx.linear4(x, low), want.bfloat16()) and (want != 0).all()

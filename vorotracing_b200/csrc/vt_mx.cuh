@@ -211,9 +211,9 @@ __device__ __forceinline__ float mx8_scale(uint32_t E)
 }
 // 2^-e and 2^e of a 4-bit block.
 __device__ __forceinline__ float mx4_inverse(uint32_t E) { return __uint_as_float((254u - E) << 23); }
-__device__ __forceinline__ float mx4_scale(uint32_t E)
+__device__ __forceinline__ float mx4_scale(uint32_t E)  // E = 0, which is never written here, is 2^-127
 {
-    return __uint_as_float(E == 255u ? 0x7fc00000u : E << 23);
+    return __uint_as_float(E == 255u ? 0x7fc00000u : E == 0u ? 0x00400000u : E << 23);
 }
 // Four 8-bit codes in a word.  Adding 1.5 2^23 rounds to the nearest whole number, ties to even, and leaves
 // it in the low byte: two instructions a pair, where conversions would share the pipe of the activations'
