@@ -406,7 +406,7 @@ VT_API vt_status vt_quantize_u8(const float *src, uint64_t count, float scale, f
  * No reference counterpart.  Microscaled formats: a row is cut into blocks of
  * 32 columns (the last one padded with zeros), each with one exponent byte E.
  *   8 bits: codes (rows, 32 B) i8, exps (rows, B) u8, B = ceil(cols / 32);
- *           value = code * 2^(E - 133), E >= 7
+ *           value = code * 2^(E - 133); written with E >= 7
  *   4 bits: codes (rows, 16 B) u8, the even column in the low nibble, exps
  *           (rows, B) u8; value = e2m1 * 2^(E - 127); written with E >= 1
  * E = 255 marks a block that held a NaN or an infinity: its values are NaN.

@@ -129,3 +129,28 @@ def test_every_exponent_of_4_bits():
     low.codes[:, 8:] = 0  # no negatives: 21 units in a row
     want = x.double() @ low.dequantize().double().t()
     assert torch.equal(mx.linear4(x, low), want.bfloat16()) and (want != 0).all()
+
+
+@pytest.mark.parametrize("outs", [5, 40, 300])
+def test_every_exponent_of_8_bits(outs):
+    """Checkpoints that were made elsewhere: scales below those that act_checkpoint writes."""
+    from vorotracing_b200 import mx
+
+    exps = torch.arange(255, device="cuda").to(torch.uint8).view(255, 1)
+    codes = (torch.arange(32, device="cuda") * 8 - 128).to(torch.int8).expand(255, 32).contiguous()
+    ckpt = mx.Checkpoint(codes, exps, 32, "identity")
+    z8 = codes.double() * torch.exp2(exps.double() - 133)
+    z8[254] = z8[254].float().double()  # -128 there is 2^128, an infinity
+    assert torch.equal(ckpt.dequantize(), z8.float()) and (ckpt.dequantize()[0, :16] < 0).all()
+    # act_backward and the slope of z below zero and above
+    ckpt = mx.Checkpoint(codes, exps, 32, "relu")
+    dz = mx.act_backward(torch.ones((255, 32), device="cuda"), ckpt)
+    assert torch.equal(dz, (z8 > 0).float())
+    # the smallest scales alone: dW is the sum of a row's values times a large number
+    few = mx.Checkpoint(codes[:8].contiguous(), exps[:8].contiguous(), 32, "identity")
+    dy = torch.zeros((8, outs), dtype=torch.bfloat16, device="cuda")
+    dy[0], dy[6] = 2.0 ** 100, 2.0 ** 100
+    w = torch.ones((outs, 32), dtype=torch.bfloat16, device="cuda")
+    dw = mx.linear_backward(dy, w, few)[1]
+    want = dy.double().t() @ z8[:8].bfloat16().double()
+    assert torch.equal(dw, want.bfloat16()) and (want[:, 20:] > 0).all()

@@ -203,11 +203,12 @@ __device__ __forceinline__ uint32_t mx4_exponent(uint32_t top_bits)
     const uint32_t f = top_bits >> 23;
     return f == 255u ? 255u : f < 3u ? 1u : f - 2u;
 }
-// 2^(6 - e) and 2^(e - 6) of an 8-bit block.  E = 255 gives 2^-122 (its codes are set to zero) and NaN.
+// 2^(6 - e) and 2^(e - 6) of an 8-bit block.  E = 255 gives 2^-122 (its codes are set to zero) and NaN.  Below 7,
+// which is never written here, the scale is a subnormal number.
 __device__ __forceinline__ float mx8_inverse(uint32_t E) { return __uint_as_float((260u - E) << 23); }
 __device__ __forceinline__ float mx8_scale(uint32_t E)
 {
-    return __uint_as_float(E == 255u ? 0x7fc00000u : (E - 6u) << 23);
+    return __uint_as_float(E == 255u ? 0x7fc00000u : E < 7u ? 1u << (E + 16u) : (E - 6u) << 23);
 }
 // 2^-e and 2^e of a 4-bit block.
 __device__ __forceinline__ float mx4_inverse(uint32_t E) { return __uint_as_float((254u - E) << 23); }
@@ -291,8 +292,8 @@ __device__ __forceinline__ void act_pair(f32x2 x, f32x2 &value, f32x2 &slope)
     if constexpr (ACT == ACT_RELU) {
         const float2 v = unpair(x);
         value = pair(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
-        if constexpr (SLOPE)  // x * 0 hands a NaN on
-            slope = pair(v.x > 0.0f ? 1.0f : v.x * 0.0f, v.y > 0.0f ? 1.0f : v.y * 0.0f);
+        if constexpr (SLOPE)  // of a zero itself, and of a NaN
+            slope = pair(v.x > 0.0f ? 1.0f : v.x < 0.0f ? 0.0f : v.x, v.y > 0.0f ? 1.0f : v.y < 0.0f ? 0.0f : v.y);
     } else if constexpr (ACT == ACT_SILU) {
         const f32x2 p = logistic2(mul2(x, both(-LOG2_E)));
         value = mul2(x, p);
