@@ -197,3 +197,31 @@ def test_activations_beyond_float16(outs):
     z = z.clamp(max=65504).half()
     _, ckpt = mx.act_checkpoint(z, "relu")
     assert all(g.isfinite().all() for g in mx.linear_backward(dy.half() / 1024, w.half(), ckpt))
+
+
+def test_the_4_bit_decoder_is_off_by_its_format_alone():
+    """Against its layers in 64 bits on the 4-bit values of weights and inputs, each output rounded to bfloat16 as the
+    operator's is.  A sum in binary32 may round to the other neighbour in bfloat16 (about one in a thousand: 2^-23 times
+    some terms for steps of 2^-8), and a few of those tip a 4-bit code of the next layer: far less than a hundredth of
+    the squared error that the codes themselves cost."""
+    import mx_reference as R
+    from test_gpu_decoder import view
+    from vorotracing_b200.decoder import RayDecoder, ray_features
+
+    rgba, rays = view()
+    x = ray_features(rgba, rays).view(-1, 16)
+    torch.manual_seed(5)
+    decoder = RayDecoder(features=16, hidden=64, layers=2)
+    with torch.no_grad():
+        for b in decoder.biases:
+            b.uniform_(-0.2, 0.2)
+        whole = decoder(x)
+    y4 = decoder.quantized()(x)
+    y = x
+    for i, (w, b) in enumerate(zip(decoder.weights, decoder.biases)):
+        last = i + 1 == len(decoder.weights)
+        pre = R.round4(y)[0] @ R.round4(w.detach())[0].t() + b.detach().double()
+        y = R.act(pre, "identity" if last else "silu").bfloat16()
+    square = lambda a, b: float((a.double() - b.double()).square().mean())
+    cost = square(y, whole)
+    assert cost > 0 and square(y4, y) <= 0.01 * cost
