@@ -54,19 +54,22 @@ def test_backward_frees_the_checkpoints():
     loss still held."""
     from vorotracing_b200 import mx
 
+    def asked_for():  # of the allocator, whose blocks may be larger
+        return torch.cuda.memory_stats()["requested_bytes.all.current"]
+
     rows, cols = 4096, 256
     z = values(rows, cols, torch.bfloat16, scale=1.0).requires_grad_()
     w = values(64, cols, torch.bfloat16, 1, 0.1).requires_grad_()
     mx.act_linear(z, w, None, "silu").float().square().sum().backward()  # what libraries keep from their first call on
     z.grad = w.grad = None
-    before = torch.cuda.memory_allocated()
+    before = asked_for()
     y = mx.act_linear(z, w, None, "silu")
-    kept = torch.cuda.memory_allocated() - before - y.numel() * 2
+    kept = asked_for() - before - y.numel() * 2
     assert rows * cols * 33 // 32 <= kept < rows * cols * 33 // 32 + 1024
     loss = y.float().square().sum()
     del y
     loss.backward()
-    assert torch.cuda.memory_allocated() - before < (rows * cols + 64 * cols) * 2 + 4096 and loss.isfinite()
+    assert asked_for() - before < (rows * cols + 64 * cols) * 2 + 4096 and loss.isfinite()
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
