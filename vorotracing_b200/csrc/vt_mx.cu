@@ -2,14 +2,16 @@
 // activation checkpoints in 8 bits, the activation's gradient from them, and
 // 4-bit quantisation.
 //
-// All are one pass over the data and bound by HBM.  Four lanes share a block of
+// All are one pass over the data, for which HBM is the floor.  Four lanes share a block of
 // 32 columns, 8 columns a lane, so a lane reads and writes 16-byte words of the
 // 16-bit types, and a block's largest magnitude is two shuffles away.  Magnitudes
 // are compared as integers: the bits of |x| order like |x|, with infinities and
 // NaN on top, which is what the exponent rule wants.
 //
 // Measured (1088640 x 64, binary16, SiLU): checkpoint and gradient together 134 to 149 us, 4.7 to 5.2 TB/s
-// of 6.45; 4 bits and back on 1000000 x 192 binary32: 306 to 317 us, 5.5 TB/s.  The exponential and the reciprocal
+// of 6.45 (floor 109 us); 4 bits and back on 1000000 x 192 binary32: 305 to 318 us, 5.5 TB/s; 8 bits to binary16 on the first
+// matrix 44 us (floor 33), 4 bits to binary16 52 us (floor 27).  Neither HBM nor the issue slots are full: 38 to 46 % and
+// 62 to 66 % under the counters.  The exponential and the reciprocal
 // of an activation share a pipe of 16 lanes an SM, which is half busy: conversions are kept off it.  Two
 // items a thread in flight cost registers and were slower (186 us); so was a grid without a loop (151 us).
 #include "vt_mx.cuh"

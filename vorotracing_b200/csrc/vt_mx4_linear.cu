@@ -20,11 +20,12 @@
 // sums meet in distributed shared memory, where they are added in the order of k.  One launch; the
 // weight is spread over as many SMs as there are.
 //
-// Measured (bfloat16): 1088640 rows, 192 -> 64, SiLU: 115 to 123 us, 4.5 to 4.9 TB/s (floor 86 us), bound by
-// HBM; with x read by the rounding warps themselves 597 us.  One row, 4096 -> 4096: 12.5 us a call, of which
+// Measured (bfloat16): 1088640 rows, 192 -> 64, SiLU: 115 to 123 us, 4.5 to 4.9 TB/s (floor 86 us); no unit is full (DRAM 51 %,
+// issue 46 %, tensor pipe 3 % of their peaks on 500000 rows), so latency is what is left, and what of it was not
+// found.  With x read by the rounding warps themselves 597 us.  One row, 4096 -> 4096: 12.5 us a call, of which
 // the host takes 10; 77 rows, 1000 -> 333: 12.6 us (33 us in the large tiles).
-// 4096 rows, 8192 -> 8192: 161 us, 3.4 PFLOP/s, bound by waits and issue between stages (floor 83 us; tiles of 192
-// outputs with more places for scales 179 us).  277867 rows, 91 -> 195: 138 us, of which copying x to whole words 24.
+// 4096 rows, 8192 -> 8192: 157 to 162 us, 3.4 PFLOP/s (floor 83 us), of which the pass that writes x's codes and both scales
+// takes a fifth.  277867 rows, 91 -> 195: 138 us, of which copying x to whole words 24.
 #include "vt_mx_rows.cuh"
 
 namespace vt {
@@ -364,9 +365,11 @@ __global__ void __launch_bounds__(L4<TN>::THREADS, 1)
 // A pair of CTAs shares a tile of 256 rows by 224 outputs: each stages its 128 rows of x and half of the
 // outputs' weights, so a byte of shared memory serves twice the products of a CTA alone.  224 outputs leave
 // room in tensor memory for two accumulators and two places of scales.
-// Measured: 4096 x 8192 x 8192 in 161 us, 3.4 PFLOP/s, twice what the bfloat16 library product reaches here
-// (one CTA a tile: 182 us).  What bounds it: a stage's 448 cycles of products start behind a wait for the
-// products two stages before, whose scales' place it takes, and the issue of copies and products, about 470.
+// Measured: 4096 x 8192 x 8192 in 157 to 162 us, 3.4 PFLOP/s, twice what the bfloat16 library product reaches here
+// (one CTA a tile: 182 us).  Under the counters stage4_kernel takes 33 us, at two thirds of its issue slots (its bytes
+// would take 13), and pair4_kernel 116 us: 757 cycles a stage, of which the tensor cores are busy 59 % with its 448 cycles of
+// products.  The rest is waits, of which kind was not found: more places for scales, in tiles of 192 outputs, made it
+// slower (179 us).
 
 constexpr uint32_t PAIR_N = 224, PAIR_A = 16384, PAIR_B = PAIR_N / 2 * 128, PAIR_STAGE = PAIR_A + PAIR_B + 3072, PAIR_STAGES = 6,
                    PAIR_THREADS = 256, PAIR_SF_AT = 2 * PAIR_N, PAIR_SF_COLS = 24;

@@ -10,7 +10,9 @@
 // over all the CTA's rows.  Between the two products sixteen warps take dH out of tensor memory,
 // read the 8-bit z, evaluate act and act' together (one logistic serves both), write dz, and put
 // act(z8) back into the place of dH as the second product's A operand, rounded to the operands'
-// 16-bit type as the forward pass's own activations are.  The column sums of dy are one more,
+// 16-bit type: what the forward pass multiplied by W was rounded to it too, so dW is the gradient of the
+// product that was computed.  Against 64 bits dW is off by 1.15 to 1.25 times what rounding dW itself costs.  (A second
+// operand for what the rounding left would cost half as much again of the tensor cores' time in wide layers.)  The column sums of dy are one more,
 // narrow product of the staged tile.  At its end a CTA writes its part of dW in binary32; a second
 // kernel adds the parts in order, so results do not depend on timing.
 //
@@ -24,10 +26,10 @@
 // and each half of the lanes takes half of a tile's rows: the second product of a half's rows leaves the other
 // half's lanes as they are.  (Zeros in their place would make an infinity in dy a NaN of every column.)
 //
-// Measured (bfloat16, a B200, in a loop of calls): 1088640 rows, 256 -> 256, SiLU: 404 us, 3.5 TB/s of
-// what it has to read and write (floor at 6.45 TB/s: 218 us).  What bounds it: with 256 outputs dW, W and
+// Measured (bfloat16, B200s, in a loop of calls): 1088640 rows, 256 -> 256, SiLU: 398 to 429 us by the GPU, 3.3 to 3.5 TB/s
+// of what it has to read and write (floor at 6.45 TB/s: 218 us).  What bounds it: with 256 outputs dW, W and
 // the column sums leave room for three buffers of dH, so one of the four sets of activation warps always
-// waits; a tile of 32 rows takes 1030 cycles where its bytes would take 700 (399 to 429 us by the GPU).  Steps on the way: rows in the
+// waits; a tile of 32 rows takes 1030 cycles where its bytes would take 700.  Steps on the way: rows in the
 // lanes, activations through shared memory 479 us; columns in the lanes 439; W in tensor memory instead of
 // shared memory 424; column sums on the tensor cores (a warp that added took as long as all else) 404.
 // 1614080 rows, 64 -> 3, ReLU: 98 us (floor 50 us), bound by the second product's warp: its wait, issue
@@ -38,8 +40,8 @@
 // tile: dz = (dy W) * act'(z8), with the slope in the epilogue, and dW = dy^T h with h = act(z8)
 // written once, in the operands' type, by a pass before it: as an operand it is read once for
 // every 256 outputs, and evaluating it as often would cost more than the tensor cores' time.
-// Measured (binary16): 8192 rows, 4096 -> 4096, GELU: 540 us, 1.02 PFLOP/s, at 1.56 GHz under the power
-// limit; the tensor cores are busy 68 % of the time there, dW's 256 tiles fill 3.5 rounds of 74 pairs.
+// Measured (binary16): 8192 rows, 4096 -> 4096, GELU: 516 to 547 us by the GPU, 1.01 to 1.07 PFLOP/s, at 1.56 GHz under
+// the power limit; the tensor cores are busy 68 % of the time there, dW's 256 tiles fill 3.5 rounds of 74 pairs.
 #include "vt_mx_rows.cuh"
 
 namespace vt {

@@ -12,11 +12,12 @@ layouts): 8 bits for what a training step keeps of a layer's pre-activations,
     w4 = quantize4(weight)                     # once
     y = linear4(x, w4, bias, "silu")           # act(q4(x) w4^T + b)
 
-``act_linear`` is the training pair as an autograd function.  Tensors live on
-a CUDA device, kernels run on torch's current stream, outputs are new tensors
-there; matrices may have any row stride.  Elementwise operators take float32,
-float16 and bfloat16, products the 16-bit types.  A block of 32 columns that
-holds a NaN or an infinity is NaN in either format.
+``act_linear`` is the training pair as an autograd function, and alone records
+gradients.  Tensors live on a CUDA device, kernels run on torch's current
+stream, outputs are new tensors there; matrices may have any row stride.
+Elementwise operators take float32, float16 and bfloat16, products the 16-bit
+types.  A block of 32 columns that holds a NaN or an infinity is NaN in either
+format.
 
 Every wait inside a product's kernel ends after about a second.  A kernel that
 gave up has outputs that are not valid: the next product called after it has
@@ -351,8 +352,9 @@ class _ActLinear(torch.autograd.Function):
 
 
 def act_linear(z: torch.Tensor, weight: torch.Tensor, bias=None, act: str = "silu"):
-    """y = act(z) W^T + b for training: between forward and backward only the
-    8-bit form of z is kept (33/32 byte a value), neither z nor act(z).  First derivatives only.
+    """y = act(z) W^T + b for training, the product by torch: between forward
+    and backward only the 8-bit form of z is kept (33/32 byte a value), neither
+    z nor act(z).  First derivatives only.
 
     z, weight and bias have one 16-bit type; under torch.autocast they may have
     any and are brought to its type, with gradients in their own."""
