@@ -55,3 +55,18 @@ def test_4_bit_products_of_whole_numbers(rows, cols, outs, dtype):
         want = x @ w.t() + b
         want = (want.clamp(min=0) if act == "relu" else want).to(dtype)
         assert torch.equal(got, want), f"{int((got != want).sum())} of {want.numel()} differ"
+
+
+@pytest.mark.parametrize("rows,cols,outs", [(153512, 16, 224), (200003, 33, 256), (153512, 96, 200), (60001, 300, 250), (153512, 16, 192), (200003, 16, 128), (200003, 8, 8)])
+def test_gradients_come_out_the_same_each_time(rows, cols, outs):
+    """Many tiles a block whose stores are slow against its products, and many calls: what depends on timing shows."""
+    from vorotracing_b200 import mx
+
+    z, dy, w = (whole(*s, 1, i, torch.float16) for i, s in enumerate(((rows, cols), (rows, outs), (outs, cols))))
+    _, ckpt = mx.act_checkpoint(z, "identity")
+    z8 = ckpt.dequantize().double()
+    want = [t.half() for t in (dy.double() @ w.double(), dy.double().t() @ z8, dy.double().sum(0))]
+    for _ in range(60):
+        for a, b in zip(mx.linear_backward(dy, w, ckpt), want):
+            assert torch.equal(a, b)
+    mx.raise_errors()

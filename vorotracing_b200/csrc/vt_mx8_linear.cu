@@ -61,7 +61,7 @@ template <int OC, bool FOLD> struct Narrow {
     static constexpr uint32_t STAGE = DY_BYTES + TILE_ROWS * CODE_PITCH;
     struct Ctrl {
         float scale[16][TILE_ROWS];  // of the blocks in each activation warp's rows
-        uint64_t full[12], empty[12], dh_full[8], h_full[8], w_full, done, failed;
+        uint64_t full[12], empty[12], dh_full[narrow_ready(OC)], h_full[narrow_buffers(OC)], w_full, done, failed;
         uint32_t tmem;
         tc::Fail fail;
     };
@@ -69,9 +69,9 @@ template <int OC, bool FOLD> struct Narrow {
     static constexpr uint32_t ONES_AT = STAGES * STAGE, CTRL_AT = ONES_AT + ONES, SMEM = CTRL_AT + sizeof(Ctrl);
     static constexpr uint32_t TMEM = 512;
     // columns of tensor memory: dW, W, db (16 for 128 outputs), and as many of dH as there is room for, up to six
-    static constexpr uint32_t W_AT = OC * 64u, MT = (OC + 1) / 2, DB_AT = W_AT + OC * 32u, DH_AT = DB_AT + MT * 16u, BUFS = OC == 4 ? 3 : OC == 3 ? 6 : 4;
+    static constexpr uint32_t W_AT = OC * 64u, MT = (OC + 1) / 2, DB_AT = W_AT + OC * 32u, DH_AT = DB_AT + MT * 16u, BUFS = narrow_buffers(OC), READY = narrow_ready(OC);
     static constexpr int ROWS = FOLD ? TILE_ROWS / 2 : TILE_ROWS;  // of a tile an activation warp takes
-    static_assert(STAGES >= 4 && STAGES > BUFS && DH_AT + BUFS * TILE_ROWS <= TMEM, "does not fit an SM");
+    static_assert(NARROW_SETS == 4 && READY >= 4 && STAGES >= 4 && STAGES > BUFS && DH_AT + BUFS * TILE_ROWS <= TMEM, "does not fit an SM");
 };
 
 struct NarrowArgs {
@@ -131,10 +131,8 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             tc::mbar_init(&s.full[i], tiny ? 2 : 1);
             tc::mbar_init(&s.empty[i], 1);
         }
-        for (uint32_t i = 0; i < P::BUFS; ++i) {
-            tc::mbar_init(&s.dh_full[i], 1);
-            tc::mbar_init(&s.h_full[i], 4);
-        }
+        for (uint32_t i = 0; i < P::READY; ++i) tc::mbar_init(&s.dh_full[i], 1);
+        for (uint32_t i = 0; i < P::BUFS; ++i) tc::mbar_init(&s.h_full[i], 4);
         tc::mbar_init(&s.w_full, 16);
         tc::mbar_init(&s.done, 1);
         tc::mbar_init(&s.failed, 1);
@@ -188,7 +186,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
         constexpr uint32_t ID = tc::idesc_f16<BF16>(128, TILE_ROWS, false, false);
         const uint32_t st_addr = tc::smem_u32(smem);
         const bool mine = tc::elect();
-        tc::Ring r, dh, old;  // old: the stage of the tile that had this one's buffer of dH
+        tc::Ring r, dh, ready, old;  // old: the stage of the tile that had this one's buffer of dH
         bool ok = __all_sync(~0u, tc::mbar_wait(&s.w_full, 0, fail, a.err));
         for (uint32_t t = group; t < a.tiles && ok; t += a.groups) {
             ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
@@ -206,11 +204,12 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
                     for (uint32_t k = 0; k < 4; ++k)
                         tc::mma_f16_tmem(dh_at + dh.i * TILE_ROWS, tmem + P::W_AT + (c * 4u + k) * 8u, b + c * (P::CHUNK >> 4) + k * 2u,
                                          ID, c + k != 0);
-                tc::commit(&s.dh_full[dh.i]);
+                tc::commit(&s.dh_full[ready.i]);
             }
             __syncwarp();
             r.next(P::STAGES);
             dh.next(P::BUFS);
+            ready.next(P::READY);
         }
         if (!ok) {  // leave no product in flight
             if (mine) tc::commit(&s.failed);
@@ -351,9 +350,10 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&s.w_full);
         }
-        tc::Ring r, dh;
+        tc::Ring r, dh, ready;
         r.skip(set, P::STAGES);
         dh.skip(set, P::BUFS);
+        ready.skip(set, P::READY);
         bool ok = true;
         for (uint32_t t = first; t < a.tiles && ok; t += step) {
             uint32_t next_E[EXPS];
@@ -363,11 +363,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             for (int i = 0; i < EXPS; ++i) scale[i * 32 + lane] = mx8_scale(E[i]);
             __syncwarp();
             ok = __all_sync(~0u, tc::mbar_wait(&s.full[r.i], r.phase, fail, a.err));
-            // A parity tells a phase from the one before it only.  Of a buffer's last use this set knows
-            // that it is over when that was four tiles ago or earlier; with fewer buffers it asks.
-            if (P::BUFS < 4u && t >= group + P::BUFS * a.groups)
-                ok = ok && __all_sync(~0u, tc::mbar_wait(&s.dh_full[dh.i], dh.phase ^ 1u, fail, a.err));
-            ok = ok && __all_sync(~0u, tc::mbar_wait(&s.dh_full[dh.i], dh.phase, fail, a.err));
+            ok = ok && __all_sync(~0u, tc::mbar_wait(&s.dh_full[ready.i], ready.phase, fail, a.err));
             if (!ok) break;
             tc::fence_after();
             const uint8_t *codes = smem + r.i * P::STAGE + P::DY_BYTES + code0;
@@ -423,6 +419,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1)
             out += out_step;
             dh.skip(P::BUFS < 4u ? P::BUFS : 4u, P::BUFS);
             if (P::BUFS < 4u) dh.skip(4u - P::BUFS, P::BUFS);
+            ready.skip(4, P::READY);
             r.skip(4, P::STAGES);
 #pragma unroll
             for (int i = 0; i < EXPS; ++i) E[i] = next_E[i];

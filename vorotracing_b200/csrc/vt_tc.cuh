@@ -14,6 +14,7 @@
 #include <atomic>
 
 #include "vt_abi.cuh"
+#include "vt_ring.cuh"
 #include "vt_wait.cuh"
 
 namespace vt {
@@ -77,20 +78,6 @@ __device__ __forceinline__ void outlast_copies()
     const long long began = clock64();
     while (clock64() - began < WAIT_LIMIT / 100) {}
 }
-
-// Counts through the stages of a ring: index and the parity of its current use.
-struct Ring {
-    uint32_t i = 0, phase = 0;
-    __device__ __forceinline__ void next(uint32_t stages)
-    {
-        if (++i == stages) { i = 0; phase ^= 1u; }
-    }
-    __device__ __forceinline__ void skip(uint32_t n, uint32_t stages)  // n at most stages
-    {
-        i += n;
-        if (i >= stages) { i -= stages; phase ^= 1u; }
-    }
-};
 
 // ---- TMA ----
 
